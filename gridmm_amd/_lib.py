@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(_HERE, "libgridmm_hip.so")
 # overrides and the whole experiment table of tile configurations.  Only the sweep tools ask for it (load(debug=True) or
 # GRIDMM_LIB_DEBUG=1 before the first load); the product path and the tests run on the shipping library, which has neither.
 DEBUG_LIB_PATH = os.path.join(_HERE, "libgridmm_hip_dbg.so")
-ABI_VERSION = 29
+ABI_VERSION = 30
 
 _vp, _i, _f, _i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_int64
 
@@ -129,6 +129,13 @@ SIGNATURES = {
     "gridmm_linear_skinny": [_vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _vp],
     "gridmm_linear_skinny_bwd_workspace": [_i, _i, _i],
     "gridmm_linear_skinny_bwd": [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _vp],
+    # losses over a large vocabulary, top logits
+    "gridmm_vocab_loss_saved_bytes": [_vp],
+    "gridmm_vocab_loss_workspace": [_vp, _i],
+    "gridmm_vocab_loss_fwd": [_vp, _vp, _vp, ctypes.c_size_t, _vp, ctypes.c_size_t, _vp],
+    "gridmm_vocab_loss_bwd": [_vp, _vp, ctypes.c_size_t, _vp, _i64, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp],
+    "gridmm_top_logits_workspace": [_i, _i, _i],
+    "gridmm_top_logits": [_vp, _i64, _i, _i, _i, _i, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp],
     # host-side helpers of the agent loop (no device work)
     "gridmm_route_lengths": [_vp, _i, _i, _vp, _vp, _vp, _i, _vp],
     "gridmm_collate_nav_plan": [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp],
@@ -190,6 +197,9 @@ def load(debug=None):
     lib.gridmm_preln_layer_workspace.restype = ctypes.c_size_t
     lib.gridmm_linear_skinny_bwd_workspace.restype = ctypes.c_size_t
     lib.gridmm_rowdot_bwd_workspace.restype = ctypes.c_size_t
+    lib.gridmm_vocab_loss_saved_bytes.restype = ctypes.c_size_t
+    lib.gridmm_vocab_loss_workspace.restype = ctypes.c_size_t
+    lib.gridmm_top_logits_workspace.restype = ctypes.c_size_t
     lib.gridmm_nav_heads_workspace.argtypes = [_i, _i, _i]
     lib.gridmm_nav_heads_workspace.restype = ctypes.c_size_t
     v = lib.gridmm_abi_version()

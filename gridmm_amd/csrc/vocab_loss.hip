@@ -1,0 +1,968 @@
+// Losses over a large vocabulary from hidden states, in pieces of the vocabulary, without keeping the logits
+// (pretrain_src/model/pretrain_cmt.py:131-153 multiplies the masked tokens with the tied decoder of 30 522 rows and calls
+// cross_entropy on the logits):
+//   scores          z_rj = (h_r . W_j + b_j) / T          L_r = log sum_j exp z_rj
+//   cross entropy   loss_r = L_r - z_{r, y_r}             (T = 1)
+//   distillation    loss_r = T^2 sum_s p_rs (log p_rs - z_{r, id_rs} + L_r),   p_r = softmax of the teacher's top logits / T
+//   both            dS_rj = g_r T (exp(z_rj - L_r) - sum_{s: id_rs = j} p_rs)    (cross entropy: one slot, p = 1)
+//                   dh = dS W,   dW = dS^T h,   db_j = sum_r dS_rj
+// Forward: the score tile's epilogue leaves each row's (maximum, sum of exponentials) of its columns; a second, small kernel joins
+// them.  Backward: the scores are computed again piece by piece, the epilogue turns them into 16-bit dS (one piece at a time, the
+// workspace bounds its width), and two more products read it.  The entries of dS at a target are written by a kernel of their own
+// from the target's fp32 score: exp(..) - p is rounded once there, whatever cancels.
+//
+// Rows that do not count (label == ignore_index; no filled slot) are left out on the device: the counted rows are compacted into
+// the packed copy of h, the grids are sized for all rows and workgroups past the count end at once -- no host read-back.
+//
+// Number formats.  bf16 / fp16 operands: one plane, products exact, sums fp32; dS is rounded to the operands' type (2^-9 / 2^-12
+// of an entry, the size of the rounding of the gradients themselves).  fp32 operands: two fp16 planes each (22 bits) after a
+// power-of-two scale from the tensor's largest finite value, so a product is off by ~2^-22: like fp32 sums.  dS is scaled by a power of
+// two from the largest |g T| of the call (fp16 range: entries below 2^-38 of it vanish).
+// Everything runs in the base-2 domain: y = z log2 e, exp2, and ln 2 comes back in the losses.
+#include <algorithm>
+
+#include "vocab_gemm.h"
+
+namespace {
+
+using vocab::f32x16_t;
+using vocab::Operand;
+using vocab::Tile;
+using vocab::tile_of;
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int AMAX_H = 64, AMAX_W = 512;      // workgroups of the largest-value search (fp32 operands)
+constexpr int PREP_T = 1024;
+enum { F32 = 0, BF16 = 1, F16 = 2 };
+
+__device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype) {
+  if (dtype == F32) return reinterpret_cast<const float*>(p)[i];
+  const unsigned short u = reinterpret_cast<const unsigned short*>(p)[i];
+  return dtype == BF16 ? bf16_bits_to_f32(u) : (float)__builtin_bit_cast(_Float16, u);
+}
+__device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int wide) {
+  return wide ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t)reinterpret_cast<const int32_t*>(p)[i];
+}
+// fp32 -> 16 bits, to nearest even; NaN stays NaN
+__device__ __forceinline__ unsigned short to_f16(float x) { return __builtin_bit_cast(unsigned short, (_Float16)x); }
+__device__ __forceinline__ unsigned short to_bf16(float x) { return (unsigned short)(cvt_pk_bf16(x, x) & 0xffffu); }
+template <bool F16V>
+__device__ __forceinline__ unsigned short to_16(float x) {
+  if constexpr (F16V) return to_f16(x); else return to_bf16(x);
+}
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a <= 3.4028234664e38f ? a : 0.f;
+}
+// power of two that brings values of at most `amax` under 2^(top + 1): exponent top - floor(log2 amax)
+__device__ __forceinline__ int scale_exp(float amax, int top) {
+  if (!(amax > 0.f)) return 0;
+  int e;
+  (void)frexpf(amax, &e);              // amax = f 2^e, f in [1/2, 1)
+  return top + 1 - e;
+}
+
+// what the kernels share on the device: written by the preparation kernels, read by all that follow
+struct Meta {
+  int count;         // rows that count
+  int sh, sw;        // power-of-two exponents of the packed h and W
+};
+
+// ---- targets of the distillation: p = softmax(t / T) over the filled slots, the row's sum of p log p, whether it counts ----
+__global__ __launch_bounds__(256) void kd_targets_kernel(const void* __restrict__ ids, int wide, int64_t ld_ids,
+                                                         const float* __restrict__ t, int64_t ld_t, int rows, int slots,
+                                                         float inv_t, float* __restrict__ p, float* __restrict__ plogp,
+                                                         unsigned char* __restrict__ counts) {
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r >= rows) return;
+  float m = -INFINITY;
+  bool nan = false;
+  for (int s = lane; s < slots; s += 64) {
+    if (load_index(ids, r * ld_ids + s, wide) < 0) continue;
+    const float v = t[r * ld_t + s] * inv_t;
+    nan |= v != v;
+    m = fmaxf(m, v);
+  }
+  m = wave_max(m);
+  nan = __any(nan);
+  if (m == -INFINITY && !nan) {              // nothing to learn from
+    for (int s = lane; s < slots; s += 64) p[(int64_t)r * slots + s] = 0.f;
+    if (lane == 0) { counts[r] = 0; plogp[r] = 0.f; }
+    return;
+  }
+  float sum = 0.f;
+  for (int s = lane; s < slots; s += 64)
+    if (load_index(ids, r * ld_ids + s, wide) >= 0) sum += expf(t[r * ld_t + s] * inv_t - m);
+  sum = wave_sum(sum);
+  const float ls = logf(sum);
+  float h = 0.f;
+  for (int s = lane; s < slots; s += 64) {
+    float q = 0.f;
+    if (load_index(ids, r * ld_ids + s, wide) >= 0) {
+      const float lp = t[r * ld_t + s] * inv_t - m - ls;
+      q = expf(lp);
+      if (q > 0.f || q != q) h += q * lp;
+    }
+    p[(int64_t)r * slots + s] = q;
+  }
+  h = wave_sum(h);
+  if (lane == 0) { counts[r] = 1; plogp[r] = h; }
+}
+
+struct PrepArgs {
+  const void *hidden, *weight, *bias, *labels;
+  const unsigned char* counts;       // distillation; NULL: labels
+  int64_t ldh, ldw, ignore;
+  int rows, vocab, K, wide, dtype, bias_dtype, vp;
+  float inv_t;
+  Meta* meta;
+  int *rowmap, *rowinv;
+  float *loss, *biasz, *amax_h, *amax_w;
+};
+
+__device__ __forceinline__ float amax_row(const float* x, int K, int lane) {
+  float a = 0.f;
+  if (K % 4 == 0 && ((uintptr_t)x & 15) == 0) {
+    for (int k = lane * 4; k < K; k += 256) {
+      const float4 v = *reinterpret_cast<const float4*>(x + k);
+      a = fmaxf(fmaxf(a, fmaxf(finite_abs(v.x), finite_abs(v.y))), fmaxf(finite_abs(v.z), finite_abs(v.w)));
+    }
+  } else {
+    for (int k = lane; k < K; k += 64) a = fmaxf(a, finite_abs(x[k]));
+  }
+  return a;
+}
+
+// One launch: workgroup 0 compacts the counted rows; the next `nb` copy the bias (/ T, base 2, -inf past the vocabulary); for fp32
+// operands the rest find the largest finite |h| of the counted rows and |W|, one partial value a workgroup.
+__global__ __launch_bounds__(PREP_T) void prep_kernel(const PrepArgs a, int nb) {
+  __shared__ int part[16];
+  __shared__ float fpart[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto counted = [&](int r) {
+    return a.counts ? a.counts[r] != 0 : load_index(a.labels, r, a.wide) != a.ignore;
+  };
+  int blk = blockIdx.x;
+  if (blk == 0) {
+    const int64_t per = (a.rows + PREP_T - 1) / PREP_T, r0 = tid * per, r1 = min((int64_t)a.rows, r0 + per);
+    int n = 0;
+    for (int64_t r = r0; r < r1; ++r) n += counted((int)r);
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 63) part[wave] = incl;
+    __syncthreads();
+    int pos = incl - n, total = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) pos += part[w];
+      total += part[w];
+    }
+    for (int64_t r = r0; r < r1; ++r) {
+      const bool c = counted((int)r);
+      a.rowinv[r] = c ? pos : -1;
+      if (c) a.rowmap[pos++] = (int)r;
+      else a.loss[r] = 0.f;
+    }
+    if (tid == 0) { a.meta->count = total; a.meta->sh = a.meta->sw = 0; }
+    return;
+  }
+  blk -= 1;
+  if (blk < nb) {
+    const int64_t j = (int64_t)blk * PREP_T + tid;
+    if (j < a.vp)
+      a.biasz[j] = j >= a.vocab ? -INFINITY : a.bias ? load_as_f32(a.bias, j, a.bias_dtype) * (a.inv_t * LOG2E) : 0.f;
+    return;
+  }
+  blk -= nb;
+  const bool is_h = blk < AMAX_H;
+  if (!is_h) blk -= AMAX_H;
+  const int blocks = is_h ? AMAX_H : AMAX_W;
+  const float* x = reinterpret_cast<const float*>(is_h ? a.hidden : a.weight);
+  const int64_t ld = is_h ? a.ldh : a.ldw;
+  const int rows = is_h ? a.rows : a.vocab;
+  float m = 0.f;
+  for (int64_t r = blk * 16 + wave; r < rows; r += blocks * 16)
+    if (!is_h || counted((int)r)) m = fmaxf(m, amax_row(x + r * ld, a.K, lane));
+  m = wave_max(m);
+  if (lane == 0) fpart[wave] = m;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < 16; ++w) m = fmaxf(m, fpart[w]);
+    (is_h ? a.amax_h : a.amax_w)[blk] = m;
+  }
+}
+
+// ---- packing: rows -> 16-bit rows of Kp columns (zero past K), fp32 as two fp16 planes under a power-of-two scale ----
+__device__ __forceinline__ void pack8(const float (&v)[8], bool split, int sh, unsigned short* hi, unsigned short* lo) {
+  u16x8_t h, l;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float x = split ? ldexpf(v[e], sh) : v[e];
+    const _Float16 f = (_Float16)x;
+    h[e] = __builtin_bit_cast(unsigned short, f);
+    l[e] = to_f16(x - (float)f);
+  }
+  *reinterpret_cast<u16x8_t*>(hi) = h;
+  if (split) *reinterpret_cast<u16x8_t*>(lo) = l;
+}
+__device__ __forceinline__ void pack_row(const void* src, int64_t off, int dtype, int K, int Kp, int lane, int sh, bool zero,
+                                         unsigned short* hi, unsigned short* lo) {
+  if (dtype == F32) {
+    const float* x = reinterpret_cast<const float*>(src) + off;
+    const bool vec = ((uintptr_t)x & 15) == 0;
+    for (int k = lane * 8; k < Kp; k += 512) {
+      float v[8];
+      if (!zero && vec && k + 8 <= K) {
+        const float4 p = *reinterpret_cast<const float4*>(x + k), q = *reinterpret_cast<const float4*>(x + k + 4);
+        v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = !zero && k + e < K ? x[k + e] : 0.f;
+      }
+      pack8(v, true, sh, hi + k, lo + k);
+    }
+  } else {
+    const unsigned short* x = reinterpret_cast<const unsigned short*>(src) + off;
+    const bool vec = ((uintptr_t)x & 15) == 0;
+    for (int k = lane * 8; k < Kp; k += 512) {
+      u16x8_t v;
+      if (!zero && vec && k + 8 <= K) {
+        v = *reinterpret_cast<const u16x8_t*>(x + k);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = !zero && k + e < K ? x[k + e] : (unsigned short)0;
+      }
+      *reinterpret_cast<u16x8_t*>(hi + k) = v;
+    }
+  }
+}
+
+// counted rows of h -> Hp (rows past the count up to a multiple of 256: zero)
+__global__ __launch_bounds__(256) void pack_h_kernel(const void* __restrict__ hidden, int64_t ldh, int dtype, int K, int Kp, int Rp,
+                                                     const int* __restrict__ rowmap, const float* __restrict__ amax_h,
+                                                     const float* __restrict__ amax_w, Meta* __restrict__ meta,
+                                                     unsigned short* __restrict__ Hp) {
+  const int lane = threadIdx.x & 63;
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int count = meta->count;
+  int sh = 0;
+  if (dtype == F32) {
+    sh = scale_exp(wave_max(amax_h[lane]), 14);
+    if (i == 0) {
+      float m = 0.f;
+      for (int k = lane; k < AMAX_W; k += 64) m = fmaxf(m, amax_w[k]);
+      m = wave_max(m);
+      if (lane == 0) { meta->sh = sh; meta->sw = scale_exp(m, 14); }
+    }
+  }
+  if (i >= (count + 255) / 256 * 256) return;
+  const bool zero = i >= count;
+  unsigned short* hi = Hp + (int64_t)i * Kp;
+  pack_row(hidden, zero ? 0 : (int64_t)rowmap[i] * ldh, dtype, K, Kp, lane, sh, zero, hi, hi + (int64_t)Rp * Kp);
+}
+
+// rows [j0, j0 + C) of W -> Wp (zero past the vocabulary)
+__global__ __launch_bounds__(256) void pack_w_kernel(const void* __restrict__ W, int64_t ldw, int dtype, int K, int Kp, int64_t j0,
+                                                     int C, int vocab, const Meta* __restrict__ meta,
+                                                     unsigned short* __restrict__ Wp) {
+  const int lane = threadIdx.x & 63;
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= C) return;
+  const bool zero = j0 + i >= vocab;
+  unsigned short* hi = Wp + (int64_t)i * Kp;
+  pack_row(W, zero ? 0 : (j0 + i) * ldw, dtype, K, Kp, lane, meta->sw, zero, hi, hi + (int64_t)C * Kp);
+}
+
+// ---- forward: per-row (maximum, sum of exponentials) of each tile's columns ----
+template <class T>
+__global__ __launch_bounds__(T::THREADS) void score_stats_kernel(Operand A, Operand B, int nk, int64_t tn, const Meta* __restrict__ meta,
+                                                                 const float* __restrict__ biasz, float unit,
+                                                                 float2* __restrict__ stats, int64_t Rp) {
+  __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
+  __shared__ float2 wst[T::WAVES_N][T::BM];
+  const int count = meta->count;
+  int64_t ty, tx;
+  if (!tile_of(blockIdx.x, (count + T::BM - 1) / T::BM, tn, ty, tx)) return;
+  typename T::Acc acc = {};
+  T::run(A, B, ty * T::BM, tx * T::BN, 0, nk, smem, acc);
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
+  const float sc = ldexpf(unit, -(meta->sh + meta->sw));
+  float m[T::TM], s[T::TM];
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) m[i] = -INFINITY;
+#pragma unroll
+  for (int n = 0; n < T::TN; ++n)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 b = *reinterpret_cast<const float4*>(biasz + tx * T::BN + wc * T::WN + n * 32 + q * 8 + (lane >> 5) * 4);
+#pragma unroll
+      for (int i = 0; i < T::TM; ++i) {
+        f32x16_t& c = acc[i][n];
+        c[q * 4 + 0] = fmaf(c[q * 4 + 0], sc, b.x);
+        c[q * 4 + 1] = fmaf(c[q * 4 + 1], sc, b.y);
+        c[q * 4 + 2] = fmaf(c[q * 4 + 2], sc, b.z);
+        c[q * 4 + 3] = fmaf(c[q * 4 + 3], sc, b.w);
+        m[i] = fmaxf(m[i], fmaxf(fmaxf(c[q * 4], c[q * 4 + 1]), fmaxf(c[q * 4 + 2], c[q * 4 + 3])));
+      }
+    }
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) {
+    m[i] = fmaxf(m[i], __shfl_xor(m[i], 32, 64));
+    const float ref = m[i] == -INFINITY ? 0.f : m[i];      // a tile whose columns are all masked: sum 0
+    float t = 0.f;
+#pragma unroll
+    for (int n = 0; n < T::TN; ++n)
+#pragma unroll
+      for (int q = 0; q < 16; ++q) t += __builtin_amdgcn_exp2f(acc[i][n][q] - ref);
+    s[i] = t + __shfl_xor(t, 32, 64);
+    if (lane < 32) wst[wc][wr * T::WM + i * 32 + lane] = make_float2(m[i], s[i]);
+  }
+  __syncthreads();
+  for (int r = threadIdx.x; r < T::BM; r += T::THREADS) {
+    float2 a = wst[0][r];
+#pragma unroll
+    for (int w = 1; w < T::WAVES_N; ++w) {
+      const float2 b = wst[w][r];
+      const float M = fmaxf(a.x, b.x), ref = M == -INFINITY ? 0.f : M;
+      a = make_float2(M, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
+    }
+    stats[tx * Rp + ty * T::BM + r] = a;
+  }
+}
+
+// ---- scores at the targets: one wave a (row, up to 8 slots), fp32 sums over the operands as they came ----
+struct TargetArgs {
+  const void *hidden, *weight, *index;
+  int64_t ldh, ldw, ld_index;
+  int K, vocab, slots, wide, dtype, kd;      // slots >= 1
+  float unit;
+  const Meta* meta;
+  const int* rowmap;
+  const float* biasz;
+  float* zt;       // [compacted row][slots], base 2
+};
+template <int DT>
+__device__ __forceinline__ float dot_rows(const void* a, int64_t ao, const void* b, int64_t bo, int K, int lane, bool vec) {
+  float s = 0.f;
+  if constexpr (DT == F32) {
+    const float *x = (const float*)a + ao, *y = (const float*)b + bo;
+    if (vec) {
+      for (int k = lane * 4; k < K; k += 256) {
+        const float4 p = *reinterpret_cast<const float4*>(x + k), q = *reinterpret_cast<const float4*>(y + k);
+        s = fmaf(p.x, q.x, s); s = fmaf(p.y, q.y, s); s = fmaf(p.z, q.z, s); s = fmaf(p.w, q.w, s);
+      }
+      return s;
+    }
+  } else if (vec) {
+    const unsigned short *x = (const unsigned short*)a + ao, *y = (const unsigned short*)b + bo;
+    for (int k = lane * 8; k < K; k += 512) {
+      const u16x8_t p = *reinterpret_cast<const u16x8_t*>(x + k), q = *reinterpret_cast<const u16x8_t*>(y + k);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (DT == BF16) s = fmaf(bf16_bits_to_f32(p[e]), bf16_bits_to_f32(q[e]), s);
+        else s = fmaf((float)__builtin_bit_cast(_Float16, (unsigned short)p[e]), (float)__builtin_bit_cast(_Float16, (unsigned short)q[e]), s);
+      }
+    }
+    return s;
+  }
+  for (int k = lane; k < K; k += 64) s = fmaf(load_as_f32(a, ao + k, DT), load_as_f32(b, bo + k, DT), s);
+  return s;
+}
+template <int DT>
+__global__ __launch_bounds__(256) void target_scores_kernel(const TargetArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int groups = (a.slots + 7) / 8;
+  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t i = w / groups;
+  if (i >= a.meta->count) return;
+  const int s0 = (int)(w % groups) * 8, s1 = min(a.slots, s0 + 8);
+  const int64_t r = a.rowmap[i];
+  constexpr int A = DT == F32 ? 4 : 8;
+  const bool vec = a.K % A == 0 && a.ldh % A == 0 && a.ldw % A == 0 && (((uintptr_t)a.hidden | (uintptr_t)a.weight) & 15) == 0;
+  for (int s = s0; s < s1; ++s) {
+    const int64_t id = load_index(a.index, r * a.ld_index + s, a.wide);
+    float z = NAN;                                          // an id outside the vocabulary spoils its row
+    if (a.kd && id < 0) z = 0.f;                            // an empty slot
+    else if (id >= 0 && id < a.vocab) z = fmaf(wave_sum(dot_rows<DT>(a.hidden, r * a.ldh, a.weight, id * a.ldw, a.K, lane, vec)), a.unit, a.biasz[id]);
+    if (lane == 0) a.zt[i * a.slots + s] = z;
+  }
+}
+
+// ---- joins the tiles' statistics and writes the losses: 16 rows a workgroup, 16 threads a row ----
+__global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ stats, int64_t tiles, int64_t Rp, const Meta* __restrict__ meta,
+                                                   const int* __restrict__ rowmap, const float* __restrict__ zt, int slots,
+                                                   const float* __restrict__ p, const float* __restrict__ plogp, float temperature,
+                                                   float* __restrict__ lse, float* __restrict__ loss) {
+  __shared__ float2 part[16][17];
+  __shared__ float acc[16][17];
+  const int rr = threadIdx.x & 15, lanep = threadIdx.x >> 4;
+  const int count = meta->count;
+  const int64_t i = (int64_t)blockIdx.x * 16 + rr;
+  if ((int64_t)blockIdx.x * 16 >= count) return;
+  float2 a = make_float2(-INFINITY, 0.f);
+  auto join = [](float2 a, float2 b) {
+    const float M = fmaxf(a.x, b.x), ref = M == -INFINITY ? 0.f : M;
+    return make_float2(M, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
+  };
+  if (i < count)
+    for (int64_t t = lanep; t < tiles; t += 16) a = join(a, stats[t * Rp + i]);
+  part[lanep][rr] = a;
+  __syncthreads();
+  a = part[0][rr];
+  for (int w = 1; w < 16; ++w) a = join(a, part[w][rr]);
+  const float L = a.x + __builtin_amdgcn_logf(a.y);        // base 2
+  float s = 0.f;
+  bool bad = L != L;
+  if (i < count) {
+    if (p) {
+      const int64_t r = rowmap[i];
+      for (int k = lanep; k < slots; k += 16) {
+        const float q = p[r * slots + k], z = zt[i * slots + k];
+        bad |= z != z;
+        if (!(q == 0.f)) s += q * (L - z);
+      }
+    }
+  }
+  acc[lanep][rr] = bad ? NAN : s;
+  __syncthreads();
+  if (lanep != 0 || i >= count) return;
+  const int64_t r = rowmap[i];
+  float out;
+  if (p) {
+    s = 0.f;
+    for (int w = 0; w < 16; ++w) s += acc[w][rr];
+    out = temperature * temperature * (plogp[r] + s * LN2);
+  } else {
+    out = (L - zt[i]) * LN2;
+    s = zt[i];
+  }
+  loss[r] = out;
+  lse[i] = s != s ? NAN : L;                                // a bad target: its row's gradient is NaN too
+}
+
+// ---- backward ----
+// scale exponent of dS from the largest finite |g T| and the scaled factor of every compacted row (zero past the count)
+__global__ __launch_bounds__(PREP_T) void grad_scale_kernel(const float* __restrict__ g, int64_t gs, float temperature,
+                                                            const int* __restrict__ rowmap, const Meta* __restrict__ meta,
+                                                            int* __restrict__ scale, float* __restrict__ grow, int Rp) {
+  __shared__ float part[16];
+  const int tid = threadIdx.x, count = meta->count;
+  float m = 0.f;
+  for (int i = tid; i < count; i += PREP_T) m = fmaxf(m, finite_abs(g[(int64_t)rowmap[i] * gs] * temperature));
+  m = wave_max(m);
+  if ((tid & 63) == 0) part[tid >> 6] = m;
+  __syncthreads();
+  for (int w = 0; w < 16; ++w) m = fmaxf(m, part[w]);
+  const int sg = scale_exp(m, 13);
+  if (tid == 0) *scale = sg;
+  for (int i = tid; i < Rp; i += PREP_T) grow[i] = i < count ? ldexpf(g[(int64_t)rowmap[i] * gs] * temperature, sg) : 0.f;
+}
+
+// dS of the columns [j0, j0 + C): dS[r][j] = grow_r exp2(y_rj - lse_r), two planes for fp32 operands
+template <class T>
+__global__ __launch_bounds__(T::THREADS) void score_grad_kernel(Operand A, Operand B, int nk, int64_t tn, const Meta* __restrict__ meta,
+                                                                const float* __restrict__ biasz, float unit,
+                                                                const float* __restrict__ lse, const float* __restrict__ grow,
+                                                                unsigned short* __restrict__ dS, int64_t ldS, int64_t plane) {
+  __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
+  const int count = meta->count;
+  int64_t ty, tx;
+  if (!tile_of(blockIdx.x, (count + T::BM - 1) / T::BM, tn, ty, tx)) return;
+  typename T::Acc acc = {};
+  T::run(A, B, ty * T::BM, tx * T::BN, 0, nk, smem, acc);
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
+  const float sc = ldexpf(unit, -(meta->sh + meta->sw));
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) {
+    const int64_t r = ty * T::BM + wr * T::WM + i * 32 + (lane & 31);
+    const bool live = r < count;
+    const float L = live ? lse[r] : 0.f, gr = live ? grow[r] : 0.f;
+#pragma unroll
+    for (int n = 0; n < T::TN; ++n)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t c0 = tx * T::BN + wc * T::WN + n * 32 + q * 8 + (lane >> 5) * 4;
+        const float4 b = *reinterpret_cast<const float4*>(biasz + c0);
+        const float bb[4] = {b.x, b.y, b.z, b.w};
+        u16x4_t hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = live ? gr * __builtin_amdgcn_exp2f(fmaf(acc[i][n][q * 4 + e], sc, bb[e]) - L) : 0.f;
+          if constexpr (T::PL == 2) {
+            const _Float16 h = (_Float16)v;
+            hi[e] = __builtin_bit_cast(unsigned short, h);
+            lo[e] = to_f16(v - (float)h);
+          } else {
+            hi[e] = to_16<T::F16>(v);
+          }
+        }
+        *reinterpret_cast<u16x4_t*>(dS + r * ldS + c0) = hi;
+        if constexpr (T::PL == 2) *reinterpret_cast<u16x4_t*>(dS + plane + r * ldS + c0) = lo;
+      }
+  }
+}
+
+// the entries of dS at the targets in [j0, j0 + C): grow_r (exp2(zt - lse) - sum of p over the slots of the same id), rounded once
+struct FixArgs {
+  const void* index;
+  int64_t ld_index, j0, ldS, plane;
+  int wide, slots, C, vocab, dtype;
+  const Meta* meta;
+  const int* rowmap;
+  const float *p, *zt, *lse, *grow;
+  unsigned short* dS;
+};
+__global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
+  const int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = w / a.slots;
+  const int s = (int)(w % a.slots);
+  if (i >= a.meta->count) return;
+  const int64_t r = a.rowmap[i];
+  const int64_t id = load_index(a.index, r * a.ld_index + s, a.wide);
+  if (id < a.j0 || id >= a.j0 + a.C || id >= a.vocab || id < 0) return;
+  float p = 1.f;
+  if (a.p) {                                       // several slots may name one id: each of them writes the same value
+    p = 0.f;
+    for (int k = 0; k < a.slots; ++k)
+      if (load_index(a.index, r * a.ld_index + k, a.wide) == id) p += a.p[r * a.slots + k];
+  }
+  const float v = a.grow[i] * (__builtin_amdgcn_exp2f(a.zt[i * a.slots + s] - a.lse[i]) - p);
+  unsigned short* at = a.dS + i * a.ldS + (id - a.j0);
+  if (a.dtype == F32) {
+    const _Float16 h = (_Float16)v;
+    at[0] = __builtin_bit_cast(unsigned short, h);
+    at[a.plane] = to_f16(v - (float)h);
+  } else {
+    at[0] = a.dtype == F16 ? to_f16(v) : to_bf16(v);
+  }
+}
+
+// dh of this piece: partial products over the contraction ranges blockIdx.y, added to those of the pieces before
+template <class T>
+__global__ __launch_bounds__(T::THREADS) void hidden_grad_kernel(Operand A, Operand B, int steps, int64_t tn, const Meta* __restrict__ meta,
+                                                                 float* __restrict__ part, int64_t Rp, int64_t Kp, int first) {
+  __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
+  const int count = meta->count;
+  int64_t ty, tx;
+  if (!tile_of(blockIdx.x, (count + T::BM - 1) / T::BM, tn, ty, tx)) return;
+  const int per = (steps + gridDim.y - 1) / gridDim.y, s0 = blockIdx.y * per, nk = min(per, steps - s0);
+  typename T::Acc acc = {};
+  T::run(A, B, ty * T::BM, tx * T::BN, (int64_t)s0 * T::BK, nk, smem, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
+  float* out = part + (int64_t)blockIdx.y * Rp * Kp;
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) {
+    const int64_t r = ty * T::BM + wr * T::WM + i * 32 + (lane & 31);
+#pragma unroll
+    for (int n = 0; n < T::TN; ++n)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t c0 = tx * T::BN + wc * T::WN + n * 32 + q * 8 + (lane >> 5) * 4;
+        if (r >= count || c0 >= Kp) continue;
+        float4* at = reinterpret_cast<float4*>(out + r * Kp + c0);
+        float4 v = make_float4(acc[i][n][q * 4], acc[i][n][q * 4 + 1], acc[i][n][q * 4 + 2], acc[i][n][q * 4 + 3]);
+        if (!first) { const float4 o = *at; v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w; }
+        *at = v;
+      }
+  }
+}
+
+__device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v) {
+  if (dtype == F32) reinterpret_cast<float*>(p)[i] = v;
+  else reinterpret_cast<unsigned short*>(p)[i] = dtype == BF16 ? to_bf16(v) : to_f16(v);
+}
+
+// dh = the ranges' partial products in order, unscaled, to the rows they came from; zero for rows that do not count
+__global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict__ part, int splits, int64_t Rp, int64_t Kp, int K,
+                                                         int rows, const int* __restrict__ rowinv, const Meta* __restrict__ meta,
+                                                         const int* __restrict__ scale, int dtype, void* __restrict__ out) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const int pos = rowinv[r], e = -(*scale + meta->sw);
+  for (int k = lane * 4; k < K; k += 256) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (pos >= 0) {
+      for (int s = 0; s < splits; ++s) {
+        const float4 a = *reinterpret_cast<const float4*>(part + (s * Rp + pos) * Kp + k);
+        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+      }
+      v.x = ldexpf(v.x, e); v.y = ldexpf(v.y, e); v.z = ldexpf(v.z, e); v.w = ldexpf(v.w, e);
+    }
+    const float f[4] = {v.x, v.y, v.z, v.w};
+    for (int x = 0; x < 4; ++x)
+      if (k + x < K) store_as(out, r * K + k + x, dtype, f[x]);
+  }
+}
+
+// dW of this piece: rows [j0, j0 + C) complete (the contraction is all counted rows), written once in the weight's type
+template <class T>
+__global__ __launch_bounds__(T::THREADS) void weight_grad_kernel(Operand A, Operand B, int64_t tm, int64_t tn, const Meta* __restrict__ meta,
+                                                                 const int* __restrict__ scale, int dtype, int64_t j0, int vocab, int K, void* __restrict__ dW) {
+  __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
+  int64_t ty, tx;
+  if (!tile_of(blockIdx.x, tm, tn, ty, tx)) return;
+  const int count = meta->count;
+  typename T::Acc acc = {};
+  T::run(A, B, ty * T::BM, tx * T::BN, 0, (count + T::BK - 1) / T::BK, smem, acc);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
+  const int e = -(*scale + meta->sh);
+#pragma unroll
+  for (int i = 0; i < T::TM; ++i) {
+    const int64_t r = j0 + ty * T::BM + wr * T::WM + i * 32 + (lane & 31);
+    if (r >= vocab) continue;
+#pragma unroll
+    for (int n = 0; n < T::TN; ++n)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t c0 = tx * T::BN + wc * T::WN + n * 32 + q * 8 + (lane >> 5) * 4;
+        float f[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) f[x] = ldexpf(acc[i][n][q * 4 + x], e);
+        if (K % 4 == 0) {
+          if (c0 >= K) continue;
+          if (dtype == F32) {
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(dW) + r * K + c0) = make_float4(f[0], f[1], f[2], f[3]);
+          } else {
+            u16x4_t u;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) u[x] = dtype == BF16 ? to_bf16(f[x]) : to_f16(f[x]);
+            *reinterpret_cast<u16x4_t*>(reinterpret_cast<unsigned short*>(dW) + r * K + c0) = u;
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (c0 + x < K) store_as(dW, r * K + c0 + x, dtype, f[x]);
+        }
+      }
+  }
+}
+
+// db of this piece: column sums of dS, 256 columns a workgroup, 8 rows at a time, joined in order
+__global__ __launch_bounds__(256) void bias_grad_kernel(const unsigned short* __restrict__ dS, int64_t ldS, int64_t plane, int dtype,
+                                                        const Meta* __restrict__ meta, const int* __restrict__ scale, int64_t j0,
+                                                        int vocab, int bias_dtype, void* __restrict__ db) {
+  __shared__ float part[8][256 + 8];
+  const int c = (threadIdx.x & 31) * 8, rp = threadIdx.x >> 5, count = meta->count;
+  float s[8] = {};
+  for (int64_t r = rp; r < count; r += 8) {
+    const unsigned short* at = dS + r * ldS + (int64_t)blockIdx.x * 256 + c;
+    const u16x8_t h = *reinterpret_cast<const u16x8_t*>(at);
+    if (dtype == BF16) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += bf16_bits_to_f32(h[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += (float)__builtin_bit_cast(_Float16, (unsigned short)h[e]);
+    }
+    if (dtype == F32) {
+      const u16x8_t l = *reinterpret_cast<const u16x8_t*>(at + plane);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += (float)__builtin_bit_cast(_Float16, (unsigned short)l[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) part[rp][c + e] = s[e];
+  __syncthreads();
+  const int64_t j = j0 + (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (j >= vocab) return;
+  float t = 0.f;
+  for (int w = 0; w < 8; ++w) t += part[w][threadIdx.x];
+  store_as(db, j, bias_dtype, ldexpf(t, -*scale));
+}
+
+__global__ void zero_u16_kernel(unsigned short* __restrict__ p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) p[i] = 0;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// host side: what lies where, which tile, how wide a piece
+// ---------------------------------------------------------------------------------------------------------------------
+inline size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+
+struct Plan {
+  int PL, slots;               // planes; target slots a row (cross entropy: 1)
+  int64_t Rp, Kp, Vp;
+  bool pack_w;                 // W has to be split or padded; else it is read where it lies
+  int64_t C_fwd, C_bwd;        // columns a piece
+  int splits;                  // contraction ranges of dh
+  bool big;                    // 256 x 256 tiles, else 128 x 128
+  // saved
+  size_t o_meta, o_rowmap, o_rowinv, o_lse, o_zt, o_p, o_biasz, o_h, saved;
+  // forward workspace
+  size_t f_counts, f_plogp, f_amax, f_stats, f_w, fwd;
+  // backward workspace
+  size_t b_scale, b_grow, b_ds, b_w, b_part, bwd;
+};
+
+bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
+  if (!d || d->rows < 0 || d->vocab < 1 || d->hidden_size < 1 || d->slots < 0 || d->dtype < 0 || d->dtype > 2 || d->bias_dtype < 0 ||
+      d->bias_dtype > 2 || !(d->temperature > 0.f) || !(d->temperature < INFINITY) || d->rows > (1 << 28) || d->vocab > (1 << 28) ||
+      d->hidden_size > (1 << 20) || d->slots > (1 << 16) || (!d->slots && d->temperature != 1.f))
+    return false;
+  P.PL = d->dtype == F32 ? 2 : 1;
+  P.slots = d->slots ? d->slots : 1;
+  P.Rp = (int64_t)up(d->rows, 256);
+  P.Kp = (int64_t)up(d->hidden_size, 64);
+  P.Vp = (int64_t)up(d->vocab, 256);
+  P.pack_w = d->dtype == F32 || d->hidden_size % 64 || d->ld_weight % 8 || ((uintptr_t)d->weight & 15);
+  // pieces: packed W and dS at most 128 MB each (both then stay in the 256-MB Infinity Cache between the kernels that write and
+  // read them), whole tiles, 8 192 columns at least
+  const int64_t most = 128ll << 20, least = 8192;
+  auto piece = [&](int64_t bytes_a_column) {
+    int64_t c = most / bytes_a_column / 256 * 256;
+    if (c < least) c = least;
+    if (c >= P.Vp) return P.Vp;
+    const int64_t n = (P.Vp + c - 1) / c;                      // equal pieces
+    return (int64_t)up((P.Vp + n - 1) / n, 256);
+  };
+  P.C_fwd = P.pack_w ? piece(P.Kp * 2 * P.PL) : P.Vp;
+  P.C_bwd = piece(std::max<int64_t>(P.Rp, 1) * 2 * P.PL);
+  if (P.pack_w) P.C_bwd = std::min(P.C_bwd, P.C_fwd);
+  P.big = d->rows > 128 && ((d->rows + 255) / 256) * (P.Vp / 256) >= 512;
+  const int64_t T = P.big ? 256 : 128, tiles = std::max<int64_t>(1, (d->rows + T - 1) / T) * ((P.Kp + T - 1) / T);
+  const int64_t steps = P.C_bwd / 64;
+  int64_t s = (P.big ? 256 : 512) / tiles;
+  s = std::min<int64_t>(s, steps / 8);
+  P.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
+
+  const size_t R = (size_t)std::max(d->rows, 1), Rp = (size_t)std::max<int64_t>(P.Rp, 256), S = P.slots;
+  size_t o = 0;
+  auto take = [&](size_t bytes) { const size_t at = o; o += up(bytes, 256); return at; };
+  P.o_meta = take(sizeof(Meta));
+  P.o_rowmap = take(R * 4);
+  P.o_rowinv = take(R * 4);
+  P.o_lse = take(Rp * 4);
+  P.o_zt = take(R * S * 4);
+  P.o_p = take(d->slots ? R * S * 4 : 0);
+  P.o_biasz = take(P.Vp * 4);
+  P.o_h = take(Rp * P.Kp * 2 * P.PL);
+  P.saved = o;
+  o = 0;
+  P.f_counts = take(R);
+  P.f_plogp = take(R * 4);
+  P.f_amax = take((AMAX_H + AMAX_W) * 4);
+  P.f_stats = take(Rp * (size_t)(P.Vp / 128) * 8);
+  P.f_w = take(P.pack_w ? (size_t)P.C_fwd * P.Kp * 2 * P.PL : 0);
+  P.fwd = o;
+  o = 0;
+  P.b_scale = take(4);
+  P.b_grow = take(Rp * 4);
+  P.b_ds = take(Rp * (size_t)P.C_bwd * 2 * P.PL);
+  P.b_w = take(P.pack_w ? (size_t)P.C_bwd * P.Kp * 2 * P.PL : 0);
+  P.b_part = take((size_t)P.splits * Rp * P.Kp * 4);
+  P.bwd = o;
+  return true;
+}
+
+template <bool F16V, int PL, bool BIG, bool CA, bool CB>
+using TileOf = typename std::conditional<BIG, Tile<F16V, PL, 256, 256, 128, 64, CA, CB>, Tile<F16V, PL, 128, 128, 64, 64, CA, CB>>::type;
+
+// calls f(type tag) for the operands' type and the tile
+template <class F>
+int by_type(const gridmm_vocab_loss_t* d, bool big, F f) {
+  using std::bool_constant;
+  using std::integral_constant;
+  if (d->dtype == F32) return big ? f(bool_constant<true>{}, integral_constant<int, 2>{}, bool_constant<true>{})
+                                  : f(bool_constant<true>{}, integral_constant<int, 2>{}, bool_constant<false>{});
+  if (d->dtype == F16) return big ? f(bool_constant<true>{}, integral_constant<int, 1>{}, bool_constant<true>{})
+                                  : f(bool_constant<true>{}, integral_constant<int, 1>{}, bool_constant<false>{});
+  return big ? f(bool_constant<false>{}, integral_constant<int, 1>{}, bool_constant<true>{})
+             : f(bool_constant<false>{}, integral_constant<int, 1>{}, bool_constant<false>{});
+}
+
+// W's rows [j0, j0 + C) as an operand: packed into `buf` or in place
+int weight_piece(const gridmm_vocab_loss_t* d, const Plan& P, int64_t j0, int64_t C, const Meta* meta, unsigned short* buf,
+                 hipStream_t st, Operand& W) {
+  if (P.pack_w) {
+    GRIDMM_LAUNCH(pack_w_kernel, dim3((unsigned)((C + 3) / 4)), dim3(256), 0, st, d->weight, d->ld_weight, d->dtype, d->hidden_size,
+                  (int)P.Kp, j0, (int)C, d->vocab, meta, buf);
+    GRIDMM_CHECK_LAUNCH();
+    W = Operand{buf, P.Kp, C * P.Kp, C, P.Kp};
+  } else {
+    W = Operand{(const unsigned short*)d->weight + j0 * d->ld_weight, d->ld_weight, 0, d->vocab - j0, P.Kp};
+  }
+  return GRIDMM_OK;
+}
+
+bool bad_pointers(const gridmm_vocab_loss_t* d, const void* saved, bool forward) {
+  if (!d->weight || !saved || d->ld_weight < d->hidden_size || ((uintptr_t)saved & 255)) return true;
+  if (d->rows && forward && (!d->hidden || d->ld_hidden < d->hidden_size)) return true;
+  if (d->rows && d->slots && (!d->ids || d->ld_ids < d->slots)) return true;
+  if (d->rows && d->slots && forward && (!d->teacher || d->ld_teacher < d->slots)) return true;
+  if (d->rows && !d->slots && !d->labels) return true;
+  return false;
+}
+
+}  // namespace
+
+extern "C" size_t gridmm_vocab_loss_saved_bytes(const gridmm_vocab_loss_t* d) {
+  Plan P;
+  return make_plan(d, P) ? P.saved : 0;
+}
+
+extern "C" size_t gridmm_vocab_loss_workspace(const gridmm_vocab_loss_t* d, int backward) {
+  Plan P;
+  return make_plan(d, P) ? (backward ? P.bwd : P.fwd) : 0;
+}
+
+extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, void* saved, size_t saved_bytes, void* workspace,
+                                     size_t workspace_bytes, gridmm_stream_t stream) {
+  Plan P;
+  if (!make_plan(d, P) || bad_pointers(d, saved, true) || saved_bytes < P.saved || !workspace || workspace_bytes < P.fwd ||
+      ((uintptr_t)workspace & 255) || (d->rows && !loss))
+    return GRIDMM_EINVAL;
+  if (d->rows == 0) return GRIDMM_OK;
+  hipStream_t st = as_stream(stream);
+  char *sv = (char*)saved, *ws = (char*)workspace;
+  Meta* meta = (Meta*)(sv + P.o_meta);
+  int *rowmap = (int*)(sv + P.o_rowmap), *rowinv = (int*)(sv + P.o_rowinv);
+  float *lse = (float*)(sv + P.o_lse), *zt = (float*)(sv + P.o_zt), *p = d->slots ? (float*)(sv + P.o_p) : nullptr;
+  float* biasz = (float*)(sv + P.o_biasz);
+  unsigned short* Hp = (unsigned short*)(sv + P.o_h);
+  unsigned char* counts = (unsigned char*)(ws + P.f_counts);
+  float *plogp = (float*)(ws + P.f_plogp), *amax = (float*)(ws + P.f_amax);
+  float2* stats = (float2*)(ws + P.f_stats);
+  const float inv_t = 1.f / d->temperature, unit = inv_t * LOG2E;
+
+  if (d->slots) {
+    GRIDMM_LAUNCH(kd_targets_kernel, dim3((d->rows + 3) / 4), dim3(256), 0, st, d->ids, d->index64, d->ld_ids, d->teacher,
+                  d->ld_teacher, d->rows, d->slots, inv_t, p, plogp, counts);
+    GRIDMM_CHECK_LAUNCH();
+  }
+  PrepArgs a;
+  a.hidden = d->hidden; a.weight = d->weight; a.bias = d->bias; a.labels = d->labels;
+  a.counts = d->slots ? counts : nullptr;
+  a.ldh = d->ld_hidden; a.ldw = d->ld_weight; a.ignore = d->ignore_index;
+  a.rows = d->rows; a.vocab = d->vocab; a.K = d->hidden_size; a.wide = d->index64; a.dtype = d->dtype; a.bias_dtype = d->bias_dtype;
+  a.vp = (int)P.Vp; a.inv_t = inv_t; a.meta = meta; a.rowmap = rowmap; a.rowinv = rowinv; a.loss = loss; a.biasz = biasz;
+  a.amax_h = amax; a.amax_w = amax + AMAX_H;
+  const int nb = (int)((P.Vp + PREP_T - 1) / PREP_T);
+  GRIDMM_LAUNCH(prep_kernel, dim3(1 + nb + (d->dtype == F32 ? AMAX_H + AMAX_W : 0)), dim3(PREP_T), 0, st, a, nb);
+  GRIDMM_CHECK_LAUNCH();
+  GRIDMM_LAUNCH(pack_h_kernel, dim3((unsigned)(P.Rp / 4)), dim3(256), 0, st, d->hidden, d->ld_hidden, d->dtype, d->hidden_size,
+                (int)P.Kp, (int)P.Rp, rowmap, amax, amax + AMAX_H, meta, Hp);
+  GRIDMM_CHECK_LAUNCH();
+
+  const Operand H{Hp, P.Kp, P.Rp * P.Kp, P.Rp, P.Kp};
+  const int BT = P.big ? 256 : 128;
+  for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_fwd) {
+    const int64_t C = std::min(P.C_fwd, P.Vp - j0);
+    Operand W;
+    int rc = weight_piece(d, P, j0, C, meta, (unsigned short*)(ws + P.f_w), st, W);
+    if (rc != GRIDMM_OK) return rc;
+    rc = by_type(d, P.big, [&](auto f16, auto pl, auto big) {
+      using T = TileOf<decltype(f16)::value, decltype(pl)::value, decltype(big)::value, false, false>;
+      const int64_t tn = C / T::BN, tm = (d->rows + T::BM - 1) / T::BM;
+      GRIDMM_LAUNCH((score_stats_kernel<T>), dim3((unsigned)(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), tn, meta,
+                    biasz + j0, unit, stats + j0 / T::BN * P.Rp, P.Rp);
+      GRIDMM_CHECK_LAUNCH();
+      return GRIDMM_OK;
+    });
+    if (rc != GRIDMM_OK) return rc;
+  }
+  TargetArgs t;
+  t.hidden = d->hidden; t.weight = d->weight; t.index = d->slots ? d->ids : d->labels;
+  t.ldh = d->ld_hidden; t.ldw = d->ld_weight; t.ld_index = d->slots ? d->ld_ids : 1;
+  t.K = d->hidden_size; t.vocab = d->vocab; t.slots = P.slots; t.wide = d->index64; t.dtype = d->dtype; t.kd = d->slots > 0;
+  t.unit = unit; t.meta = meta; t.rowmap = rowmap; t.biasz = biasz; t.zt = zt;
+  const dim3 tg((unsigned)(((int64_t)d->rows * ((P.slots + 7) / 8) + 3) / 4));
+  if (d->dtype == F32) GRIDMM_LAUNCH(target_scores_kernel<F32>, tg, dim3(256), 0, st, t);
+  else if (d->dtype == BF16) GRIDMM_LAUNCH(target_scores_kernel<BF16>, tg, dim3(256), 0, st, t);
+  else GRIDMM_LAUNCH(target_scores_kernel<F16>, tg, dim3(256), 0, st, t);
+  GRIDMM_CHECK_LAUNCH();
+  GRIDMM_LAUNCH(loss_kernel, dim3((d->rows + 15) / 16), dim3(256), 0, st, stats, P.Vp / BT, P.Rp, meta, rowmap, zt, P.slots, p,
+                plogp, d->temperature, lse, loss);
+  GRIDMM_CHECK_LAUNCH();
+  return GRIDMM_OK;
+}
+
+extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* saved, size_t saved_bytes, const float* grad,
+                                     int64_t grad_stride, void* d_hidden, void* d_weight, void* d_bias, void* workspace,
+                                     size_t workspace_bytes, gridmm_stream_t stream) {
+  Plan P;
+  if (!make_plan(d, P) || bad_pointers(d, saved, false) || saved_bytes < P.saved || !workspace || workspace_bytes < P.bwd ||
+      ((uintptr_t)workspace & 255) || (d->rows && !grad) || (!d_hidden && !d_weight && !d_bias) || grad_stride < 0 ||
+      (d_bias && !d->bias))
+    return GRIDMM_EINVAL;
+  hipStream_t st = as_stream(stream);
+  if (d->rows == 0) {                       // nothing counts: the shared gradients are zero
+    const int64_t nw = (int64_t)d->vocab * d->hidden_size * (d->dtype == F32 ? 2 : 1), nb = (int64_t)d->vocab * (d->bias_dtype == F32 ? 2 : 1);
+    if (d_weight) GRIDMM_LAUNCH(zero_u16_kernel, dim3((unsigned)std::min<int64_t>((nw + 255) / 256, 4096)), dim3(256), 0, st, (unsigned short*)d_weight, nw);
+    if (d_bias) GRIDMM_LAUNCH(zero_u16_kernel, dim3((unsigned)std::min<int64_t>((nb + 255) / 256, 4096)), dim3(256), 0, st, (unsigned short*)d_bias, nb);
+    GRIDMM_CHECK_LAUNCH();
+    return GRIDMM_OK;
+  }
+  const char* sv = (const char*)saved;
+  char* ws = (char*)workspace;
+  const Meta* meta = (const Meta*)(sv + P.o_meta);
+  int* scale = (int*)(ws + P.b_scale);
+  const int *rowmap = (const int*)(sv + P.o_rowmap), *rowinv = (const int*)(sv + P.o_rowinv);
+  const float *lse = (const float*)(sv + P.o_lse), *zt = (const float*)(sv + P.o_zt);
+  const float *p = d->slots ? (const float*)(sv + P.o_p) : nullptr, *biasz = (const float*)(sv + P.o_biasz);
+  const unsigned short* Hp = (const unsigned short*)(sv + P.o_h);
+  float *grow = (float*)(ws + P.b_grow), *part = (float*)(ws + P.b_part);
+  unsigned short *dS = (unsigned short*)(ws + P.b_ds), *wbuf = (unsigned short*)(ws + P.b_w);
+  const float unit = LOG2E / d->temperature;
+
+  GRIDMM_LAUNCH(grad_scale_kernel, dim3(1), dim3(PREP_T), 0, st, grad, grad_stride, d->temperature, rowmap, meta, scale, grow, (int)P.Rp);
+  GRIDMM_CHECK_LAUNCH();
+  const Operand H{Hp, P.Kp, P.Rp * P.Kp, P.Rp, P.Kp};
+  for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_bwd) {
+    const int64_t C = std::min(P.C_bwd, P.Vp - j0);
+    Operand W;
+    int rc = weight_piece(d, P, j0, C, meta, wbuf, st, W);
+    if (rc != GRIDMM_OK) return rc;
+    const int64_t plane = P.Rp * C;
+    const Operand S{dS, C, plane, P.Rp, C};
+    rc = by_type(d, P.big, [&](auto f16, auto pl, auto big) {
+      constexpr bool F = decltype(f16)::value, BIG = decltype(big)::value;
+      constexpr int L = decltype(pl)::value;
+      {
+        using T = TileOf<F, L, BIG, false, false>;
+        const int64_t tn = C / T::BN, tm = (d->rows + T::BM - 1) / T::BM;
+        GRIDMM_LAUNCH((score_grad_kernel<T>), dim3((unsigned)(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), tn, meta,
+                      biasz + j0, unit, lse, grow, dS, C, plane);
+        GRIDMM_CHECK_LAUNCH();
+      }
+      FixArgs f;
+      f.index = d->slots ? d->ids : d->labels; f.ld_index = d->slots ? d->ld_ids : 1; f.j0 = j0; f.ldS = C; f.plane = plane;
+      f.wide = d->index64; f.slots = P.slots; f.C = (int)C; f.vocab = d->vocab; f.dtype = d->dtype; f.meta = meta; f.rowmap = rowmap;
+      f.p = p; f.zt = zt; f.lse = lse; f.grow = grow; f.dS = dS;
+      GRIDMM_LAUNCH(target_grad_kernel, dim3((unsigned)(((int64_t)d->rows * P.slots + 255) / 256)), dim3(256), 0, st, f);
+      GRIDMM_CHECK_LAUNCH();
+      if (d_hidden) {
+        using T = TileOf<F, L, BIG, false, true>;
+        const int64_t tn = (P.Kp + T::BN - 1) / T::BN, tm = (d->rows + T::BM - 1) / T::BM;
+        GRIDMM_LAUNCH((hidden_grad_kernel<T>), dim3((unsigned)(tm * tn), P.splits), dim3(T::THREADS), 0, st, S, W, (int)(C / T::BK), tn,
+                      meta, part, P.Rp, P.Kp, j0 == 0);
+        GRIDMM_CHECK_LAUNCH();
+      }
+      if (d_weight) {
+        using T = TileOf<F, L, BIG, true, true>;
+        const int64_t tn = (P.Kp + T::BN - 1) / T::BN, tm = C / T::BM;
+        GRIDMM_LAUNCH((weight_grad_kernel<T>), dim3((unsigned)(tm * tn)), dim3(T::THREADS), 0, st, S, H, tm, tn, meta, scale, d->dtype, j0,
+                      d->vocab, d->hidden_size, d_weight);
+        GRIDMM_CHECK_LAUNCH();
+      }
+      if (d_bias) {
+        GRIDMM_LAUNCH(bias_grad_kernel, dim3((unsigned)(C / 256)), dim3(256), 0, st, dS, C, plane, d->dtype, meta, scale, j0,
+                      d->vocab, d->bias_dtype, d_bias);
+        GRIDMM_CHECK_LAUNCH();
+      }
+      return GRIDMM_OK;
+    });
+    if (rc != GRIDMM_OK) return rc;
+  }
+  if (d_hidden) {
+    GRIDMM_LAUNCH(hidden_out_kernel, dim3((d->rows + 3) / 4), dim3(256), 0, st, part, P.splits, P.Rp, P.Kp, d->hidden_size, d->rows,
+                  rowinv, meta, scale, d->dtype, d_hidden);
+    GRIDMM_CHECK_LAUNCH();
+  }
+  return GRIDMM_OK;
+}

@@ -1,0 +1,188 @@
+"""Losses over a large vocabulary without keeping the logits, and a teacher's top logits.
+
+  vocab_cross_entropy   softmax cross entropy of hidden states against decoder rows, forward and backward in pieces of the
+                        vocabulary (gridmm_vocab_loss_fwd / _bwd).  Beside autograd.linear + torch's cross_entropy, which is what
+                        GlocalTextPathCMTPreTraining.forward_mlm (pretrain_src/model/pretrain_cmt.py:131-153) computes and which
+                        keeps rows x vocabulary fp32 logits for the backward
+  vocab_distillation    the same head against a teacher's top logits: T^2 KL(teacher over its slots || student over everything)
+  top_logits            the k largest logits of every row, their ids and the row's log-sum-exp: the teacher's side
+
+There is no CPU fallback: the functions raise on non-GPU tensors.
+"""
+import contextlib
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib, ops
+from .autograd import DEFERRED
+from .ops import _p, _stream
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_TOP = 1024
+
+
+class _Desc(ctypes.Structure):
+    """gridmm_vocab_loss_t of include/gridmm.h."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("hidden", "weight", "bias", "labels", "ids", "teacher")]
+                + [(n, ctypes.c_int64) for n in ("ld_hidden", "ld_weight", "ld_ids", "ld_teacher", "ignore_index")]
+                + [(n, ctypes.c_int) for n in ("rows", "vocab", "hidden_size", "slots", "dtype", "bias_dtype", "index64")]
+                + [("temperature", ctypes.c_float)])
+
+
+def _on(device):
+    """The tensors' own device as the current one (the kernels go to its current stream)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _rows(t):
+    """(..., C) -> its rows as (M, C) with a contiguous last dimension and one row stride, and that stride."""
+    C = t.shape[-1]
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= C:
+        return t, t.stride(0)
+    t = t.contiguous().view(-1, C) if C else t.reshape(0, 0)
+    return t, C
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _check_head(hidden, weight, bias, **index):
+    for name, t in dict(hidden=hidden, weight=weight, bias=bias, **index).items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.GridmmLibraryError("gridmm ops need GPU tensors (%s is on %s); no CPU fallback exists" % (name, t.device))
+        _need(t.device == hidden.device, "%s is on %s, hidden on %s" % (name, t.device, hidden.device))
+    _need(hidden.dtype in _DTYPES, "hidden is fp32, bf16 or fp16, not %s" % hidden.dtype)
+    _need(weight.dtype == hidden.dtype, "weight is %s, hidden %s: one type for both" % (weight.dtype, hidden.dtype))
+    _need(hidden.dim() >= 1 and weight.dim() == 2 and weight.shape[1] == hidden.shape[-1],
+          "hidden (..., K) and weight (V, K), not %s and %s" % (tuple(hidden.shape), tuple(weight.shape)))
+    _need(weight.shape[0] >= 1 and weight.shape[1] >= 1, "an empty weight %s" % (tuple(weight.shape),))
+    if bias is not None:
+        _need(tuple(bias.shape) == (weight.shape[0],), "bias (V,), not %s" % (tuple(bias.shape),))
+        _need(bias.dtype in (torch.float32, weight.dtype), "bias is %s: fp32 or the weight's type" % bias.dtype)
+
+
+class _VocabLoss(torch.autograd.Function):
+    """hidden (R, K), weight (V, K), bias (V,) or None, index (R,) labels or (R, S) ids, teacher None or (R, S) -> losses (R,)."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, index, teacher, ignore_index, temperature):
+        lib = _lib.load()
+        ctx.set_materialize_grads(False)
+        w, ldw = _rows(weight)
+        b = None if bias is None else bias.contiguous()
+        d = _Desc()
+        d.weight, d.bias = w.data_ptr(), None if b is None else b.data_ptr()
+        d.ld_weight, d.rows, d.vocab, d.hidden_size = ldw, hidden.shape[0], w.shape[0], w.shape[1]
+        d.dtype, d.bias_dtype = _DTYPES[w.dtype], 0 if b is None else _DTYPES[b.dtype]
+        d.index64, d.temperature, d.ignore_index = int(index.dtype == torch.int64), temperature, ignore_index
+        if teacher is None:
+            d.labels, d.slots = index.data_ptr(), 0
+        else:
+            d.ids, d.ld_ids, d.slots = index.data_ptr(), index.stride(0), index.shape[1]
+            d.teacher, d.ld_teacher = teacher.data_ptr(), teacher.stride(0)
+        d.hidden, d.ld_hidden = hidden.data_ptr(), hidden.stride(0)
+        need = any(ctx.needs_input_grad[:3])
+        dev = hidden.device
+        n_saved, n_ws = lib.gridmm_vocab_loss_saved_bytes(ctypes.byref(d)), lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 0)
+        if n_saved == 0 or n_ws == 0:
+            raise ValueError("sizes the vocabulary losses do not take: rows %d, vocabulary %d, hidden %d, slots %d"
+                             % (d.rows, d.vocab, d.hidden_size, d.slots))
+        loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
+        saved = torch.empty(n_saved, dtype=torch.uint8, device=dev)
+        ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
+        _lib.check(lib.gridmm_vocab_loss_fwd(ctypes.byref(d), _p(loss), _p(saved), n_saved, _p(ws), n_ws, _stream()),
+                   "gridmm_vocab_loss_fwd")
+        if need:
+            ctx.save_for_backward(w, b, index, saved)
+            ctx.desc, ctx.prm, ctx.shape = d, (weight, bias), hidden.shape
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        if g is None:
+            return (None,) * 7
+        lib = _lib.load()
+        w, b, index, saved = ctx.saved_tensors
+        d = ctx.desc
+        dev = w.device
+        if g.dtype != torch.float32:
+            g = g.float()
+        need_h, need_w, need_b = ctx.needs_input_grad[:3]
+        dh = torch.empty(ctx.shape, dtype=w.dtype, device=dev) if need_h else None
+        dw = torch.empty(w.shape, dtype=w.dtype, device=dev) if need_w else None
+        db = torch.empty(b.shape, dtype=b.dtype, device=dev) if need_b else None
+        with _on(dev):
+            n_ws = lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 1)
+            ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
+            _lib.check(lib.gridmm_vocab_loss_bwd(ctypes.byref(d), _p(saved), saved.numel(), _p(g), g.stride(0), _p(dh), _p(dw),
+                                                 _p(db), _p(ws), n_ws, _stream()), "gridmm_vocab_loss_bwd")
+        return dh, DEFERRED.hand(ctx.prm[0], dw), DEFERRED.hand(ctx.prm[1], db), None, None, None, None
+
+
+def vocab_cross_entropy(hidden, weight, labels, bias=None, ignore_index=-1):
+    """Cross entropy of softmax(hidden weight^T + bias) against labels: fp32 losses of labels' shape, 0 where the label is
+    ignore_index (those rows cost nothing and get no gradient).  hidden (..., K) and weight (V, K) in one of fp32 / bf16 / fp16,
+    bias (V,) in that type or fp32, labels (...) int64 or int32.  Gradients of hidden, weight and bias in their types.
+
+    A label outside [0, V) that is not ignore_index makes its row's loss NaN, and with it the gradients that it reaches."""
+    _check_head(hidden, weight, bias, labels=labels)
+    _need(tuple(labels.shape) == tuple(hidden.shape[:-1]), "labels %s for hidden %s" % (tuple(labels.shape), tuple(hidden.shape)))
+    _need(labels.dtype in (torch.int64, torch.int32), "labels are int64 or int32, not %s" % labels.dtype)
+    with _on(hidden.device):
+        h, _ = _rows(hidden)
+        return _VocabLoss.apply(h, weight, bias, labels.reshape(-1).contiguous(), None, int(ignore_index), 1.0).view(labels.shape)
+
+
+def vocab_distillation(hidden, weight, teacher_ids, teacher_logits, bias=None, temperature=1.0):
+    """Distillation from a teacher's top logits over the same head: with p = softmax(teacher_logits / T) over the slots of a row and
+    q = softmax((hidden weight^T + bias) / T) over the whole vocabulary, T^2 sum_s p_s (log p_s - log q[id_s]) as fp32 losses of
+    hidden's leading shape.  teacher_ids (..., S) int64 or int32: an id < 0 is an empty slot, an id >= V makes its row NaN, ids may
+    repeat; teacher_logits (..., S) (top_logits gives both).  A row without a filled slot above -inf: loss 0, no gradient.
+    Gradients of hidden, weight and bias; the teacher gets none."""
+    _check_head(hidden, weight, bias, teacher_ids=teacher_ids, teacher_logits=teacher_logits)
+    _need(teacher_ids.dim() >= 1 and teacher_ids.shape == teacher_logits.shape
+          and tuple(teacher_ids.shape[:-1]) == tuple(hidden.shape[:-1]) and teacher_ids.shape[-1] >= 1,
+          "teacher_ids %s and teacher_logits %s for hidden %s" % (tuple(teacher_ids.shape), tuple(teacher_logits.shape),
+                                                                  tuple(hidden.shape)))
+    _need(teacher_ids.dtype in (torch.int64, torch.int32), "teacher_ids are int64 or int32, not %s" % teacher_ids.dtype)
+    _need(teacher_logits.dtype in _DTYPES, "teacher_logits are fp32, bf16 or fp16, not %s" % teacher_logits.dtype)
+    T = float(temperature)
+    _need(0.0 < T < float("inf"), "a temperature above 0, not %r" % (temperature,))
+    with _on(hidden.device):
+        h, _ = _rows(hidden)
+        ids, _ = _rows(teacher_ids)
+        t, _ = _rows(teacher_logits.detach().float())
+        return _VocabLoss.apply(h, weight, bias, ids, t, -1, T).view(hidden.shape[:-1])
+
+
+def top_logits(logits, k):
+    """The k largest of every row of logits (..., V): (values (..., k) in the logits' type, ids (..., k) int64, lse (...) fp32 = the
+    row's log-sum-exp).  Sorted by value, among equal values by id (the lowest first; -0 equals +0), NaN before everything.
+    1 <= k <= min(V, 1024).  No gradients: a teacher's scores."""
+    if not logits.is_cuda:
+        raise _lib.GridmmLibraryError("gridmm ops need GPU tensors (got %s); no CPU fallback exists" % logits.device)
+    _need(logits.dtype in _DTYPES, "logits are fp32, bf16 or fp16, not %s" % logits.dtype)
+    k = int(k)
+    _need(logits.dim() >= 1 and 1 <= k <= min(logits.shape[-1], MAX_TOP), "1 <= k <= min(V, %d): k = %d of %s"
+          % (MAX_TOP, k, tuple(logits.shape)))
+    lib = _lib.load()
+    with _on(logits.device):
+        x, ld = _rows(logits.detach())
+        lead, dev, R, V = logits.shape[:-1], logits.device, x.shape[0], x.shape[1]
+        values = torch.empty(*lead, k, dtype=x.dtype, device=dev)
+        ids = torch.empty(*lead, k, dtype=torch.int64, device=dev)
+        lse = torch.empty(lead, dtype=torch.float32, device=dev)
+        n = lib.gridmm_top_logits_workspace(R, V, k)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        _lib.check(lib.gridmm_top_logits(_p(x), ld, _DTYPES[x.dtype], R, V, k, _p(values), _p(ids), _p(lse), _p(ws), n, _stream()),
+                   "gridmm_top_logits")
+    return values, ids, lse

@@ -811,6 +811,47 @@ int gridmm_preln_layer_bwd(const gridmm_preln_layer_t* L, const float* X, const 
 int gridmm_dropout_add(const float* x, const float* r, float* y, void* y_hi, void* y_lo, int64_t n, float p,
                        unsigned long long seed, const unsigned long long* seed_dev, gridmm_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Losses over a large vocabulary, in pieces of the vocabulary, without keeping the logits: the masked-token head
+ * (pretrain_src/model/pretrain_cmt.py:131-153: decoder over 30 522 rows + cross_entropy, reduction "none") and its
+ * distillation from a teacher's top logits.  z_rj = (h_r . W_j + b_j) / T,  L_r = log sum_j exp z_rj;
+ *   cross entropy (slots == 0, T must be 1):  loss_r = L_r - z_{r, label_r};  label == ignore_index: loss 0, no gradient
+ *   distillation (slots >= 1):  p_r = softmax over the filled slots of teacher_r / T;
+ *                               loss_r = T^2 sum_s p_rs (log p_rs - z_{r, ids_rs} + L_r);  an id < 0 is an empty slot, a row
+ *                               without a filled slot above -inf: loss 0, no gradient; ids of one row may repeat
+ * A label / id >= vocab (a label < 0 that is not ignore_index) reads nothing out of range: its row's loss and gradients are NaN.
+ *   hidden [rows][hidden_size], weight [vocab][hidden_size] in dtype (0 fp32, 1 bf16, 2 fp16), row strides ld_*; bias [vocab] in
+ *   bias_dtype or NULL; labels [rows], ids [rows][slots] int64 (index64 != 0) or int32; teacher fp32 [rows][slots].
+ * fp32 operands run as two fp16 planes under a power-of-two scale of the tensor (22 bits), 16-bit ones as they are; sums,
+ * maxima and losses are fp32.  Deterministic.  Rows that do not count are left out on the device (no read-back): a capture
+ * may replay the call with other labels.
+ *   saved      >= gridmm_vocab_loss_saved_bytes, 256-byte aligned: filled by _fwd, read (not changed) by _bwd
+ *   workspace  >= gridmm_vocab_loss_workspace(d, 0 forward / 1 backward) bytes, 256-byte aligned
+ *   backward   grad: d loss_r at grad[r * grad_stride] (0: one value for all rows); d_hidden [rows][hidden_size],
+ *              d_weight [vocab][hidden_size] dense in dtype, d_bias [vocab] in bias_dtype, each overwritten, each may be NULL (one
+ *              at least is not); hidden and teacher are not read. */
+typedef struct {
+  const void *hidden, *weight, *bias, *labels, *ids;
+  const float* teacher;
+  int64_t ld_hidden, ld_weight, ld_ids, ld_teacher, ignore_index;
+  int rows, vocab, hidden_size, slots, dtype, bias_dtype, index64;
+  float temperature;
+} gridmm_vocab_loss_t;
+size_t gridmm_vocab_loss_saved_bytes(const gridmm_vocab_loss_t* d);
+size_t gridmm_vocab_loss_workspace(const gridmm_vocab_loss_t* d, int backward);
+int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, void* saved, size_t saved_bytes, void* workspace,
+                          size_t workspace_bytes, gridmm_stream_t stream);
+int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* saved, size_t saved_bytes, const float* grad,
+                          int64_t grad_stride, void* d_hidden, void* d_weight, void* d_bias, void* workspace,
+                          size_t workspace_bytes, gridmm_stream_t stream);
+
+/* The k largest of every row of logits [rows][vocab] (dtype as above, row stride ld), their ids and the row's log-sum-exp:
+ * the teacher's side of the distillation.  Order: value descending, id ascending among equal values (-0 equals +0), NaN first.
+ *   1 <= k <= min(vocab, 1024);  values [rows][k] in dtype, ids [rows][k] int64, lse [rows] fp32
+ *   workspace  >= gridmm_top_logits_workspace(rows, vocab, k) bytes, 256-byte aligned (NULL if that is 0) */
+size_t gridmm_top_logits_workspace(int rows, int vocab, int k);
+int gridmm_top_logits(const void* logits, int64_t ld, int dtype, int rows, int vocab, int k, void* values, int64_t* ids,
+                      float* lse, void* workspace, size_t workspace_bytes, gridmm_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
  * Host-side helpers of the agent loop's collation (HOST pointers, no device work, no stream)

@@ -1,0 +1,609 @@
+"""Losses over a large vocabulary (gridmm_amd/vocab.py, csrc/vocab_loss.hip) and the selection of top logits (csrc/top_logits.hip)
+against their definitions in 64 bits.
+
+Tolerances are bounds, derived from the arithmetic (u = 2^-24 is half a step of fp32):
+  score      two fp16 planes hold 22 bits of an fp32 operand and the lo lo product is left out: 3 2^-22 of |h| |W|; 16-bit products
+             are exact; an fp32 sum of n terms is off by n u of the sum of their sizes; three roundings and a base-2 scale on |z|
+             e_z = (c + K u) |h| . |W| + 4 u |z|,   c = 3 2^-22 (fp32), 0 (16 bits)
+  loss       L is off by at most max e_z + the sum of exponentials (V u + 2 steps of exp2 / log2) -> + (V + 8) u (|L| + 1)
+  dS entry   exp(z - L) is off by its own size times (e_z + e_L); a target adds its p times 4 u; then one rounding: half a step of
+             the 16-bit type, 2^-22 for two fp16 planes; fp16 has no step below 2^-24, and dS is scaled to 2^13 at most: 2^-36 of
+             the largest |g T|
+  gradients  the entries' errors times the other factor, plus (c + n u) of the sum of sizes, plus half a step of the output's type
+"""
+import os
+
+import pytest
+import torch
+
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+DT = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def _inputs(dtype, R, V, K, bias=True, seed=0, device="cuda", spread=2.0):
+    g = torch.Generator().manual_seed(seed)
+    dt = DT[dtype]
+    h = torch.randn(R, K, generator=g).to(dt).to(device)
+    w = (torch.randn(V, K, generator=g) * (spread / K ** 0.5)).to(dt).to(device)
+    b = (torch.randn(V, generator=g) * 0.5).to(dt).to(device) if bias else None
+    return h, w, b, g
+
+
+def _oracle(h, w, b, ids, p, T, g):
+    """Losses, gradients and their error bounds in fp64; ids / p (R, S): targets (p rows of 0: the row does not count); g (R,)."""
+    K, V, dt = h.shape[1], w.shape[0], h.dtype
+    H, W = h.double(), w.double()
+    z = H @ W.t()
+    size = H.abs() @ W.abs().t()
+    if b is not None:
+        z = z + b.double()
+        size = size + b.double().abs()
+    z, size = z / T, size / T
+    c = 3 * 2.0 ** -22 if dt == torch.float32 else 0.0
+    e_z = (c + K * U) * size + 4 * U * z.abs().nan_to_num(posinf=0.0)
+    L = torch.logsumexp(z, 1)
+    live = (p.sum(1) > 0).double()
+    slot = ids.clamp(min=0)
+    e_max = e_z.max(1)[0]
+    e_L = e_max + (V + 8) * U * (L.abs() + 1)
+    zt = z.gather(1, slot)
+    logp = torch.where(p > 0, p.log(), torch.zeros_like(p))
+    loss = live * T * T * (p * (logp - torch.where(p > 0, zt, torch.zeros_like(zt)) + L[:, None])).sum(1)
+    e_loss = live * T * T * (e_max + e_L + 16 * U * ((p * (logp.abs() + torch.where(p > 0, zt, torch.zeros_like(zt)).abs())).sum(1)
+                                                        + L.abs() + 1) + ids.shape[1] * U)
+    q = (z - L[:, None]).exp()
+    target = torch.zeros_like(q).scatter_add_(1, slot, torch.where(ids >= 0, p, torch.zeros_like(p)))
+    gt = (g.double() * T * live)[:, None]
+    dS = gt * (q - target)
+    rnd = HALF[dt] if dt != torch.float32 else 2.0 ** -22
+    e_S = gt.abs() * (q * (e_z + e_L[:, None]) * 1.01 + 8 * U * (target + q)) + 4 * U * dS.abs()
+    e_S = e_S + rnd * (dS.abs() + e_S) + (2.0 ** -36 * gt.abs().max() if dt != torch.bfloat16 else 0.0)
+    out = {"loss": (loss, e_loss)}
+
+    def product(x, ex, y, n):
+        v = x @ y
+        e = (ex @ y.abs()) + (c + n * U) * (x.abs() @ y.abs())
+        return v, e + HALF[dt] * (v.abs() + e) + 2.0 ** -140
+    out["d_hidden"] = product(dS, e_S, W, V)
+    out["d_weight"] = product(dS.t(), e_S.t(), H, h.shape[0])
+    if b is not None:
+        v, e = dS.sum(0), e_S.sum(0) + h.shape[0] * U * dS.abs().sum(0)
+        out["d_bias"] = (v, e + HALF[b.dtype] * (v.abs() + e) + 2.0 ** -140)
+    return out
+
+
+def _hold(got, want, what):
+    v, e = want
+    d = (got.double() - v).abs()
+    if got.dtype == torch.float16:
+        e = e + 2.0 ** -25                        # fp16 has no finer step
+    bad = ~(d <= e)
+    assert not bool(bad.any()), "%s: %d of %d over the bound, worst %.3g of a bound of %.3g" % (
+        what, int(bad.sum()), d.numel(), float(d[bad].max()), float(e.expand_as(d)[bad][d[bad].argmax()]))
+
+
+def _leaves(h, w, b):
+    return [t.detach().clone().requires_grad_() if t is not None else None for t in (h, w, b)]
+
+
+def _run_ce(h, w, b, labels, g, ignore=-1):
+    from gridmm_amd import vocab
+    hl, wl, bl = _leaves(h, w, b)
+    loss = vocab.vocab_cross_entropy(hl, wl, labels, bias=bl, ignore_index=ignore)
+    loss.backward(g)
+    got = {"loss": loss.detach(), "d_hidden": hl.grad, "d_weight": wl.grad}
+    if b is not None:
+        got["d_bias"] = bl.grad
+    return got
+
+
+def _check_ce(h, w, b, labels, g, ignore=-1):
+    got = _run_ce(h, w, b, labels, g, ignore)
+    p = (labels != ignore).double()[:, None]
+    want = _oracle(h, w, b, torch.where(labels == ignore, torch.zeros_like(labels), labels).long()[:, None], p, 1.0, g)
+    for k, v in want.items():
+        assert got[k].dtype == (torch.float32 if k == "loss" else w.dtype if k != "d_bias" else b.dtype)
+        _hold(got[k], v, k)
+    return got
+
+
+CE = [("fp32", 1, 1, 1), ("fp32", 1, 300, 64), ("bf16", 1, 257, 64), ("fp16", 3, 1000, 72), ("fp32", 37, 1000, 256), ("bf16", 129, 511, 128),
+      ("fp16", 64, 256, 64), ("fp32", 200, 777, 33), ("bf16", 65, 1025, 200), ("fp16", 130, 2049, 96), ("fp32", 257, 513, 768),
+      ("bf16", 300, 70000, 64), ("fp32", 300, 70000, 64), ("bf16", 7, 40000, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,R,V,K", CE)
+@pytest.mark.parametrize("bias", [False, True])
+def test_cross_entropy_and_its_gradients(dtype, R, V, K, bias):
+    h, w, b, g = _inputs(dtype, R, V, K, bias, seed=R + V + K)
+    labels = torch.randint(0, V, (R,), generator=g)
+    if R > 2:
+        labels[torch.rand(R, generator=g) < 0.3] = -1
+    labels[0], labels[-1] = 0, V - 1
+    _check_ce(h, w, b, labels.cuda(), (torch.rand(R, generator=g) - 0.3).cuda())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_cross_entropy_over_several_pieces(dtype):
+    """More columns than one piece of dS holds: rows x vocabulary over 128 MB of 16-bit values, and packed weight pieces."""
+    R, V, K = 4100, 20011, 72
+    h, w, b, g = _inputs(dtype, R, V, K, True, seed=5)
+    labels = torch.randint(0, V, (R,), generator=g).cuda()
+    _check_ce(h, w, b, labels, (torch.rand(R, generator=g) / R).cuda())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_cross_entropy_of_rows_that_are_all_ignored(dtype):
+    h, w, b, _ = _inputs(dtype, 70, 300, 64)
+    h[3] = float("nan")                            # an ignored row's values are never read into a result
+    got = _run_ce(h, w, b, torch.full((70,), -100, device="cuda"), torch.ones(70, device="cuda"), ignore=-100)
+    for v in got.values():
+        assert bool((v == 0).all())
+
+
+@pytest.mark.gpu
+def test_ignored_rows_may_hold_anything():
+    h, w, b, g = _inputs("fp32", 40, 500, 64)
+    labels = torch.randint(0, 500, (40,), generator=g).cuda()
+    labels[::3] = -1
+    clean = _run_ce(h, w, b, labels, torch.ones(40, device="cuda"))
+    h[0], h[3] = float("nan"), 3.0e38
+    dirty = _run_ce(h, w, b, labels, torch.ones(40, device="cuda"))
+    for k in clean:
+        assert torch.equal(clean[k], dirty[k]), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("index", [torch.int64, torch.int32])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_cross_entropy_of_strided_operands(dtype, index):
+    """Rows of a wider matrix, off a 16-byte boundary; a transposed weight; a batch of sequences."""
+    R, V, K = 50, 333, 64
+    g = torch.Generator().manual_seed(3)
+    big = torch.randn(R, K + 19, generator=g).to(DT[dtype]).cuda()
+    wt = (torch.randn(K, V, generator=g) / 4).to(DT[dtype]).cuda()
+    wbig = (torch.randn(V, 2 * K + 5, generator=g) / 4).to(DT[dtype]).cuda()
+    labels = torch.randint(0, V, (R,), generator=g).to(index).cuda()
+    gr = torch.rand(R, generator=g).cuda()
+    for h, w in ((big[:, 3:3 + K], wbig[:, 7:7 + K]), (big[:, :K], wt.t()), (big.view(-1)[:R * K].view(R, K), wbig[:, :K])):
+        _check_ce(h, w, None, labels, gr)
+    from gridmm_amd import vocab
+    w = wt.t().contiguous()
+    h3 = big[:, :K].contiguous().view(5, 10, K)
+    a = vocab.vocab_cross_entropy(h3, w, labels.view(5, 10))
+    assert a.shape == (5, 10) and torch.equal(a.view(-1), vocab.vocab_cross_entropy(h3.reshape(R, K), w, labels))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_bias_of_minus_infinity_masks_a_column(dtype):
+    h, w, b, g = _inputs(dtype, 33, 600, 64)
+    labels = torch.randint(0, 300, (33,), generator=g).cuda()
+    b[300:] = float("-inf")                        # whole tiles without a live column
+    w[400] = 60.0
+    hl, wl, bl = _leaves(h, w, b)
+    from gridmm_amd import vocab
+    gr = torch.rand(33, generator=g).cuda()
+    loss = vocab.vocab_cross_entropy(hl, wl, labels, bias=bl)
+    loss.backward(gr)
+    want = _oracle(h, w[:300], b[:300], labels[:, None], torch.ones(33, 1, device="cuda", dtype=torch.float64), 1.0, gr)
+    for k, t in (("loss", loss.detach()), ("d_hidden", hl.grad), ("d_weight", wl.grad[:300]), ("d_bias", bl.grad[:300])):
+        v, e = want[k]
+        _hold(t, (v, e * 8), k)                    # w[400] sets the scale of the fp32 planes: 60 against a spread of 1/4 is 8 bits less range, not precision
+    assert bool((wl.grad[300:] == 0).all()) and bool((bl.grad[300:] == 0).all())
+
+
+@pytest.mark.gpu
+def test_a_label_outside_the_vocabulary_spoils_its_row_and_nothing_else():
+    h, w, b, g = _inputs("fp32", 20, 100, 64)
+    labels = torch.randint(0, 100, (20,), generator=g).cuda()
+    good = _run_ce(h, w, b, labels, torch.ones(20, device="cuda"))
+    for bad in (100, -2, 2 ** 31 - 1, -2 ** 40):
+        lab = labels.clone()
+        lab[7] = bad
+        got = _run_ce(h, w, b, lab, torch.ones(20, device="cuda"))
+        keep = torch.arange(20, device="cuda") != 7
+        assert bool(torch.isnan(got["loss"][7])) and torch.equal(got["loss"][keep], good["loss"][keep])
+        assert bool(torch.isnan(got["d_hidden"][7]).all()) and torch.equal(got["d_hidden"][keep], good["d_hidden"][keep])
+        assert bool(torch.isnan(got["d_bias"]).all())
+
+
+@pytest.mark.gpu
+def test_a_row_of_nan_or_infinity_stays_its_own():
+    for bad in (float("nan"), float("inf")):
+        h, w, b, g = _inputs("fp32", 20, 100, 64)
+        labels = torch.randint(0, 100, (20,), generator=g).cuda()
+        good = _run_ce(h, w, b, labels, torch.ones(20, device="cuda"))
+        h[5, 3] = bad
+        got = _run_ce(h, w, b, labels, torch.ones(20, device="cuda"))
+        keep = torch.arange(20, device="cuda") != 5
+        assert bool(torch.isnan(got["loss"][5]))
+        scale = good["loss"][keep].abs().max()
+        assert float((got["loss"][keep] - good["loss"][keep]).abs().max()) <= 8 * U * 64 * float(scale + 8)
+
+
+def _kd_inputs(dtype, R, V, K, S, seed):
+    h, w, b, g = _inputs(dtype, R, V, K, True, seed)
+    ids = torch.stack([torch.randperm(V, generator=g)[:S] for _ in range(R)])
+    t = torch.randn(R, S, generator=g) * 3
+    return h, w, b, ids, t, g
+
+
+def _teacher(ids, t, T):
+    t = torch.where(ids >= 0, t.double() / T, torch.full_like(t.double(), float("-inf")))
+    p = torch.softmax(t, 1)
+    return torch.nan_to_num(p)
+
+
+def _check_kd(h, w, b, ids, t, g, T):
+    from gridmm_amd import vocab
+    hl, wl, bl = _leaves(h, w, b)
+    loss = vocab.vocab_distillation(hl, wl, ids, t, bias=bl, temperature=T)
+    loss.backward(g)
+    want = _oracle(h, w, b, ids.long(), _teacher(ids, t, T), T, g)
+    got = {"loss": loss.detach(), "d_hidden": hl.grad, "d_weight": wl.grad, "d_bias": bl.grad}
+    for k, v in want.items():
+        _hold(got[k], v, k)
+
+
+KD = [("fp32", 1, 1, 64, 1, 1.0), ("fp32", 5, 300, 64, 8, 2.0), ("bf16", 130, 1000, 128, 32, 1.0), ("fp16", 77, 513, 72, 100, 0.5),
+      ("fp32", 300, 2000, 100, 17, 4.0), ("bf16", 3, 40000, 64, 256, 1.5), ("fp32", 64, 256, 64, 256, 1.0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,R,V,K,S,T", KD)
+def test_distillation_and_its_gradients(dtype, R, V, K, S, T):
+    h, w, b, ids, t, g = _kd_inputs(dtype, R, V, K, S, seed=R + S)
+    if R > 4:
+        ids[torch.rand(R, S, generator=g) < 0.2] = -1
+        ids[1] = -1                                    # a row without a target
+        t[2] = float("-inf")                           # a row whose teacher says nothing
+        t[3, 0] = float("-inf")
+    _check_kd(h, w, b, ids.cuda(), t.cuda(), torch.rand(R, generator=g).cuda(), T)
+
+
+@pytest.mark.gpu
+def test_distillation_where_ids_repeat_and_are_int32_columns_of_a_wider_table():
+    h, w, b, ids, t, g = _kd_inputs("fp32", 40, 90, 64, 12, seed=1)
+    ids = torch.randint(0, 5, (40, 15), generator=g)
+    t = torch.randn(40, 20, generator=g)
+    _check_kd(h, w, b, ids.int().cuda()[:, 2:14], t.cuda()[:, 3:15], torch.rand(40, generator=g).cuda(), 1.0)
+
+
+@pytest.mark.gpu
+def test_distillation_of_an_id_past_the_vocabulary():
+    from gridmm_amd import vocab
+    h, w, b, ids, t, g = _kd_inputs("bf16", 10, 300, 64, 4, seed=1)
+    good = vocab.vocab_distillation(h, w, ids.cuda(), t.cuda(), bias=b)
+    ids[4, 2] = 300
+    got = vocab.vocab_distillation(h, w, ids.cuda(), t.cuda(), bias=b)
+    keep = torch.arange(10, device="cuda") != 4
+    assert bool(torch.isnan(got[4])) and torch.equal(got[keep], good[keep])
+
+
+@pytest.mark.gpu
+def test_one_slot_at_temperature_one_is_cross_entropy():
+    from gridmm_amd import vocab
+    h, w, b, g = _inputs("fp32", 50, 700, 128)
+    labels = torch.randint(0, 700, (50,), generator=g).cuda()
+    a = vocab.vocab_cross_entropy(h, w, labels, bias=b)
+    k = vocab.vocab_distillation(h, w, labels[:, None], torch.randn(50, 1, device="cuda"), bias=b)
+    assert float((a - k).abs().max()) <= 4 * U * float(a.abs().max() + 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_gradients_against_differences(dtype):
+    """Central differences of the fp32 losses along random directions: step d, error of the difference O(d^2) + noise / d."""
+    from gridmm_amd import vocab
+    R, V, K, d = 24, 200, 64, 2.0 ** -6
+    h, w, b, g = _inputs("fp32", R, V, K, True, seed=9, spread=1.0)
+    ids = torch.stack([torch.randperm(V, generator=g)[:6] for _ in range(R)]).cuda()
+    t = torch.randn(R, 6, generator=g).cuda()
+    labels = torch.randint(0, V, (R,), generator=g).cuda()
+    cast = DT[dtype]
+    for f in (lambda a, m, c: vocab.vocab_cross_entropy(a, m, labels, bias=c),
+              lambda a, m, c: vocab.vocab_distillation(a, m, ids, t, bias=c, temperature=2.0)):
+        hl, wl, bl = _leaves(h.to(cast), w.to(cast), b.to(cast))
+        f(hl, wl, bl).sum().backward()
+        for leaf in (hl, wl, bl):
+            u = torch.randn(leaf.shape, generator=g).cuda()
+            u = u / u.norm() * d
+            args = [x.detach().float() for x in (hl, wl, bl)]
+            i = [x is leaf for x in (hl, wl, bl)].index(True)
+            up, dn = list(args), list(args)
+            up[i], dn[i] = args[i] + u, args[i] - u
+            slope = float((f(*up).double().sum() - f(*dn).double().sum()) / 2)
+            want = float((leaf.grad.double() * u.double()).sum())
+            # third derivative of a log-sum-exp along a step of size s (in scores): s^3 / 3 a row at most; noise: R losses of ~8 off by 2^-20
+            step = float((u.double().norm()) * max(float(h.double().norm(dim=1).max()), float(w.double().norm(dim=1).max()), 1.0))
+            bound = R * step ** 3 + R * 8 * 2.0 ** -19 + (2 * HALF[cast] if dtype != "fp32" else 2.0 ** -18) * float((leaf.grad.double().abs() * u.double().abs()).sum())
+            assert abs(slope - want) <= bound, (slope, want, bound)
+
+
+@pytest.mark.gpu
+def test_only_the_gradients_that_are_asked_for():
+    from gridmm_amd import vocab
+    h, w, b, g = _inputs("fp32", 30, 400, 64)
+    labels = torch.randint(0, 400, (30,), generator=g).cuda()
+    full = _run_ce(h, w, b, labels, torch.ones(30, device="cuda"))
+    for mask in range(1, 8):
+        ts = [t.detach().clone().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate((h, w, b))]
+        vocab.vocab_cross_entropy(ts[0], ts[1], labels, bias=ts[2]).sum().backward()      # (a gradient of stride 0)
+        for i, k in enumerate(("d_hidden", "d_weight", "d_bias")):
+            if mask >> i & 1:
+                assert torch.equal(ts[i].grad, full[k]), (mask, k)
+            else:
+                assert ts[i].grad is None
+
+
+@pytest.mark.gpu
+def test_runs_repeat_bit_for_bit_and_leave_their_inputs():
+    h, w, b, g = _inputs("bf16", 300, 3000, 128)
+    labels = torch.randint(0, 3000, (300,), generator=g).cuda()
+    gr = torch.rand(300, generator=g).cuda()
+    copies = [t.clone() for t in (h, w, b, labels, gr)]
+    first = _run_ce(h, w, b, labels, gr)
+    for _ in range(3):
+        again = _run_ce(h, w, b, labels, gr)
+        for k in first:
+            assert torch.equal(first[k], again[k]), k
+    for a, c in zip((h, w, b, labels, gr), copies):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
+def test_backward_twice_of_a_retained_graph_with_other_gradients():
+    from gridmm_amd import vocab
+    h, w, b, g = _inputs("fp16", 40, 500, 64)
+    labels = torch.randint(0, 500, (40,), generator=g).cuda()
+    hl, wl, bl = _leaves(h, w, b)
+    loss = vocab.vocab_cross_entropy(hl, wl, labels, bias=bl)
+    for scale in (1.0, 1e-4, 64.0):
+        gr = (torch.rand(40, generator=g) * scale).cuda()
+        got = torch.autograd.grad(loss, (hl, wl, bl), gr, retain_graph=True)
+        want = _run_ce(h, w, b, labels, gr)
+        for x, k in zip(got, ("d_hidden", "d_weight", "d_bias")):
+            assert torch.equal(x, want[k])
+
+
+@pytest.mark.gpu
+def test_a_weight_changed_before_the_backward_is_refused():
+    from gridmm_amd import vocab
+    h, w, b, g = _inputs("fp32", 10, 100, 64)
+    hl, wl, bl = _leaves(h, w, b)
+    loss = vocab.vocab_cross_entropy(hl, wl, torch.zeros(10, dtype=torch.long, device="cuda"), bias=bl)
+    with torch.no_grad():
+        wl.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.sum().backward()
+
+
+@pytest.mark.gpu
+def test_no_rows():
+    from gridmm_amd import vocab
+    h, w, b, _ = _inputs("bf16", 0, 100, 64)
+    got = _run_ce(h, w, b, torch.zeros(0, dtype=torch.long, device="cuda"), torch.zeros(0, device="cuda"))
+    assert got["loss"].shape == (0,) and got["d_hidden"].shape == (0, 64)
+    assert bool((got["d_weight"] == 0).all()) and bool((got["d_bias"] == 0).all())
+    v, i, l = vocab.top_logits(torch.zeros(0, 10, device="cuda"), 3)
+    assert v.shape == (0, 3) and i.shape == (0, 3) and l.shape == (0,)
+
+
+@pytest.mark.gpu
+def test_on_another_stream():
+    h, w, b, g = _inputs("fp32", 100, 2000, 128)
+    labels = torch.randint(0, 2000, (100,), generator=g).cuda()
+    gr = torch.rand(100, generator=g).cuda()
+    want = _run_ce(h, w, b, labels, gr)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        got = _run_ce(h, w, b, labels, gr)
+    torch.cuda.current_stream().wait_stream(st)
+    for k in want:
+        assert torch.equal(want[k], got[k])
+
+
+@pytest.mark.gpu
+def test_captured_step_replays_with_other_labels_and_other_counts():
+    """Forward and backward in one hipGraph; between the replays the labels (and with them the number of rows that count) change and
+    eager work of the same operators runs."""
+    from gridmm_amd import vocab
+    h, w, b, g = _inputs("fp32", 300, 1500, 128)
+    hl, wl, bl = _leaves(h, w, b)
+    labels = torch.randint(0, 1500, (300,), generator=g).cuda()
+    gr = torch.rand(300, generator=g).cuda()
+
+    def step():
+        loss = vocab.vocab_cross_entropy(hl, wl, labels, bias=bl)
+        return (loss,) + torch.autograd.grad(loss, (hl, wl, bl), gr)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(st)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for drop in (0.0, 0.5, 1.0, 0.1):
+        new = torch.randint(0, 1500, (300,), generator=g)
+        new[torch.rand(300, generator=g) < drop] = -1
+        labels.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _run_ce(h, w, b, labels, gr)
+        for x, k in zip(out, ("loss", "d_hidden", "d_weight", "d_bias")):
+            assert torch.equal(x, want[k]), (drop, k)
+
+
+# ---- top logits ----
+def _top_oracle(x, k):
+    key = x.float().cpu()
+    key = torch.where(torch.isnan(key), torch.full_like(key, float("inf")), key)
+    nan = torch.isnan(x.float().cpu())
+    out = []
+    for r in range(x.shape[0]):
+        order = sorted(range(x.shape[1]), key=lambda j: (not bool(nan[r, j]), -float(key[r, j]), j))[:k]
+        out.append(order)
+    return torch.tensor(out, dtype=torch.int64)
+
+
+def _check_top(x, k):
+    from gridmm_amd import vocab
+    values, ids, lse = vocab.top_logits(x, k)
+    want = _top_oracle(x, k)
+    assert torch.equal(ids.cpu(), want)
+    assert torch.equal(torch.nan_to_num(values, nan=7.0), torch.nan_to_num(x.gather(1, want.to(x.device)), nan=7.0))
+    z = torch.logsumexp(x.double(), 1)
+    fine = torch.isfinite(z)
+    assert torch.equal(torch.isnan(z), torch.isnan(lse)) and torch.equal(z[~fine & ~torch.isnan(z)].float(), lse[~fine & ~torch.isnan(z)])
+    # a sum of V fp32 exponentials in pieces, each off by 2 steps of exp and one of its argument
+    bound = (x.shape[1] ** 0.5 + 16) * U * (z[fine].abs() + x[fine].double().nan_to_num(neginf=0.0).abs().amax(1) + 1)
+    assert bool(((lse[fine].double() - z[fine]).abs() <= bound).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("R,V,k", [(1, 1, 1), (1, 5, 5), (3, 64, 7), (7, 1000, 1), (2, 1025, 1024), (5, 4099, 100), (1, 70001, 256),
+                                   (2, 30522, 32), (300, 257, 16)])
+def test_top_logits(dtype, R, V, k):
+    g = torch.Generator().manual_seed(V + k)
+    _check_top((torch.randn(R, V, generator=g) * 3).to(DT[dtype]).cuda(), k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_top_logits_of_rows_that_are_hard_to_select_from(dtype):
+    dt, V = DT[dtype], 9001
+    rows = [torch.zeros(V), torch.arange(V) / 64.0, -torch.arange(V) / 64.0, torch.full((V,), float("-inf")), torch.full((V,), float("inf"))]
+    few = torch.full((V,), float("-inf"))
+    few[[17, 4000, 8999]] = torch.tensor([1.0, -3.0, 1.0])
+    signed = torch.zeros(V)
+    signed[::2] = -0.0
+    nan = torch.randn(V, generator=torch.Generator().manual_seed(0))
+    nan[[5, 7000]] = float("nan")
+    big = torch.randn(V, generator=torch.Generator().manual_seed(1)) * 1e4
+    two = torch.where(torch.arange(V) % 3 == 0, 2.0, 1.0)
+    x = torch.stack(rows + [few, signed, nan, big, two]).to(dt).cuda()
+    for k in (1, 3, 64, 1000):
+        _check_top(x, k)
+
+
+@pytest.mark.gpu
+def test_top_logits_of_rows_of_a_wider_matrix_and_of_a_batch():
+    from gridmm_amd import vocab
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(6, 1000, generator=g).bfloat16().cuda()
+    _check_top(x[:, 3:990], 20)
+    _check_top(x.t()[:500, :5].t(), 9)
+    v, i, l = vocab.top_logits(x.view(2, 3, 1000), 4)
+    v2, i2, l2 = vocab.top_logits(x, 4)
+    assert v.shape == i.shape == (2, 3, 4) and l.shape == (2, 3)
+    assert torch.equal(v.view(6, 4), v2) and torch.equal(i.view(6, 4), i2) and torch.equal(l.view(6), l2)
+    v1, i1, l1 = vocab.top_logits(x[0], 4)
+    assert torch.equal(v1, v2[0]) and torch.equal(i1, i2[0]) and torch.equal(l1, l2[0])
+
+
+@pytest.mark.gpu
+def test_teacher_to_student():
+    """The three together, as they are used: a teacher's scores, its top logits, the student's two losses in one backward."""
+    from gridmm_amd import vocab
+    R, V, K, k, T = 90, 3000, 128, 20, 2.0
+    h, w, b, g = _inputs("fp32", R, V, K, True, seed=4)
+    teacher = (torch.randn(R, K, generator=g).cuda() + 0.5 * h) @ w.t()
+    values, ids, lse = vocab.top_logits(teacher, k)
+    assert bool((lse >= values[:, 0]).all())
+    labels = torch.randint(0, V, (R,), generator=g).cuda()
+    hl, wl, bl = _leaves(h, w, b)
+    loss = vocab.vocab_cross_entropy(hl, wl, labels, bias=bl).mean() + 0.5 * vocab.vocab_distillation(hl, wl, ids, values, bias=bl,
+                                                                                                      temperature=T).mean()
+    loss.backward()
+    one = torch.ones(R, 1, device="cuda", dtype=torch.float64)
+    a = _oracle(h, w, b, labels[:, None], one, 1.0, torch.full((R,), 1.0 / R, device="cuda"))
+    c = _oracle(h, w, b, ids, _teacher(ids, values, T), T, torch.full((R,), 0.5 / R, device="cuda"))
+    for name, t in (("d_hidden", hl.grad), ("d_weight", wl.grad), ("d_bias", bl.grad)):
+        v = a[name][0] + c[name][0]
+        _hold(t, (v, (a[name][1] + c[name][1]) * 1.001 + 2 * U * v.abs()), name)
+
+
+# ---- refusals (no kernel runs) ----
+def test_refusals_on_the_cpu():
+    from gridmm_amd import _lib, vocab
+    h, w, y = torch.zeros(4, 8), torch.zeros(10, 8), torch.zeros(4, dtype=torch.long)
+    for call in (lambda: vocab.vocab_cross_entropy(h, w, y), lambda: vocab.vocab_distillation(h, w, y[:, None], h[:, :1]),
+                 lambda: vocab.top_logits(h, 2)):
+        with pytest.raises(_lib.GridmmLibraryError):
+            call()
+
+
+def _descriptor(**over):
+    from gridmm_amd import vocab
+    d = vocab._Desc()
+    d.rows, d.vocab, d.hidden_size, d.slots, d.temperature = 4, 100, 64, 0, 1.0
+    d.ld_hidden = d.ld_weight = 64
+    for k, v in over.items():
+        setattr(d, k, v)
+    return d
+
+
+def test_the_c_entry_refuses_bad_sizes_and_pointers():
+    """The library is called without a GPU: every one of these returns before anything is launched."""
+    import ctypes
+    from gridmm_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        import __graft_entry__ as g
+        g.build()
+    lib = _lib.load()
+    EINVAL = -1
+    assert lib.gridmm_vocab_loss_saved_bytes(ctypes.byref(_descriptor())) > 0
+    for over in (dict(rows=-1), dict(vocab=0), dict(hidden_size=0), dict(slots=-1), dict(dtype=3), dict(bias_dtype=-1),
+                 dict(temperature=0.0), dict(temperature=float("nan")), dict(temperature=float("inf")), dict(temperature=2.0),
+                 dict(rows=2 ** 30), dict(vocab=2 ** 30), dict(hidden_size=2 ** 21), dict(slots=2 ** 17)):
+        d = _descriptor(**over)
+        assert lib.gridmm_vocab_loss_saved_bytes(ctypes.byref(d)) == 0, over
+        assert lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 0) == 0 and lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 1) == 0
+        assert lib.gridmm_vocab_loss_fwd(ctypes.byref(d), 256, 256, 1 << 40, 256, 1 << 40, None) == EINVAL
+    n, ws = lib.gridmm_vocab_loss_saved_bytes(ctypes.byref(_descriptor())), lib.gridmm_vocab_loss_workspace(ctypes.byref(_descriptor()), 0)
+    ok = dict(hidden=256, weight=256, labels=256)
+    for over, args in ((dict(hidden=0), (256, 256, n, 256, ws)), (dict(weight=0), (256, 256, n, 256, ws)), (dict(labels=0), (256, 256, n, 256, ws)),
+                       (dict(ld_hidden=63), (256, 256, n, 256, ws)), (dict(ld_weight=63), (256, 256, n, 256, ws)),
+                       ({}, (0, 256, n, 256, ws)), ({}, (256, 0, n, 256, ws)), ({}, (256, 256, n - 1, 256, ws)),
+                       ({}, (256, 256, n, 0, ws)), ({}, (256, 256, n, 256, ws - 1)), ({}, (256, 16, n, 256, ws)), ({}, (256, 256, n, 16, ws)),
+                       (dict(slots=4, ids=256, ld_ids=4, ld_teacher=4), (256, 256, 1 << 40, 256, 1 << 40)),
+                       (dict(slots=4, ids=256, teacher=256, ld_ids=3, ld_teacher=4), (256, 256, 1 << 40, 256, 1 << 40))):
+        assert lib.gridmm_vocab_loss_fwd(ctypes.byref(_descriptor(**{**ok, **over})), *args, None) == EINVAL, (over, args)
+    wb = lib.gridmm_vocab_loss_workspace(ctypes.byref(_descriptor()), 1)
+    for over, args in (({}, (256, n, 0, 1, 256, 256, 0, 256, wb)), ({}, (256, n, 256, 1, 0, 0, 0, 256, wb)), ({}, (256, n, 256, -1, 256, 0, 0, 256, wb)),
+                       ({}, (256, n, 256, 1, 256, 0, 256, 256, wb)), ({}, (256, n, 256, 1, 256, 0, 0, 256, wb - 1))):
+        assert lib.gridmm_vocab_loss_bwd(ctypes.byref(_descriptor(**{**ok, **over})), *args, None) == EINVAL, (over, args)
+    for a in ((256, 9, 0, 1, 10, 2), (256, 10, 3, 1, 10, 2), (256, 10, 0, -1, 10, 2), (256, 10, 0, 1, 10, 0), (256, 10, 0, 1, 10, 11),
+              (256, 2000, 0, 1, 2000, 1025), (0, 10, 0, 1, 10, 2)):
+        assert lib.gridmm_top_logits(*a, 256, 256, 256, 256, 1 << 40, None) == EINVAL, a
+
+
+@pytest.mark.gpu
+def test_the_wrappers_refuse():
+    from gridmm_amd import vocab
+    h, w, y = torch.zeros(4, 8).cuda(), torch.zeros(10, 8).cuda(), torch.zeros(4, dtype=torch.long).cuda()
+    t = torch.zeros(4, 3).cuda()
+    ids = torch.zeros(4, 3, dtype=torch.long).cuda()
+    for call in (lambda: vocab.vocab_cross_entropy(h.double(), w.double(), y), lambda: vocab.vocab_cross_entropy(h, w.half(), y),
+                 lambda: vocab.vocab_cross_entropy(h[:, :7], w, y), lambda: vocab.vocab_cross_entropy(h, w[0], y),
+                 lambda: vocab.vocab_cross_entropy(h, w, y[:3]), lambda: vocab.vocab_cross_entropy(h, w, y.float()),
+                 lambda: vocab.vocab_cross_entropy(h, w, y, bias=w[:, 0][:9]), lambda: vocab.vocab_cross_entropy(h, w, y, bias=w[:, 0].half()),
+                 lambda: vocab.vocab_cross_entropy(h, w[:0], y), lambda: vocab.vocab_cross_entropy(h[:, :0], w[:, :0], y),
+                 lambda: vocab.vocab_distillation(h, w, ids, t[:, :2]), lambda: vocab.vocab_distillation(h, w, ids[:3], t[:3]),
+                 lambda: vocab.vocab_distillation(h, w, ids, t, temperature=0.0), lambda: vocab.vocab_distillation(h, w, ids, t, temperature=float("nan")),
+                 lambda: vocab.vocab_distillation(h, w, ids.float(), t), lambda: vocab.vocab_distillation(h, w, ids, ids),
+                 lambda: vocab.vocab_distillation(h, w, ids[:, :0], t[:, :0]),
+                 lambda: vocab.top_logits(h, 0), lambda: vocab.top_logits(h, 9), lambda: vocab.top_logits(h.long(), 1),
+                 lambda: vocab.top_logits(torch.zeros(2, 3000).cuda(), 1025)):
+        with pytest.raises(ValueError):
+            call()
