@@ -27,9 +27,11 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef short s16x8_t __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ void dma16(const unsigned short* src, unsigned short* lds) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                   (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+// 64 x 16 bytes from base + offset (the base and the destination alike for the wave) to LDS.  Inline assembly, because behind the
+// builtin the compiler waits for every transfer in flight before the next read of LDS, the current stage's fragments among them:
+// whoever reads the destination waits for vmcnt and passes a barrier first.
+__device__ __forceinline__ void dma16(const unsigned short* base, unsigned byte_offset, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(byte_offset), "s"(base) : "memory", "m0");
 }
 
 template <bool F16>
@@ -43,7 +45,7 @@ __device__ __forceinline__ f32x16_t mma(s16x8_t a, s16x8_t b, f32x16_t c) {
 struct Operand {
   const unsigned short* p;
   int64_t ld;       // elements between rows of the stored matrix
-  int64_t plane;    // elements between the hi and the lo plane (PL = 2)
+  int64_t plane;    // elements between the hi and the lo plane of a row (PL = 2)
   int64_t rows;     // stored rows that may be read; what lies past them is read as the last one again
   int64_t cols;     // stored columns that may be read (a multiple of 8), likewise
 };
@@ -65,57 +67,67 @@ struct Tile {
   // Accumulates contraction steps [k0, k0 + nk * BK) of the tile at (bm, bn).  Lane l ends with, for output row
   // bm + wr WM + 32 i + (l & 31), the columns bn + wc WN + 32 j + 8 (q >> 2) + 4 (l >> 5) + (q & 3), q < 16: the B operand is the
   // first of the matrix instruction, so a lane holds runs of 4 columns of one row.  Every wave of the workgroup calls it.
+  //
+  // Two-stage ring, fragments one sub-step (16 contraction steps) ahead in registers: in front of the last sub-step of a stage
+  // every fragment of the stage is in registers, so ONE barrier says both that the next stage has landed and that this one's
+  // buffer is free; the transfers of the stage after next start right there and have a whole stage of matrix work to land.
   static __device__ __forceinline__ void run(const Operand& A, const Operand& B, int64_t bm, int64_t bn, int64_t k0, int nk,
                                              unsigned short* smem, Acc& acc) {
+    if (nk <= 0) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave / WAVES_N, wc = wave % WAVES_N;
 
-    // ---- the DMA pieces of this wave: 8 image rows x 128 bytes each
-    const unsigned short* src[PPW];
-    int64_t step[PPW];
+    // ---- the DMA pieces of this wave: 8 image rows x 128 bytes each; byte offsets from the operand's first tile element
+    static_assert(BM / 8 % PPW == 0 || PPW % (BM / 8) == 0, "a wave's pieces belong to one operand");
+    const bool isA = wave * PPW < BM / 8;
+    const Operand& O = isA ? A : B;
+    const bool col = isA ? COLA : COLB;
+    const int64_t b0 = isA ? bm : bn, r0 = b0 < O.rows ? b0 : O.rows - 1;      // (a row operand's first row)
+    const unsigned short* base = O.p + (col ? k0 * O.ld : r0 * O.ld + k0);
+    const int64_t step = col ? BK * O.ld : BK;
+    const unsigned ld = (unsigned)O.ld;
+    unsigned off[PPW];
+    [[maybe_unused]] int krow[PPW];
 #pragma unroll
     for (int i = 0; i < PPW; ++i) {
-      const int p = wave * PPW + i;
-      const bool isA = p < BM / 8;
-      const bool col = isA ? COLA : COLB;
-      const Operand& O = isA ? A : B;
-      const int64_t b0 = isA ? bm : bn;
-      const int q = isA ? p : p - BM / 8;
-      const int slot = lane & 7;
+      const int q = wave * PPW + i - (isA ? 0 : BM / 8), slot = lane & 7;
       if (!col) {
-        const int row = q * 8 + (lane >> 3);
+        const int64_t last = O.rows - 1 - r0;
+        int row = q * 8 + (lane >> 3);
         const int c = slot ^ ((row >> 1) & 7);
-        const int64_t m = b0 + row < O.rows ? b0 + row : O.rows - 1;
-        src[i] = O.p + (PL == 2 ? (c >> 2) * O.plane : 0) + m * O.ld + k0 + (PL == 2 ? c & 3 : c) * 8;
-        step[i] = BK;
+        if (row > last) row = (int)last;
+        off[i] = ((unsigned)row * ld + (PL == 2 ? (c >> 2) * (unsigned)O.plane + (c & 3) * 8 : c * 8)) * 2;
+        krow[i] = 0;
       } else {
         const int panel = q >> 3, rr = (q & 7) * 8 + (lane >> 3);
         const int c = slot ^ (((rr >> 1) & 1) << 2);
         int64_t cc = b0 + panel * 64 + c * 8;
         if (cc > O.cols - 8) cc = O.cols - 8;
-        src[i] = O.p + (PL == 2 ? (rr >> 5) * O.plane : 0) + cc;      // + the contraction row's offset, see issue()
-        step[i] = k0 + (PL == 2 ? rr & 31 : rr);                      // that row at the first stage
+        krow[i] = PL == 2 ? rr & 31 : rr;
+        off[i] = ((unsigned)krow[i] * ld + (PL == 2 ? (rr >> 5) * (unsigned)O.plane : 0) + (unsigned)cc) * 2;
       }
     }
-    auto issue = [&](int kt) {
-      unsigned short* to = smem + (kt & 1) * STAGE;
-#pragma unroll
-      for (int i = 0; i < PPW; ++i) {
-        const int p = wave * PPW + i;
-        const bool isA = p < BM / 8;
-        if (!(isA ? COLA : COLB)) {
-          dma16(src[i] + kt * BK, to + p * 512);
-        } else {
-          const Operand& O = isA ? A : B;
-          int64_t r = step[i] + (int64_t)kt * BK;
-          if (r >= O.rows) r = O.rows - 1;
-          dma16(src[i] + r * O.ld, to + p * 512);
-        }
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned short*)smem + wave * PPW * 1024;
+    auto issue_piece = [&](int kt, int i, bool tail) {
+      const unsigned short* from = base + kt * step;
+      unsigned o = off[i];
+      if ((COLA || COLB) && tail) {           // contraction rows past the last stored one: that one again
+        const int64_t first = k0 + (int64_t)kt * BK, have = O.rows - 1 - first;
+        const int keep = have < 0 ? 0 : krow[i] < have ? krow[i] : (int)have;
+        if (have < 0) from = O.p + (O.rows - 1) * O.ld;
+        o -= (unsigned)(krow[i] - keep) * ld * 2;
       }
+      dma16(from, o, lds0 + (kt & 1) * (STAGE * 2) + i * 1024);
+    };
+    auto is_tail = [&](int kt) { return (COLA || COLB) && col && k0 + (int64_t)(kt + 1) * BK > O.rows; };
+    auto issue = [&](int kt) {
+      const bool tail = is_tail(kt);
+#pragma unroll
+      for (int i = 0; i < PPW; ++i) issue_piece(kt, i, tail);
     };
 
-    // ---- fragment addresses (u16 inside a section)
+    // ---- fragments
     const int l31 = lane & 31, half = lane >> 5, j = lane & 15, g = lane >> 4;
     auto frag = [&](auto colc, const unsigned short* sec, int w0, int ks, int lo) -> s16x8_t {
       if constexpr (!decltype(colc)::value) {
@@ -132,37 +144,58 @@ struct Tile {
     };
     using CA = std::integral_constant<bool, COLA>;
     using CB = std::integral_constant<bool, COLB>;
-
-    if (nk <= 0) return;
-    issue(0);
-    for (int kt = 0; kt < nk; ++kt) {
-      // this wave's pieces of stage kt have landed and its reads of the other buffer are in registers
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();          // stage kt visible to every wave; the other buffer is free
-      asm volatile("" ::: "memory");
-      if (kt + 1 < nk) issue(kt + 1);
+    constexpr int KS = BK / 16;
+    s16x8_t a[2][PL][TM], b[2][PL][TN];
+    auto read = [&](int set, int kt, int ks) {
       const unsigned short* sa = smem + (kt & 1) * STAGE;
       const unsigned short* sb = sa + BM * 64;
 #pragma unroll
-      for (int ks = 0; ks < BK / 16; ++ks) {
-        s16x8_t a[PL][TM], b[PL][TN];
+      for (int pl = 0; pl < PL; ++pl) {
 #pragma unroll
-        for (int pl = 0; pl < PL; ++pl) {
+        for (int n = 0; n < TN; ++n) b[set][pl][n] = frag(CB{}, sb, wc * WN + n * 32, ks, pl);
 #pragma unroll
-          for (int i = 0; i < TM; ++i) a[pl][i] = frag(CA{}, sa, wr * WM + i * 32, ks, pl);
+        for (int i = 0; i < TM; ++i) a[set][pl][i] = frag(CA{}, sa, wr * WM + i * 32, ks, pl);
+      }
+    };
+    auto barrier = [&] {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
+
+    issue(0);
+    barrier();
+    if (nk > 1) issue(1);
+    read(0, 0, 0);
+    for (int kt = 0; kt < nk; ++kt) {
 #pragma unroll
-          for (int n = 0; n < TN; ++n) b[pl][n] = frag(CB{}, sb, wc * WN + n * 32, ks, pl);
+      for (int ks = 0; ks < KS; ++ks) {
+        const int set = ks & 1;
+        bool next = false, tail = false;
+        if (ks + 1 < KS) {
+          read(set ^ 1, kt, ks + 1);
+        } else if (kt + 1 < nk) {
+          barrier();
+          read(set ^ 1, kt + 1, 0);
+          next = kt + 2 < nk;
+          tail = next && is_tail(kt + 2);
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
           for (int n = 0; n < TN; ++n) {
             if constexpr (PL == 2) {
-              acc[i][n] = mma<F16>(b[1][n], a[0][i], acc[i][n]);
-              acc[i][n] = mma<F16>(b[0][n], a[1][i], acc[i][n]);
+              acc[i][n] = mma<F16>(b[set][1][n], a[set][0][i], acc[i][n]);
+              acc[i][n] = mma<F16>(b[set][0][n], a[set][1][i], acc[i][n]);
             }
-            acc[i][n] = mma<F16>(b[0][n], a[0][i], acc[i][n]);
+            acc[i][n] = mma<F16>(b[set][0][n], a[set][0][i], acc[i][n]);
           }
+        if (next) {
+#pragma unroll
+          for (int q = 0; q < PPW; ++q) issue_piece(kt + 2, q, tail);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }

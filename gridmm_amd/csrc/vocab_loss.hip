@@ -241,7 +241,7 @@ __device__ __forceinline__ void pack_row(const void* src, int64_t off, int dtype
 }
 
 // counted rows of h -> Hp (rows past the count up to a multiple of 256: zero)
-__global__ __launch_bounds__(256) void pack_h_kernel(const void* __restrict__ hidden, int64_t ldh, int dtype, int K, int Kp, int Rp,
+__global__ __launch_bounds__(256) void pack_h_kernel(const void* __restrict__ hidden, int64_t ldh, int dtype, int K, int Kp,
                                                      const int* __restrict__ rowmap, const float* __restrict__ amax_h,
                                                      const float* __restrict__ amax_w, Meta* __restrict__ meta,
                                                      unsigned short* __restrict__ Hp) {
@@ -260,8 +260,8 @@ __global__ __launch_bounds__(256) void pack_h_kernel(const void* __restrict__ hi
   }
   if (i >= (count + 255) / 256 * 256) return;
   const bool zero = i >= count;
-  unsigned short* hi = Hp + (int64_t)i * Kp;
-  pack_row(hidden, zero ? 0 : (int64_t)rowmap[i] * ldh, dtype, K, Kp, lane, sh, zero, hi, hi + (int64_t)Rp * Kp);
+  unsigned short* hi = Hp + (int64_t)i * Kp * (dtype == F32 ? 2 : 1);
+  pack_row(hidden, zero ? 0 : (int64_t)rowmap[i] * ldh, dtype, K, Kp, lane, sh, zero, hi, hi + Kp);
 }
 
 // rows [j0, j0 + C) of W -> Wp (zero past the vocabulary)
@@ -272,8 +272,8 @@ __global__ __launch_bounds__(256) void pack_w_kernel(const void* __restrict__ W,
   const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= C) return;
   const bool zero = j0 + i >= vocab;
-  unsigned short* hi = Wp + (int64_t)i * Kp;
-  pack_row(W, zero ? 0 : (j0 + i) * ldw, dtype, K, Kp, lane, meta->sw, zero, hi, hi + (int64_t)C * Kp);
+  unsigned short* hi = Wp + (int64_t)i * Kp * (dtype == F32 ? 2 : 1);
+  pack_row(W, zero ? 0 : (j0 + i) * ldw, dtype, K, Kp, lane, meta->sw, zero, hi, hi + Kp);
 }
 
 // ---- forward: per-row (maximum, sum of exponentials) of each tile's columns ----
@@ -783,7 +783,7 @@ int weight_piece(const gridmm_vocab_loss_t* d, const Plan& P, int64_t j0, int64_
     GRIDMM_LAUNCH(pack_w_kernel, dim3((unsigned)((C + 3) / 4)), dim3(256), 0, st, d->weight, d->ld_weight, d->dtype, d->hidden_size,
                   (int)P.Kp, j0, (int)C, d->vocab, meta, buf);
     GRIDMM_CHECK_LAUNCH();
-    W = Operand{buf, P.Kp, C * P.Kp, C, P.Kp};
+    W = Operand{buf, P.PL * P.Kp, P.Kp, C, P.Kp};
   } else {
     W = Operand{(const unsigned short*)d->weight + j0 * d->ld_weight, d->ld_weight, 0, d->vocab - j0, P.Kp};
   }
@@ -846,10 +846,10 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   GRIDMM_LAUNCH(prep_kernel, dim3(1 + nb + (d->dtype == F32 ? AMAX_H + AMAX_W : 0)), dim3(PREP_T), 0, st, a, nb);
   GRIDMM_CHECK_LAUNCH();
   GRIDMM_LAUNCH(pack_h_kernel, dim3((unsigned)(P.Rp / 4)), dim3(256), 0, st, d->hidden, d->ld_hidden, d->dtype, d->hidden_size,
-                (int)P.Kp, (int)P.Rp, rowmap, amax, amax + AMAX_H, meta, Hp);
+                (int)P.Kp, rowmap, amax, amax + AMAX_H, meta, Hp);
   GRIDMM_CHECK_LAUNCH();
 
-  const Operand H{Hp, P.Kp, P.Rp * P.Kp, P.Rp, P.Kp};
+  const Operand H{Hp, P.PL * P.Kp, P.Kp, P.Rp, P.Kp};
   const int BT = P.big ? 256 : 128;
   for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_fwd) {
     const int64_t C = std::min(P.C_fwd, P.Vp - j0);
@@ -912,14 +912,14 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
 
   GRIDMM_LAUNCH(grad_scale_kernel, dim3(1), dim3(PREP_T), 0, st, grad, grad_stride, d->temperature, rowmap, meta, scale, grow, (int)P.Rp);
   GRIDMM_CHECK_LAUNCH();
-  const Operand H{Hp, P.Kp, P.Rp * P.Kp, P.Rp, P.Kp};
+  const Operand H{Hp, P.PL * P.Kp, P.Kp, P.Rp, P.Kp};
   for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_bwd) {
     const int64_t C = std::min(P.C_bwd, P.Vp - j0);
     Operand W;
     int rc = weight_piece(d, P, j0, C, meta, wbuf, st, W);
     if (rc != GRIDMM_OK) return rc;
-    const int64_t plane = P.Rp * C;
-    const Operand S{dS, C, plane, P.Rp, C};
+    const int64_t ldS = P.PL * C;
+    const Operand S{dS, ldS, C, P.Rp, C};
     rc = by_type(d, P.big, [&](auto f16, auto pl, auto big) {
       constexpr bool F = decltype(f16)::value, BIG = decltype(big)::value;
       constexpr int L = decltype(pl)::value;
@@ -927,11 +927,11 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
         using T = TileOf<F, L, BIG, false, false>;
         const int64_t tn = C / T::BN, tm = (d->rows + T::BM - 1) / T::BM;
         GRIDMM_LAUNCH((score_grad_kernel<T>), dim3((unsigned)(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), tn, meta,
-                      biasz + j0, unit, lse, grow, dS, C, plane);
+                      biasz + j0, unit, lse, grow, dS, ldS, C);
         GRIDMM_CHECK_LAUNCH();
       }
       FixArgs f;
-      f.index = d->slots ? d->ids : d->labels; f.ld_index = d->slots ? d->ld_ids : 1; f.j0 = j0; f.ldS = C; f.plane = plane;
+      f.index = d->slots ? d->ids : d->labels; f.ld_index = d->slots ? d->ld_ids : 1; f.j0 = j0; f.ldS = ldS; f.plane = C;
       f.wide = d->index64; f.slots = P.slots; f.C = (int)C; f.vocab = d->vocab; f.dtype = d->dtype; f.meta = meta; f.rowmap = rowmap;
       f.p = p; f.zt = zt; f.lse = lse; f.grow = grow; f.dS = dS;
       GRIDMM_LAUNCH(target_grad_kernel, dim3((unsigned)(((int64_t)d->rows * P.slots + 255) / 256)), dim3(256), 0, st, f);
@@ -951,7 +951,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
         GRIDMM_CHECK_LAUNCH();
       }
       if (d_bias) {
-        GRIDMM_LAUNCH(bias_grad_kernel, dim3((unsigned)(C / 256)), dim3(256), 0, st, dS, C, plane, d->dtype, meta, scale, j0,
+        GRIDMM_LAUNCH(bias_grad_kernel, dim3((unsigned)(C / 256)), dim3(256), 0, st, dS, ldS, C, d->dtype, meta, scale, j0,
                       d->vocab, d->bias_dtype, d_bias);
         GRIDMM_CHECK_LAUNCH();
       }
