@@ -42,6 +42,26 @@ __device__ __forceinline__ f32x16_t mma(s16x8_t a, s16x8_t b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
+// sum of 8 16-bit values + c
+template <bool F16>
+__device__ __forceinline__ float sum8(s16x8_t v, float c) {
+  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+  typedef short s16x2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const s16x2_t x = {v[2 * e], v[2 * e + 1]};
+    if constexpr (F16) {
+      const f16x2_t one = {(_Float16)1.f, (_Float16)1.f};
+      c = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, x), one, c, false);
+    } else {
+      const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
+      c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x), one, c, false);
+    }
+  }
+  return c;
+}
+
 struct Operand {
   const unsigned short* p;
   int64_t ld;       // elements between rows of the stored matrix
@@ -71,8 +91,12 @@ struct Tile {
   // Two-stage ring, fragments one sub-step (16 contraction steps) ahead in registers: in front of the last sub-step of a stage
   // every fragment of the stage is in registers, so ONE barrier says both that the next stage has landed and that this one's
   // buffer is free; the transfers of the stage after next start right there and have a whole stage of matrix work to land.
+  //
+  // SUMA and sum (alike for the wave): asum (TM values) also takes the sums of A over the contraction, lane l those of the steps
+  // that it holds of row 32 i + (l & 31); lanes l and l ^ 32 together hold all.
+  template <bool SUMA = false>
   static __device__ __forceinline__ void run(const Operand& A, const Operand& B, int64_t bm, int64_t bn, int64_t k0, int nk,
-                                             unsigned short* smem, Acc& acc) {
+                                             unsigned short* smem, Acc& acc, float* asum = nullptr, bool sum = false) {
     if (nk <= 0) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -145,17 +169,21 @@ struct Tile {
     using CA = std::integral_constant<bool, COLA>;
     using CB = std::integral_constant<bool, COLB>;
     constexpr int KS = BK / 16;
-    s16x8_t a[2][PL][TM], b[2][PL][TN];
-    auto read = [&](int set, int kt, int ks) {
+    s16x8_t a[2][TM], b[2][TN];                                 // (hi) planes, two sub-steps
+    [[maybe_unused]] s16x8_t al[TM], bl[TN];                    // lo planes of the current one
+    auto read = [&](s16x8_t (&fa)[TM], s16x8_t (&fb)[TN], int kt, int ks, int lo) {
       const unsigned short* sa = smem + (kt & 1) * STAGE;
       const unsigned short* sb = sa + BM * 64;
 #pragma unroll
-      for (int pl = 0; pl < PL; ++pl) {
+      for (int n = 0; n < TN; ++n) fb[n] = frag(CB{}, sb, wc * WN + n * 32, ks, lo);
 #pragma unroll
-        for (int n = 0; n < TN; ++n) b[set][pl][n] = frag(CB{}, sb, wc * WN + n * 32, ks, pl);
+      for (int i = 0; i < TM; ++i) fa[i] = frag(CA{}, sa, wr * WM + i * 32, ks, lo);
+    };
+    auto product = [&](const s16x8_t (&fa)[TM], const s16x8_t (&fb)[TN]) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) a[set][pl][i] = frag(CA{}, sa, wr * WM + i * 32, ks, pl);
-      }
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int n = 0; n < TN; ++n) acc[i][n] = mma<F16>(fb[n], fa[i], acc[i][n]);
     };
     auto barrier = [&] {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -166,31 +194,34 @@ struct Tile {
     issue(0);
     barrier();
     if (nk > 1) issue(1);
-    read(0, 0, 0);
+    read(a[0], b[0], 0, 0, 0);
     for (int kt = 0; kt < nk; ++kt) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         const int set = ks & 1;
         bool next = false, tail = false;
+        if constexpr (PL == 2) read(al, bl, kt, ks, 1);
         if (ks + 1 < KS) {
-          read(set ^ 1, kt, ks + 1);
+          read(a[set ^ 1], b[set ^ 1], kt, ks + 1, 0);
         } else if (kt + 1 < nk) {
           barrier();
-          read(set ^ 1, kt + 1, 0);
+          read(a[set ^ 1], b[set ^ 1], kt + 1, 0, 0);
           next = kt + 2 < nk;
           tail = next && is_tail(kt + 2);
         }
         __builtin_amdgcn_sched_barrier(0);
+        product(a[set], b[set]);
+        if constexpr (PL == 2) {
+          product(a[set], bl);
+          product(al, b[set]);
+        }
+        if (SUMA && sum) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int n = 0; n < TN; ++n) {
-            if constexpr (PL == 2) {
-              acc[i][n] = mma<F16>(b[set][1][n], a[set][0][i], acc[i][n]);
-              acc[i][n] = mma<F16>(b[set][0][n], a[set][1][i], acc[i][n]);
-            }
-            acc[i][n] = mma<F16>(b[set][0][n], a[set][0][i], acc[i][n]);
+          for (int i = 0; i < TM; ++i) {
+            asum[i] = sum8<F16>(a[set][i], asum[i]);
+            if constexpr (PL == 2) asum[i] = sum8<F16>(al[i], asum[i]);
           }
+        }
         if (next) {
 #pragma unroll
           for (int q = 0; q < PPW; ++q) issue_piece(kt + 2, q, tail);

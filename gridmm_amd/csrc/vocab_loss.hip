@@ -33,6 +33,7 @@ using vocab::tile_of;
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 constexpr int AMAX_H = 64, AMAX_W = 512;      // workgroups of the largest-value search (fp32 operands)
 constexpr int PREP_T = 1024;
+constexpr int64_t PIECE_MB = 512;
 enum { F32 = 0, BF16 = 1, F16 = 2 };
 
 __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype) {
@@ -67,6 +68,19 @@ struct Meta {
   int count;         // rows that count
   int sh, sw;        // power-of-two exponents of the packed h and W
 };
+
+// Tiles of the products over the counted rows.  256 x 256 where they fill the chip (one workgroup of 8 waves a CU), else 128 x 128 (two
+// of 4 waves a CU).  The host does not know the count: where both may be right it launches both, each sized for its own range, and the
+// workgroups of the one whose turn it is not end at once.
+constexpr int BIG_TILES = 384;       // 1.5 rounds of 256 CUs
+__host__ __device__ inline bool big_tiles(int64_t count, int64_t C) { return count > 128 && (count + 255) / 256 * (C / 256) >= BIG_TILES; }
+// contraction ranges of dh: enough workgroups for two rounds of the chip, at least 8 stages of 64 columns a range
+__host__ __device__ inline int hidden_splits(int64_t count, int64_t Kp, int64_t C, bool big) {
+  const int64_t T = big ? 256 : 128, tiles = ((count + T - 1) / T) * ((Kp + T - 1) / T);
+  int64_t s = (big ? 256 : 512) / (tiles > 0 ? tiles : 1);
+  if (s > C / 512) s = C / 512;
+  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
 
 // ---- targets of the distillation: p = softmax(t / T) over the filled slots, the row's sum of p log p, whether it counts ----
 __global__ __launch_bounds__(256) void kd_targets_kernel(const void* __restrict__ ids, int wide, int64_t ld_ids,
@@ -285,7 +299,7 @@ __global__ __launch_bounds__(T::THREADS) void score_stats_kernel(Operand A, Oper
   __shared__ float2 wst[T::WAVES_N][T::BM];
   const int count = meta->count;
   int64_t ty, tx;
-  if (!tile_of(blockIdx.x, (count + T::BM - 1) / T::BM, tn, ty, tx)) return;
+  if (big_tiles(count, tn * T::BN) != (T::BM == 256) || !tile_of(blockIdx.x, (count + T::BM - 1) / T::BM, tn, ty, tx)) return;
   typename T::Acc acc = {};
   T::run(A, B, ty * T::BM, tx * T::BN, 0, nk, smem, acc);
 
@@ -330,11 +344,11 @@ __global__ __launch_bounds__(T::THREADS) void score_stats_kernel(Operand A, Oper
       const float M = fmaxf(a.x, b.x), ref = M == -INFINITY ? 0.f : M;
       a = make_float2(M, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
     }
-    stats[tx * Rp + ty * T::BM + r] = a;
+    stats[tx * (T::BN / 128) * Rp + ty * T::BM + r] = a;
   }
 }
 
-// ---- scores at the targets: one wave a (row, up to 8 slots), fp32 sums over the operands as they came ----
+// ---- scores at the targets: one wave a (row, NS slots), fp32 sums over the operands as they came ----
 struct TargetArgs {
   const void *hidden, *weight, *index;
   int64_t ldh, ldw, ld_index;
@@ -345,55 +359,73 @@ struct TargetArgs {
   const float* biasz;
   float* zt;       // [compacted row][slots], base 2
 };
-template <int DT>
-__device__ __forceinline__ float dot_rows(const void* a, int64_t ao, const void* b, int64_t bo, int K, int lane, bool vec) {
-  float s = 0.f;
-  if constexpr (DT == F32) {
-    const float *x = (const float*)a + ao, *y = (const float*)b + bo;
-    if (vec) {
-      for (int k = lane * 4; k < K; k += 256) {
-        const float4 p = *reinterpret_cast<const float4*>(x + k), q = *reinterpret_cast<const float4*>(y + k);
-        s = fmaf(p.x, q.x, s); s = fmaf(p.y, q.y, s); s = fmaf(p.z, q.z, s); s = fmaf(p.w, q.w, s);
-      }
-      return s;
-    }
-  } else if (vec) {
-    const unsigned short *x = (const unsigned short*)a + ao, *y = (const unsigned short*)b + bo;
-    for (int k = lane * 8; k < K; k += 512) {
-      const u16x8_t p = *reinterpret_cast<const u16x8_t*>(x + k), q = *reinterpret_cast<const u16x8_t*>(y + k);
+// NS dot products of one row of h with rows of W, their loads in flight together
+template <int DT, int NS>
+__device__ __forceinline__ void dots(const TargetArgs& a, int64_t r, const int64_t (&id)[NS], int lane, bool vec, float (&out)[NS]) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (DT == BF16) s = fmaf(bf16_bits_to_f32(p[e]), bf16_bits_to_f32(q[e]), s);
-        else s = fmaf((float)__builtin_bit_cast(_Float16, (unsigned short)p[e]), (float)__builtin_bit_cast(_Float16, (unsigned short)q[e]), s);
-      }
+  for (int s = 0; s < NS; ++s) out[s] = 0.f;
+  if (!vec) {
+    for (int k = lane; k < a.K; k += 64) {
+      const float x = load_as_f32(a.hidden, r * a.ldh + k, DT);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) out[s] = fmaf(x, load_as_f32(a.weight, id[s] * a.ldw + k, DT), out[s]);
     }
-    return s;
+  } else if constexpr (DT == F32) {
+    const float *x = (const float*)a.hidden + r * a.ldh, *W = (const float*)a.weight;
+    for (int k = lane * 4; k < a.K; k += 256) {
+      const float4 p = *reinterpret_cast<const float4*>(x + k);
+      float4 q[NS];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) q[s] = *reinterpret_cast<const float4*>(W + id[s] * a.ldw + k);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) out[s] = fmaf(p.x, q[s].x, fmaf(p.y, q[s].y, fmaf(p.z, q[s].z, fmaf(p.w, q[s].w, out[s]))));
+    }
+  } else {
+    const unsigned short *x = (const unsigned short*)a.hidden + r * a.ldh, *W = (const unsigned short*)a.weight;
+    auto f = [](unsigned short u) { return DT == BF16 ? bf16_bits_to_f32(u) : (float)__builtin_bit_cast(_Float16, u); };
+    for (int k = lane * 8; k < a.K; k += 512) {
+      const u16x8_t p = *reinterpret_cast<const u16x8_t*>(x + k);
+      u16x8_t q[NS];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) q[s] = *reinterpret_cast<const u16x8_t*>(W + id[s] * a.ldw + k);
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[s] = fmaf(f(p[e]), f(q[s][e]), out[s]);
+    }
   }
-  for (int k = lane; k < K; k += 64) s = fmaf(load_as_f32(a, ao + k, DT), load_as_f32(b, bo + k, DT), s);
-  return s;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) out[s] = wave_sum(out[s]);
 }
-template <int DT>
+template <int DT, int NS>
 __global__ __launch_bounds__(256) void target_scores_kernel(const TargetArgs a) {
   const int lane = threadIdx.x & 63;
-  const int groups = (a.slots + 7) / 8;
+  const int groups = (a.slots + NS - 1) / NS;
   const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int64_t i = w / groups;
   if (i >= a.meta->count) return;
-  const int s0 = (int)(w % groups) * 8, s1 = min(a.slots, s0 + 8);
+  const int s0 = (int)(w % groups) * NS;
   const int64_t r = a.rowmap[i];
   constexpr int A = DT == F32 ? 4 : 8;
   const bool vec = a.K % A == 0 && a.ldh % A == 0 && a.ldw % A == 0 && (((uintptr_t)a.hidden | (uintptr_t)a.weight) & 15) == 0;
-  for (int s = s0; s < s1; ++s) {
-    const int64_t id = load_index(a.index, r * a.ld_index + s, a.wide);
-    float z = NAN;                                          // an id outside the vocabulary spoils its row
-    if (a.kd && id < 0) z = 0.f;                            // an empty slot
-    else if (id >= 0 && id < a.vocab) z = fmaf(wave_sum(dot_rows<DT>(a.hidden, r * a.ldh, a.weight, id * a.ldw, a.K, lane, vec)), a.unit, a.biasz[id]);
-    if (lane == 0) a.zt[i * a.slots + s] = z;
+  int64_t id[NS], at[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    id[s] = s0 + s < a.slots ? load_index(a.index, r * a.ld_index + s0 + s, a.wide) : -1;
+    at[s] = id[s] >= 0 && id[s] < a.vocab ? id[s] : 0;      // (row 0 in place of a row that is not there)
+  }
+  float z[NS];
+  dots<DT, NS>(a, r, at, lane, vec, z);
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    if (lane != s || s0 + s >= a.slots) continue;
+    // an id outside the vocabulary spoils its row; an empty slot has no score
+    a.zt[i * a.slots + s0 + s] = a.kd && id[s] < 0 ? 0.f : id[s] < 0 || id[s] >= a.vocab ? NAN : fmaf(z[s], a.unit, a.biasz[at[s]]);
   }
 }
 
 // ---- joins the tiles' statistics and writes the losses: 16 rows a workgroup, 16 threads a row ----
-__global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ stats, int64_t tiles, int64_t Rp, const Meta* __restrict__ meta,
+__global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ stats, int64_t Vp, int64_t C, int64_t Rp, const Meta* __restrict__ meta,
                                                    const int* __restrict__ rowmap, const float* __restrict__ zt, int slots,
                                                    const float* __restrict__ p, const float* __restrict__ plogp, float temperature,
                                                    float* __restrict__ lse, float* __restrict__ loss) {
@@ -401,6 +433,9 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
   __shared__ float acc[16][17];
   const int rr = threadIdx.x & 15, lanep = threadIdx.x >> 4;
   const int count = meta->count;
+  const int64_t T = big_tiles(count, C) ? 256 : 128;
+  // statistics of the tile at column j lie at j / 128 (a last piece may have taken the other tile)
+  const int64_t last = Vp % C ? (big_tiles(count, Vp % C) ? 256 : 128) : T, whole = Vp / C * C;
   const int64_t i = (int64_t)blockIdx.x * 16 + rr;
   if ((int64_t)blockIdx.x * 16 >= count) return;
   float2 a = make_float2(-INFINITY, 0.f);
@@ -409,7 +444,10 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
     return make_float2(M, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
   };
   if (i < count)
-    for (int64_t t = lanep; t < tiles; t += 16) a = join(a, stats[t * Rp + i]);
+  {
+    for (int64_t j = lanep * T; j < whole; j += 16 * T) a = join(a, stats[j / 128 * Rp + i]);
+    for (int64_t j = whole + lanep * last; j < Vp; j += 16 * last) a = join(a, stats[j / 128 * Rp + i]);
+  }
   part[lanep][rr] = a;
   __syncthreads();
   a = part[0][rr];
@@ -471,7 +509,7 @@ __global__ __launch_bounds__(T::THREADS) void score_grad_kernel(Operand A, Opera
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
   const int count = meta->count;
   int64_t ty, tx;
-  if (!tile_of(blockIdx.x, (count + T::BM - 1) / T::BM, tn, ty, tx)) return;
+  if (big_tiles(count, tn * T::BN) != (T::BM == 256) || !tile_of(blockIdx.x, (count + T::BM - 1) / T::BM, tn, ty, tx)) return;
   typename T::Acc acc = {};
   T::run(A, B, ty * T::BM, tx * T::BN, 0, nk, smem, acc);
 
@@ -517,20 +555,7 @@ struct FixArgs {
   const float *p, *zt, *lse, *grow;
   unsigned short* dS;
 };
-__global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
-  const int64_t w = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t i = w / a.slots;
-  const int s = (int)(w % a.slots);
-  if (i >= a.meta->count) return;
-  const int64_t r = a.rowmap[i];
-  const int64_t id = load_index(a.index, r * a.ld_index + s, a.wide);
-  if (id < a.j0 || id >= a.j0 + a.C || id >= a.vocab || id < 0) return;
-  float p = 1.f;
-  if (a.p) {                                       // several slots may name one id: each of them writes the same value
-    p = 0.f;
-    for (int k = 0; k < a.slots; ++k)
-      if (load_index(a.index, r * a.ld_index + k, a.wide) == id) p += a.p[r * a.slots + k];
-  }
+__device__ __forceinline__ void target_entry(const FixArgs& a, int64_t i, int s, int64_t id, float p) {
   const float v = a.grow[i] * (__builtin_amdgcn_exp2f(a.zt[i * a.slots + s] - a.lse[i]) - p);
   unsigned short* at = a.dS + i * a.ldS + (id - a.j0);
   if (a.dtype == F32) {
@@ -541,20 +566,57 @@ __global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
     at[0] = a.dtype == F16 ? to_f16(v) : to_bf16(v);
   }
 }
+__global__ __launch_bounds__(256) void label_grad_kernel(const FixArgs a) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.meta->count) return;
+  const int64_t id = load_index(a.index, a.rowmap[i], a.wide);
+  if (id >= a.j0 && id < a.j0 + a.C && id < a.vocab && id >= 0) target_entry(a, i, 0, id, 1.f);
+}
+// one row a workgroup, 256 of its slots in LDS at a time; several slots may name one id: each of them writes the same value
+__global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
+  __shared__ int sid[256];
+  __shared__ float sp[256];
+  const int64_t i = blockIdx.x;
+  if (i >= a.meta->count) return;
+  const int64_t r = a.rowmap[i];
+  for (int s0 = 0; s0 < a.slots; s0 += 256) {
+    const int s = s0 + threadIdx.x;
+    const int64_t id = s < a.slots ? load_index(a.index, r * a.ld_index + s, a.wide) : -1;
+    const bool mine = id >= a.j0 && id < a.j0 + a.C && id < a.vocab && id >= 0;
+    float p = 0.f;
+    for (int t0 = 0; t0 < a.slots; t0 += 256) {
+      __syncthreads();
+      const int t = t0 + threadIdx.x;
+      if (t < a.slots) {
+        const int64_t o = load_index(a.index, r * a.ld_index + t, a.wide);
+        sid[threadIdx.x] = o < 0 || o >= a.vocab ? -1 : (int)o;
+        sp[threadIdx.x] = a.p[r * a.slots + t];
+      }
+      __syncthreads();
+      if (mine)
+        for (int k = 0; k < min(256, a.slots - t0); ++k) p += sid[k] == (int)id ? sp[k] : 0.f;
+    }
+    if (mine) target_entry(a, i, s, id, p);
+  }
+}
 
-// dh of this piece: partial products over the contraction ranges blockIdx.y, added to those of the pieces before
+// dh of this piece: partial products over the contraction ranges blockIdx.y, added to those of the pieces before.  `C`: the columns of
+// a whole piece, which fix the tile and the number of ranges for all pieces.
 template <class T>
-__global__ __launch_bounds__(T::THREADS) void hidden_grad_kernel(Operand A, Operand B, int steps, int64_t tn, const Meta* __restrict__ meta,
-                                                                 float* __restrict__ part, int64_t Rp, int64_t Kp, int first) {
+__global__ __launch_bounds__(T::THREADS) void hidden_grad_kernel(Operand A, Operand B, int steps, int64_t tn, int64_t C,
+                                                                 const Meta* __restrict__ meta, float* __restrict__ part, int64_t Kp,
+                                                                 int first) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
   const int count = meta->count;
+  const bool big = big_tiles(count, C);
+  const int splits = hidden_splits(count, Kp, C, big);
   int64_t ty, tx;
-  if (!tile_of(blockIdx.x, (count + T::BM - 1) / T::BM, tn, ty, tx)) return;
-  const int per = (steps + gridDim.y - 1) / gridDim.y, s0 = blockIdx.y * per, nk = min(per, steps - s0);
+  if (big != (T::BM == 256) || (int)blockIdx.y >= splits || !tile_of(blockIdx.x, (count + T::BM - 1) / T::BM, tn, ty, tx)) return;
+  const int per = (steps + splits - 1) / splits, s0 = blockIdx.y * per, nk = min(per, steps - s0);
   typename T::Acc acc = {};
   T::run(A, B, ty * T::BM, tx * T::BN, (int64_t)s0 * T::BK, nk, smem, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
-  float* out = part + (int64_t)blockIdx.y * Rp * Kp;
+  float* out = part + (int64_t)blockIdx.y * count * Kp;
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) {
     const int64_t r = ty * T::BM + wr * T::WM + i * 32 + (lane & 31);
@@ -577,40 +639,61 @@ __device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v)
   else reinterpret_cast<unsigned short*>(p)[i] = dtype == BF16 ? to_bf16(v) : to_f16(v);
 }
 
-// dh = the ranges' partial products in order, unscaled, to the rows they came from; zero for rows that do not count
-__global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict__ part, int splits, int64_t Rp, int64_t Kp, int K,
-                                                         int rows, const int* __restrict__ rowinv, const Meta* __restrict__ meta,
+// dh = the ranges' partial products in order, unscaled, to the rows they came from; zero for rows that do not count.  A workgroup
+// takes 64 runs of 4 columns of one row, 4 threads a run, each every fourth range.
+__global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict__ part, int64_t C, int64_t Kp, int K, int rows,
+                                                         const int* __restrict__ rowinv, const Meta* __restrict__ meta,
                                                          const int* __restrict__ scale, int dtype, void* __restrict__ out) {
-  const int lane = threadIdx.x & 63;
-  const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
-  const int pos = rowinv[r], e = -(*scale + meta->sw);
-  for (int k = lane * 4; k < K; k += 256) {
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (pos >= 0) {
-      for (int s = 0; s < splits; ++s) {
-        const float4 a = *reinterpret_cast<const float4*>(part + (s * Rp + pos) * Kp + k);
-        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
-      }
-      v.x = ldexpf(v.x, e); v.y = ldexpf(v.y, e); v.z = ldexpf(v.z, e); v.w = ldexpf(v.w, e);
+  __shared__ float4 sums[3][64];
+  const int t = threadIdx.x & 63, sp = threadIdx.x >> 6;
+  const int64_t r = blockIdx.x;
+  const int k = blockIdx.y * 256 + t * 4;
+  const int count = meta->count, pos = rowinv[r], e = -(*scale + meta->sw);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (pos >= 0 && k < Kp) {
+    const int splits = hidden_splits(count, Kp, C, big_tiles(count, C));
+    const float* at = part + (int64_t)pos * Kp + k;
+#pragma unroll 4
+    for (int s = sp; s < splits; s += 4) {
+      const float4 a = *reinterpret_cast<const float4*>(at + (int64_t)s * count * Kp);
+      v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
     }
-    const float f[4] = {v.x, v.y, v.z, v.w};
-    for (int x = 0; x < 4; ++x)
-      if (k + x < K) store_as(out, r * K + k + x, dtype, f[x]);
   }
+  if (sp) sums[sp - 1][t] = v;
+  __syncthreads();
+  if (sp || k >= K) return;
+#pragma unroll
+  for (int s = 0; s < 3; ++s) { const float4 a = sums[s][t]; v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w; }
+  const float f[4] = {ldexpf(v.x, e), ldexpf(v.y, e), ldexpf(v.z, e), ldexpf(v.w, e)};
+  for (int x = 0; x < 4; ++x)
+    if (k + x < K) store_as(out, r * K + k + x, dtype, f[x]);
 }
 
-// dW of this piece: rows [j0, j0 + C) complete (the contraction is all counted rows), written once in the weight's type
+// dW of this piece: rows [j0, j0 + C) complete (the contraction is all counted rows), written once in the weight's type; the first
+// tile column also sums dS over the rows: db
 template <class T>
 __global__ __launch_bounds__(T::THREADS) void weight_grad_kernel(Operand A, Operand B, int64_t tm, int64_t tn, const Meta* __restrict__ meta,
-                                                                 const int* __restrict__ scale, int dtype, int64_t j0, int vocab, int K, void* __restrict__ dW) {
+                                                                 const int* __restrict__ scale, int dtype, int64_t j0, int vocab, int K, void* __restrict__ dW,
+                                                                 int bias_dtype, void* __restrict__ db) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
   int64_t ty, tx;
   if (!tile_of(blockIdx.x, tm, tn, ty, tx)) return;
   const int count = meta->count;
   typename T::Acc acc = {};
-  T::run(A, B, ty * T::BM, tx * T::BN, 0, (count + T::BK - 1) / T::BK, smem, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
+  const int nk = (count + T::BK - 1) / T::BK;
+  float sums[T::TM] = {};
+  const bool sum = db && tx == 0 && wc == 0;
+  T::template run<true>(A, B, ty * T::BM, tx * T::BN, 0, nk, smem, acc, sums, sum);
+  if (sum) {
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) {
+      const float s = sums[i] + __shfl_xor(sums[i], 32, 64);
+      const int64_t j = j0 + ty * T::BM + wr * T::WM + i * 32 + (lane & 31);
+      if (lane < 32 && j < vocab) store_as(db, j, bias_dtype, ldexpf(s, -*scale));
+    }
+  }
+  if (!dW) return;
   const int e = -(*scale + meta->sh);
 #pragma unroll
   for (int i = 0; i < T::TM; ++i) {
@@ -643,39 +726,6 @@ __global__ __launch_bounds__(T::THREADS) void weight_grad_kernel(Operand A, Oper
   }
 }
 
-// db of this piece: column sums of dS, 256 columns a workgroup, 8 rows at a time, joined in order
-__global__ __launch_bounds__(256) void bias_grad_kernel(const unsigned short* __restrict__ dS, int64_t ldS, int64_t plane, int dtype,
-                                                        const Meta* __restrict__ meta, const int* __restrict__ scale, int64_t j0,
-                                                        int vocab, int bias_dtype, void* __restrict__ db) {
-  __shared__ float part[8][256 + 8];
-  const int c = (threadIdx.x & 31) * 8, rp = threadIdx.x >> 5, count = meta->count;
-  float s[8] = {};
-  for (int64_t r = rp; r < count; r += 8) {
-    const unsigned short* at = dS + r * ldS + (int64_t)blockIdx.x * 256 + c;
-    const u16x8_t h = *reinterpret_cast<const u16x8_t*>(at);
-    if (dtype == BF16) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += bf16_bits_to_f32(h[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += (float)__builtin_bit_cast(_Float16, (unsigned short)h[e]);
-    }
-    if (dtype == F32) {
-      const u16x8_t l = *reinterpret_cast<const u16x8_t*>(at + plane);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] += (float)__builtin_bit_cast(_Float16, (unsigned short)l[e]);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) part[rp][c + e] = s[e];
-  __syncthreads();
-  const int64_t j = j0 + (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (j >= vocab) return;
-  float t = 0.f;
-  for (int w = 0; w < 8; ++w) t += part[w][threadIdx.x];
-  store_as(db, j, bias_dtype, ldexpf(t, -*scale));
-}
-
 __global__ void zero_u16_kernel(unsigned short* __restrict__ p, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) p[i] = 0;
 }
@@ -690,8 +740,6 @@ struct Plan {
   int64_t Rp, Kp, Vp;
   bool pack_w;                 // W has to be split or padded; else it is read where it lies
   int64_t C_fwd, C_bwd;        // columns a piece
-  int splits;                  // contraction ranges of dh
-  bool big;                    // 256 x 256 tiles, else 128 x 128
   // saved
   size_t o_meta, o_rowmap, o_rowinv, o_lse, o_zt, o_p, o_biasz, o_h, saved;
   // forward workspace
@@ -702,7 +750,7 @@ struct Plan {
 
 bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   if (!d || d->rows < 0 || d->vocab < 1 || d->hidden_size < 1 || d->slots < 0 || d->dtype < 0 || d->dtype > 2 || d->bias_dtype < 0 ||
-      d->bias_dtype > 2 || !(d->temperature > 0.f) || !(d->temperature < INFINITY) || d->rows > (1 << 28) || d->vocab > (1 << 28) ||
+      d->bias_dtype > 2 || !(d->temperature > 0.f) || !(d->temperature < INFINITY) || d->rows > (1 << 20) || d->vocab > (1 << 28) ||
       d->hidden_size > (1 << 20) || d->slots > (1 << 16) || (!d->slots && d->temperature != 1.f))
     return false;
   P.PL = d->dtype == F32 ? 2 : 1;
@@ -711,9 +759,10 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.Kp = (int64_t)up(d->hidden_size, 64);
   P.Vp = (int64_t)up(d->vocab, 256);
   P.pack_w = d->dtype == F32 || d->hidden_size % 64 || d->ld_weight % 8 || ((uintptr_t)d->weight & 15);
-  // pieces: packed W and dS at most 128 MB each (both then stay in the 256-MB Infinity Cache between the kernels that write and
-  // read them), whole tiles, 8 192 columns at least
-  const int64_t most = 128ll << 20, least = 8192;
+  // (grids: at most 2^32 threads)
+  if ((P.Rp / 128) * (P.Vp / 128) > (1 << 23) || (int64_t)d->rows * ((P.slots + 7) / 8) > (1 << 25)) return false;
+  // pieces: packed W and dS at most MOST bytes each, whole tiles, 8 192 columns at least
+  const int64_t most = PIECE_MB << 20, least = 8192;
   auto piece = [&](int64_t bytes_a_column) {
     int64_t c = most / bytes_a_column / 256 * 256;
     if (c < least) c = least;
@@ -724,13 +773,6 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.C_fwd = P.pack_w ? piece(P.Kp * 2 * P.PL) : P.Vp;
   P.C_bwd = piece(std::max<int64_t>(P.Rp, 1) * 2 * P.PL);
   if (P.pack_w) P.C_bwd = std::min(P.C_bwd, P.C_fwd);
-  P.big = d->rows > 128 && ((d->rows + 255) / 256) * (P.Vp / 256) >= 512;
-  const int64_t T = P.big ? 256 : 128, tiles = std::max<int64_t>(1, (d->rows + T - 1) / T) * ((P.Kp + T - 1) / T);
-  const int64_t steps = P.C_bwd / 64;
-  int64_t s = (P.big ? 256 : 512) / tiles;
-  s = std::min<int64_t>(s, steps / 8);
-  P.splits = (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
-
   const size_t R = (size_t)std::max(d->rows, 1), Rp = (size_t)std::max<int64_t>(P.Rp, 256), S = P.slots;
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o += up(bytes, 256); return at; };
@@ -755,7 +797,8 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.b_grow = take(Rp * 4);
   P.b_ds = take(Rp * (size_t)P.C_bwd * 2 * P.PL);
   P.b_w = take(P.pack_w ? (size_t)P.C_bwd * P.Kp * 2 * P.PL : 0);
-  P.b_part = take((size_t)P.splits * Rp * P.Kp * 4);
+  // with more than one range the ranges' tiles number at most 512 of 128 x 128 or 256 of 256 x 256, else the rows' product once
+  P.b_part = take(std::max<size_t>(Rp * (size_t)P.Kp, std::min<size_t>(64 * Rp * (size_t)P.Kp, 256 * 256 * 256)) * 4);
   P.bwd = o;
   return true;
 }
@@ -763,17 +806,23 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
 template <bool F16V, int PL, bool BIG, bool CA, bool CB>
 using TileOf = typename std::conditional<BIG, Tile<F16V, PL, 256, 256, 128, 64, CA, CB>, Tile<F16V, PL, 128, 128, 64, 64, CA, CB>>::type;
 
-// calls f(type tag) for the operands' type and the tile
+// calls f(fp16?, planes) for the operands' type
 template <class F>
-int by_type(const gridmm_vocab_loss_t* d, bool big, F f) {
+int by_type(const gridmm_vocab_loss_t* d, F f) {
   using std::bool_constant;
   using std::integral_constant;
-  if (d->dtype == F32) return big ? f(bool_constant<true>{}, integral_constant<int, 2>{}, bool_constant<true>{})
-                                  : f(bool_constant<true>{}, integral_constant<int, 2>{}, bool_constant<false>{});
-  if (d->dtype == F16) return big ? f(bool_constant<true>{}, integral_constant<int, 1>{}, bool_constant<true>{})
-                                  : f(bool_constant<true>{}, integral_constant<int, 1>{}, bool_constant<false>{});
-  return big ? f(bool_constant<false>{}, integral_constant<int, 1>{}, bool_constant<true>{})
-             : f(bool_constant<false>{}, integral_constant<int, 1>{}, bool_constant<false>{});
+  if (d->dtype == F32) return f(bool_constant<true>{}, integral_constant<int, 2>{});
+  if (d->dtype == F16) return f(bool_constant<true>{}, integral_constant<int, 1>{});
+  return f(bool_constant<false>{}, integral_constant<int, 1>{});
+}
+// calls f(big?, rows) for each tile that a count of at most `rows` may ask for, with the most rows it is asked for
+template <class F>
+int by_tile(int rows, int64_t C, F f) {
+  // the largest count that takes the small tile
+  const int64_t small = std::max<int64_t>(128, (BIG_TILES + C / 256 - 1) / (C / 256) * 256 - 256);
+  int rc = f(std::bool_constant<false>{}, (int)std::min<int64_t>(rows, small));
+  if (rc == GRIDMM_OK && rows > small) rc = f(std::bool_constant<true>{}, rows);
+  return rc;
 }
 
 // W's rows [j0, j0 + C) as an operand: packed into `buf` or in place
@@ -850,19 +899,20 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   GRIDMM_CHECK_LAUNCH();
 
   const Operand H{Hp, P.PL * P.Kp, P.Kp, P.Rp, P.Kp};
-  const int BT = P.big ? 256 : 128;
   for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_fwd) {
     const int64_t C = std::min(P.C_fwd, P.Vp - j0);
     Operand W;
     int rc = weight_piece(d, P, j0, C, meta, (unsigned short*)(ws + P.f_w), st, W);
     if (rc != GRIDMM_OK) return rc;
-    rc = by_type(d, P.big, [&](auto f16, auto pl, auto big) {
-      using T = TileOf<decltype(f16)::value, decltype(pl)::value, decltype(big)::value, false, false>;
-      const int64_t tn = C / T::BN, tm = (d->rows + T::BM - 1) / T::BM;
-      GRIDMM_LAUNCH((score_stats_kernel<T>), dim3((unsigned)(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), tn, meta,
-                    biasz + j0, unit, stats + j0 / T::BN * P.Rp, P.Rp);
-      GRIDMM_CHECK_LAUNCH();
-      return GRIDMM_OK;
+    rc = by_type(d, [&](auto f16, auto pl) {
+      return by_tile(d->rows, C, [&](auto big, int rows) {
+        using T = TileOf<decltype(f16)::value, decltype(pl)::value, decltype(big)::value, false, false>;
+        const int64_t tn = C / T::BN, tm = (rows + T::BM - 1) / T::BM;
+        GRIDMM_LAUNCH((score_stats_kernel<T>), dim3((unsigned)(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), tn, meta,
+                      biasz + j0, unit, stats + j0 / 128 * P.Rp, P.Rp);
+        GRIDMM_CHECK_LAUNCH();
+        return GRIDMM_OK;
+      });
     });
     if (rc != GRIDMM_OK) return rc;
   }
@@ -871,12 +921,17 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   t.ldh = d->ld_hidden; t.ldw = d->ld_weight; t.ld_index = d->slots ? d->ld_ids : 1;
   t.K = d->hidden_size; t.vocab = d->vocab; t.slots = P.slots; t.wide = d->index64; t.dtype = d->dtype; t.kd = d->slots > 0;
   t.unit = unit; t.meta = meta; t.rowmap = rowmap; t.biasz = biasz; t.zt = zt;
-  const dim3 tg((unsigned)(((int64_t)d->rows * ((P.slots + 7) / 8) + 3) / 4));
-  if (d->dtype == F32) GRIDMM_LAUNCH(target_scores_kernel<F32>, tg, dim3(256), 0, st, t);
-  else if (d->dtype == BF16) GRIDMM_LAUNCH(target_scores_kernel<BF16>, tg, dim3(256), 0, st, t);
-  else GRIDMM_LAUNCH(target_scores_kernel<F16>, tg, dim3(256), 0, st, t);
+  auto scores = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    const dim3 grid((unsigned)(((int64_t)d->rows * (d->slots ? (P.slots + 7) / 8 : 1) + 3) / 4));
+    if (d->slots) GRIDMM_LAUNCH((target_scores_kernel<DT, 8>), grid, dim3(256), 0, st, t);
+    else GRIDMM_LAUNCH((target_scores_kernel<DT, 1>), grid, dim3(256), 0, st, t);
+  };
+  if (d->dtype == F32) scores(std::integral_constant<int, F32>{});
+  else if (d->dtype == BF16) scores(std::integral_constant<int, BF16>{});
+  else scores(std::integral_constant<int, F16>{});
   GRIDMM_CHECK_LAUNCH();
-  GRIDMM_LAUNCH(loss_kernel, dim3((d->rows + 15) / 16), dim3(256), 0, st, stats, P.Vp / BT, P.Rp, meta, rowmap, zt, P.slots, p,
+  GRIDMM_LAUNCH(loss_kernel, dim3((d->rows + 15) / 16), dim3(256), 0, st, stats, P.Vp, P.C_fwd, P.Rp, meta, rowmap, zt, P.slots, p,
                 plogp, d->temperature, lse, loss);
   GRIDMM_CHECK_LAUNCH();
   return GRIDMM_OK;
@@ -920,48 +975,55 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
     if (rc != GRIDMM_OK) return rc;
     const int64_t ldS = P.PL * C;
     const Operand S{dS, ldS, C, P.Rp, C};
-    rc = by_type(d, P.big, [&](auto f16, auto pl, auto big) {
-      constexpr bool F = decltype(f16)::value, BIG = decltype(big)::value;
+    rc = by_type(d, [&](auto f16, auto pl) {
+      constexpr bool F = decltype(f16)::value;
       constexpr int L = decltype(pl)::value;
-      {
-        using T = TileOf<F, L, BIG, false, false>;
-        const int64_t tn = C / T::BN, tm = (d->rows + T::BM - 1) / T::BM;
+      int rc = by_tile(d->rows, C, [&](auto big, int rows) {
+        using T = TileOf<F, L, decltype(big)::value, false, false>;
+        const int64_t tn = C / T::BN, tm = (rows + T::BM - 1) / T::BM;
         GRIDMM_LAUNCH((score_grad_kernel<T>), dim3((unsigned)(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), tn, meta,
                       biasz + j0, unit, lse, grow, dS, ldS, C);
         GRIDMM_CHECK_LAUNCH();
-      }
+        return GRIDMM_OK;
+      });
+      if (rc != GRIDMM_OK) return rc;
       FixArgs f;
       f.index = d->slots ? d->ids : d->labels; f.ld_index = d->slots ? d->ld_ids : 1; f.j0 = j0; f.ldS = ldS; f.plane = C;
       f.wide = d->index64; f.slots = P.slots; f.C = (int)C; f.vocab = d->vocab; f.dtype = d->dtype; f.meta = meta; f.rowmap = rowmap;
       f.p = p; f.zt = zt; f.lse = lse; f.grow = grow; f.dS = dS;
-      GRIDMM_LAUNCH(target_grad_kernel, dim3((unsigned)(((int64_t)d->rows * P.slots + 255) / 256)), dim3(256), 0, st, f);
+      if (d->slots) GRIDMM_LAUNCH(target_grad_kernel, dim3(d->rows), dim3(256), 0, st, f);
+      else GRIDMM_LAUNCH(label_grad_kernel, dim3((d->rows + 255) / 256), dim3(256), 0, st, f);
       GRIDMM_CHECK_LAUNCH();
       if (d_hidden) {
-        using T = TileOf<F, L, BIG, false, true>;
-        const int64_t tn = (P.Kp + T::BN - 1) / T::BN, tm = (d->rows + T::BM - 1) / T::BM;
-        GRIDMM_LAUNCH((hidden_grad_kernel<T>), dim3((unsigned)(tm * tn), P.splits), dim3(T::THREADS), 0, st, S, W, (int)(C / T::BK), tn,
-                      meta, part, P.Rp, P.Kp, j0 == 0);
-        GRIDMM_CHECK_LAUNCH();
+        rc = by_tile(d->rows, P.C_bwd, [&](auto big, int rows) {
+          using T = TileOf<F, L, decltype(big)::value, false, true>;
+          const int64_t tn = (P.Kp + T::BN - 1) / T::BN, tm = (rows + T::BM - 1) / T::BM;
+          GRIDMM_LAUNCH((hidden_grad_kernel<T>), dim3((unsigned)(tm * tn), hidden_splits(1, P.Kp, P.C_bwd, T::BM == 256)), dim3(T::THREADS),
+                        0, st, S, W, (int)(C / T::BK), tn, P.C_bwd, meta, part, P.Kp, j0 == 0);
+          GRIDMM_CHECK_LAUNCH();
+          return GRIDMM_OK;
+        });
+        if (rc != GRIDMM_OK) return rc;
       }
-      if (d_weight) {
-        using T = TileOf<F, L, BIG, true, true>;
-        const int64_t tn = (P.Kp + T::BN - 1) / T::BN, tm = C / T::BM;
-        GRIDMM_LAUNCH((weight_grad_kernel<T>), dim3((unsigned)(tm * tn)), dim3(T::THREADS), 0, st, S, H, tm, tn, meta, scale, d->dtype, j0,
-                      d->vocab, d->hidden_size, d_weight);
-        GRIDMM_CHECK_LAUNCH();
-      }
-      if (d_bias) {
-        GRIDMM_LAUNCH(bias_grad_kernel, dim3((unsigned)(C / 256)), dim3(256), 0, st, dS, ldS, C, d->dtype, meta, scale, j0,
-                      d->vocab, d->bias_dtype, d_bias);
-        GRIDMM_CHECK_LAUNCH();
+      if (d_weight || d_bias) {
+        auto weight = [&](auto big) {
+          using T = TileOf<F, L, decltype(big)::value, true, true>;
+          const int64_t tn = d_weight ? (P.Kp + T::BN - 1) / T::BN : 1, tm = C / T::BM;      // (db alone: the first tile column)
+          GRIDMM_LAUNCH((weight_grad_kernel<T>), dim3((unsigned)(tm * tn)), dim3(T::THREADS), 0, st, S, H, tm, tn, meta, scale, d->dtype, j0,
+                        d->vocab, d->hidden_size, d_weight, d->bias_dtype, d_bias);
+          GRIDMM_CHECK_LAUNCH();
+          return GRIDMM_OK;
+        };
+        rc = C / 256 * ((P.Kp + 255) / 256) >= BIG_TILES ? weight(std::true_type{}) : weight(std::false_type{});
+        if (rc != GRIDMM_OK) return rc;
       }
       return GRIDMM_OK;
     });
     if (rc != GRIDMM_OK) return rc;
   }
   if (d_hidden) {
-    GRIDMM_LAUNCH(hidden_out_kernel, dim3((d->rows + 3) / 4), dim3(256), 0, st, part, P.splits, P.Rp, P.Kp, d->hidden_size, d->rows,
-                  rowinv, meta, scale, d->dtype, d_hidden);
+    GRIDMM_LAUNCH(hidden_out_kernel, dim3(d->rows, (unsigned)((P.Kp + 255) / 256)), dim3(256), 0, st, part, P.C_bwd, P.Kp,
+                  d->hidden_size, d->rows, rowinv, meta, scale, d->dtype, d_hidden);
     GRIDMM_CHECK_LAUNCH();
   }
   return GRIDMM_OK;
