@@ -499,6 +499,26 @@ def test_top_logits_of_rows_that_are_hard_to_select_from(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("V,k,R", [(131071, 64, 1), (131072, 1000, 3), (20000, 1024, 7), (8193, 200, 40), (50021, 1, 5), (50021, 16, 700)])
+def test_top_logits_of_long_rows(dtype, V, k, R):
+    """Rows cut into segments or read by one workgroup in many chunks; rising rows, where every value enters, and constant ones."""
+    from gridmm_amd import vocab
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(R, V, generator=g) * 3
+    x[0] = torch.arange(V) / 512.0
+    if R > 1:
+        x[1] = 1.5
+        x[2, : V - 5] = float("-inf")
+    x = x.to(DT[dtype]).cuda()
+    values, ids, lse = vocab.top_logits(x, k)
+    want, order = x.float().sort(dim=1, descending=True, stable=True)
+    assert torch.equal(ids, order[:, :k]) and torch.equal(values.float(), want[:, :k])
+    z = torch.logsumexp(x.double(), 1)
+    assert bool(((lse.double() - z).abs() <= (V ** 0.5 + 16) * U * (z.abs() + want[:, 0].double().abs() + 1)).all())
+
+
+@pytest.mark.gpu
 def test_top_logits_of_rows_of_a_wider_matrix_and_of_a_batch():
     from gridmm_amd import vocab
     g = torch.Generator().manual_seed(2)
