@@ -1,0 +1,367 @@
+// The vocabulary losses for few rows (vocab_loss.hip takes it up to FEW_ROWS rows): a handful of tokens against the whole vocabulary
+// is bound by the read of W and, backward, the write of dW; tiles of 128 rows, packed copies and a dozen launches cost more than the
+// work.  Two launches forward, three backward, rows where they lie, nothing packed:
+//   few_scores   16 vocabulary rows a wave, RT tiles of 16 rows of h: each W value is loaded once, straight into the fragment layout
+//                of the 16x16 matrix instructions (fp32: 16x16x4 fp32, products and sums in fp32; 16 bits: 16x16x32, products exact).
+//                Forward: each row's (maximum, sum of exponentials) of the workgroup's 64 columns, and the targets' scores.
+//                Backward: the same scores again -> dS [vocabulary][rows] in fp32
+//   few_loss     joins the statistics, the teacher's softmax, the losses
+//   few_products dh = dS W over ranges of the vocabulary and dW = dS^T h, db, on the fp32 matrix instruction (16-bit operands are
+//                widened: exact), as two kinds of workgroups of one launch
+//   few_hidden   joins the ranges of dh
+// dS is never rounded to 16 bits here.  A row that does not count has dS = 0 and its h is read as 0.
+#pragma once
+#include "vocab_gemm.h"
+
+namespace {
+
+typedef float few_f4 __attribute__((ext_vector_type(4)));
+
+struct FewArgs {
+  const void *hidden, *weight, *bias, *index;
+  const float* teacher;
+  int64_t ldh, ldw, ld_index, ld_teacher, ignore;
+  int rows, vocab, K, slots, wide, dtype, bias_dtype, kd;
+  float inv_t, unit, temperature;
+  float2* stats;                 // [workgroup][RP]
+  float *lse, *zt, *p, *flag;    // saved: [RP], [rows][slots], [rows][slots], [RP]: 1 for rows that count
+  float* loss;
+  const float* grad;
+  int64_t grad_stride;
+  float *dS, *part;              // [vocab up to 64][RP], [ranges][RP][K up to 4]
+  void *dh, *dW, *db;
+  int ranges, range;             // of the vocabulary in dh, rows a range (a multiple of 4)
+};
+
+template <int DT>
+__device__ __forceinline__ float few_1(const void* p, int64_t i) { return load_as_f32(p, i, DT); }
+
+// values k .. k + 3 of a row, widened (zero from K on)
+template <int DT, bool VEC>
+__device__ __forceinline__ few_f4 few_load4(const void* p, int64_t off, int k, int K) {
+  few_f4 v = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (VEC) {                       // K % 4 == 0
+    const int at = k < K ? k : 0;
+    if constexpr (DT == F32) {
+      v = *reinterpret_cast<const few_f4*>((const float*)p + off + at);
+    } else {
+      const u16x4_t u = *reinterpret_cast<const u16x4_t*>((const unsigned short*)p + off + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = DT == BF16 ? bf16_bits_to_f32(u[e]) : (float)__builtin_bit_cast(_Float16, (unsigned short)u[e]);
+    }
+    if (k >= K) v = (few_f4){0.f, 0.f, 0.f, 0.f};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (k + e < K) v[e] = few_1<DT>(p, off + k + e);
+  }
+  return v;
+}
+// values k .. k + 7 of a 16-bit row as they are (zero from K on)
+template <bool VEC>
+__device__ __forceinline__ vocab::s16x8_t few_load8(const void* p, int64_t off, int k, int K) {
+  vocab::s16x8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
+  const short* x = (const short*)p + off;
+  if constexpr (VEC) {                                 // K % 8 == 0
+    v = *reinterpret_cast<const vocab::s16x8_t*>(x + (k < K ? k : 0));
+    if (k >= K) v = (vocab::s16x8_t){0, 0, 0, 0, 0, 0, 0, 0};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (k + e < K) v[e] = x[k + e];
+  }
+  return v;
+}
+
+// Scores of the wave's 16 vocabulary rows from j0 on: lane l has rows of h 16 t + (l & 15), columns j0 + 4 (l >> 4) + i, base 2, bias
+// in; -inf past the vocabulary.
+template <int DT, int RT, bool VEC>
+__device__ __forceinline__ void few_tile(const FewArgs& a, int64_t j0, f32x4_t (&acc)[RT]) {
+  const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
+  const int64_t j = j0 + l15 < a.vocab ? j0 + l15 : a.vocab - 1;
+  int64_t ho[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int r = t * 16 + l15;
+    ho[t] = (int64_t)(r < a.rows ? r : a.rows - 1) * a.ldh;
+    acc[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  }
+  // 16 bits: U steps' loads in flight together (fp32 measured slower so: 372 against 240 us at 131072 x 2048)
+  if constexpr (DT == F32) {
+#pragma unroll 4
+    for (int k0 = 0; k0 < a.K; k0 += 16) {
+      const few_f4 w = few_load4<DT, VEC>(a.weight, j * a.ldw, k0 + 4 * g, a.K);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const few_f4 h = few_load4<DT, VEC>(a.hidden, ho[t], k0 + 4 * g, a.K);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e], h[e], acc[t], 0, 0, 0);
+      }
+    }
+  } else {
+    constexpr int U = RT == 1 ? 8 : RT == 2 ? 6 : 4;
+    for (int k0 = 0; k0 < a.K; k0 += 32 * U) {
+      vocab::s16x8_t w[U], h[U][RT];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + 32 * u + 8 * g;
+        w[u] = few_load8<VEC>(a.weight, j * a.ldw, k, a.K);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) h[u][t] = few_load8<VEC>(a.hidden, ho[t], k, a.K);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          if constexpr (DT == BF16)
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w[u]), __builtin_bit_cast(bf16x8_t, h[u][t]), acc[t], 0, 0, 0);
+          else
+            acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w[u]), __builtin_bit_cast(f16x8_t, h[u][t]), acc[t], 0, 0, 0);
+        }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t c = j0 + 4 * g + i;
+    const float b = c >= a.vocab ? -INFINITY : a.bias ? load_as_f32(a.bias, c, a.bias_dtype) * a.unit : 0.f;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) acc[t][i] = c >= a.vocab ? -INFINITY : fmaf(acc[t][i], a.unit, b);
+  }
+}
+
+__device__ __forceinline__ bool few_counts(const FewArgs& a, int r) {       // cross entropy: known from the label
+  return load_index(a.index, r * a.ld_index, a.wide) != a.ignore;
+}
+
+// VEC: the rows of h and W are whole 16-byte vectors on their boundaries (decided once a call: a choice at each load would wait for it)
+template <int DT, int RT, bool VEC, bool GRAD>
+__global__ __launch_bounds__(256) void few_scores_kernel(const FewArgs a) {
+  __shared__ float2 wst[4][RT * 16];
+  constexpr int RP = RT * 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+  const int64_t j0 = (int64_t)blockIdx.x * 64 + wave * 16, jl = j0 + 4 * g;
+  f32x4_t y[RT];
+  few_tile<DT, RT, VEC>(a, j0, y);
+  if constexpr (!GRAD) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int r = t * 16 + l15;
+      float m = fmaxf(fmaxf(y[t][0], y[t][1]), fmaxf(y[t][2], y[t][3]));
+      m = fmaxf(m, __shfl_xor(m, 16, 64));
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      const float ref = m == -INFINITY ? 0.f : m;
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f(y[t][i] - ref);
+      s += __shfl_xor(s, 16, 64);
+      s += __shfl_xor(s, 32, 64);
+      if (g == 0) wst[wave][r] = make_float2(m, s);
+      if (r < a.rows)                           // the scores at the row's targets
+        for (int k = 0; k < a.slots; ++k) {
+          const int64_t d = load_index(a.index, r * a.ld_index + k, a.wide) - jl;
+          if (d >= 0 && d < 4 && jl + d < a.vocab) a.zt[(int64_t)r * a.slots + k] = d < 2 ? (d == 0 ? y[t][0] : y[t][1]) : (d == 2 ? y[t][2] : y[t][3]);
+        }
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r < RP; r += 256) {
+      float2 s = wst[0][r];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) s = join_stats(s, wst[w][r]);
+      a.stats[(int64_t)blockIdx.x * RP + r] = s;
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int r = t * 16 + l15;
+      const bool live = r < a.rows && a.flag[r] != 0.f;
+      const float gt = live ? a.grad[r * a.grad_stride] * a.temperature : 0.f, L = live ? a.lse[r] : 0.f;
+      float p[4] = {0.f, 0.f, 0.f, 0.f};
+      if (live)
+        for (int k = 0; k < a.slots; ++k) {
+          const int64_t d = load_index(a.index, r * a.ld_index + k, a.wide) - jl;
+          if (d < 0 || d >= 4) continue;
+          const float q = a.kd ? a.p[(int64_t)r * a.slots + k] : 1.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[i] += d == i ? q : 0.f;
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        a.dS[(jl + i) * RP + r] = live ? gt * (__builtin_amdgcn_exp2f(y[t][i] - L) - p[i]) : 0.f;
+    }
+  }
+}
+
+// one row a workgroup: wave 0 the teacher's softmax, all the join of the statistics
+__global__ __launch_bounds__(256) void few_loss_kernel(const FewArgs a, int64_t tiles, int RP) {
+  __shared__ float2 part[4];
+  const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float2 s = make_float2(-INFINITY, 0.f);
+  for (int64_t t = threadIdx.x; t < tiles; t += 256) s = join_stats(s, a.stats[t * RP + r]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s = join_stats(s, make_float2(__shfl_xor(s.x, o, 64), __shfl_xor(s.y, o, 64)));
+  if (lane == 0) part[wave] = s;
+  __syncthreads();
+  if (wave) return;
+  s = part[0];
+  for (int w = 1; w < 4; ++w) s = join_stats(s, part[w]);
+  float L = s.x + __builtin_amdgcn_logf(s.y), out = 0.f;
+  bool live;
+  if (a.kd) {
+    float plogp;
+    live = teacher_row(a.index, a.wide, a.ld_index, a.teacher, a.ld_teacher, r, a.slots, a.inv_t, a.p, plogp);
+    float cross = 0.f;
+    bool bad = false;
+    for (int k = lane; k < a.slots; k += 64) {
+      const int64_t id = load_index(a.index, r * a.ld_index + k, a.wide);
+      const float q = a.p[(int64_t)r * a.slots + k];
+      if (id < 0) continue;
+      bad |= id >= a.vocab;
+      if (id < a.vocab && !(q == 0.f)) cross += q * (L - a.zt[(int64_t)r * a.slots + k]);
+    }
+    cross = wave_sum(cross);
+    out = __any(bad) ? NAN : a.temperature * a.temperature * (plogp + cross * LN2);
+    if (__any(bad)) L = NAN;
+  } else {
+    const int64_t y = load_index(a.index, r * a.ld_index, a.wide);
+    live = y != a.ignore;
+    if (y < 0 || y >= a.vocab) L = NAN;                 // a label outside the vocabulary spoils its row
+    else out = (L - a.zt[r]) * LN2;
+    if (L != L) out = NAN;
+  }
+  if (lane == 0) {
+    a.loss[r] = live ? out : 0.f;
+    a.lse[r] = L;
+    a.flag[r] = live ? 1.f : 0.f;
+  }
+}
+
+template <int DT, int RT, bool VEC>
+__global__ __launch_bounds__(256) void few_products_kernel(const FewArgs a, int h_blocks, int k_blocks) {
+  constexpr int RP = RT * 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+  // Lane l of a first operand loads 4 columns from 4 perm on, one matrix instruction each; the result's rows 4 g + i are then the columns
+  // 16 i + 4 g + e: a store of 4 columns is 64 contiguous bytes a row over the wave.
+  const int perm = 4 * (l15 & 3) + (l15 >> 2);
+  if ((int)blockIdx.x < h_blocks) {
+    // dh: 256 columns a workgroup, 64 a wave; lane l ends with row 16 t + l15, columns k0 + 16 i + 4 g + e
+    const int ranges = h_blocks / k_blocks, range = blockIdx.x % ranges, k0 = blockIdx.x / ranges * 256 + wave * 64;
+    const int64_t j0 = (int64_t)range * a.range, j1 = j0 + a.range < a.vocab ? j0 + a.range : a.vocab;
+    if (k0 >= a.K) return;
+    f32x4_t acc[4][RT];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) acc[e][t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    constexpr int U = 8;
+    for (int64_t jb = j0; jb < j1; jb += 4 * U) {
+      few_f4 w[U];
+      float s[U][RT];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t j = jb + 4 * u + g, jj = j < j1 ? j : j1 - 1;
+        w[u] = few_load4<DT, VEC>(a.weight, jj * a.ldw, k0 + 4 * perm, a.K);
+#pragma unroll
+        for (int t = 0; t < RT; ++t) s[u][t] = a.dS[jj * RP + t * 16 + l15];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const float v = jb + 4 * u + g < j1 ? s[u][t] : 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[u][e], v, acc[e][t], 0, 0, 0);
+        }
+    }
+    const int64_t Kq = (a.K + 3) / 4 * 4;
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = k0 + 16 * i + 4 * g;
+        if (k < a.K)
+          *reinterpret_cast<float4*>(a.part + ((int64_t)range * RP + t * 16 + l15) * Kq + k) =
+              make_float4(acc[0][t][i], acc[1][t][i], acc[2][t][i], acc[3][t][i]);
+      }
+    return;
+  }
+  // dW: 16 vocabulary rows a workgroup, every fourth run of 64 columns a wave; lane l ends with row j0 + l15, columns k0 + 16 i + 4 g + e
+  const int64_t j = ((int64_t)blockIdx.x - h_blocks) * 16 + l15;      // (dS has rows up to a multiple of 64)
+  float s[4 * RT];
+#pragma unroll
+  for (int q = 0; q < 4 * RT; ++q) s[q] = a.dS[j * RP + 4 * q + g];
+  if (a.db && wave == 0) {
+    float sum = 0.f;
+#pragma unroll
+    for (int q = 0; q < 4 * RT; ++q) sum += s[q];
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (g == 0 && j < a.vocab) store_as(a.db, j, a.bias_dtype, sum);
+  }
+  if (!a.dW) return;
+  bool in[4 * RT];
+  int64_t ho[4 * RT];
+#pragma unroll
+  for (int q = 0; q < 4 * RT; ++q) {
+    const int r = 4 * q + g;
+    in[q] = r < a.rows && a.flag[r] != 0.f;
+    ho[q] = in[q] ? r * a.ldh : 0;
+  }
+  for (int k0 = wave * 64; k0 < a.K; k0 += 256) {
+    f32x4_t acc[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 4 * RT; ++q) {
+      if (4 * q >= a.rows) break;
+      few_f4 h = few_load4<DT, VEC>(a.hidden, ho[q], k0 + 4 * perm, a.K);
+      if (!in[q]) h = (few_f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(h[e], s[q], acc[e], 0, 0, 0);
+    }
+    if (j >= a.vocab) continue;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = k0 + 16 * i + 4 * g;
+      const float f[4] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+      if (a.K % 4 == 0) {
+        if (k >= a.K) continue;
+        if constexpr (DT == F32) {
+          *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.dW) + j * a.K + k) = make_float4(f[0], f[1], f[2], f[3]);
+        } else {
+          u16x4_t u;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[e] = DT == BF16 ? to_bf16(f[e]) : to_f16(f[e]);
+          *reinterpret_cast<u16x4_t*>(reinterpret_cast<unsigned short*>(a.dW) + j * a.K + k) = u;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (k + e < a.K) store_as(a.dW, j * a.K + k + e, DT, f[e]);
+      }
+    }
+  }
+}
+
+// dh = the ranges in order: 16 runs of 4 columns of one row a workgroup, 16 threads a run, each every 16th range
+__global__ __launch_bounds__(256) void few_hidden_kernel(const FewArgs a, int RP) {
+  __shared__ float4 sums[16][17];
+  const int t = threadIdx.x & 15, sp = threadIdx.x >> 4, r = blockIdx.x, k = blockIdx.y * 64 + t * 4;
+  const int64_t Kq = (a.K + 3) / 4 * 4;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (k < a.K) {
+#pragma unroll 4
+    for (int s = sp; s < a.ranges; s += 16) {
+      const float4 x = *reinterpret_cast<const float4*>(a.part + ((int64_t)s * RP + r) * Kq + k);
+      v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+    }
+  }
+  sums[sp][t] = v;
+  __syncthreads();
+  if (sp || k >= a.K) return;
+  for (int s = 1; s < 16; ++s) { const float4 x = sums[s][t]; v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w; }
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  for (int e = 0; e < 4; ++e)
+    if (k + e < a.K) store_as(a.dh, (int64_t)r * a.K + k + e, a.dtype, f[e]);
+}
+
+}  // namespace

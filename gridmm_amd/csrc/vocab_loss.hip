@@ -82,13 +82,19 @@ __host__ __device__ inline int hidden_splits(int64_t count, int64_t Kp, int64_t 
   return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 
-// ---- targets of the distillation: p = softmax(t / T) over the filled slots, the row's sum of p log p, whether it counts ----
-__global__ __launch_bounds__(256) void kd_targets_kernel(const void* __restrict__ ids, int wide, int64_t ld_ids,
-                                                         const float* __restrict__ t, int64_t ld_t, int rows, int slots,
-                                                         float inv_t, float* __restrict__ p, float* __restrict__ plogp,
-                                                         unsigned char* __restrict__ counts) {
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (r >= rows) return;
+__device__ __forceinline__ float2 join_stats(float2 a, float2 b) {        // (maximum, sum of 2^(y - maximum))
+  const float M = fmaxf(a.x, b.x), ref = M == -INFINITY ? 0.f : M;        // nothing but masked columns: sum 0
+  return make_float2(M, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
+}
+__device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v) {
+  if (dtype == F32) reinterpret_cast<float*>(p)[i] = v;
+  else reinterpret_cast<unsigned short*>(p)[i] = dtype == BF16 ? to_bf16(v) : to_f16(v);
+}
+
+// ---- targets of the distillation: one wave, one row: p = softmax(t / T) over the filled slots, sum of p log p; does the row count? ----
+__device__ __forceinline__ bool teacher_row(const void* ids, int wide, int64_t ld_ids, const float* t, int64_t ld_t, int64_t r, int slots,
+                                            float inv_t, float* p, float& plogp) {
+  const int lane = threadIdx.x & 63;
   float m = -INFINITY;
   bool nan = false;
   for (int s = lane; s < slots; s += 64) {
@@ -98,11 +104,10 @@ __global__ __launch_bounds__(256) void kd_targets_kernel(const void* __restrict_
     m = fmaxf(m, v);
   }
   m = wave_max(m);
-  nan = __any(nan);
-  if (m == -INFINITY && !nan) {              // nothing to learn from
-    for (int s = lane; s < slots; s += 64) p[(int64_t)r * slots + s] = 0.f;
-    if (lane == 0) { counts[r] = 0; plogp[r] = 0.f; }
-    return;
+  plogp = 0.f;
+  if (m == -INFINITY && !__any(nan)) {              // nothing to learn from
+    for (int s = lane; s < slots; s += 64) p[r * slots + s] = 0.f;
+    return false;
   }
   float sum = 0.f;
   for (int s = lane; s < slots; s += 64)
@@ -117,10 +122,20 @@ __global__ __launch_bounds__(256) void kd_targets_kernel(const void* __restrict_
       q = expf(lp);
       if (q > 0.f || q != q) h += q * lp;
     }
-    p[(int64_t)r * slots + s] = q;
+    p[r * slots + s] = q;
   }
-  h = wave_sum(h);
-  if (lane == 0) { counts[r] = 1; plogp[r] = h; }
+  plogp = wave_sum(h);
+  return true;
+}
+__global__ __launch_bounds__(256) void kd_targets_kernel(const void* __restrict__ ids, int wide, int64_t ld_ids,
+                                                         const float* __restrict__ t, int64_t ld_t, int rows, int slots,
+                                                         float inv_t, float* __restrict__ p, float* __restrict__ plogp,
+                                                         unsigned char* __restrict__ counts) {
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  float h;
+  const bool live = teacher_row(ids, wide, ld_ids, t, ld_t, r, slots, inv_t, p, h);
+  if ((threadIdx.x & 63) == 0) { counts[r] = live; plogp[r] = h; }
 }
 
 struct PrepArgs {
@@ -340,9 +355,7 @@ __global__ __launch_bounds__(T::THREADS) void score_stats_kernel(Operand A, Oper
     float2 a = wst[0][r];
 #pragma unroll
     for (int w = 1; w < T::WAVES_N; ++w) {
-      const float2 b = wst[w][r];
-      const float M = fmaxf(a.x, b.x), ref = M == -INFINITY ? 0.f : M;
-      a = make_float2(M, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
+      a = join_stats(a, wst[w][r]);
     }
     stats[tx * (T::BN / 128) * Rp + ty * T::BM + r] = a;
   }
@@ -439,19 +452,15 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
   const int64_t i = (int64_t)blockIdx.x * 16 + rr;
   if ((int64_t)blockIdx.x * 16 >= count) return;
   float2 a = make_float2(-INFINITY, 0.f);
-  auto join = [](float2 a, float2 b) {
-    const float M = fmaxf(a.x, b.x), ref = M == -INFINITY ? 0.f : M;
-    return make_float2(M, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
-  };
   if (i < count)
   {
-    for (int64_t j = lanep * T; j < whole; j += 16 * T) a = join(a, stats[j / 128 * Rp + i]);
-    for (int64_t j = whole + lanep * last; j < Vp; j += 16 * last) a = join(a, stats[j / 128 * Rp + i]);
+    for (int64_t j = lanep * T; j < whole; j += 16 * T) a = join_stats(a, stats[j / 128 * Rp + i]);
+    for (int64_t j = whole + lanep * last; j < Vp; j += 16 * last) a = join_stats(a, stats[j / 128 * Rp + i]);
   }
   part[lanep][rr] = a;
   __syncthreads();
   a = part[0][rr];
-  for (int w = 1; w < 16; ++w) a = join(a, part[w][rr]);
+  for (int w = 1; w < 16; ++w) a = join_stats(a, part[w][rr]);
   const float L = a.x + __builtin_amdgcn_logf(a.y);        // base 2
   float s = 0.f;
   bool bad = L != L;
@@ -634,11 +643,6 @@ __global__ __launch_bounds__(T::THREADS) void hidden_grad_kernel(Operand A, Oper
   }
 }
 
-__device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v) {
-  if (dtype == F32) reinterpret_cast<float*>(p)[i] = v;
-  else reinterpret_cast<unsigned short*>(p)[i] = dtype == BF16 ? to_bf16(v) : to_f16(v);
-}
-
 // dh = the ranges' partial products in order, unscaled, to the rows they came from; zero for rows that do not count.  A workgroup
 // takes 64 runs of 4 columns of one row, 4 threads a run, each every fourth range.
 __global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict__ part, int64_t C, int64_t Kp, int K, int rows,
@@ -730,13 +734,25 @@ __global__ void zero_u16_kernel(unsigned short* __restrict__ p, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) p[i] = 0;
 }
 
+}  // namespace
+
+#include "vocab_few.h"
+
+namespace {
+
 // ---------------------------------------------------------------------------------------------------------------------
 // host side: what lies where, which tile, how wide a piece
 // ---------------------------------------------------------------------------------------------------------------------
 inline size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
+// Up to this many rows the kernels of vocab_few.h.  Forward and backward, us, them against the others: fp32 131072 x 2048, 32 rows 1500 : 2300;
+// bf16 5 rows 530 : 731, 32 rows 860 : 736; 30522 x 768 at one row, forward, fp32 41 : 90.
+constexpr int FEW_ROWS_F32 = 32, FEW_ROWS_16 = 16;
+
 struct Plan {
   int PL, slots;               // planes; target slots a row (cross entropy: 1)
+  bool few;
+  int RP, ranges, range;       // few rows: rows padded to 16 or 32; ranges of the vocabulary in dh and their rows
   int64_t Rp, Kp, Vp;
   bool pack_w;                 // W has to be split or padded; else it is read where it lies
   int64_t C_fwd, C_bwd;        // columns a piece
@@ -773,6 +789,30 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.C_fwd = P.pack_w ? piece(P.Kp * 2 * P.PL) : P.Vp;
   P.C_bwd = piece(std::max<int64_t>(P.Rp, 1) * 2 * P.PL);
   if (P.pack_w) P.C_bwd = std::min(P.C_bwd, P.C_fwd);
+  P.few = d->rows <= (d->dtype == F32 ? FEW_ROWS_F32 : FEW_ROWS_16);
+  if (P.few) {
+    P.RP = d->rows <= 16 ? 16 : 32;
+    // dh: four workgroups of 256 columns a CU (512, 1024, 2048 of them: 348, 238, 240 us at 131072 x 2048 fp32), at least 64 vocabulary rows a range
+    const int64_t kb = (d->hidden_size + 255) / 256, n = std::max<int64_t>(1, std::min<int64_t>((1024 + kb - 1) / kb, d->vocab / 64));
+    P.range = (int)up((d->vocab + n - 1) / n, 4);
+    P.ranges = (d->vocab + P.range - 1) / P.range;
+    size_t o = 0;
+    auto take = [&](size_t bytes) { const size_t at = o; o += up(bytes, 256); return at; };
+    const size_t V64 = up(d->vocab, 64), S = (size_t)d->rows * P.slots;
+    P.o_lse = take(P.RP * 4);
+    P.o_meta = take(P.RP * 4);                       // 1 for rows that count
+    P.o_zt = take(S * 4);
+    P.o_p = take(d->slots ? S * 4 : 0);
+    P.saved = o;
+    o = 0;
+    P.f_stats = take(V64 / 64 * P.RP * 8);
+    P.fwd = o;
+    o = 0;
+    P.b_ds = take(V64 * P.RP * 4);
+    P.b_part = take((size_t)P.ranges * P.RP * up(d->hidden_size, 4) * 4);
+    P.bwd = o;
+    return true;
+  }
   const size_t R = (size_t)std::max(d->rows, 1), Rp = (size_t)std::max<int64_t>(P.Rp, 256), S = P.slots;
   size_t o = 0;
   auto take = [&](size_t bytes) { const size_t at = o; o += up(bytes, 256); return at; };
@@ -841,11 +881,39 @@ int weight_piece(const gridmm_vocab_loss_t* d, const Plan& P, int64_t j0, int64_
 
 bool bad_pointers(const gridmm_vocab_loss_t* d, const void* saved, bool forward) {
   if (!d->weight || !saved || d->ld_weight < d->hidden_size || ((uintptr_t)saved & 255)) return true;
-  if (d->rows && forward && (!d->hidden || d->ld_hidden < d->hidden_size)) return true;
+  if (d->rows && (!d->hidden || d->ld_hidden < d->hidden_size)) return true;
   if (d->rows && d->slots && (!d->ids || d->ld_ids < d->slots)) return true;
   if (d->rows && d->slots && forward && (!d->teacher || d->ld_teacher < d->slots)) return true;
   if (d->rows && !d->slots && !d->labels) return true;
   return false;
+}
+
+// calls f(type, tiles of 16 rows, whole vectors)
+template <class F>
+int by_few(const gridmm_vocab_loss_t* d, const Plan& P, F f) {
+  const int A = d->dtype == F32 ? 4 : 8;
+  const bool vec = d->hidden_size % A == 0 && d->ld_hidden % A == 0 && d->ld_weight % A == 0 &&
+                   (((uintptr_t)d->hidden | (uintptr_t)d->weight) & 15) == 0;
+  auto rows = [&](auto dt) {
+    auto one = [&](auto rt) { return vec ? f(dt, rt, std::true_type{}) : f(dt, rt, std::false_type{}); };
+    return P.RP == 16 ? one(std::integral_constant<int, 1>{}) : one(std::integral_constant<int, 2>{});
+  };
+  if (d->dtype == F32) return rows(std::integral_constant<int, F32>{});
+  if (d->dtype == BF16) return rows(std::integral_constant<int, BF16>{});
+  return rows(std::integral_constant<int, F16>{});
+}
+FewArgs few_args(const gridmm_vocab_loss_t* d, const Plan& P, const void* saved) {
+  FewArgs a{};
+  char* sv = (char*)saved;
+  a.hidden = d->hidden; a.weight = d->weight; a.bias = d->bias; a.index = d->slots ? d->ids : d->labels; a.teacher = d->teacher;
+  a.ldh = d->ld_hidden; a.ldw = d->ld_weight; a.ld_index = d->slots ? d->ld_ids : 1; a.ld_teacher = d->ld_teacher; a.ignore = d->ignore_index;
+  a.rows = d->rows; a.vocab = d->vocab; a.K = d->hidden_size; a.slots = P.slots; a.wide = d->index64; a.dtype = d->dtype;
+  a.bias_dtype = d->bias_dtype; a.kd = d->slots > 0;
+  a.inv_t = 1.f / d->temperature; a.unit = a.inv_t * LOG2E; a.temperature = d->temperature;
+  a.lse = (float*)(sv + P.o_lse); a.flag = (float*)(sv + P.o_meta); a.zt = (float*)(sv + P.o_zt);
+  a.p = d->slots ? (float*)(sv + P.o_p) : nullptr;
+  a.ranges = P.ranges; a.range = P.range;
+  return a;
 }
 
 }  // namespace
@@ -869,6 +937,21 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   if (d->rows == 0) return GRIDMM_OK;
   hipStream_t st = as_stream(stream);
   char *sv = (char*)saved, *ws = (char*)workspace;
+  if (P.few) {
+    FewArgs a = few_args(d, P, saved);
+    a.stats = (float2*)(ws + P.f_stats);
+    a.loss = loss;
+    const int tiles = (d->vocab + 63) / 64;
+    const int rc = by_few(d, P, [&](auto dt, auto rt, auto vec) {
+      GRIDMM_LAUNCH((few_scores_kernel<decltype(dt)::value, decltype(rt)::value, decltype(vec)::value, false>), dim3(tiles), dim3(256), 0, st, a);
+      GRIDMM_CHECK_LAUNCH();
+      return GRIDMM_OK;
+    });
+    if (rc != GRIDMM_OK) return rc;
+    GRIDMM_LAUNCH(few_loss_kernel, dim3(d->rows), dim3(256), 0, st, a, (int64_t)tiles, P.RP);
+    GRIDMM_CHECK_LAUNCH();
+    return GRIDMM_OK;
+  }
   Meta* meta = (Meta*)(sv + P.o_meta);
   int *rowmap = (int*)(sv + P.o_rowmap), *rowinv = (int*)(sv + P.o_rowinv);
   float *lse = (float*)(sv + P.o_lse), *zt = (float*)(sv + P.o_zt), *p = d->slots ? (float*)(sv + P.o_p) : nullptr;
@@ -955,6 +1038,27 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
   }
   const char* sv = (const char*)saved;
   char* ws = (char*)workspace;
+  if (P.few) {
+    FewArgs a = few_args(d, P, saved);
+    a.grad = grad; a.grad_stride = grad_stride;
+    a.dS = (float*)(ws + P.b_ds); a.part = (float*)(ws + P.b_part);
+    a.dh = d_hidden; a.dW = d_weight; a.db = d_bias;
+    const int tiles = (d->vocab + 63) / 64, kb = (d->hidden_size + 255) / 256;
+    const int hb = d_hidden ? kb * P.ranges : 0, wb = d_weight || d_bias ? (d->vocab + 15) / 16 : 0;
+    const int rc = by_few(d, P, [&](auto dt, auto rt, auto vec) {
+      GRIDMM_LAUNCH((few_scores_kernel<decltype(dt)::value, decltype(rt)::value, decltype(vec)::value, true>), dim3(tiles), dim3(256), 0, st, a);
+      GRIDMM_CHECK_LAUNCH();
+      GRIDMM_LAUNCH((few_products_kernel<decltype(dt)::value, decltype(rt)::value, decltype(vec)::value>), dim3(hb + wb), dim3(256), 0, st, a, hb, kb);
+      GRIDMM_CHECK_LAUNCH();
+      return GRIDMM_OK;
+    });
+    if (rc != GRIDMM_OK) return rc;
+    if (d_hidden) {
+      GRIDMM_LAUNCH(few_hidden_kernel, dim3(d->rows, (d->hidden_size + 63) / 64), dim3(256), 0, st, a, P.RP);
+      GRIDMM_CHECK_LAUNCH();
+    }
+    return GRIDMM_OK;
+  }
   const Meta* meta = (const Meta*)(sv + P.o_meta);
   int* scale = (int*)(ws + P.b_scale);
   const int *rowmap = (const int*)(sv + P.o_rowmap), *rowinv = (const int*)(sv + P.o_rowinv);

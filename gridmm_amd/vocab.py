@@ -31,10 +31,13 @@ class _Desc(ctypes.Structure):
                 + [("temperature", ctypes.c_float)])
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(device):
     """The tensors' own device as the current one (the kernels go to its current stream)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.index == ops._CUR_DEVICE():
+        return _HERE
     return torch.cuda.device(device)
 
 
@@ -52,21 +55,28 @@ def _need(ok, what):
         raise ValueError(what)
 
 
-def _check_head(hidden, weight, bias, **index):
-    for name, t in dict(hidden=hidden, weight=weight, bias=bias, **index).items():
+def _check_head(hidden, weight, bias, *index):
+    for t in (hidden, weight, bias) + index:
         if t is None:
             continue
         if not t.is_cuda:
-            raise _lib.GridmmLibraryError("gridmm ops need GPU tensors (%s is on %s); no CPU fallback exists" % (name, t.device))
-        _need(t.device == hidden.device, "%s is on %s, hidden on %s" % (name, t.device, hidden.device))
-    _need(hidden.dtype in _DTYPES, "hidden is fp32, bf16 or fp16, not %s" % hidden.dtype)
-    _need(weight.dtype == hidden.dtype, "weight is %s, hidden %s: one type for both" % (weight.dtype, hidden.dtype))
-    _need(hidden.dim() >= 1 and weight.dim() == 2 and weight.shape[1] == hidden.shape[-1],
-          "hidden (..., K) and weight (V, K), not %s and %s" % (tuple(hidden.shape), tuple(weight.shape)))
-    _need(weight.shape[0] >= 1 and weight.shape[1] >= 1, "an empty weight %s" % (tuple(weight.shape),))
+            raise _lib.GridmmLibraryError("gridmm ops need GPU tensors (got %s); no CPU fallback exists" % t.device)
+        if t.device != hidden.device:
+            raise ValueError("a tensor is on %s, hidden on %s" % (t.device, hidden.device))
+    dt, ws = hidden.dtype, weight.shape
+    if dt not in _DTYPES:
+        raise ValueError("hidden is fp32, bf16 or fp16, not %s" % dt)
+    if weight.dtype != dt:
+        raise ValueError("weight is %s, hidden %s: one type for both" % (weight.dtype, dt))
+    if hidden.dim() < 1 or len(ws) != 2 or ws[1] != hidden.shape[-1]:
+        raise ValueError("hidden (..., K) and weight (V, K), not %s and %s" % (tuple(hidden.shape), tuple(ws)))
+    if ws[0] < 1 or ws[1] < 1:
+        raise ValueError("an empty weight %s" % (tuple(ws),))
     if bias is not None:
-        _need(tuple(bias.shape) == (weight.shape[0],), "bias (V,), not %s" % (tuple(bias.shape),))
-        _need(bias.dtype in (torch.float32, weight.dtype), "bias is %s: fp32 or the weight's type" % bias.dtype)
+        if bias.dim() != 1 or bias.shape[0] != ws[0]:
+            raise ValueError("bias (V,), not %s" % (tuple(bias.shape),))
+        if bias.dtype != torch.float32 and bias.dtype != dt:
+            raise ValueError("bias is %s: fp32 or the weight's type" % bias.dtype)
 
 
 class _VocabLoss(torch.autograd.Function):
@@ -101,8 +111,8 @@ class _VocabLoss(torch.autograd.Function):
         _lib.check(lib.gridmm_vocab_loss_fwd(ctypes.byref(d), _p(loss), _p(saved), n_saved, _p(ws), n_ws, _stream()),
                    "gridmm_vocab_loss_fwd")
         if need:
-            ctx.save_for_backward(w, b, index, saved)
-            ctx.desc, ctx.prm, ctx.shape = d, (weight, bias), hidden.shape
+            ctx.save_for_backward(hidden, w, b, index, saved)
+            ctx.desc, ctx.prm, ctx.n_ws = d, (weight, bias), lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 1)
         return loss
 
     @staticmethod
@@ -111,19 +121,18 @@ class _VocabLoss(torch.autograd.Function):
         if g is None:
             return (None,) * 7
         lib = _lib.load()
-        w, b, index, saved = ctx.saved_tensors
-        d = ctx.desc
-        dev = w.device
+        hidden, w, b, index, saved = ctx.saved_tensors
         if g.dtype != torch.float32:
             g = g.float()
         need_h, need_w, need_b = ctx.needs_input_grad[:3]
-        dh = torch.empty(ctx.shape, dtype=w.dtype, device=dev) if need_h else None
+        dev = w.device
+        dh = torch.empty(hidden.shape, dtype=w.dtype, device=dev) if need_h else None
         dw = torch.empty(w.shape, dtype=w.dtype, device=dev) if need_w else None
-        db = torch.empty(b.shape, dtype=b.dtype, device=dev) if need_b else None
+        db = torch.empty_like(b) if need_b else None
         with _on(dev):
-            n_ws = lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 1)
+            n_ws = ctx.n_ws
             ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
-            _lib.check(lib.gridmm_vocab_loss_bwd(ctypes.byref(d), _p(saved), saved.numel(), _p(g), g.stride(0), _p(dh), _p(dw),
+            _lib.check(lib.gridmm_vocab_loss_bwd(ctypes.byref(ctx.desc), _p(saved), saved.numel(), _p(g), g.stride(0), _p(dh), _p(dw),
                                                  _p(db), _p(ws), n_ws, _stream()), "gridmm_vocab_loss_bwd")
         return dh, DEFERRED.hand(ctx.prm[0], dw), DEFERRED.hand(ctx.prm[1], db), None, None, None, None
 
@@ -134,12 +143,16 @@ def vocab_cross_entropy(hidden, weight, labels, bias=None, ignore_index=-1):
     bias (V,) in that type or fp32, labels (...) int64 or int32.  Gradients of hidden, weight and bias in their types.
 
     A label outside [0, V) that is not ignore_index makes its row's loss NaN, and with it the gradients that it reaches."""
-    _check_head(hidden, weight, bias, labels=labels)
-    _need(tuple(labels.shape) == tuple(hidden.shape[:-1]), "labels %s for hidden %s" % (tuple(labels.shape), tuple(hidden.shape)))
-    _need(labels.dtype in (torch.int64, torch.int32), "labels are int64 or int32, not %s" % labels.dtype)
+    _check_head(hidden, weight, bias, labels)
+    if labels.shape != hidden.shape[:-1]:
+        raise ValueError("labels %s for hidden %s" % (tuple(labels.shape), tuple(hidden.shape)))
+    if labels.dtype != torch.int64 and labels.dtype != torch.int32:
+        raise ValueError("labels are int64 or int32, not %s" % labels.dtype)
     with _on(hidden.device):
-        h, _ = _rows(hidden)
-        return _VocabLoss.apply(h, weight, bias, labels.reshape(-1).contiguous(), None, int(ignore_index), 1.0).view(labels.shape)
+        if labels.dim() == 1:
+            return _VocabLoss.apply(_rows(hidden)[0], weight, bias, labels.contiguous(), None, int(ignore_index), 1.0)
+        y = labels.reshape(-1).contiguous()
+        return _VocabLoss.apply(_rows(hidden)[0], weight, bias, y, None, int(ignore_index), 1.0).view(labels.shape)
 
 
 def vocab_distillation(hidden, weight, teacher_ids, teacher_logits, bias=None, temperature=1.0):
@@ -148,7 +161,7 @@ def vocab_distillation(hidden, weight, teacher_ids, teacher_logits, bias=None, t
     hidden's leading shape.  teacher_ids (..., S) int64 or int32: an id < 0 is an empty slot, an id >= V makes its row NaN, ids may
     repeat; teacher_logits (..., S) (top_logits gives both).  A row without a filled slot above -inf: loss 0, no gradient.
     Gradients of hidden, weight and bias; the teacher gets none."""
-    _check_head(hidden, weight, bias, teacher_ids=teacher_ids, teacher_logits=teacher_logits)
+    _check_head(hidden, weight, bias, teacher_ids, teacher_logits)
     _need(teacher_ids.dim() >= 1 and teacher_ids.shape == teacher_logits.shape
           and tuple(teacher_ids.shape[:-1]) == tuple(hidden.shape[:-1]) and teacher_ids.shape[-1] >= 1,
           "teacher_ids %s and teacher_logits %s for hidden %s" % (tuple(teacher_ids.shape), tuple(teacher_logits.shape),
@@ -161,7 +174,8 @@ def vocab_distillation(hidden, weight, teacher_ids, teacher_logits, bias=None, t
         h, _ = _rows(hidden)
         ids, _ = _rows(teacher_ids)
         t, _ = _rows(teacher_logits.detach().float())
-        return _VocabLoss.apply(h, weight, bias, ids, t, -1, T).view(hidden.shape[:-1])
+        loss = _VocabLoss.apply(h, weight, bias, ids, t, -1, T)
+        return loss if hidden.dim() == 2 else loss.view(hidden.shape[:-1])
 
 
 def top_logits(logits, k):
