@@ -62,12 +62,26 @@ __device__ __forceinline__ float sum8(s16x8_t v, float c) {
   return c;
 }
 
+// a pointer that is the same for the wave, in scalar registers
+__device__ __forceinline__ const unsigned short* uniform(const unsigned short* p) {
+  const uint64_t u = (uint64_t)p;
+  return (const unsigned short*)(((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(u >> 32)) << 32) |
+                                 (unsigned)__builtin_amdgcn_readfirstlane((int)u));
+}
+
 struct Operand {
   const unsigned short* p;
   int64_t ld;       // elements between rows of the stored matrix
   int64_t plane;    // elements between the hi and the lo plane of a row (PL = 2)
   int64_t rows;     // stored rows that may be read; what lies past them is read as the last one again
   int64_t cols;     // stored columns that may be read (a multiple of 8), likewise
+};
+
+// A piece of work for a workgroup: one output tile over one range of the contraction.
+struct Item {
+  int64_t bm, bn, k0;
+  int nk;              // stages; 0: the tile is 0
+  int extra;           // the caller's
 };
 
 template <bool F16_, int PL_, int BM_, int BN_, int WM_, int WN_, bool COLA_, bool COLB_>
@@ -80,75 +94,92 @@ struct Tile {
   static constexpr int STAGE = (BM + BN) * 64;           // u16 a stage
   static constexpr int PIECES = (BM + BN) / 8, PPW = PIECES / NW;
   static constexpr int LDS = 2 * STAGE;                  // u16 of the two-stage ring
+  static constexpr int SCRATCH = NW * 2048;              // u16: 4 KB a wave for an epilogue's stores
+  static constexpr int PER_CU = BM == 256 ? 1 : 2;       // workgroups that a CU's 160 KB of LDS take
   static_assert(PIECES % NW == 0 && WM % 32 == 0 && WN % 32 == 0 && BM % 64 == 0 && BN % 64 == 0, "tile shape");
+  static_assert(BM / 8 % PPW == 0 || PPW % (BM / 8) == 0, "a wave's pieces belong to one operand");
 
   using Acc = f32x16_t[TM][TN];
 
-  // Accumulates contraction steps [k0, k0 + nk * BK) of the tile at (bm, bn).  Lane l ends with, for output row
-  // bm + wr WM + 32 i + (l & 31), the columns bn + wc WN + 32 j + 8 (q >> 2) + 4 (l >> 5) + (q & 3), q < 16: the B operand is the
-  // first of the matrix instruction, so a lane holds runs of 4 columns of one row.  Every wave of the workgroup calls it.
+  // The workgroup's loop over its items: work(i, item) gives the i-th or false, done(item, acc, sums) takes the finished tile.  Lane l
+  // ends with, for output row bm + wr WM + 32 i + (l & 31), the columns bn + wc WN + 32 j + 8 (q >> 2) + 4 (l >> 5) + (q & 3), q < 16:
+  // the B operand is the first of the matrix instruction, so a lane holds runs of 4 columns of one row.
   //
-  // Two-stage ring, fragments one sub-step (16 contraction steps) ahead in registers: in front of the last sub-step of a stage
-  // every fragment of the stage is in registers, so ONE barrier says both that the next stage has landed and that this one's
-  // buffer is free; the transfers of the stage after next start right there and have a whole stage of matrix work to land.
+  // Two-stage ring that runs on from item to item, fragments one sub-step (16 contraction steps) ahead in registers: in front of the
+  // last sub-step of a stage every fragment of the stage is in registers, so ONE barrier says both that the next stage has landed and
+  // that this one's buffer is free; the transfers of the stage after next -- of the next tile, near a tile's end -- start right there.
+  // While done() works on a tile the next one's first fragments are in registers and its second stage is on the way.
   //
-  // SUMA and sum (alike for the wave): asum (TM values) also takes the sums of A over the contraction, lane l those of the steps
-  // that it holds of row 32 i + (l & 31); lanes l and l ^ 32 together hold all.
-  template <bool SUMA = false>
-  static __device__ __forceinline__ void run(const Operand& A, const Operand& B, int64_t bm, int64_t bn, int64_t k0, int nk,
-                                             unsigned short* smem, Acc& acc, float* asum = nullptr, bool sum = false) {
-    if (nk <= 0) return;
+  // SUMA: sums also takes the sums of A over the contraction for the waves that want_sums(item) names, lane l those of the steps that
+  // it holds of row 32 i + (l & 31); lanes l and l ^ 32 together hold all.
+  template <bool SUMA = false, class Work, class Want, class Done>
+  static __device__ __forceinline__ void run(const Operand& A, const Operand& B, unsigned short* smem, Work work, Want want_sums, Done done) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave / WAVES_N, wc = wave % WAVES_N;
 
-    // ---- the DMA pieces of this wave: 8 image rows x 128 bytes each; byte offsets from the operand's first tile element
-    static_assert(BM / 8 % PPW == 0 || PPW % (BM / 8) == 0, "a wave's pieces belong to one operand");
+    // ---- the transfers: this wave's pieces are 8 image rows x 128 bytes each, byte offsets from the operand's first tile element
     const bool isA = wave * PPW < BM / 8;
     const Operand& O = isA ? A : B;
     const bool col = isA ? COLA : COLB;
-    const int64_t b0 = isA ? bm : bn, r0 = b0 < O.rows ? b0 : O.rows - 1;      // (a row operand's first row)
-    const unsigned short* base = O.p + (col ? k0 * O.ld : r0 * O.ld + k0);
     const int64_t step = col ? BK * O.ld : BK;
     const unsigned ld = (unsigned)O.ld;
-    unsigned off[PPW];
-    [[maybe_unused]] int krow[PPW];
-#pragma unroll
-    for (int i = 0; i < PPW; ++i) {
-      const int q = wave * PPW + i - (isA ? 0 : BM / 8), slot = lane & 7;
-      if (!col) {
-        const int64_t last = O.rows - 1 - r0;
-        int row = q * 8 + (lane >> 3);
-        const int c = slot ^ ((row >> 1) & 7);
-        if (row > last) row = (int)last;
-        off[i] = ((unsigned)row * ld + (PL == 2 ? (c >> 2) * (unsigned)O.plane + (c & 3) * 8 : c * 8)) * 2;
-        krow[i] = 0;
-      } else {
-        const int panel = q >> 3, rr = (q & 7) * 8 + (lane >> 3);
-        const int c = slot ^ (((rr >> 1) & 1) << 2);
-        int64_t cc = b0 + panel * 64 + c * 8;
-        if (cc > O.cols - 8) cc = O.cols - 8;
-        krow[i] = PL == 2 ? rr & 31 : rr;
-        off[i] = ((unsigned)krow[i] * ld + (PL == 2 ? (rr >> 5) * (unsigned)O.plane : 0) + (unsigned)cc) * 2;
-      }
-    }
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned short*)smem + wave * PPW * 1024;
-    auto issue_piece = [&](int kt, int i, bool tail) {
-      const unsigned short* from = base + kt * step;
-      unsigned o = off[i];
-      if ((COLA || COLB) && tail) {           // contraction rows past the last stored one: that one again
-        const int64_t first = k0 + (int64_t)kt * BK, have = O.rows - 1 - first;
-        const int keep = have < 0 ? 0 : krow[i] < have ? krow[i] : (int)have;
-        if (have < 0) from = O.p + (O.rows - 1) * O.ld;
-        o -= (unsigned)(krow[i] - keep) * ld * 2;
-      }
-      dma16(from, o, lds0 + (kt & 1) * (STAGE * 2) + i * 1024);
+    const unsigned short* base = O.p;
+    unsigned off[PPW];
+    Item ahead;                          // the item whose stage `akt` is transferred next
+    int ai = 0, akt = 0, issued = 0;
+    bool have;
+    auto krow = [&](int i) {             // (a column operand's contraction row within the stage)
+      const int q = wave * PPW + i - (isA ? 0 : BM / 8), rr = (q & 7) * 8 + (lane >> 3);
+      return PL == 2 ? rr & 31 : rr;
     };
-    auto is_tail = [&](int kt) { return (COLA || COLB) && col && k0 + (int64_t)(kt + 1) * BK > O.rows; };
-    auto issue = [&](int kt) {
-      const bool tail = is_tail(kt);
+    auto aim = [&] {
+      const int64_t b0 = isA ? ahead.bm : ahead.bn, r0 = b0 < O.rows ? b0 : O.rows - 1;      // (a row operand's first row)
+      base = O.p + (col ? ahead.k0 * O.ld : r0 * O.ld + ahead.k0);
 #pragma unroll
-      for (int i = 0; i < PPW; ++i) issue_piece(kt, i, tail);
+      for (int i = 0; i < PPW; ++i) {
+        const int q = wave * PPW + i - (isA ? 0 : BM / 8), slot = lane & 7;
+        if (!col) {
+          int row = q * 8 + (lane >> 3);
+          const int c = slot ^ ((row >> 1) & 7);
+          if (row > O.rows - 1 - r0) row = (int)(O.rows - 1 - r0);
+          off[i] = ((unsigned)row * ld + (PL == 2 ? (c >> 2) * (unsigned)O.plane + (c & 3) * 8 : c * 8)) * 2;
+        } else {
+          const int panel = q >> 3, rr = (q & 7) * 8 + (lane >> 3);
+          const int c = slot ^ (((rr >> 1) & 1) << 2);
+          int64_t cc = b0 + panel * 64 + c * 8;
+          if (cc > O.cols - 8) cc = O.cols - 8;
+          off[i] = ((unsigned)krow(i) * ld + (PL == 2 ? (rr >> 5) * (unsigned)O.plane : 0) + (unsigned)cc) * 2;
+        }
+      }
+    };
+    auto next_item = [&] {
+      do have = work(ai++, ahead); while (have && ahead.nk <= 0);
+      akt = 0;
+      if (have) aim();
+    };
+    auto issue = [&] {
+      const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + (issued & 1) * (STAGE * 2));
+      if (COLA || COLB) {
+        const int64_t first = ahead.k0 + (int64_t)akt * BK, last = O.rows - 1 - first;      // (of a column operand)
+        if (col && last < BK - 1) {              // contraction rows past the last stored one: that one again
+          const unsigned short* from = uniform(last < 0 ? O.p + (O.rows - 1) * O.ld : base + akt * step);
+#pragma unroll
+          for (int i = 0; i < PPW; ++i) {
+            const int kr = krow(i), keep = last < 0 ? 0 : kr < last ? kr : (int)last;
+            dma16(from, off[i] - (unsigned)(kr - keep) * ld * 2, to + i * 1024);
+          }
+          ++issued;
+          if (++akt == ahead.nk) next_item();
+          return;
+        }
+      }
+      const unsigned short* from = uniform(base + akt * step);
+#pragma unroll
+      for (int i = 0; i < PPW; ++i) dma16(from, off[i], to + i * 1024);
+      ++issued;
+      if (++akt == ahead.nk) next_item();
     };
 
     // ---- fragments
@@ -171,14 +202,15 @@ struct Tile {
     constexpr int KS = BK / 16;
     s16x8_t a[2][TM], b[2][TN];                                 // (hi) planes, two sub-steps
     [[maybe_unused]] s16x8_t al[TM], bl[TN];                    // lo planes of the current one
-    auto read = [&](s16x8_t (&fa)[TM], s16x8_t (&fb)[TN], int kt, int ks, int lo) {
-      const unsigned short* sa = smem + (kt & 1) * STAGE;
+    auto read = [&](s16x8_t (&fa)[TM], s16x8_t (&fb)[TN], int stage, int ks, int lo) {
+      const unsigned short* sa = smem + (stage & 1) * STAGE;
       const unsigned short* sb = sa + BM * 64;
 #pragma unroll
       for (int n = 0; n < TN; ++n) fb[n] = frag(CB{}, sb, wc * WN + n * 32, ks, lo);
 #pragma unroll
       for (int i = 0; i < TM; ++i) fa[i] = frag(CA{}, sa, wr * WM + i * 32, ks, lo);
     };
+    Acc acc;
     auto product = [&](const s16x8_t (&fa)[TM], const s16x8_t (&fb)[TN]) {
 #pragma unroll
       for (int i = 0; i < TM; ++i)
@@ -186,68 +218,85 @@ struct Tile {
         for (int n = 0; n < TN; ++n) acc[i][n] = mma<F16>(fb[n], fa[i], acc[i][n]);
     };
     auto barrier = [&] {
+      // this wave's pieces of the next stage have landed and its reads of the current one are in registers
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     };
 
-    issue(0);
-    barrier();
-    if (nk > 1) issue(1);
-    read(a[0], b[0], 0, 0, 0);
-    for (int kt = 0; kt < nk; ++kt) {
+    next_item();
+    if (have) {
+      issue();
+      barrier();
+      if (have) issue();
+      read(a[0], b[0], 0, 0, 0);
+    }
+    Item item;
+    int stage = 0;
+    for (int n = 0; work(n, item); ++n) {
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const int set = ks & 1;
-        bool next = false, tail = false;
-        if constexpr (PL == 2) read(al, bl, kt, ks, 1);
-        if (ks + 1 < KS) {
-          read(a[set ^ 1], b[set ^ 1], kt, ks + 1, 0);
-        } else if (kt + 1 < nk) {
-          barrier();
-          read(a[set ^ 1], b[set ^ 1], kt + 1, 0, 0);
-          next = kt + 2 < nk;
-          tail = next && is_tail(kt + 2);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        product(a[set], b[set]);
-        if constexpr (PL == 2) {
-          product(a[set], bl);
-          product(al, b[set]);
-        }
-        if (SUMA && sum) {
+      for (int i = 0; i < TM; ++i)
 #pragma unroll
-          for (int i = 0; i < TM; ++i) {
-            asum[i] = sum8<F16>(a[set][i], asum[i]);
-            if constexpr (PL == 2) asum[i] = sum8<F16>(al[i], asum[i]);
+        for (int c = 0; c < TN; ++c)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) acc[i][c][q] = 0.f;
+      float sums[TM] = {};
+      const bool sum = SUMA && want_sums(item);
+      for (int kt = 0; kt < item.nk; ++kt, ++stage) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const int set = ks & 1;
+          bool more = false;
+          if constexpr (PL == 2) read(al, bl, stage, ks, 1);
+          if (ks + 1 < KS) {
+            read(a[set ^ 1], b[set ^ 1], stage, ks + 1, 0);
+          } else if (stage + 1 < issued) {
+            barrier();
+            read(a[set ^ 1], b[set ^ 1], stage + 1, 0, 0);
+            more = have;
           }
-        }
-        if (next) {
+          __builtin_amdgcn_sched_barrier(0);
+          product(a[set], b[set]);
+          if constexpr (PL == 2) {
+            product(a[set], bl);
+            product(al, b[set]);
+          }
+          if (SUMA && sum) {
 #pragma unroll
-          for (int q = 0; q < PPW; ++q) issue_piece(kt + 2, q, tail);
+            for (int i = 0; i < TM; ++i) {
+              sums[i] = sum8<F16>(a[set][i], sums[i]);
+              if constexpr (PL == 2) sums[i] = sum8<F16>(al[i], sums[i]);
+            }
+          }
+          if (more) issue();
+          __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
+      done(item, acc, sums);
     }
   }
 };
 
-// Workgroup b -> tile (ty, tx) of a tm x tn grid of tiles, false past the last.  Workgroup b runs on XCD b % 8, each with an L2 of
-// its own: every XCD gets a contiguous part of a list that walks strips of 8 tile columns row by row, so the workgroups that run
-// together on one share their A and B rows through it.
-__device__ __forceinline__ bool tile_of(int64_t b, int64_t tm, int64_t tn, int64_t& ty, int64_t& tx) {
-  const int64_t T = tm * tn;
-  if (b >= T) return false;
-  const int64_t xcd = b & 7, i = b >> 3, q = T >> 3, rem = T & 7;
-  const int64_t t = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + i;
-  constexpr int64_t W = 8;
-  const int64_t nfs = tn / W, full = nfs * tm * W;
+// The n-th tile (ty, tx) of workgroup b of `blocks`, of a tm x tn grid of tiles, and which of `layers` grids; false past the last.
+// Workgroup b runs on XCD b % 8, each with an L2 of its own: every XCD gets a contiguous part of a list that walks strips of 8 tile
+// columns row by row, and its workgroups take the list's next tiles in turn, so those that run together share their A and B rows.
+__device__ __forceinline__ bool tile_of(unsigned b, unsigned blocks, unsigned n, unsigned tm, unsigned tn, unsigned layers, unsigned& ty,
+                                        unsigned& tx, unsigned& layer) {
+  const unsigned T = tm * tn * layers, x = b & 7, q = T >> 3, rem = T & 7;
+  const unsigned mine = q + (x < rem), per = (blocks - x + 7) >> 3;           // tiles of this XCD, its workgroups
+  const unsigned i = (b >> 3) + n * per;
+  if (i >= mine) return false;
+  unsigned t = (x < rem ? x * (q + 1) : rem * (q + 1) + (x - rem) * q) + i;
+  layer = t / (tm * tn);
+  t -= layer * (tm * tn);
+  constexpr unsigned W = 8;
+  const unsigned nfs = tn / W, full = nfs * tm * W;
   if (t < full) {
-    const int64_t strip = t / (tm * W), r = t - strip * tm * W;
+    const unsigned strip = t / (tm * W), r = t - strip * tm * W;
     ty = r / W;
     tx = strip * W + r % W;
   } else {
-    const int64_t w = tn - nfs * W, r = t - full;
+    const unsigned w = tn - nfs * W, r = t - full;
     ty = r / w;
     tx = nfs * W + r % w;
   }

@@ -26,6 +26,7 @@
 namespace {
 
 using vocab::f32x16_t;
+using vocab::Item;
 using vocab::Operand;
 using vocab::Tile;
 using vocab::tile_of;
@@ -307,58 +308,63 @@ __global__ __launch_bounds__(256) void pack_w_kernel(const void* __restrict__ W,
 
 // ---- forward: per-row (maximum, sum of exponentials) of each tile's columns ----
 template <class T>
-__global__ __launch_bounds__(T::THREADS) void score_stats_kernel(Operand A, Operand B, int nk, int64_t tn, const Meta* __restrict__ meta,
+__global__ __launch_bounds__(T::THREADS, 2) void score_stats_kernel(Operand A, Operand B, int nk, int tn, const Meta* __restrict__ meta,
                                                                  const float* __restrict__ biasz, float unit,
                                                                  float2* __restrict__ stats, int64_t Rp) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
   __shared__ float2 wst[T::WAVES_N][T::BM];
-  const int count = meta->count;
-  int64_t ty, tx;
-  if (big_tiles(count, tn * T::BN) != (T::BM == 256) || !tile_of(blockIdx.x, (count + T::BM - 1) / T::BM, tn, ty, tx)) return;
-  typename T::Acc acc = {};
-  T::run(A, B, ty * T::BM, tx * T::BN, 0, nk, smem, acc);
-
+  const int count = __builtin_amdgcn_readfirstlane(meta->count), tm = (count + T::BM - 1) / T::BM;
+  if (big_tiles(count, (int64_t)tn * T::BN) != (T::BM == 256)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
   const float sc = ldexpf(unit, -(meta->sh + meta->sw));
-  float m[T::TM], s[T::TM];
+  T::run(
+      A, B, smem,
+      [&](int n, Item& it) {
+        unsigned ty, tx, layer;
+        if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, 1, ty, tx, layer)) return false;
+        it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, 0, nk, 0};
+        return true;
+      },
+      [](const Item&) { return false; },
+      [&](const Item& it, typename T::Acc& acc, const float*) {
+        float m[T::TM];
 #pragma unroll
-  for (int i = 0; i < T::TM; ++i) m[i] = -INFINITY;
+        for (int i = 0; i < T::TM; ++i) m[i] = -INFINITY;
 #pragma unroll
-  for (int n = 0; n < T::TN; ++n)
+        for (int n = 0; n < T::TN; ++n)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float4 b = *reinterpret_cast<const float4*>(biasz + tx * T::BN + wc * T::WN + n * 32 + q * 8 + (lane >> 5) * 4);
+          for (int q = 0; q < 4; ++q) {
+            const float4 b = *reinterpret_cast<const float4*>(biasz + it.bn + wc * T::WN + n * 32 + q * 8 + (lane >> 5) * 4);
 #pragma unroll
-      for (int i = 0; i < T::TM; ++i) {
-        f32x16_t& c = acc[i][n];
-        c[q * 4 + 0] = fmaf(c[q * 4 + 0], sc, b.x);
-        c[q * 4 + 1] = fmaf(c[q * 4 + 1], sc, b.y);
-        c[q * 4 + 2] = fmaf(c[q * 4 + 2], sc, b.z);
-        c[q * 4 + 3] = fmaf(c[q * 4 + 3], sc, b.w);
-        m[i] = fmaxf(m[i], fmaxf(fmaxf(c[q * 4], c[q * 4 + 1]), fmaxf(c[q * 4 + 2], c[q * 4 + 3])));
-      }
-    }
+            for (int i = 0; i < T::TM; ++i) {
+              f32x16_t& c = acc[i][n];
+              c[q * 4 + 0] = fmaf(c[q * 4 + 0], sc, b.x);
+              c[q * 4 + 1] = fmaf(c[q * 4 + 1], sc, b.y);
+              c[q * 4 + 2] = fmaf(c[q * 4 + 2], sc, b.z);
+              c[q * 4 + 3] = fmaf(c[q * 4 + 3], sc, b.w);
+              m[i] = fmaxf(m[i], fmaxf(fmaxf(c[q * 4], c[q * 4 + 1]), fmaxf(c[q * 4 + 2], c[q * 4 + 3])));
+            }
+          }
 #pragma unroll
-  for (int i = 0; i < T::TM; ++i) {
-    m[i] = fmaxf(m[i], __shfl_xor(m[i], 32, 64));
-    const float ref = m[i] == -INFINITY ? 0.f : m[i];      // a tile whose columns are all masked: sum 0
-    float t = 0.f;
+        for (int i = 0; i < T::TM; ++i) {
+          m[i] = fmaxf(m[i], __shfl_xor(m[i], 32, 64));
+          const float ref = m[i] == -INFINITY ? 0.f : m[i];      // a tile whose columns are all masked: sum 0
+          float t = 0.f;
 #pragma unroll
-    for (int n = 0; n < T::TN; ++n)
+          for (int n = 0; n < T::TN; ++n)
 #pragma unroll
-      for (int q = 0; q < 16; ++q) t += __builtin_amdgcn_exp2f(acc[i][n][q] - ref);
-    s[i] = t + __shfl_xor(t, 32, 64);
-    if (lane < 32) wst[wc][wr * T::WM + i * 32 + lane] = make_float2(m[i], s[i]);
-  }
-  __syncthreads();
-  for (int r = threadIdx.x; r < T::BM; r += T::THREADS) {
-    float2 a = wst[0][r];
+            for (int q = 0; q < 16; ++q) t += __builtin_amdgcn_exp2f(acc[i][n][q] - ref);
+          t += __shfl_xor(t, 32, 64);
+          if (lane < 32) wst[wc][wr * T::WM + i * 32 + lane] = make_float2(m[i], t);
+        }
+        __syncthreads();
+        for (int r = threadIdx.x; r < T::BM; r += T::THREADS) {
+          float2 a = wst[0][r];
 #pragma unroll
-    for (int w = 1; w < T::WAVES_N; ++w) {
-      a = join_stats(a, wst[w][r]);
-    }
-    stats[tx * (T::BN / 128) * Rp + ty * T::BM + r] = a;
-  }
+          for (int w = 1; w < T::WAVES_N; ++w) a = join_stats(a, wst[w][r]);
+          stats[it.bn / 128 * Rp + it.bm + r] = a;
+        }
+      });
 }
 
 // ---- scores at the targets: one wave a (row, NS slots), fp32 sums over the operands as they came ----
@@ -509,49 +515,92 @@ __global__ __launch_bounds__(PREP_T) void grad_scale_kernel(const float* __restr
   for (int i = tid; i < Rp; i += PREP_T) grow[i] = i < count ? ldexpf(g[(int64_t)rowmap[i] * gs] * temperature, sg) : 0.f;
 }
 
+// A wave's 32 x 64 values of an epilogue, of 16 or 32 bits, through its own LDS: lane l puts the runs of 4 columns it holds of row
+// l & 31, and takes 16 bytes at a time of rows that lie whole in 8 (16 bits) or 16 (32 bits, 32 columns a pass) lanes: 128 contiguous
+// bytes a row instead of 16 or 32.
+template <class Put>
+__device__ __forceinline__ void rows_of_16(unsigned short* scratch, const u16x4_t (&v)[8], Put put) {
+  const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+  // run n q (8 columns 8 (4 n + q) ..) half h: 8 bytes at column 32 n + 8 q + 4 h, 16-byte chunks swizzled by the row
+#pragma unroll
+  for (int i = 0; i < 8; ++i) *reinterpret_cast<u16x4_t*>(scratch + r * 64 + ((i ^ (r & 7)) * 8) + h * 4) = v[i];
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int row = p * 8 + (lane >> 3), c = lane & 7;
+    put(row, c * 8, *reinterpret_cast<const u16x8_t*>(scratch + row * 64 + ((c ^ (row & 7)) * 8)));
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+template <class Put>
+__device__ __forceinline__ void rows_of_32(unsigned short* scratch, const float4 (&v)[4], Put put) {       // 32 x 32
+  const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+  float* s = reinterpret_cast<float*>(scratch);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) *reinterpret_cast<float4*>(s + r * 32 + (((2 * q + h) ^ (r & 7)) * 4)) = v[q];
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int row = p * 8 + (lane >> 3), c = lane & 7;
+    put(row, c * 4, *reinterpret_cast<const float4*>(s + row * 32 + ((c ^ (row & 7)) * 4)));
+  }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+}
+
 // dS of the columns [j0, j0 + C): dS[r][j] = grow_r exp2(y_rj - lse_r), two planes for fp32 operands
 template <class T>
-__global__ __launch_bounds__(T::THREADS) void score_grad_kernel(Operand A, Operand B, int nk, int64_t tn, const Meta* __restrict__ meta,
+__global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Operand B, int nk, int tn, const Meta* __restrict__ meta,
                                                                 const float* __restrict__ biasz, float unit,
                                                                 const float* __restrict__ lse, const float* __restrict__ grow,
                                                                 unsigned short* __restrict__ dS, int64_t ldS, int64_t plane) {
-  __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
-  const int count = meta->count;
-  int64_t ty, tx;
-  if (big_tiles(count, tn * T::BN) != (T::BM == 256) || !tile_of(blockIdx.x, (count + T::BM - 1) / T::BM, tn, ty, tx)) return;
-  typename T::Acc acc = {};
-  T::run(A, B, ty * T::BM, tx * T::BN, 0, nk, smem, acc);
-
+  __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
+  const int count = __builtin_amdgcn_readfirstlane(meta->count), tm = (count + T::BM - 1) / T::BM;
+  if (big_tiles(count, (int64_t)tn * T::BN) != (T::BM == 256)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
   const float sc = ldexpf(unit, -(meta->sh + meta->sw));
+  unsigned short* scratch = smem + T::LDS + wave * 2048;
+  static_assert(T::TN == 2, "64 columns a wave");
+  T::run(
+      A, B, smem,
+      [&](int n, Item& it) {
+        unsigned ty, tx, layer;
+        if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, 1, ty, tx, layer)) return false;
+        it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, 0, nk, 0};
+        return true;
+      },
+      [](const Item&) { return false; },
+      [&](const Item& it, typename T::Acc& acc, const float*) {
+        const int64_t r0 = it.bm + wr * T::WM, c0 = it.bn + wc * T::WN;
+        const float* bz = biasz + c0 + (lane >> 5) * 4;
 #pragma unroll
-  for (int i = 0; i < T::TM; ++i) {
-    const int64_t r = ty * T::BM + wr * T::WM + i * 32 + (lane & 31);
-    const bool live = r < count;
-    const float L = live ? lse[r] : 0.f, gr = live ? grow[r] : 0.f;
+        for (int i = 0; i < T::TM; ++i) {
+          __builtin_amdgcn_sched_barrier(0);
+          const int64_t r = r0 + i * 32 + (lane & 31);
+          const bool live = r < count;
+          const float L = live ? lse[r] : 0.f, gr = live ? grow[r] : 0.f;
+          u16x4_t hi[8], lo[8];
 #pragma unroll
-    for (int n = 0; n < T::TN; ++n)
+          for (int c = 0; c < 8; ++c) {
+            const float4 b = *reinterpret_cast<const float4*>(bz + c * 8);
+            const float bb[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t c0 = tx * T::BN + wc * T::WN + n * 32 + q * 8 + (lane >> 5) * 4;
-        const float4 b = *reinterpret_cast<const float4*>(biasz + c0);
-        const float bb[4] = {b.x, b.y, b.z, b.w};
-        u16x4_t hi, lo;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = live ? gr * __builtin_amdgcn_exp2f(fmaf(acc[i][n][q * 4 + e], sc, bb[e]) - L) : 0.f;
-          if constexpr (T::PL == 2) {
-            const _Float16 h = (_Float16)v;
-            hi[e] = __builtin_bit_cast(unsigned short, h);
-            lo[e] = to_f16(v - (float)h);
-          } else {
-            hi[e] = to_16<T::F16>(v);
+            for (int e = 0; e < 4; ++e) {
+              const float v = live ? gr * __builtin_amdgcn_exp2f(fmaf(acc[i][c >> 2][(c & 3) * 4 + e], sc, bb[e]) - L) : 0.f;
+              if constexpr (T::PL == 2) {
+                const _Float16 h = (_Float16)v;
+                hi[c][e] = __builtin_bit_cast(unsigned short, h);
+                lo[c][e] = to_f16(v - (float)h);
+              } else {
+                hi[c][e] = to_16<T::F16>(v);
+              }
+            }
           }
+          unsigned short* at = dS + (r0 + i * 32) * ldS + c0;
+          rows_of_16(scratch, hi, [&](int row, int cc, u16x8_t v) { *reinterpret_cast<u16x8_t*>(at + row * ldS + cc) = v; });
+          if constexpr (T::PL == 2)
+            rows_of_16(scratch, lo, [&](int row, int cc, u16x8_t v) { *reinterpret_cast<u16x8_t*>(at + plane + row * ldS + cc) = v; });
         }
-        *reinterpret_cast<u16x4_t*>(dS + r * ldS + c0) = hi;
-        if constexpr (T::PL == 2) *reinterpret_cast<u16x4_t*>(dS + plane + r * ldS + c0) = lo;
-      }
-  }
+      });
 }
 
 // the entries of dS at the targets in [j0, j0 + C): grow_r (exp2(zt - lse) - sum of p over the slots of the same id), rounded once
@@ -612,35 +661,44 @@ __global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
 // dh of this piece: partial products over the contraction ranges blockIdx.y, added to those of the pieces before.  `C`: the columns of
 // a whole piece, which fix the tile and the number of ranges for all pieces.
 template <class T>
-__global__ __launch_bounds__(T::THREADS) void hidden_grad_kernel(Operand A, Operand B, int steps, int64_t tn, int64_t C,
+__global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, Operand B, int steps, int tn, int64_t C,
                                                                  const Meta* __restrict__ meta, float* __restrict__ part, int64_t Kp,
                                                                  int first) {
-  __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
-  const int count = meta->count;
+  __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
+  const int count = __builtin_amdgcn_readfirstlane(meta->count), tm = (count + T::BM - 1) / T::BM;
   const bool big = big_tiles(count, C);
-  const int splits = hidden_splits(count, Kp, C, big);
-  int64_t ty, tx;
-  if (big != (T::BM == 256) || (int)blockIdx.y >= splits || !tile_of(blockIdx.x, (count + T::BM - 1) / T::BM, tn, ty, tx)) return;
-  const int per = (steps + splits - 1) / splits, s0 = blockIdx.y * per, nk = min(per, steps - s0);
-  typename T::Acc acc = {};
-  T::run(A, B, ty * T::BM, tx * T::BN, (int64_t)s0 * T::BK, nk, smem, acc);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
-  float* out = part + (int64_t)blockIdx.y * count * Kp;
+  if (big != (T::BM == 256)) return;
+  const int splits = hidden_splits(count, Kp, C, big), per = (steps + splits - 1) / splits;
+  const int wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
+  unsigned short* scratch = smem + T::LDS + wave * 2048;
+  T::run(
+      A, B, smem,
+      [&](int n, Item& it) {
+        unsigned ty, tx, split;
+        if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, splits, ty, tx, split)) return false;
+        it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, (int64_t)split * per * T::BK, min(per, steps - (int)split * per), (int)split};
+        return true;
+      },
+      [](const Item&) { return false; },
+      [&](const Item& it, typename T::Acc& acc, const float*) {
+        float* out = part + (int64_t)it.extra * count * Kp;
 #pragma unroll
-  for (int i = 0; i < T::TM; ++i) {
-    const int64_t r = ty * T::BM + wr * T::WM + i * 32 + (lane & 31);
+        for (int i = 0; i < T::TM; ++i)
 #pragma unroll
-    for (int n = 0; n < T::TN; ++n)
+          for (int n = 0; n < T::TN; ++n) {
+            __builtin_amdgcn_sched_barrier(0);
+            const int64_t r0 = it.bm + wr * T::WM + i * 32, c0 = it.bn + wc * T::WN + n * 32;
+            float4 v[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t c0 = tx * T::BN + wc * T::WN + n * 32 + q * 8 + (lane >> 5) * 4;
-        if (r >= count || c0 >= Kp) continue;
-        float4* at = reinterpret_cast<float4*>(out + r * Kp + c0);
-        float4 v = make_float4(acc[i][n][q * 4], acc[i][n][q * 4 + 1], acc[i][n][q * 4 + 2], acc[i][n][q * 4 + 3]);
-        if (!first) { const float4 o = *at; v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w; }
-        *at = v;
-      }
-  }
+            for (int q = 0; q < 4; ++q) v[q] = make_float4(acc[i][n][q * 4], acc[i][n][q * 4 + 1], acc[i][n][q * 4 + 2], acc[i][n][q * 4 + 3]);
+            rows_of_32(scratch, v, [&](int row, int cc, float4 x) {
+              if (r0 + row >= count || c0 + cc >= Kp) return;
+              float4* at = reinterpret_cast<float4*>(out + (r0 + row) * Kp + c0 + cc);
+              if (!first) { const float4 o = *at; x.x += o.x; x.y += o.y; x.z += o.z; x.w += o.w; }
+              *at = x;
+            });
+          }
+      });
 }
 
 // dh = the ranges' partial products in order, unscaled, to the rows they came from; zero for rows that do not count.  A workgroup
@@ -652,7 +710,7 @@ __global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict
   const int t = threadIdx.x & 63, sp = threadIdx.x >> 6;
   const int64_t r = blockIdx.x;
   const int k = blockIdx.y * 256 + t * 4;
-  const int count = meta->count, pos = rowinv[r], e = -(*scale + meta->sw);
+  const int count = __builtin_amdgcn_readfirstlane(meta->count), pos = rowinv[r], e = -(*scale + meta->sw);
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (pos >= 0 && k < Kp) {
     const int splits = hidden_splits(count, Kp, C, big_tiles(count, C));
@@ -676,58 +734,79 @@ __global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict
 // dW of this piece: rows [j0, j0 + C) complete (the contraction is all counted rows), written once in the weight's type; the first
 // tile column also sums dS over the rows: db
 template <class T>
-__global__ __launch_bounds__(T::THREADS) void weight_grad_kernel(Operand A, Operand B, int64_t tm, int64_t tn, const Meta* __restrict__ meta,
-                                                                 const int* __restrict__ scale, int dtype, int64_t j0, int vocab, int K, void* __restrict__ dW,
-                                                                 int bias_dtype, void* __restrict__ db) {
-  __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
-  int64_t ty, tx;
-  if (!tile_of(blockIdx.x, tm, tn, ty, tx)) return;
-  const int count = meta->count;
-  typename T::Acc acc = {};
+__global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, Operand B, int tm, int tn, const Meta* __restrict__ meta,
+                                                                 const int* __restrict__ scale, int dtype, int64_t j0, int vocab, int K,
+                                                                 void* __restrict__ dW, int bias_dtype, void* __restrict__ db) {
+  __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
+  const int count = __builtin_amdgcn_readfirstlane(meta->count), nk = (count + T::BK - 1) / T::BK;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
-  const int nk = (count + T::BK - 1) / T::BK;
-  float sums[T::TM] = {};
-  const bool sum = db && tx == 0 && wc == 0;
-  T::template run<true>(A, B, ty * T::BM, tx * T::BN, 0, nk, smem, acc, sums, sum);
-  if (sum) {
+  const int sg = *scale;
+  const float un = ldexpf(1.f, -sg), unw = ldexpf(1.f, -meta->sh);       // (two factors: their product may leave fp32's range)
+  unsigned short* scratch = smem + T::LDS + wave * 2048;
+  static_assert(T::TN == 2, "64 columns a wave");
+  T::template run<true>(
+      A, B, smem,
+      [&](int n, Item& it) {
+        unsigned ty, tx, layer;
+        if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, 1, ty, tx, layer)) return false;
+        it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, 0, nk, 0};
+        return true;
+      },
+      [&](const Item& it) { return db && it.bn == 0 && wc == 0; },
+      [&](const Item& it, typename T::Acc& acc, const float* sums) {
+        const int64_t r0 = j0 + it.bm + wr * T::WM, c0 = it.bn + wc * T::WN;
+        if (db && it.bn == 0 && wc == 0) {
 #pragma unroll
-    for (int i = 0; i < T::TM; ++i) {
-      const float s = sums[i] + __shfl_xor(sums[i], 32, 64);
-      const int64_t j = j0 + ty * T::BM + wr * T::WM + i * 32 + (lane & 31);
-      if (lane < 32 && j < vocab) store_as(db, j, bias_dtype, ldexpf(s, -*scale));
-    }
-  }
-  if (!dW) return;
-  const int e = -(*scale + meta->sh);
-#pragma unroll
-  for (int i = 0; i < T::TM; ++i) {
-    const int64_t r = j0 + ty * T::BM + wr * T::WM + i * 32 + (lane & 31);
-    if (r >= vocab) continue;
-#pragma unroll
-    for (int n = 0; n < T::TN; ++n)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t c0 = tx * T::BN + wc * T::WN + n * 32 + q * 8 + (lane >> 5) * 4;
-        float f[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) f[x] = ldexpf(acc[i][n][q * 4 + x], e);
-        if (K % 4 == 0) {
-          if (c0 >= K) continue;
-          if (dtype == F32) {
-            *reinterpret_cast<float4*>(reinterpret_cast<float*>(dW) + r * K + c0) = make_float4(f[0], f[1], f[2], f[3]);
-          } else {
-            u16x4_t u;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) u[x] = dtype == BF16 ? to_bf16(f[x]) : to_f16(f[x]);
-            *reinterpret_cast<u16x4_t*>(reinterpret_cast<unsigned short*>(dW) + r * K + c0) = u;
+          for (int i = 0; i < T::TM; ++i) {
+            const float s = sums[i] + __shfl_xor(sums[i], 32, 64);
+            const int64_t j = r0 + i * 32 + (lane & 31);
+            if (lane < 32 && j < vocab) store_as(db, j, bias_dtype, s * un);
           }
-        } else {
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (c0 + x < K) store_as(dW, r * K + c0 + x, dtype, f[x]);
         }
-      }
-  }
+        if (!dW) return;
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (dtype == F32) {
+            float* out = reinterpret_cast<float*>(dW);
+#pragma unroll
+            for (int n = 0; n < T::TN; ++n) {
+              float4 v[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                v[q] = make_float4(acc[i][n][q * 4] * un * unw, acc[i][n][q * 4 + 1] * un * unw, acc[i][n][q * 4 + 2] * un * unw, acc[i][n][q * 4 + 3] * un * unw);
+              rows_of_32(scratch, v, [&](int row, int cc, float4 x) {
+                const int64_t r = r0 + i * 32 + row, c = c0 + n * 32 + cc;
+                if (r >= vocab || c >= K) return;
+                if (K % 4 == 0) {
+                  *reinterpret_cast<float4*>(out + r * K + c) = x;
+                } else {
+                  const float f[4] = {x.x, x.y, x.z, x.w};
+                  for (int e = 0; e < 4; ++e)
+                    if (c + e < K) out[r * K + c + e] = f[e];
+                }
+              });
+            }
+          } else {
+            unsigned short* out = reinterpret_cast<unsigned short*>(dW);
+            u16x4_t v[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[c][e] = to_16<T::F16>(acc[i][c >> 2][(c & 3) * 4 + e] * un * unw);
+            rows_of_16(scratch, v, [&](int row, int cc, u16x8_t x) {
+              const int64_t r = r0 + i * 32 + row, c = c0 + cc;
+              if (r >= vocab || c >= K) return;
+              if (K % 8 == 0) {
+                *reinterpret_cast<u16x8_t*>(out + r * K + c) = x;
+              } else {
+                for (int e = 0; e < 8; ++e)
+                  if (c + e < K) out[r * K + c + e] = x[e];
+              }
+            });
+          }
+        }
+      });
 }
 
 __global__ void zero_u16_kernel(unsigned short* __restrict__ p, int64_t n) {
@@ -845,6 +924,10 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
 
 template <bool F16V, int PL, bool BIG, bool CA, bool CB>
 using TileOf = typename std::conditional<BIG, Tile<F16V, PL, 256, 256, 128, 64, CA, CB>, Tile<F16V, PL, 128, 128, 64, 64, CA, CB>>::type;
+
+// workgroups for so many tiles: what the chip holds at once, each then walks several
+template <class T>
+unsigned blocks(int64_t tiles) { return (unsigned)std::min<int64_t>(tiles, 256 * T::PER_CU); }
 
 // calls f(fp16?, planes) for the operands' type
 template <class F>
@@ -991,7 +1074,7 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
       return by_tile(d->rows, C, [&](auto big, int rows) {
         using T = TileOf<decltype(f16)::value, decltype(pl)::value, decltype(big)::value, false, false>;
         const int64_t tn = C / T::BN, tm = (rows + T::BM - 1) / T::BM;
-        GRIDMM_LAUNCH((score_stats_kernel<T>), dim3((unsigned)(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), tn, meta,
+        GRIDMM_LAUNCH((score_stats_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), (int)tn, meta,
                       biasz + j0, unit, stats + j0 / 128 * P.Rp, P.Rp);
         GRIDMM_CHECK_LAUNCH();
         return GRIDMM_OK;
@@ -1085,7 +1168,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
       int rc = by_tile(d->rows, C, [&](auto big, int rows) {
         using T = TileOf<F, L, decltype(big)::value, false, false>;
         const int64_t tn = C / T::BN, tm = (rows + T::BM - 1) / T::BM;
-        GRIDMM_LAUNCH((score_grad_kernel<T>), dim3((unsigned)(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), tn, meta,
+        GRIDMM_LAUNCH((score_grad_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), (int)tn, meta,
                       biasz + j0, unit, lse, grow, dS, ldS, C);
         GRIDMM_CHECK_LAUNCH();
         return GRIDMM_OK;
@@ -1102,8 +1185,8 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
         rc = by_tile(d->rows, P.C_bwd, [&](auto big, int rows) {
           using T = TileOf<F, L, decltype(big)::value, false, true>;
           const int64_t tn = (P.Kp + T::BN - 1) / T::BN, tm = (rows + T::BM - 1) / T::BM;
-          GRIDMM_LAUNCH((hidden_grad_kernel<T>), dim3((unsigned)(tm * tn), hidden_splits(1, P.Kp, P.C_bwd, T::BM == 256)), dim3(T::THREADS),
-                        0, st, S, W, (int)(C / T::BK), tn, P.C_bwd, meta, part, P.Kp, j0 == 0);
+          GRIDMM_LAUNCH((hidden_grad_kernel<T>), dim3(blocks<T>(tm * tn * hidden_splits(1, P.Kp, P.C_bwd, T::BM == 256))), dim3(T::THREADS),
+                        0, st, S, W, (int)(C / T::BK), (int)tn, P.C_bwd, meta, part, P.Kp, j0 == 0);
           GRIDMM_CHECK_LAUNCH();
           return GRIDMM_OK;
         });
@@ -1113,7 +1196,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
         auto weight = [&](auto big) {
           using T = TileOf<F, L, decltype(big)::value, true, true>;
           const int64_t tn = d_weight ? (P.Kp + T::BN - 1) / T::BN : 1, tm = C / T::BM;      // (db alone: the first tile column)
-          GRIDMM_LAUNCH((weight_grad_kernel<T>), dim3((unsigned)(tm * tn)), dim3(T::THREADS), 0, st, S, H, tm, tn, meta, scale, d->dtype, j0,
+          GRIDMM_LAUNCH((weight_grad_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, S, H, (int)tm, (int)tn, meta, scale, d->dtype, j0,
                         d->vocab, d->hidden_size, d_weight, d->bias_dtype, d_bias);
           GRIDMM_CHECK_LAUNCH();
           return GRIDMM_OK;
