@@ -270,30 +270,6 @@ __device__ __forceinline__ void pack_row(const void* src, int64_t off, int dtype
   }
 }
 
-// counted rows of h -> Hp (rows past the count up to a multiple of 256: zero)
-__global__ __launch_bounds__(256) void pack_h_kernel(const void* __restrict__ hidden, int64_t ldh, int dtype, int K, int Kp,
-                                                     const int* __restrict__ rowmap, const float* __restrict__ amax_h,
-                                                     const float* __restrict__ amax_w, Meta* __restrict__ meta,
-                                                     unsigned short* __restrict__ Hp) {
-  const int lane = threadIdx.x & 63;
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int count = meta->count;
-  int sh = 0;
-  if (dtype == F32) {
-    sh = scale_exp(wave_max(amax_h[lane]), 14);
-    if (i == 0) {
-      float m = 0.f;
-      for (int k = lane; k < AMAX_W; k += 64) m = fmaxf(m, amax_w[k]);
-      m = wave_max(m);
-      if (lane == 0) { meta->sh = sh; meta->sw = scale_exp(m, 14); }
-    }
-  }
-  if (i >= (count + 255) / 256 * 256) return;
-  const bool zero = i >= count;
-  unsigned short* hi = Hp + (int64_t)i * Kp * (dtype == F32 ? 2 : 1);
-  pack_row(hidden, zero ? 0 : (int64_t)rowmap[i] * ldh, dtype, K, Kp, lane, sh, zero, hi, hi + Kp);
-}
-
 // rows [j0, j0 + C) of W -> Wp (zero past the vocabulary)
 __global__ __launch_bounds__(256) void pack_w_kernel(const void* __restrict__ W, int64_t ldw, int dtype, int K, int Kp, int64_t j0,
                                                      int C, int vocab, const Meta* __restrict__ meta,
@@ -371,7 +347,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_stats_kernel(Operand A, O
 struct TargetArgs {
   const void *hidden, *weight, *index;
   int64_t ldh, ldw, ld_index;
-  int K, vocab, slots, wide, dtype, kd;      // slots >= 1
+  int K, vocab, slots, wide, kd;      // slots >= 1
   float unit;
   const Meta* meta;
   const int* rowmap;
@@ -417,10 +393,10 @@ __device__ __forceinline__ void dots(const TargetArgs& a, int64_t r, const int64
   for (int s = 0; s < NS; ++s) out[s] = wave_sum(out[s]);
 }
 template <int DT, int NS>
-__global__ __launch_bounds__(256) void target_scores_kernel(const TargetArgs a) {
+__device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block) {
   const int lane = threadIdx.x & 63;
   const int groups = (a.slots + NS - 1) / NS;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t w = block * 4 + (threadIdx.x >> 6);
   const int64_t i = w / groups;
   if (i >= a.meta->count) return;
   const int s0 = (int)(w % groups) * NS;
@@ -441,6 +417,33 @@ __global__ __launch_bounds__(256) void target_scores_kernel(const TargetArgs a) 
     // an id outside the vocabulary spoils its row; an empty slot has no score
     a.zt[i * a.slots + s0 + s] = a.kd && id[s] < 0 ? 0.f : id[s] < 0 || id[s] >= a.vocab ? NAN : fmaf(z[s], a.unit, a.biasz[at[s]]);
   }
+}
+
+// One launch behind prep_kernel: the first `blocks` workgroups pack the counted rows of h into Hp (rows past the count up to a multiple
+// of 256: zero), the others compute the scores at the targets.
+template <int DT, int NS>
+__global__ __launch_bounds__(256) void rows_kernel(const TargetArgs t, int blocks, int Kp,
+                                                     const float* __restrict__ amax_h,
+                                                     const float* __restrict__ amax_w, Meta* __restrict__ meta,
+                                                     unsigned short* __restrict__ Hp) {
+  if ((int)blockIdx.x >= blocks) return target_scores<DT, NS>(t, blockIdx.x - blocks);
+  const int lane = threadIdx.x & 63;
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int count = meta->count;
+  int sh = 0;
+  if constexpr (DT == F32) {
+    sh = scale_exp(wave_max(amax_h[lane]), 14);
+    if (i == 0) {
+      float m = 0.f;
+      for (int k = lane; k < AMAX_W; k += 64) m = fmaxf(m, amax_w[k]);
+      m = wave_max(m);
+      if (lane == 0) { meta->sh = sh; meta->sw = scale_exp(m, 14); }
+    }
+  }
+  if (i >= (count + 255) / 256 * 256) return;
+  const bool zero = i >= count;
+  unsigned short* hi = Hp + (int64_t)i * Kp * (DT == F32 ? 2 : 1);
+  pack_row(t.hidden, zero ? 0 : (int64_t)t.rowmap[i] * t.ldh, DT, t.K, Kp, lane, sh, zero, hi, hi + Kp);
 }
 
 // ---- joins the tiles' statistics and writes the losses: 16 rows a workgroup, 16 threads a row ----
@@ -834,9 +837,10 @@ struct Plan {
   int RP, ranges, range;       // few rows: rows padded to 16 or 32; ranges of the vocabulary in dh and their rows
   int64_t Rp, Kp, Vp;
   bool pack_w;                 // W has to be split or padded; else it is read where it lies
+  bool keep_w;                 // ... and its copy, one piece, stays for the backward (28 us of 396 at 30522 x 768 fp32)
   int64_t C_fwd, C_bwd;        // columns a piece
   // saved
-  size_t o_meta, o_rowmap, o_rowinv, o_lse, o_zt, o_p, o_biasz, o_h, saved;
+  size_t o_meta, o_rowmap, o_rowinv, o_lse, o_zt, o_p, o_biasz, o_h, o_w, saved;
   // forward workspace
   size_t f_counts, f_plogp, f_amax, f_stats, f_w, fwd;
   // backward workspace
@@ -867,6 +871,7 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   };
   P.C_fwd = P.pack_w ? piece(P.Kp * 2 * P.PL) : P.Vp;
   P.C_bwd = piece(std::max<int64_t>(P.Rp, 1) * 2 * P.PL);
+  P.keep_w = P.pack_w && P.C_fwd == P.Vp;
   if (P.pack_w) P.C_bwd = std::min(P.C_bwd, P.C_fwd);
   P.few = d->rows <= (d->dtype == F32 ? FEW_ROWS_F32 : FEW_ROWS_16);
   if (P.few) {
@@ -903,19 +908,20 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.o_p = take(d->slots ? R * S * 4 : 0);
   P.o_biasz = take(P.Vp * 4);
   P.o_h = take(Rp * P.Kp * 2 * P.PL);
+  P.o_w = take(P.keep_w ? (size_t)P.Vp * P.Kp * 2 * P.PL : 0);
   P.saved = o;
   o = 0;
   P.f_counts = take(R);
   P.f_plogp = take(R * 4);
   P.f_amax = take((AMAX_H + AMAX_W) * 4);
   P.f_stats = take(Rp * (size_t)(P.Vp / 128) * 8);
-  P.f_w = take(P.pack_w ? (size_t)P.C_fwd * P.Kp * 2 * P.PL : 0);
+  P.f_w = take(P.pack_w && !P.keep_w ? (size_t)P.C_fwd * P.Kp * 2 * P.PL : 0);
   P.fwd = o;
   o = 0;
   P.b_scale = take(4);
   P.b_grow = take(Rp * 4);
   P.b_ds = take(Rp * (size_t)P.C_bwd * 2 * P.PL);
-  P.b_w = take(P.pack_w ? (size_t)P.C_bwd * P.Kp * 2 * P.PL : 0);
+  P.b_w = take(P.pack_w && !P.keep_w ? (size_t)P.C_bwd * P.Kp * 2 * P.PL : 0);
   // with more than one range the ranges' tiles number at most 512 of 128 x 128 or 256 of 256 x 256, else the rows' product once
   P.b_part = take(std::max<size_t>(Rp * (size_t)P.Kp, std::min<size_t>(64 * Rp * (size_t)P.Kp, 256 * 256 * 256)) * 4);
   P.bwd = o;
@@ -929,6 +935,13 @@ using TileOf = typename std::conditional<BIG, Tile<F16V, PL, 256, 256, 128, 64, 
 template <class T>
 unsigned blocks(int64_t tiles) { return (unsigned)std::min<int64_t>(tiles, 256 * T::PER_CU); }
 
+// calls f(type)
+template <class F>
+int by_dtype(const gridmm_vocab_loss_t* d, F f) {
+  if (d->dtype == F32) return f(std::integral_constant<int, F32>{});
+  if (d->dtype == BF16) return f(std::integral_constant<int, BF16>{});
+  return f(std::integral_constant<int, F16>{});
+}
 // calls f(fp16?, planes) for the operands' type
 template <class F>
 int by_type(const gridmm_vocab_loss_t* d, F f) {
@@ -948,17 +961,20 @@ int by_tile(int rows, int64_t C, F f) {
   return rc;
 }
 
-// W's rows [j0, j0 + C) as an operand: packed into `buf` or in place
-int weight_piece(const gridmm_vocab_loss_t* d, const Plan& P, int64_t j0, int64_t C, const Meta* meta, unsigned short* buf,
-                 hipStream_t st, Operand& W) {
-  if (P.pack_w) {
+// W's rows [j0, j0 + C) as an operand: packed into `buf` (kept: all of it in `kept`, where the forward packs it) or in place
+int weight_piece(const gridmm_vocab_loss_t* d, const Plan& P, int64_t j0, int64_t C, const Meta* meta, unsigned short* kept, bool forward,
+                 unsigned short* buf, hipStream_t st, Operand& W) {
+  if (!P.pack_w) {
+    W = Operand{(const unsigned short*)d->weight + j0 * d->ld_weight, d->ld_weight, 0, d->vocab - j0, P.Kp};
+    return GRIDMM_OK;
+  }
+  if (P.keep_w) buf = kept + j0 * P.PL * P.Kp;
+  if (forward || !P.keep_w) {
     GRIDMM_LAUNCH(pack_w_kernel, dim3((unsigned)((C + 3) / 4)), dim3(256), 0, st, d->weight, d->ld_weight, d->dtype, d->hidden_size,
                   (int)P.Kp, j0, (int)C, d->vocab, meta, buf);
     GRIDMM_CHECK_LAUNCH();
-    W = Operand{buf, P.PL * P.Kp, P.Kp, C, P.Kp};
-  } else {
-    W = Operand{(const unsigned short*)d->weight + j0 * d->ld_weight, d->ld_weight, 0, d->vocab - j0, P.Kp};
   }
+  W = Operand{buf, P.PL * P.Kp, P.Kp, C, P.Kp};
   return GRIDMM_OK;
 }
 
@@ -981,9 +997,7 @@ int by_few(const gridmm_vocab_loss_t* d, const Plan& P, F f) {
     auto one = [&](auto rt) { return vec ? f(dt, rt, std::true_type{}) : f(dt, rt, std::false_type{}); };
     return P.RP == 16 ? one(std::integral_constant<int, 1>{}) : one(std::integral_constant<int, 2>{});
   };
-  if (d->dtype == F32) return rows(std::integral_constant<int, F32>{});
-  if (d->dtype == BF16) return rows(std::integral_constant<int, BF16>{});
-  return rows(std::integral_constant<int, F16>{});
+  return by_dtype(d, rows);
 }
 FewArgs few_args(const gridmm_vocab_loss_t* d, const Plan& P, const void* saved) {
   FewArgs a{};
@@ -1060,15 +1074,27 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   const int nb = (int)((P.Vp + PREP_T - 1) / PREP_T);
   GRIDMM_LAUNCH(prep_kernel, dim3(1 + nb + (d->dtype == F32 ? AMAX_H + AMAX_W : 0)), dim3(PREP_T), 0, st, a, nb);
   GRIDMM_CHECK_LAUNCH();
-  GRIDMM_LAUNCH(pack_h_kernel, dim3((unsigned)(P.Rp / 4)), dim3(256), 0, st, d->hidden, d->ld_hidden, d->dtype, d->hidden_size,
-                (int)P.Kp, rowmap, amax, amax + AMAX_H, meta, Hp);
-  GRIDMM_CHECK_LAUNCH();
+  TargetArgs t;
+  t.hidden = d->hidden; t.weight = d->weight; t.index = d->slots ? d->ids : d->labels;
+  t.ldh = d->ld_hidden; t.ldw = d->ld_weight; t.ld_index = d->slots ? d->ld_ids : 1;
+  t.K = d->hidden_size; t.vocab = d->vocab; t.slots = P.slots; t.wide = d->index64; t.kd = d->slots > 0;
+  t.unit = unit; t.meta = meta; t.rowmap = rowmap; t.biasz = biasz; t.zt = zt;
+  const int rc = by_dtype(d, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    const int hb = (int)(P.Rp / 4);
+    const dim3 grid((unsigned)(hb + ((int64_t)d->rows * (d->slots ? (P.slots + 7) / 8 : 1) + 3) / 4));
+    if (d->slots) GRIDMM_LAUNCH((rows_kernel<DT, 8>), grid, dim3(256), 0, st, t, hb, (int)P.Kp, amax, amax + AMAX_H, meta, Hp);
+    else GRIDMM_LAUNCH((rows_kernel<DT, 1>), grid, dim3(256), 0, st, t, hb, (int)P.Kp, amax, amax + AMAX_H, meta, Hp);
+    GRIDMM_CHECK_LAUNCH();
+    return GRIDMM_OK;
+  });
+  if (rc != GRIDMM_OK) return rc;
 
   const Operand H{Hp, P.PL * P.Kp, P.Kp, P.Rp, P.Kp};
   for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_fwd) {
     const int64_t C = std::min(P.C_fwd, P.Vp - j0);
     Operand W;
-    int rc = weight_piece(d, P, j0, C, meta, (unsigned short*)(ws + P.f_w), st, W);
+    int rc = weight_piece(d, P, j0, C, meta, (unsigned short*)(sv + P.o_w), true, (unsigned short*)(ws + P.f_w), st, W);
     if (rc != GRIDMM_OK) return rc;
     rc = by_type(d, [&](auto f16, auto pl) {
       return by_tile(d->rows, C, [&](auto big, int rows) {
@@ -1082,21 +1108,6 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
     });
     if (rc != GRIDMM_OK) return rc;
   }
-  TargetArgs t;
-  t.hidden = d->hidden; t.weight = d->weight; t.index = d->slots ? d->ids : d->labels;
-  t.ldh = d->ld_hidden; t.ldw = d->ld_weight; t.ld_index = d->slots ? d->ld_ids : 1;
-  t.K = d->hidden_size; t.vocab = d->vocab; t.slots = P.slots; t.wide = d->index64; t.dtype = d->dtype; t.kd = d->slots > 0;
-  t.unit = unit; t.meta = meta; t.rowmap = rowmap; t.biasz = biasz; t.zt = zt;
-  auto scores = [&](auto dt) {
-    constexpr int DT = decltype(dt)::value;
-    const dim3 grid((unsigned)(((int64_t)d->rows * (d->slots ? (P.slots + 7) / 8 : 1) + 3) / 4));
-    if (d->slots) GRIDMM_LAUNCH((target_scores_kernel<DT, 8>), grid, dim3(256), 0, st, t);
-    else GRIDMM_LAUNCH((target_scores_kernel<DT, 1>), grid, dim3(256), 0, st, t);
-  };
-  if (d->dtype == F32) scores(std::integral_constant<int, F32>{});
-  else if (d->dtype == BF16) scores(std::integral_constant<int, BF16>{});
-  else scores(std::integral_constant<int, F16>{});
-  GRIDMM_CHECK_LAUNCH();
   GRIDMM_LAUNCH(loss_kernel, dim3((d->rows + 15) / 16), dim3(256), 0, st, stats, P.Vp, P.C_fwd, P.Rp, meta, rowmap, zt, P.slots, p,
                 plogp, d->temperature, lse, loss);
   GRIDMM_CHECK_LAUNCH();
@@ -1158,7 +1169,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
   for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_bwd) {
     const int64_t C = std::min(P.C_bwd, P.Vp - j0);
     Operand W;
-    int rc = weight_piece(d, P, j0, C, meta, wbuf, st, W);
+    int rc = weight_piece(d, P, j0, C, meta, (unsigned short*)(sv + P.o_w), false, wbuf, st, W);
     if (rc != GRIDMM_OK) return rc;
     const int64_t ldS = P.PL * C;
     const Operand S{dS, ldS, C, P.Rp, C};
