@@ -22,7 +22,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import autograd as ag, hostsync as hs, vilmodel as V, vilmodel_train as VT
+from . import autograd as ag, hostsync as hs, vilmodel as V, vilmodel_train as VT, vocab
 
 N_CELLS = 196
 
@@ -310,7 +310,12 @@ class GlocalTextPathCMTPreTraining(nn.Module):
 
     def forward_mlm(self, batch, compute_loss=True):
         """pretrain_cmt.py:131-153 + vilmodel.py:767-856: the text attends to [gmap | vp] through
-        forward_lang2visn of every local cross-modal layer, then the tied-decoder MLM head on masked tokens."""
+        forward_lang2visn of every local cross-modal layer, then the tied-decoder MLM head on masked tokens.
+
+        config.mlm_in_pieces (default False): the losses come from vocab.vocab_cross_entropy, which multiplies with the decoder in
+        pieces of the vocabulary and keeps no logits (fp32 accuracy; the default head multiplies in three bf16 terms).
+        batch["txt_teacher_ids"] / ["txt_teacher_logits"] (masked tokens in order, slots; mlm_teacher gives them): the losses also hold
+        config.mlm_distill_weight (1) times the distillation at config.mlm_distill_temperature (1); then always in pieces."""
         txt = self.bert._mlm_text(self._front(batch))
         labels = batch["txt_labels"]
         sel = labels != -1
@@ -318,6 +323,15 @@ class GlocalTextPathCMTPreTraining(nn.Module):
         p = self.mlm_head.predictions
         h = ag.layer_norm(ag.gelu(ag.linear(hidden, p.transform.dense.weight, p.transform.dense.bias)),
                           p.transform.LayerNorm)
+        c = self.config
+        ids = batch.get("txt_teacher_ids")
+        if compute_loss and (ids is not None or getattr(c, "mlm_in_pieces", False)):
+            w, b = p.decoder.weight, p.bias
+            loss = vocab.vocab_cross_entropy(h, w, hs.select(labels, sel).long(), bias=b)
+            if ids is not None:
+                loss = loss + getattr(c, "mlm_distill_weight", 1.0) * vocab.vocab_distillation(
+                    h, w, ids, batch["txt_teacher_logits"], bias=b, temperature=getattr(c, "mlm_distill_temperature", 1.0))
+            return loss
         # decoder(h) + bias.  The vocabulary (30 522 rows) is not a multiple of 8, which the plane GEMMs and the row-major weight
         # gradient need: the tied matrix and its bias are extended by zero rows for the call (one cat each; the gradient of the
         # cat is the row slice) and the extra logit columns cut off -- instead of the fp32-A fallback kernels (5 calls of ~260 us
@@ -333,6 +347,13 @@ class GlocalTextPathCMTPreTraining(nn.Module):
         if compute_loss:
             return F.cross_entropy(scores, hs.select(labels, sel).long(), reduction="none")
         return scores
+
+    @torch.no_grad()
+    def mlm_teacher(self, batch, k):
+        """What this model, as a teacher, hands to a student's forward_mlm: the k largest scores of every masked token, as
+        dict(txt_teacher_ids=(n, k) int64, txt_teacher_logits=(n, k) fp32)."""
+        values, ids, _ = vocab.top_logits(self(batch, task="mlm", compute_loss=False), k)
+        return dict(txt_teacher_ids=ids, txt_teacher_logits=values)
 
     @staticmethod
     def _region_head(head, x):

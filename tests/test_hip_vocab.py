@@ -555,6 +555,91 @@ def test_teacher_to_student():
         _hold(t, (v, (a[name][1] + c[name][1]) * 1.001 + 2 * U * v.abs()), name)
 
 
+# ---- the masked-token head ----
+def _mlm_model():
+    from conftest import load_golden
+    from test_hip_pretrain import _model
+    return _model(load_golden("pretrain_reduced.npz"))
+
+
+def _mlm_batch():
+    from gridmm_amd.synthetic import batch_to
+    from oracle import gen_golden
+    return batch_to(gen_golden.pretrain_batch("mlm"), "cuda")
+
+
+@pytest.mark.gpu
+def test_masked_token_head_in_pieces_equals_the_head_that_keeps_its_logits():
+    """The same losses and gradients as torch's cross entropy of the kept logits, to what that head's three bf16 terms leave: products
+    off by 3 2^-17 of |h| |W| (2^-16 with the bias's share); measured against the reference's gradients elsewhere at 5e-3."""
+    m = _mlm_model()
+    losses, grads = [], []
+    for pieces in (False, True):
+        m.config.mlm_in_pieces = pieces
+        m.zero_grad()
+        loss = m(_mlm_batch(), task="mlm", compute_loss=True)
+        loss.mean().backward()
+        losses.append(loss.detach())
+        grads.append({k: p.grad.clone() for k, p in m.named_parameters() if p.grad is not None})
+    m.config.mlm_in_pieces = False
+    assert losses[0].shape == losses[1].shape and losses[0].dtype == losses[1].dtype
+    # |h| <= sqrt(K) (LayerNorm's rows, unit gain up to a factor 2), rows of W of norm |W|: two scores each off by 2^-15 of the product
+    w = m.mlm_head.predictions.decoder.weight
+    bound = 2 * 2.0 ** -15 * 2 * w.shape[1] ** 0.5 * float(w.detach().norm(dim=1).max()) + 2.0 ** -20 * float(losses[0].abs().max())
+    assert float((losses[0] - losses[1]).abs().max()) <= bound
+    assert sorted(grads[0]) == sorted(grads[1])
+    scale = max(float(g.norm()) for g in grads[0].values())
+    for k in grads[0]:
+        a, b = grads[0][k].double(), grads[1][k].double()
+        tol = 2e-2 if "text_proj" in k else 5e-3      # (text_proj: arg-max routes, see the reference's own gradients)
+        assert float((a - b).norm()) <= tol * max(float(a.norm()), 1e-3 * scale), k
+
+
+@pytest.mark.gpu
+def test_masked_token_head_learns_from_a_teacher():
+    """Losses and gradients with a teacher's top logits: cross entropy plus the weighted distillation, of the same hidden states."""
+    from gridmm_amd import vocab
+    m = _mlm_model()
+    batch = _mlm_batch()
+    other = dict(batch, **m.mlm_teacher(batch, 12))
+    n = other["txt_teacher_ids"].shape[0]
+    assert other["txt_teacher_ids"].shape == other["txt_teacher_logits"].shape == (n, 12)
+    m.config.mlm_in_pieces = True
+    plain = m(_mlm_batch(), task="mlm", compute_loss=True)
+    m.config.mlm_distill_weight, m.config.mlm_distill_temperature = 0.5, 2.0
+    both = m(other, task="mlm", compute_loss=True)
+    # the teacher is the student: the distillation is T^2 KL(p over 12 slots || q over everything) = -T^2 log(q's mass on the slots)
+    scores = m(_mlm_batch(), task="mlm", compute_loss=False).detach().double() / 2.0
+    mass = torch.log_softmax(scores, 1).gather(1, other["txt_teacher_ids"]).logsumexp(1)
+    want = plain.detach().double() - 0.5 * 4.0 * mass
+    w = m.mlm_head.predictions.decoder.weight
+    bound = 8 * 2.0 ** -15 * 2 * w.shape[1] ** 0.5 * float(w.detach().norm(dim=1).max()) + 2.0 ** -18 * float(want.abs().max())
+    assert float((both.detach().double() - want).abs().max()) <= bound
+    both.mean().backward()
+    assert all(torch.isfinite(p.grad).all() for p in m.parameters() if p.grad is not None)
+    assert float(m.mlm_head.predictions.bias.grad.abs().max()) > 0
+
+
+@pytest.mark.gpu
+def test_captured_training_step_with_the_head_in_pieces():
+    """Optimizer steps of the captured pre-training step equal the eager ones when the masked-token head runs in pieces and learns from
+    a teacher: losses, gradient norms and parameters."""
+    import copy
+    import train_graph_cases as cases
+    from gridmm_amd.pretrain_loop import PreTrainer, default_opts
+    from gridmm_amd.train_graph import GraphedTrainStep
+    model, batches = cases._setup(0.0)
+    model.config.mlm_in_pieces = True
+    batch = dict(batches["mlm"], **model.mlm_teacher(batches["mlm"], 8))
+    ma, mb = copy.deepcopy(model), copy.deepcopy(model)
+    ta, tb = PreTrainer(ma, default_opts(warmup_steps=10)), PreTrainer(mb, default_opts(warmup_steps=10))
+    for _ in range(2):                                   # what the graphed object runs while it is built: record + warm-up
+        ta.train_step(batch, "mlm")
+    g = GraphedTrainStep(tb, batch, "mlm")
+    for it in range(4):
+        cases._compare_step(ta, tb, lambda: ta.train_step(batch, "mlm"), g, it)
+
+
 # ---- refusals (no kernel runs) ----
 def test_refusals_on_the_cpu():
     from gridmm_amd import _lib, vocab
