@@ -17,11 +17,15 @@
 
 namespace {
 
-constexpr int T = 512;                 // threads
-constexpr int CUT = 2048;              // more entries than this: cut down to k
-constexpr int BUF = 2 * CUT;           // what does not fit is taken 4 values a thread at a time: 2048
 constexpr int BINS = 2048, DIGIT = 11;
-constexpr int PER = BUF / T;           // entries a thread holds during a selection
+// With T threads a workgroup:
+template <int T>
+struct Size {
+  static constexpr int CUT = 4 * T;      // more entries than this: cut down to k
+  static constexpr int BUF = 2 * CUT;    // what does not fit is taken 4 values a thread at a time
+  static constexpr int PER = BUF / T;    // entries a thread holds during a selection
+  static constexpr int OWN = BINS / T;   // bins a thread owns
+};
 constexpr int MAX_K = 1024;
 constexpr int GROUP = 4;               // chunks (of T vectors) read and looked at together
 enum { F32 = 0, BF16 = 1, F16 = 2 };
@@ -64,8 +68,9 @@ __device__ __forceinline__ unsigned wave_scan(unsigned v) {
   return v;
 }
 
+template <int T>
 struct Shared {
-  u64 buf[BUF];
+  u64 buf[Size<T>::BUF];
   unsigned hist[BINS];
   unsigned wsum[T / 64];
   unsigned n, bin, left, size, added[3];
@@ -73,26 +78,33 @@ struct Shared {
 
 // One digit of a radix selection: `count(add)` calls add(bin) for every entry that matches what is known; of the bins counted from the
 // largest down the one that holds the left-th entry is returned, and `left` becomes its place in that bin.
-template <class Count>
-__device__ __forceinline__ unsigned select_digit(Shared& sh, unsigned& left, bool& whole, Count count) {
+template <int T, class Count>
+__device__ __forceinline__ unsigned select_digit(Shared<T>& sh, unsigned& left, bool& whole, Count count) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  *reinterpret_cast<uint4*>(&sh.hist[tid * 4]) = make_uint4(0u, 0u, 0u, 0u);
+  constexpr int OWN = Size<T>::OWN;
+#pragma unroll
+  for (int b = 0; b < OWN; b += 4) *reinterpret_cast<uint4*>(&sh.hist[tid * OWN + b]) = make_uint4(0u, 0u, 0u, 0u);
   __syncthreads();
   count([&](unsigned bin) { atomicAdd(&sh.hist[bin], 1u); });
   __syncthreads();
-  // thread t owns the bins BINS - 4 t - 1 .. BINS - 4 t - 4
-  const uint4 c4 = *reinterpret_cast<const uint4*>(&sh.hist[BINS - 4 - tid * 4]);
-  const unsigned c[4] = {c4.w, c4.z, c4.y, c4.x};
-  const unsigned own = c[0] + c[1] + c[2] + c[3], incl = wave_scan(own);
+  // thread t owns the bins BINS - OWN t - 1 .. BINS - OWN (t + 1), in that order
+  unsigned c[OWN], own = 0;
+#pragma unroll
+  for (int b = 0; b < OWN; b += 4) {
+    const uint4 c4 = *reinterpret_cast<const uint4*>(&sh.hist[BINS - 4 - b - tid * OWN]);
+    c[b] = c4.w; c[b + 1] = c4.z; c[b + 2] = c4.y; c[b + 3] = c4.x;
+    own += c4.w + c4.z + c4.y + c4.x;
+  }
+  const unsigned incl = wave_scan(own);
   if (lane == 63) sh.wsum[wave] = incl;
   __syncthreads();
   unsigned before = incl - own;
 #pragma unroll
   for (int w = 0; w < T / 64; ++w) before += w < wave ? sh.wsum[w] : 0u;
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
+  for (int b = 0; b < OWN; ++b) {
     if (before < left && before + c[b] >= left) {
-      sh.bin = BINS - 1 - (tid * 4 + b);
+      sh.bin = BINS - 1 - (tid * OWN + b);
       sh.left = left - before;
       sh.size = c[b];
     }
@@ -107,7 +119,9 @@ __device__ __forceinline__ unsigned select_digit(Shared& sh, unsigned& left, boo
 // Of the n entries (of `bits` bits) in sh.buf keeps the k largest, in sh.buf[0, k) in any order, and sets sh.n = k; n > k.  Returns a
 // floor of what is kept: entries below it are not.  Called by all threads with the same n; entries of 0 are "nothing" and lose to
 // everything.
-__device__ u64 keep_largest(Shared& sh, int n, int k, int bits) {
+template <int T>
+__device__ u64 keep_largest(Shared<T>& sh, int n, int k, int bits) {
+  constexpr int PER = Size<T>::PER;
   const int tid = threadIdx.x, lane = tid & 63;
   u64 e[PER];
 #pragma unroll
@@ -158,8 +172,8 @@ __device__ u64 keep_largest(Shared& sh, int n, int k, int bits) {
 // The k largest of the n >= k entries of sh.buf, sorted, as values and ids: each entry's place is the number of larger ones.  n is at
 // most RANK_MOST or k.
 constexpr int RANK_MOST = 512;
-template <int DT>
-__device__ void write_sorted(Shared& sh, int n, int k, int id_bits, const void* logits, int64_t base, void* values, int64_t* ids,
+template <int DT, int T>
+__device__ void write_sorted(Shared<T>& sh, int n, int k, int id_bits, const void* logits, int64_t base, void* values, int64_t* ids,
                              int64_t at) {
   for (int i = threadIdx.x; i < n; i += T) sh.hist[i] = 0;
   __syncthreads();
@@ -189,12 +203,13 @@ __device__ __forceinline__ float2 join_sums(float2 a, float2 b) {       // (refe
   return make_float2(m, a.y * __builtin_amdgcn_exp2f((a.x - m) * LOG2E) + b.y * __builtin_amdgcn_exp2f((b.x - m) * LOG2E));
 }
 
-template <int DT>
+template <int DT, int T>
 __global__ __launch_bounds__(T, 4) void top_scan_kernel(const void* __restrict__ logits, int64_t ld, int V, int k, int id_bits, int segs, int cap,
                                                         u64* __restrict__ kept, float2* __restrict__ sums, void* __restrict__ values,
                                                         int64_t* __restrict__ ids, float* __restrict__ lse) {
   constexpr int E = DT == F32 ? 4 : 8;          // values in 16 bytes
-  __shared__ Shared sh;
+  constexpr int CUT = Size<T>::CUT, BUF = Size<T>::BUF;
+  __shared__ Shared<T> sh;
   __shared__ float2 wst[T / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t r = blockIdx.x / segs, seg = blockIdx.x % segs, base = r * ld;
@@ -430,18 +445,18 @@ __global__ __launch_bounds__(T, 4) void top_scan_kernel(const void* __restrict__
   for (int w = 0; w < T / 64; ++w) a = w ? join_sums(a, wst[w]) : wst[0];
   if (segs == 1) {
     if (tid == 0) lse[r] = fmaf(__builtin_amdgcn_logf(a.y), LN2, a.x);
-    write_sorted<DT>(sh, n, k, id_bits, logits, base, values, ids, r * k);
+    write_sorted<DT, T>(sh, n, k, id_bits, logits, base, values, ids, r * k);
   } else {
     if (tid == 0) sums[blockIdx.x] = a;
     for (int i = tid; i < cap; i += T) kept[(int64_t)blockIdx.x * cap + i] = i < n ? sh.buf[i] : 0;
   }
 }
 
-template <int DT>
+template <int DT, int T>
 __global__ __launch_bounds__(T) void top_join_kernel(const void* __restrict__ logits, int64_t ld, int k, int id_bits, int segs, int cap,
                                                      const u64* __restrict__ kept, const float2* __restrict__ sums,
                                                      void* __restrict__ values, int64_t* __restrict__ ids, float* __restrict__ lse) {
-  __shared__ Shared sh;
+  __shared__ Shared<T> sh;
   const int64_t r = blockIdx.x;
   int n = segs * cap;
   for (int i = threadIdx.x; i < n; i += T) sh.buf[i] = kept[r * n + i];
@@ -455,18 +470,24 @@ __global__ __launch_bounds__(T) void top_join_kernel(const void* __restrict__ lo
     keep_largest(sh, n, k, id_bits + (DT == F32 ? 32 : 16));
     n = k;
   }
-  write_sorted<DT>(sh, n, k, id_bits, logits, r * ld, values, ids, r * k);
+  write_sorted<DT, T>(sh, n, k, id_bits, logits, r * ld, values, ids, r * k);
 }
 
-// segments a row: enough workgroups for the chip (two a CU), none shorter than a chunk, their survivors no more than the buffer
+// Threads a workgroup: 256 where the rows fill the chip four times over (four rows a CU in different phases: 302 against 326 us at 4096 x
+// 131072 bf16, 38 : 73 at 4096 x 2000), else 512 (20.6 : 33.7 at 384 x 30522 fp32); 512 also where k is more than a quarter of
+// the vectors that the floor comes from.
+int threads(int rows, int k) { return rows >= 1024 && k <= 256 ? 256 : 512; }
+// segments a row: a workgroup a CU (one segment and no join at 384 rows: 20.6 us, two: 27.5), none shorter than 4096 values, their
+// survivors no more than the joining workgroup's buffer
+constexpr int JOIN_T = 512;
 int segments(int rows, int vocab, int k) {
-  int64_t s = (512 + rows - 1) / rows;
-  s = s < (vocab + 4095) / 4096 ? s : (vocab + 4095) / 4096;
-  s = s < BUF / k ? s : BUF / k;
+  int64_t s = (256 + rows - 1) / rows;
+  s = std::min<int64_t>(s, (vocab + 4095) / 4096);
+  s = std::min<int64_t>(s, Size<JOIN_T>::BUF / k);
   return s < 1 ? 1 : (int)s;
 }
 // entries a segment may hand over: what it holds is cut down to k only if it is more than this
-int handed(int segs, int k) { return std::min(BUF / segs, 4 * k); }
+int handed(int segs, int k) { return std::min(Size<JOIN_T>::BUF / segs, 4 * k); }
 
 }  // namespace
 
@@ -494,11 +515,17 @@ extern "C" int gridmm_top_logits(const void* logits, int64_t ld, int dtype, int 
   float2* sums = (float2*)(kept + (size_t)rows * segs * cap);
   auto run = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    GRIDMM_LAUNCH((top_scan_kernel<DT>), dim3((unsigned)(rows * segs)), dim3(T), 0, st, logits, ld, vocab, k, id_bits, segs, cap, kept, sums,
-                  values, ids, lse);
+    auto scan = [&](auto t) {
+      constexpr int T = decltype(t)::value;
+      GRIDMM_LAUNCH((top_scan_kernel<DT, T>), dim3((unsigned)(rows * segs)), dim3(T), 0, st, logits, ld, vocab, k, id_bits, segs, cap,
+                    kept, sums, values, ids, lse);
+    };
+    if (threads(rows, k) == 256) scan(std::integral_constant<int, 256>{});
+    else scan(std::integral_constant<int, 512>{});
     GRIDMM_CHECK_LAUNCH();
     if (segs > 1) {
-      GRIDMM_LAUNCH((top_join_kernel<DT>), dim3(rows), dim3(T), 0, st, logits, ld, k, id_bits, segs, cap, kept, sums, values, ids, lse);
+      GRIDMM_LAUNCH((top_join_kernel<DT, JOIN_T>), dim3(rows), dim3(JOIN_T), 0, st, logits, ld, k, id_bits, segs, cap, kept, sums, values,
+                    ids, lse);
       GRIDMM_CHECK_LAUNCH();
     }
     return GRIDMM_OK;
