@@ -1,10 +1,11 @@
-// The vocabulary losses for few rows (vocab_loss.hip takes it up to FEW_ROWS rows): a handful of tokens against the whole vocabulary
-// is bound by the read of W and, backward, the write of dW; tiles of 128 rows, packed copies and a dozen launches cost more than the
-// work.  Two launches forward, three backward, rows where they lie, nothing packed:
-//   few_scores   16 vocabulary rows a wave, RT tiles of 16 rows of h: each W value is loaded once, straight into the fragment layout
+// The vocabulary losses for few rows, and for small products of any number of rows (few_rows() in vocab_loss.hip): a handful of tokens
+// against the whole vocabulary is bound by the read of W and, backward, the write of dW, a small head by its launches; tiles of 128
+// rows, packed copies and a dozen launches cost more than the work.  Two launches forward, three backward, rows where they lie,
+// nothing packed.  Rows go in groups of RP = 16 RT:
+//   few_scores   16 vocabulary rows a wave, a group's RT tiles of 16 rows of h: each W value is loaded once, straight into the fragment layout
 //                of the 16x16 matrix instructions (fp32: 16x16x4 fp32, products and sums in fp32; 16 bits: 16x16x32, products exact).
 //                Forward: each row's (maximum, sum of exponentials) of the workgroup's 64 columns, and the targets' scores.
-//                Backward: the same scores again -> dS [vocabulary][rows] in fp32
+//                Backward: the same scores again -> dS [group][vocabulary][RP] in fp32
 //   few_loss     joins the statistics, the teacher's softmax, the losses
 //   few_products dh = dS W over ranges of the vocabulary and dW = dS^T h, db, on the fp32 matrix instruction (16-bit operands are
 //                widened: exact), as two kinds of workgroups of one launch
@@ -23,14 +24,16 @@ struct FewArgs {
   int64_t ldh, ldw, ld_index, ld_teacher, ignore;
   int rows, vocab, K, slots, wide, dtype, bias_dtype, kd;
   float inv_t, unit, temperature;
-  float2* stats;                 // [workgroup][RP]
-  float *lse, *zt, *p, *flag;    // saved: [RP], [rows][slots], [rows][slots], [RP]: 1 for rows that count
+  float2* stats;                 // [workgroup][groups RP]
+  float *lse, *zt, *p, *flag;    // saved: [groups RP], [rows][slots], [rows][slots], [groups RP]: 1 for rows that count
   float* loss;
   const float* grad;
   int64_t grad_stride;
-  float *dS, *part;              // [vocab up to 64][RP], [ranges][RP][K up to 4]
+  float *dS, *part;              // [group][vocab up to 64][RP], [ranges][groups RP][K up to 4]
   void *dh, *dW, *db;
   int ranges, range;             // of the vocabulary in dh, rows a range (a multiple of 4)
+  int groups;
+  int64_t group_dS;              // values of dS a group
 };
 
 template <int DT>
@@ -73,16 +76,16 @@ __device__ __forceinline__ vocab::s16x8_t few_load8(const void* p, int64_t off, 
   return v;
 }
 
-// Scores of the wave's 16 vocabulary rows from j0 on: lane l has rows of h 16 t + (l & 15), columns j0 + 4 (l >> 4) + i, base 2, bias
+// Scores of the wave's 16 vocabulary rows from j0 on: lane l has rows of h r0 + 16 t + (l & 15), columns j0 + 4 (l >> 4) + i, base 2, bias
 // in; -inf past the vocabulary.
 template <int DT, int RT, bool VEC>
-__device__ __forceinline__ void few_tile(const FewArgs& a, int64_t j0, f32x4_t (&acc)[RT]) {
+__device__ __forceinline__ void few_tile(const FewArgs& a, int r0, int64_t j0, f32x4_t (&acc)[RT]) {
   const int lane = threadIdx.x & 63, l15 = lane & 15, g = lane >> 4;
   const int64_t j = j0 + l15 < a.vocab ? j0 + l15 : a.vocab - 1;
   int64_t ho[RT];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
-    const int r = t * 16 + l15;
+    const int r = r0 + t * 16 + l15;
     ho[t] = (int64_t)(r < a.rows ? r : a.rows - 1) * a.ldh;
     acc[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   }
@@ -129,8 +132,17 @@ __device__ __forceinline__ void few_tile(const FewArgs& a, int64_t j0, f32x4_t (
   }
 }
 
-__device__ __forceinline__ bool few_counts(const FewArgs& a, int r) {       // cross entropy: known from the label
-  return load_index(a.index, r * a.ld_index, a.wide) != a.ignore;
+// f(slot, d) for the targets of row r among the 4 columns from jl on, in the order of the slots; 8 of them loaded at a time
+template <class F>
+__device__ __forceinline__ void few_targets(const FewArgs& a, int64_t r, int64_t jl, F f) {
+  for (int k0 = 0; k0 < a.slots; k0 += 8) {
+    int64_t d[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) d[u] = load_index(a.index, r * a.ld_index + (k0 + u < a.slots ? k0 + u : a.slots - 1), a.wide) - jl;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (k0 + u < a.slots && (uint64_t)d[u] < 4) f(k0 + u, (int)d[u]);
+  }
 }
 
 // VEC: the rows of h and W are whole 16-byte vectors on their boundaries (decided once a call: a choice at each load would wait for it)
@@ -141,11 +153,12 @@ __global__ __launch_bounds__(256) void few_scores_kernel(const FewArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
   const int64_t j0 = (int64_t)blockIdx.x * 64 + wave * 16, jl = j0 + 4 * g;
   f32x4_t y[RT];
-  few_tile<DT, RT, VEC>(a, j0, y);
+  const int r0 = blockIdx.y * RP;
+  few_tile<DT, RT, VEC>(a, r0, j0, y);
   if constexpr (!GRAD) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const int r = t * 16 + l15;
+      const int r = r0 + t * 16 + l15;
       float m = fmaxf(fmaxf(y[t][0], y[t][1]), fmaxf(y[t][2], y[t][3]));
       m = fmaxf(m, __shfl_xor(m, 16, 64));
       m = fmaxf(m, __shfl_xor(m, 32, 64));
@@ -155,38 +168,35 @@ __global__ __launch_bounds__(256) void few_scores_kernel(const FewArgs a) {
       for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f(y[t][i] - ref);
       s += __shfl_xor(s, 16, 64);
       s += __shfl_xor(s, 32, 64);
-      if (g == 0) wst[wave][r] = make_float2(m, s);
+      if (g == 0) wst[wave][t * 16 + l15] = make_float2(m, s);
       if (r < a.rows)                           // the scores at the row's targets
-        for (int k = 0; k < a.slots; ++k) {
-          const int64_t d = load_index(a.index, r * a.ld_index + k, a.wide) - jl;
-          if (d >= 0 && d < 4 && jl + d < a.vocab) a.zt[(int64_t)r * a.slots + k] = d < 2 ? (d == 0 ? y[t][0] : y[t][1]) : (d == 2 ? y[t][2] : y[t][3]);
-        }
+        few_targets(a, r, jl, [&](int k, int d) {
+          if (jl + d < a.vocab) a.zt[(int64_t)r * a.slots + k] = d < 2 ? (d == 0 ? y[t][0] : y[t][1]) : (d == 2 ? y[t][2] : y[t][3]);
+        });
     }
     __syncthreads();
     for (int r = threadIdx.x; r < RP; r += 256) {
       float2 s = wst[0][r];
 #pragma unroll
       for (int w = 1; w < 4; ++w) s = join_stats(s, wst[w][r]);
-      a.stats[(int64_t)blockIdx.x * RP + r] = s;
+      a.stats[((int64_t)blockIdx.x * a.groups + blockIdx.y) * RP + r] = s;
     }
   } else {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      const int r = t * 16 + l15;
+      const int r = r0 + t * 16 + l15;
       const bool live = r < a.rows && a.flag[r] != 0.f;
       const float gt = live ? a.grad[r * a.grad_stride] * a.temperature : 0.f, L = live ? a.lse[r] : 0.f;
       float p[4] = {0.f, 0.f, 0.f, 0.f};
       if (live)
-        for (int k = 0; k < a.slots; ++k) {
-          const int64_t d = load_index(a.index, r * a.ld_index + k, a.wide) - jl;
-          if (d < 0 || d >= 4) continue;
+        few_targets(a, r, jl, [&](int k, int d) {
           const float q = a.kd ? a.p[(int64_t)r * a.slots + k] : 1.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[i] += d == i ? q : 0.f;
-        }
+        });
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        a.dS[(jl + i) * RP + r] = live ? gt * (__builtin_amdgcn_exp2f(y[t][i] - L) - p[i]) : 0.f;
+        a.dS[blockIdx.y * a.group_dS + (jl + i) * RP + t * 16 + l15] = live ? gt * (__builtin_amdgcn_exp2f(y[t][i] - L) - p[i]) : 0.f;
     }
   }
 }
@@ -196,7 +206,7 @@ __global__ __launch_bounds__(256) void few_loss_kernel(const FewArgs a, int64_t 
   __shared__ float2 part[4];
   const int r = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float2 s = make_float2(-INFINITY, 0.f);
-  for (int64_t t = threadIdx.x; t < tiles; t += 256) s = join_stats(s, a.stats[t * RP + r]);
+  for (int64_t t = threadIdx.x; t < tiles; t += 256) s = join_stats(s, a.stats[t * a.groups * RP + r]);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s = join_stats(s, make_float2(__shfl_xor(s.x, o, 64), __shfl_xor(s.y, o, 64)));
   if (lane == 0) part[wave] = s;
@@ -244,7 +254,8 @@ __global__ __launch_bounds__(256) void few_products_kernel(const FewArgs a, int 
   const int perm = 4 * (l15 & 3) + (l15 >> 2);
   if ((int)blockIdx.x < h_blocks) {
     // dh: 256 columns a workgroup, 64 a wave; lane l ends with row 16 t + l15, columns k0 + 16 i + 4 g + e
-    const int ranges = h_blocks / k_blocks, range = blockIdx.x % ranges, k0 = blockIdx.x / ranges * 256 + wave * 64;
+    const int range = blockIdx.x % a.ranges, q = blockIdx.x / a.ranges, group = q / k_blocks, k0 = q % k_blocks * 256 + wave * 64;
+    const float* dS = a.dS + group * a.group_dS;
     const int64_t j0 = (int64_t)range * a.range, j1 = j0 + a.range < a.vocab ? j0 + a.range : a.vocab;
     if (k0 >= a.K) return;
     f32x4_t acc[4][RT];
@@ -261,7 +272,7 @@ __global__ __launch_bounds__(256) void few_products_kernel(const FewArgs a, int 
         const int64_t j = jb + 4 * u + g, jj = j < j1 ? j : j1 - 1;
         w[u] = few_load4<DT, VEC>(a.weight, jj * a.ldw, k0 + 4 * perm, a.K);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) s[u][t] = a.dS[jj * RP + t * 16 + l15];
+        for (int t = 0; t < RT; ++t) s[u][t] = dS[jj * RP + t * 16 + l15];
       }
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -279,44 +290,40 @@ __global__ __launch_bounds__(256) void few_products_kernel(const FewArgs a, int 
       for (int i = 0; i < 4; ++i) {
         const int k = k0 + 16 * i + 4 * g;
         if (k < a.K)
-          *reinterpret_cast<float4*>(a.part + ((int64_t)range * RP + t * 16 + l15) * Kq + k) =
+          *reinterpret_cast<float4*>(a.part + (((int64_t)range * a.groups + group) * RP + t * 16 + l15) * Kq + k) =
               make_float4(acc[0][t][i], acc[1][t][i], acc[2][t][i], acc[3][t][i]);
       }
     return;
   }
   // dW: 16 vocabulary rows a workgroup, every fourth run of 64 columns a wave; lane l ends with row j0 + l15, columns k0 + 16 i + 4 g + e
   const int64_t j = ((int64_t)blockIdx.x - h_blocks) * 16 + l15;      // (dS has rows up to a multiple of 64)
-  float s[4 * RT];
-#pragma unroll
-  for (int q = 0; q < 4 * RT; ++q) s[q] = a.dS[j * RP + 4 * q + g];
   if (a.db && wave == 0) {
     float sum = 0.f;
+    for (int group = 0; group < a.groups; ++group)
 #pragma unroll
-    for (int q = 0; q < 4 * RT; ++q) sum += s[q];
+      for (int q = 0; q < 4 * RT; ++q) sum += a.dS[group * a.group_dS + j * RP + 4 * q + g];
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
     if (g == 0 && j < a.vocab) store_as(a.db, j, a.bias_dtype, sum);
   }
   if (!a.dW) return;
-  bool in[4 * RT];
-  int64_t ho[4 * RT];
-#pragma unroll
-  for (int q = 0; q < 4 * RT; ++q) {
-    const int r = 4 * q + g;
-    in[q] = r < a.rows && a.flag[r] != 0.f;
-    ho[q] = in[q] ? r * a.ldh : 0;
-  }
   for (int k0 = wave * 64; k0 < a.K; k0 += 256) {
     f32x4_t acc[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    for (int group = 0; group < a.groups; ++group) {
+      const int r0 = group * RP;
+      const float* dS = a.dS + group * a.group_dS + j * RP;
 #pragma unroll
-    for (int q = 0; q < 4 * RT; ++q) {
-      if (4 * q >= a.rows) break;
-      few_f4 h = few_load4<DT, VEC>(a.hidden, ho[q], k0 + 4 * perm, a.K);
-      if (!in[q]) h = (few_f4){0.f, 0.f, 0.f, 0.f};
+      for (int q = 0; q < 4 * RT; ++q) {
+        const int r = r0 + 4 * q + g;
+        const bool in = r < a.rows && a.flag[r] != 0.f;
+        few_f4 h = few_load4<DT, VEC>(a.hidden, in ? r * a.ldh : 0, k0 + 4 * perm, a.K);
+        if (!in) h = (few_f4){0.f, 0.f, 0.f, 0.f};
+        const float s = dS[4 * q + g];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(h[e], s[q], acc[e], 0, 0, 0);
+        for (int e = 0; e < 4; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(h[e], s, acc[e], 0, 0, 0);
+      }
     }
     if (j >= a.vocab) continue;
 #pragma unroll
@@ -351,7 +358,7 @@ __global__ __launch_bounds__(256) void few_hidden_kernel(const FewArgs a, int RP
   if (k < a.K) {
 #pragma unroll 4
     for (int s = sp; s < a.ranges; s += 16) {
-      const float4 x = *reinterpret_cast<const float4*>(a.part + ((int64_t)s * RP + r) * Kq + k);
+      const float4 x = *reinterpret_cast<const float4*>(a.part + ((int64_t)s * a.groups * RP + r) * Kq + k);
       v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
     }
   }

@@ -830,11 +830,19 @@ inline size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 // Up to this many rows the kernels of vocab_few.h.  Forward and backward, us, them against the others: fp32 131072 x 2048, 32 rows 1500 : 2300;
 // bf16 5 rows 530 : 731, 32 rows 860 : 736; 30522 x 768 at one row, forward, fp32 41 : 90.
 constexpr int FEW_ROWS_F32 = 32, FEW_ROWS_16 = 16;
+// and for products of at most this many operations, and target comparisons, whatever the rows.  Forward and backward of 6000 x 512 fp32 at
+// 48, 128, 400 rows (0.3, 0.8, 2.5e9), device us: 71, 118, 265 against 96, 99, 116, and 5 launches against 12 (~4 us of the host each)
+constexpr double FEW_OPS = 6e8, FEW_TARGETS = 1e8;
+bool few_rows(const gridmm_vocab_loss_t* d) {
+  const double rv = (double)d->rows * d->vocab;
+  return d->rows <= (d->dtype == F32 ? FEW_ROWS_F32 : FEW_ROWS_16) ||
+         (2. * rv * d->hidden_size <= FEW_OPS && rv * d->slots <= FEW_TARGETS);
+}
 
 struct Plan {
   int PL, slots;               // planes; target slots a row (cross entropy: 1)
   bool few;
-  int RP, ranges, range;       // few rows: rows padded to 16 or 32; ranges of the vocabulary in dh and their rows
+  int RP, groups, ranges, range;      // few rows: rows a group (16 or 32), groups; ranges of the vocabulary in dh and their rows
   int64_t Rp, Kp, Vp;
   bool pack_w;                 // W has to be split or padded; else it is read where it lies
   bool keep_w;                 // ... and its copy, one piece, stays for the backward (28 us of 396 at 30522 x 768 fp32)
@@ -873,27 +881,30 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.C_bwd = piece(std::max<int64_t>(P.Rp, 1) * 2 * P.PL);
   P.keep_w = P.pack_w && P.C_fwd == P.Vp;
   if (P.pack_w) P.C_bwd = std::min(P.C_bwd, P.C_fwd);
-  P.few = d->rows <= (d->dtype == F32 ? FEW_ROWS_F32 : FEW_ROWS_16);
+  P.few = few_rows(d);
   if (P.few) {
     P.RP = d->rows <= 16 ? 16 : 32;
-    // dh: four workgroups of 256 columns a CU (512, 1024, 2048 of them: 348, 238, 240 us at 131072 x 2048 fp32), at least 64 vocabulary rows a range
-    const int64_t kb = (d->hidden_size + 255) / 256, n = std::max<int64_t>(1, std::min<int64_t>((1024 + kb - 1) / kb, d->vocab / 64));
+    P.groups = std::max(1, (d->rows + P.RP - 1) / P.RP);
+    // dh: four workgroups of 256 columns a CU (512, 1024, 2048 of them: 348, 238, 240 us at 131072 x 2048 fp32), at least 64
+    // vocabulary rows a range
+    const int64_t kb = (int64_t)((d->hidden_size + 255) / 256) * P.groups;
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>((1024 + kb - 1) / kb, d->vocab / 64));
     P.range = (int)up((d->vocab + n - 1) / n, 4);
     P.ranges = (d->vocab + P.range - 1) / P.range;
     size_t o = 0;
     auto take = [&](size_t bytes) { const size_t at = o; o += up(bytes, 256); return at; };
-    const size_t V64 = up(d->vocab, 64), S = (size_t)d->rows * P.slots;
-    P.o_lse = take(P.RP * 4);
-    P.o_meta = take(P.RP * 4);                       // 1 for rows that count
+    const size_t V64 = up(d->vocab, 64), S = (size_t)d->rows * P.slots, GR = (size_t)P.groups * P.RP;
+    P.o_lse = take(GR * 4);
+    P.o_meta = take(GR * 4);                         // 1 for rows that count
     P.o_zt = take(S * 4);
     P.o_p = take(d->slots ? S * 4 : 0);
     P.saved = o;
     o = 0;
-    P.f_stats = take(V64 / 64 * P.RP * 8);
+    P.f_stats = take(V64 / 64 * GR * 8);
     P.fwd = o;
     o = 0;
-    P.b_ds = take(V64 * P.RP * 4);
-    P.b_part = take((size_t)P.ranges * P.RP * up(d->hidden_size, 4) * 4);
+    P.b_ds = take(V64 * GR * 4);
+    P.b_part = take((size_t)P.ranges * GR * up(d->hidden_size, 4) * 4);
     P.bwd = o;
     return true;
   }
@@ -1009,7 +1020,8 @@ FewArgs few_args(const gridmm_vocab_loss_t* d, const Plan& P, const void* saved)
   a.inv_t = 1.f / d->temperature; a.unit = a.inv_t * LOG2E; a.temperature = d->temperature;
   a.lse = (float*)(sv + P.o_lse); a.flag = (float*)(sv + P.o_meta); a.zt = (float*)(sv + P.o_zt);
   a.p = d->slots ? (float*)(sv + P.o_p) : nullptr;
-  a.ranges = P.ranges; a.range = P.range;
+  a.ranges = P.ranges; a.range = P.range; a.groups = P.groups;
+  a.group_dS = (int64_t)up(d->vocab, 64) * P.RP;
   return a;
 }
 
@@ -1040,7 +1052,7 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
     a.loss = loss;
     const int tiles = (d->vocab + 63) / 64;
     const int rc = by_few(d, P, [&](auto dt, auto rt, auto vec) {
-      GRIDMM_LAUNCH((few_scores_kernel<decltype(dt)::value, decltype(rt)::value, decltype(vec)::value, false>), dim3(tiles), dim3(256), 0, st, a);
+      GRIDMM_LAUNCH((few_scores_kernel<decltype(dt)::value, decltype(rt)::value, decltype(vec)::value, false>), dim3(tiles, P.groups), dim3(256), 0, st, a);
       GRIDMM_CHECK_LAUNCH();
       return GRIDMM_OK;
     });
@@ -1138,9 +1150,9 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
     a.dS = (float*)(ws + P.b_ds); a.part = (float*)(ws + P.b_part);
     a.dh = d_hidden; a.dW = d_weight; a.db = d_bias;
     const int tiles = (d->vocab + 63) / 64, kb = (d->hidden_size + 255) / 256;
-    const int hb = d_hidden ? kb * P.ranges : 0, wb = d_weight || d_bias ? (d->vocab + 15) / 16 : 0;
+    const int hb = d_hidden ? kb * P.ranges * P.groups : 0, wb = d_weight || d_bias ? (d->vocab + 15) / 16 : 0;
     const int rc = by_few(d, P, [&](auto dt, auto rt, auto vec) {
-      GRIDMM_LAUNCH((few_scores_kernel<decltype(dt)::value, decltype(rt)::value, decltype(vec)::value, true>), dim3(tiles), dim3(256), 0, st, a);
+      GRIDMM_LAUNCH((few_scores_kernel<decltype(dt)::value, decltype(rt)::value, decltype(vec)::value, true>), dim3(tiles, P.groups), dim3(256), 0, st, a);
       GRIDMM_CHECK_LAUNCH();
       GRIDMM_LAUNCH((few_products_kernel<decltype(dt)::value, decltype(rt)::value, decltype(vec)::value>), dim3(hb + wb), dim3(256), 0, st, a, hb, kb);
       GRIDMM_CHECK_LAUNCH();

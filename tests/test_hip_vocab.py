@@ -125,6 +125,18 @@ def test_cross_entropy_and_its_gradients(dtype, R, V, K, bias):
     _check_ce(h, w, b, labels.cuda(), (torch.rand(R, generator=g) - 0.3).cuda())
 
 
+# over 6e8 operations and 32 rows: the kernels on packed tiles (the smaller ones above take those for few rows)
+CE_TILES = [("fp32", 33, 30011, 320), ("bf16", 17, 40000, 513), ("fp16", 129, 4099, 600), ("fp32", 257, 1300, 1000), ("bf16", 511, 3001, 264),
+            ("fp16", 1025, 1025, 320), ("fp32", 700, 20001, 33), ("bf16", 2000, 700, 256), ("fp16", 300, 33000, 65), ("fp32", 129, 3000, 800)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,R,V,K", CE_TILES)
+@pytest.mark.parametrize("bias", [False, True])
+def test_cross_entropy_on_tiles(dtype, R, V, K, bias):
+    test_cross_entropy_and_its_gradients(dtype, R, V, K, bias)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("drop", [0.0, 0.98])
@@ -139,8 +151,9 @@ def test_cross_entropy_over_several_pieces(dtype, drop):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
-def test_cross_entropy_of_rows_that_are_all_ignored(dtype):
-    h, w, b, _ = _inputs(dtype, 70, 300, 64)
+@pytest.mark.parametrize("V,K", [(300, 64), (30000, 192)])
+def test_cross_entropy_of_rows_that_are_all_ignored(dtype, V, K):
+    h, w, b, _ = _inputs(dtype, 70, V, K)
     h[3] = float("nan")                            # an ignored row's values are never read into a result
     got = _run_ce(h, w, b, torch.full((70,), -100, device="cuda"), torch.ones(70, device="cuda"), ignore=-100)
     for v in got.values():
@@ -148,9 +161,10 @@ def test_cross_entropy_of_rows_that_are_all_ignored(dtype):
 
 
 @pytest.mark.gpu
-def test_ignored_rows_may_hold_anything():
-    h, w, b, g = _inputs("fp32", 40, 500, 64)
-    labels = torch.randint(0, 500, (40,), generator=g).cuda()
+@pytest.mark.parametrize("V,K", [(500, 64), (40000, 256)])
+def test_ignored_rows_may_hold_anything(V, K):
+    h, w, b, g = _inputs("fp32", 40, V, K)
+    labels = torch.randint(0, V, (40,), generator=g).cuda()
     labels[::3] = -1
     clean = _run_ce(h, w, b, labels, torch.ones(40, device="cuda"))
     h[0], h[3] = float("nan"), 3.0e38
@@ -162,9 +176,9 @@ def test_ignored_rows_may_hold_anything():
 @pytest.mark.gpu
 @pytest.mark.parametrize("index", [torch.int64, torch.int32])
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
-def test_cross_entropy_of_strided_operands(dtype, index):
+@pytest.mark.parametrize("R,V,K", [(50, 333, 64), (200, 12001, 128)])
+def test_cross_entropy_of_strided_operands(dtype, index, R, V, K):
     """Rows of a wider matrix, off a 16-byte boundary; a transposed weight; a batch of sequences."""
-    R, V, K = 50, 333, 64
     g = torch.Generator().manual_seed(3)
     big = torch.randn(R, K + 19, generator=g).to(DT[dtype]).cuda()
     wt = (torch.randn(K, V, generator=g) / 4).to(DT[dtype]).cuda()
@@ -175,15 +189,16 @@ def test_cross_entropy_of_strided_operands(dtype, index):
         _check_ce(h, w, None, labels, gr)
     from gridmm_amd import vocab
     w = wt.t().contiguous()
-    h3 = big[:, :K].contiguous().view(5, 10, K)
-    a = vocab.vocab_cross_entropy(h3, w, labels.view(5, 10))
-    assert a.shape == (5, 10) and torch.equal(a.view(-1), vocab.vocab_cross_entropy(h3.reshape(R, K), w, labels))
+    h3 = big[:, :K].contiguous().view(5, R // 5, K)
+    a = vocab.vocab_cross_entropy(h3, w, labels.view(5, R // 5))
+    assert a.shape == (5, R // 5) and torch.equal(a.view(-1), vocab.vocab_cross_entropy(h3.reshape(R, K), w, labels))
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
-def test_bias_of_minus_infinity_masks_a_column(dtype):
-    h, w, b, g = _inputs(dtype, 33, 600, 64)
+@pytest.mark.parametrize("V,K", [(600, 64), (40000, 256)])
+def test_bias_of_minus_infinity_masks_a_column(dtype, V, K):
+    h, w, b, g = _inputs(dtype, 33, V, K)
     labels = torch.randint(0, 300, (33,), generator=g).cuda()
     b[300:] = float("-inf")                        # whole tiles without a live column
     w[400] = 60.0
@@ -200,32 +215,34 @@ def test_bias_of_minus_infinity_masks_a_column(dtype):
 
 
 @pytest.mark.gpu
-def test_a_label_outside_the_vocabulary_spoils_its_row_and_nothing_else():
-    h, w, b, g = _inputs("fp32", 20, 100, 64)
-    labels = torch.randint(0, 100, (20,), generator=g).cuda()
-    good = _run_ce(h, w, b, labels, torch.ones(20, device="cuda"))
-    for bad in (100, -2, 2 ** 31 - 1, -2 ** 40):
+@pytest.mark.parametrize("R,V,K", [(20, 100, 64), (40, 40000, 256)])
+def test_a_label_outside_the_vocabulary_spoils_its_row_and_nothing_else(R, V, K):
+    h, w, b, g = _inputs("fp32", R, V, K)
+    labels = torch.randint(0, V, (R,), generator=g).cuda()
+    good = _run_ce(h, w, b, labels, torch.ones(R, device="cuda"))
+    for bad in (V, -2, 2 ** 31 - 1, -2 ** 40):
         lab = labels.clone()
         lab[7] = bad
-        got = _run_ce(h, w, b, lab, torch.ones(20, device="cuda"))
-        keep = torch.arange(20, device="cuda") != 7
+        got = _run_ce(h, w, b, lab, torch.ones(R, device="cuda"))
+        keep = torch.arange(R, device="cuda") != 7
         assert bool(torch.isnan(got["loss"][7])) and torch.equal(got["loss"][keep], good["loss"][keep])
         assert bool(torch.isnan(got["d_hidden"][7]).all()) and torch.equal(got["d_hidden"][keep], good["d_hidden"][keep])
         assert bool(torch.isnan(got["d_bias"]).all())
 
 
 @pytest.mark.gpu
-def test_a_row_of_nan_or_infinity_stays_its_own():
+@pytest.mark.parametrize("R,V,K", [(20, 100, 64), (40, 40000, 256)])
+def test_a_row_of_nan_or_infinity_stays_its_own(R, V, K):
     for bad in (float("nan"), float("inf")):
-        h, w, b, g = _inputs("fp32", 20, 100, 64)
-        labels = torch.randint(0, 100, (20,), generator=g).cuda()
-        good = _run_ce(h, w, b, labels, torch.ones(20, device="cuda"))
+        h, w, b, g = _inputs("fp32", R, V, K)
+        labels = torch.randint(0, V, (R,), generator=g).cuda()
+        good = _run_ce(h, w, b, labels, torch.ones(R, device="cuda"))
         h[5, 3] = bad
-        got = _run_ce(h, w, b, labels, torch.ones(20, device="cuda"))
-        keep = torch.arange(20, device="cuda") != 5
+        got = _run_ce(h, w, b, labels, torch.ones(R, device="cuda"))
+        keep = torch.arange(R, device="cuda") != 5
         assert bool(torch.isnan(got["loss"][5]))
         scale = good["loss"][keep].abs().max()
-        assert float((got["loss"][keep] - good["loss"][keep]).abs().max()) <= 8 * U * 64 * float(scale + 8)
+        assert float((got["loss"][keep] - good["loss"][keep]).abs().max()) <= 8 * U * K * float(scale + 8)
 
 
 def _kd_inputs(dtype, R, V, K, S, seed):
@@ -252,7 +269,8 @@ def _check_kd(h, w, b, ids, t, g, T):
         _hold(got[k], v, k)
 
 
-KD = [("fp32", 1, 1, 64, 1, 1.0), ("fp32", 5, 300, 64, 8, 2.0), ("bf16", 130, 1000, 128, 32, 1.0), ("fp16", 77, 513, 72, 100, 0.5),
+KD = [("fp32", 300, 9001, 130, 17, 2.0), ("bf16", 200, 20001, 128, 300, 1.0), ("fp16", 1030, 2500, 200, 5, 0.5), ("fp32", 60, 30522, 256, 64, 1.0),
+      ("fp32", 1, 1, 64, 1, 1.0), ("fp32", 5, 300, 64, 8, 2.0), ("bf16", 130, 1000, 128, 32, 1.0), ("fp16", 77, 513, 72, 100, 0.5),
       ("fp32", 300, 2000, 100, 17, 4.0), ("bf16", 3, 40000, 64, 256, 1.5), ("fp32", 64, 256, 64, 256, 1.0)]
 
 
@@ -269,21 +287,23 @@ def test_distillation_and_its_gradients(dtype, R, V, K, S, T):
 
 
 @pytest.mark.gpu
-def test_distillation_where_ids_repeat_and_are_int32_columns_of_a_wider_table():
-    h, w, b, ids, t, g = _kd_inputs("fp32", 40, 90, 64, 12, seed=1)
+@pytest.mark.parametrize("V,K", [(90, 64), (40000, 256)])
+def test_distillation_where_ids_repeat_and_are_int32_columns_of_a_wider_table(V, K):
+    h, w, b, ids, t, g = _kd_inputs("fp32", 40, V, K, 12, seed=1)
     ids = torch.randint(0, 5, (40, 15), generator=g)
     t = torch.randn(40, 20, generator=g)
     _check_kd(h, w, b, ids.int().cuda()[:, 2:14], t.cuda()[:, 3:15], torch.rand(40, generator=g).cuda(), 1.0)
 
 
 @pytest.mark.gpu
-def test_distillation_of_an_id_past_the_vocabulary():
+@pytest.mark.parametrize("R,V,K", [(10, 300, 64), (40, 40000, 256)])
+def test_distillation_of_an_id_past_the_vocabulary(R, V, K):
     from gridmm_amd import vocab
-    h, w, b, ids, t, g = _kd_inputs("bf16", 10, 300, 64, 4, seed=1)
+    h, w, b, ids, t, g = _kd_inputs("bf16", R, V, K, 4, seed=1)
     good = vocab.vocab_distillation(h, w, ids.cuda(), t.cuda(), bias=b)
-    ids[4, 2] = 300
+    ids[4, 2] = V
     got = vocab.vocab_distillation(h, w, ids.cuda(), t.cuda(), bias=b)
-    keep = torch.arange(10, device="cuda") != 4
+    keep = torch.arange(R, device="cuda") != 4
     assert bool(torch.isnan(got[4])) and torch.equal(got[keep], good[keep])
 
 
@@ -328,11 +348,12 @@ def test_gradients_against_differences(dtype):
 
 
 @pytest.mark.gpu
-def test_only_the_gradients_that_are_asked_for():
+@pytest.mark.parametrize("R,V,K", [(30, 400, 64), (40, 40000, 256)])
+def test_only_the_gradients_that_are_asked_for(R, V, K):
     from gridmm_amd import vocab
-    h, w, b, g = _inputs("fp32", 30, 400, 64)
-    labels = torch.randint(0, 400, (30,), generator=g).cuda()
-    full = _run_ce(h, w, b, labels, torch.ones(30, device="cuda"))
+    h, w, b, g = _inputs("fp32", R, V, K)
+    labels = torch.randint(0, V, (R,), generator=g).cuda()
+    full = _run_ce(h, w, b, labels, torch.ones(R, device="cuda"))
     for mask in range(1, 8):
         ts = [t.detach().clone().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate((h, w, b))]
         vocab.vocab_cross_entropy(ts[0], ts[1], labels, bias=ts[2]).sum().backward()      # (a gradient of stride 0)
@@ -344,9 +365,10 @@ def test_only_the_gradients_that_are_asked_for():
 
 
 @pytest.mark.gpu
-def test_runs_repeat_bit_for_bit_and_leave_their_inputs():
-    h, w, b, g = _inputs("bf16", 300, 3000, 128)
-    labels = torch.randint(0, 3000, (300,), generator=g).cuda()
+@pytest.mark.parametrize("V", [3000, 30000])
+def test_runs_repeat_bit_for_bit_and_leave_their_inputs(V):
+    h, w, b, g = _inputs("bf16", 300, V, 128)
+    labels = torch.randint(0, V, (300,), generator=g).cuda()
     gr = torch.rand(300, generator=g).cuda()
     copies = [t.clone() for t in (h, w, b, labels, gr)]
     first = _run_ce(h, w, b, labels, gr)
@@ -359,10 +381,11 @@ def test_runs_repeat_bit_for_bit_and_leave_their_inputs():
 
 
 @pytest.mark.gpu
-def test_backward_twice_of_a_retained_graph_with_other_gradients():
+@pytest.mark.parametrize("V,K", [(500, 64), (40000, 256)])
+def test_backward_twice_of_a_retained_graph_with_other_gradients(V, K):
     from gridmm_amd import vocab
-    h, w, b, g = _inputs("fp16", 40, 500, 64)
-    labels = torch.randint(0, 500, (40,), generator=g).cuda()
+    h, w, b, g = _inputs("fp16", 40, V, K)
+    labels = torch.randint(0, V, (40,), generator=g).cuda()
     hl, wl, bl = _leaves(h, w, b)
     loss = vocab.vocab_cross_entropy(hl, wl, labels, bias=bl)
     for scale in (1.0, 1e-4, 64.0):
@@ -397,9 +420,10 @@ def test_no_rows():
 
 
 @pytest.mark.gpu
-def test_on_another_stream():
-    h, w, b, g = _inputs("fp32", 100, 2000, 128)
-    labels = torch.randint(0, 2000, (100,), generator=g).cuda()
+@pytest.mark.parametrize("V", [2000, 40000])
+def test_on_another_stream(V):
+    h, w, b, g = _inputs("fp32", 100, V, 128)
+    labels = torch.randint(0, V, (100,), generator=g).cuda()
     gr = torch.rand(100, generator=g).cuda()
     want = _run_ce(h, w, b, labels, gr)
     st = torch.cuda.Stream()
@@ -412,13 +436,14 @@ def test_on_another_stream():
 
 
 @pytest.mark.gpu
-def test_captured_step_replays_with_other_labels_and_other_counts():
+@pytest.mark.parametrize("V", [1500, 15000])
+def test_captured_step_replays_with_other_labels_and_other_counts(V):
     """Forward and backward in one hipGraph; between the replays the labels (and with them the number of rows that count) change and
     eager work of the same operators runs."""
     from gridmm_amd import vocab
-    h, w, b, g = _inputs("fp32", 300, 1500, 128)
+    h, w, b, g = _inputs("fp32", 300, V, 128)
     hl, wl, bl = _leaves(h, w, b)
-    labels = torch.randint(0, 1500, (300,), generator=g).cuda()
+    labels = torch.randint(0, V, (300,), generator=g).cuda()
     gr = torch.rand(300, generator=g).cuda()
 
     def step():
@@ -435,7 +460,7 @@ def test_captured_step_replays_with_other_labels_and_other_counts():
     with torch.cuda.graph(graph):
         out = step()
     for drop in (0.0, 0.5, 1.0, 0.1):
-        new = torch.randint(0, 1500, (300,), generator=g)
+        new = torch.randint(0, V, (300,), generator=g)
         new[torch.rand(300, generator=g) < drop] = -1
         labels.copy_(new)
         graph.replay()
