@@ -132,16 +132,52 @@ __device__ __forceinline__ void few_tile(const FewArgs& a, int r0, int64_t j0, f
   }
 }
 
-// f(slot, d) for the targets of row r among the 4 columns from jl on, in the order of the slots; 8 of them loaded at a time
+// The targets of a group's rows among a workgroup's 64 columns, found together: wave w looks through the rows w, w + 4, .. and keeps a
+// list of its own, in the order of (row, slot).  With few slots, or more hits than a list holds, each lane looks through its row.
+struct FewTargets {
+  unsigned list[4][256];
+  int n[4];
+};
+constexpr int FEW_SLOTS_EACH = 4;
+template <int RP>
+__device__ __forceinline__ void few_collect(const FewArgs& a, int r0, FewTargets& T) {
+  if (a.slots <= FEW_SLOTS_EACH) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t j0 = (int64_t)blockIdx.x * 64;
+  int n = 0;
+  for (int r = wave; r < RP && r0 + r < a.rows; r += 4)
+    for (int s0 = 0; s0 < a.slots; s0 += 64) {
+      const int s = s0 + lane;
+      const int64_t id = s < a.slots ? load_index(a.index, (int64_t)(r0 + r) * a.ld_index + s, a.wide) : -1;
+      const bool hit = id >= j0 && id < j0 + 64 && id < a.vocab;
+      const uint64_t b = __ballot(hit);
+      const int at = n + __popcll(b & ((1ull << lane) - 1));
+      if (hit && at < 256) T.list[wave][at] = (unsigned)r | (unsigned)(id - j0) << 5 | (unsigned)s << 11;
+      n += __popcll(b);
+    }
+  if (lane == 0) T.n[wave] = n;
+  __syncthreads();
+}
+// f(slot, d) for the targets of row r = r0 + local among the lane's 4 columns from jl on, in the order of the slots
 template <class F>
-__device__ __forceinline__ void few_targets(const FewArgs& a, int64_t r, int64_t jl, F f) {
+__device__ __forceinline__ void few_targets(const FewArgs& a, const FewTargets& T, int r0, int local, int64_t jl, F f) {
+  if (a.slots > FEW_SLOTS_EACH && T.n[0] <= 256 && T.n[1] <= 256 && T.n[2] <= 256 && T.n[3] <= 256) {
+    const unsigned c0 = (unsigned)(jl - (int64_t)blockIdx.x * 64);
+    const int w = local & 3;
+    for (int e = 0; e < T.n[w]; ++e) {
+      const unsigned v = T.list[w][e], d = ((v >> 5) & 63) - c0;
+      if ((int)(v & 31) == local && d < 4) f((int)(v >> 11), (int)d);
+    }
+    return;
+  }
   for (int k0 = 0; k0 < a.slots; k0 += 8) {
     int64_t d[8];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) d[u] = load_index(a.index, r * a.ld_index + (k0 + u < a.slots ? k0 + u : a.slots - 1), a.wide) - jl;
+    for (int u = 0; u < 8; ++u)
+      d[u] = load_index(a.index, (int64_t)(r0 + local) * a.ld_index + (k0 + u < a.slots ? k0 + u : a.slots - 1), a.wide) - jl;
 #pragma unroll
     for (int u = 0; u < 8; ++u)
-      if (k0 + u < a.slots && (uint64_t)d[u] < 4) f(k0 + u, (int)d[u]);
+      if (k0 + u < a.slots && (uint64_t)d[u] < 4 && jl + d[u] < a.vocab) f(k0 + u, (int)d[u]);
   }
 }
 
@@ -149,11 +185,13 @@ __device__ __forceinline__ void few_targets(const FewArgs& a, int64_t r, int64_t
 template <int DT, int RT, bool VEC, bool GRAD>
 __global__ __launch_bounds__(256) void few_scores_kernel(const FewArgs a) {
   __shared__ float2 wst[4][RT * 16];
+  __shared__ FewTargets T;
   constexpr int RP = RT * 16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
   const int64_t j0 = (int64_t)blockIdx.x * 64 + wave * 16, jl = j0 + 4 * g;
   f32x4_t y[RT];
   const int r0 = blockIdx.y * RP;
+  few_collect<RP>(a, r0, T);
   few_tile<DT, RT, VEC>(a, r0, j0, y);
   if constexpr (!GRAD) {
 #pragma unroll
@@ -170,8 +208,8 @@ __global__ __launch_bounds__(256) void few_scores_kernel(const FewArgs a) {
       s += __shfl_xor(s, 32, 64);
       if (g == 0) wst[wave][t * 16 + l15] = make_float2(m, s);
       if (r < a.rows)                           // the scores at the row's targets
-        few_targets(a, r, jl, [&](int k, int d) {
-          if (jl + d < a.vocab) a.zt[(int64_t)r * a.slots + k] = d < 2 ? (d == 0 ? y[t][0] : y[t][1]) : (d == 2 ? y[t][2] : y[t][3]);
+        few_targets(a, T, r0, t * 16 + l15, jl, [&](int k, int d) {
+          a.zt[(int64_t)r * a.slots + k] = d < 2 ? (d == 0 ? y[t][0] : y[t][1]) : (d == 2 ? y[t][2] : y[t][3]);
         });
     }
     __syncthreads();
@@ -189,7 +227,7 @@ __global__ __launch_bounds__(256) void few_scores_kernel(const FewArgs a) {
       const float gt = live ? a.grad[r * a.grad_stride] * a.temperature : 0.f, L = live ? a.lse[r] : 0.f;
       float p[4] = {0.f, 0.f, 0.f, 0.f};
       if (live)
-        few_targets(a, r, jl, [&](int k, int d) {
+        few_targets(a, T, r0, t * 16 + l15, jl, [&](int k, int d) {
           const float q = a.kd ? a.p[(int64_t)r * a.slots + k] : 1.f;
 #pragma unroll
           for (int i = 0; i < 4; ++i) p[i] += d == i ? q : 0.f;
