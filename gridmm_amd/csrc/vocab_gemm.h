@@ -130,11 +130,8 @@ struct Tile {
     Item ahead;                          // the item whose stage `akt` is transferred next
     int ai = 0, akt = 0, issued = 0;
     bool have;
-    auto krow = [&](int i) {             // (a column operand's contraction row within the stage)
-      const int q = wave * PPW + i - (isA ? 0 : BM / 8), rr = (q & 7) * 8 + (lane >> 3);
-      return PL == 2 ? rr & 31 : rr;
-    };
-    auto aim = [&] {
+    // byte offsets of the pieces; a column operand's contraction rows past `last` of the stage are that one again
+    auto aim = [&](int last) {
       const int64_t b0 = isA ? ahead.bm : ahead.bn, r0 = b0 < O.rows ? b0 : O.rows - 1;      // (a row operand's first row)
       base = O.p + (col ? ahead.k0 * O.ld : r0 * O.ld + ahead.k0);
 #pragma unroll
@@ -150,36 +147,37 @@ struct Tile {
           const int c = slot ^ (((rr >> 1) & 1) << 2);
           int64_t cc = b0 + panel * 64 + c * 8;
           if (cc > O.cols - 8) cc = O.cols - 8;
-          off[i] = ((unsigned)krow(i) * ld + (PL == 2 ? (rr >> 5) * (unsigned)O.plane : 0) + (unsigned)cc) * 2;
+          const int kr = min(PL == 2 ? rr & 31 : rr, last);
+          off[i] = ((unsigned)kr * ld + (PL == 2 ? (rr >> 5) * (unsigned)O.plane : 0) + (unsigned)cc) * 2;
         }
       }
     };
     auto next_item = [&] {
       do have = work(ai++, ahead); while (have && ahead.nk <= 0);
       akt = 0;
-      if (have) aim();
+      if (have) aim(BK - 1);
     };
-    auto issue = [&] {
-      const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + (issued & 1) * (STAGE * 2));
+    // The next stage's transfers: point() says where from and to, piece(i) starts one, moved() steps on.  Past the last stage of all they
+    // bring that one again, into the buffer that nobody reads any more.
+    const unsigned short* from = base;
+    unsigned to = 0;
+    auto point = [&] {
+      to = __builtin_amdgcn_readfirstlane(lds0 + (issued & 1) * (STAGE * 2));
+      if (!have) return;
+      from = base + akt * step;
       if (COLA || COLB) {
-        const int64_t first = ahead.k0 + (int64_t)akt * BK, last = O.rows - 1 - first;      // (of a column operand)
-        if (col && last < BK - 1) {              // contraction rows past the last stored one: that one again
-          const unsigned short* from = uniform(last < 0 ? O.p + (O.rows - 1) * O.ld : base + akt * step);
-#pragma unroll
-          for (int i = 0; i < PPW; ++i) {
-            const int kr = krow(i), keep = last < 0 ? 0 : kr < last ? kr : (int)last;
-            dma16(from, off[i] - (unsigned)(kr - keep) * ld * 2, to + i * 1024);
-          }
-          ++issued;
-          if (++akt == ahead.nk) next_item();
-          return;
+        const int64_t first = ahead.k0 + (int64_t)akt * BK, last = O.rows - 1 - first;
+        if (col && last < BK - 1) {              // (the last stages of an item: the next item aims anew)
+          if (last < 0) from = O.p + (O.rows - 1) * O.ld;
+          aim(last < 0 ? 0 : (int)last);
         }
       }
-      const unsigned short* from = uniform(base + akt * step);
-#pragma unroll
-      for (int i = 0; i < PPW; ++i) dma16(from, off[i], to + i * 1024);
+      from = uniform(from);
+    };
+    auto piece = [&](int i) { dma16(from, off[i], to + i * 1024); };
+    auto moved = [&] {
       ++issued;
-      if (++akt == ahead.nk) next_item();
+      if (have && ++akt == ahead.nk) next_item();
     };
 
     // ---- fragments
@@ -200,23 +198,17 @@ struct Tile {
     using CA = std::integral_constant<bool, COLA>;
     using CB = std::integral_constant<bool, COLB>;
     constexpr int KS = BK / 16;
-    s16x8_t a[2][TM], b[2][TN];                                 // (hi) planes, two sub-steps
-    [[maybe_unused]] s16x8_t al[TM], bl[TN];                    // lo planes of the current one
-    auto read = [&](s16x8_t (&fa)[TM], s16x8_t (&fb)[TN], int stage, int ks, int lo) {
+    s16x8_t a[2][TM], b[2][TN];                 // (hi) planes, two sub-steps
+    s16x8_t al[TM], bl[TN];                     // lo planes of the current one (PL = 2)
+    // fragment f of TN + TM, in the order in which the products want them: B 0, A 0, the rest of B, the rest of A
+    auto read1 = [&](s16x8_t (&fa)[TM], s16x8_t (&fb)[TN], int f, int stage, int ks, int lo) {
       const unsigned short* sa = smem + (stage & 1) * STAGE;
       const unsigned short* sb = sa + BM * 64;
-#pragma unroll
-      for (int n = 0; n < TN; ++n) fb[n] = frag(CB{}, sb, wc * WN + n * 32, ks, lo);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) fa[i] = frag(CA{}, sa, wr * WM + i * 32, ks, lo);
+      const int n = f == 0 ? 0 : f - 1, i = f == 1 ? 0 : f - TN;
+      if (f == 0 || (f >= 2 && f <= TN)) fb[n] = frag(CB{}, sb, wc * WN + n * 32, ks, lo);
+      else fa[i] = frag(CA{}, sa, wr * WM + i * 32, ks, lo);
     };
     Acc acc;
-    auto product = [&](const s16x8_t (&fa)[TM], const s16x8_t (&fb)[TN]) {
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int n = 0; n < TN; ++n) acc[i][n] = mma<F16>(fb[n], fa[i], acc[i][n]);
-    };
     auto barrier = [&] {
       // this wave's pieces of the next stage have landed and its reads of the current one are in registers
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -226,40 +218,57 @@ struct Tile {
 
     next_item();
     if (have) {
-      issue();
-      barrier();
-      if (have) issue();
-      read(a[0], b[0], 0, 0, 0);
+      for (int twice = 0; twice < 2; ++twice) {
+        point();
+#pragma unroll
+        for (int i = 0; i < PPW; ++i) piece(i);
+        moved();
+        if (twice == 0) barrier();
+      }
+#pragma unroll
+      for (int f = 0; f < TM + TN; ++f) read1(a[0], b[0], f, 0, 0, 0);
     }
     Item item;
     int stage = 0;
     for (int n = 0; work(n, item); ++n) {
+      float sums[TM];
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int i = 0; i < TM; ++i) {
+        sums[i] = 0.f;
 #pragma unroll
         for (int c = 0; c < TN; ++c)
 #pragma unroll
           for (int q = 0; q < 16; ++q) acc[i][c][q] = 0.f;
-      float sums[TM] = {};
+      }
       const bool sum = SUMA && want_sums(item);
+      // One stage: its products, with the reads of the fragments ahead and the transfers of the stage after next between them, one
+      // after each matrix instruction, so that none of them waits for a burst of the others.
       for (int kt = 0; kt < item.nk; ++kt, ++stage) {
+        constexpr int NP = PL == 2 ? 3 : 1, NM = TM * TN, AT = PL == 2 ? NM - 1 : 0;      // the barrier follows product AT of the last sub-step
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           const int set = ks & 1;
-          bool more = false;
-          if constexpr (PL == 2) read(al, bl, stage, ks, 1);
-          if (ks + 1 < KS) {
-            read(a[set ^ 1], b[set ^ 1], stage, ks + 1, 0);
-          } else if (stage + 1 < issued) {
-            barrier();
-            read(a[set ^ 1], b[set ^ 1], stage + 1, 0, 0);
-            more = have;
-          }
-          __builtin_amdgcn_sched_barrier(0);
-          product(a[set], b[set]);
-          if constexpr (PL == 2) {
-            product(a[set], bl);
-            product(al, b[set]);
+          const bool last = ks == KS - 1;
+#pragma unroll
+          for (int m = 0; m < NP * NM; ++m) {
+            const int p = m / NM, i = m % NM / TN, n2 = m % TN;
+            acc[i][n2] = p == 0 ? mma<F16>(b[set][n2], a[set][i], acc[i][n2]) : p == 1 ? mma<F16>(bl[n2], a[set][i], acc[i][n2]) : mma<F16>(b[set][n2], al[i], acc[i][n2]);
+            if (PL == 2 && m < TM + TN) read1(al, bl, m, stage, ks, 1);
+            if (last && m == AT) {
+              barrier();
+              point();
+            }
+            constexpr int ROOM = NP * NM - 1 - AT, RPS = (TM + TN + ROOM - 1) / ROOM;      // products behind the barrier, reads at each
+#pragma unroll
+            for (int f = 0; f < TM + TN; ++f)
+              if (m > AT && f / RPS == m - AT - 1) read1(a[set ^ 1], b[set ^ 1], f, last ? stage + 1 : stage, last ? 0 : ks + 1, 0);
+            if (last && m > AT) {
+              const int q0 = (m - AT - 1) * PPW / ROOM, q1 = (m - AT) * PPW / ROOM;
+#pragma unroll
+              for (int q = 0; q < PPW; ++q)
+                if (q >= q0 && q < q1) piece(q);
+            }
+            __builtin_amdgcn_sched_barrier(0);
           }
           if (SUMA && sum) {
 #pragma unroll
@@ -268,12 +277,12 @@ struct Tile {
               if constexpr (PL == 2) sums[i] = sum8<F16>(al[i], sums[i]);
             }
           }
-          if (more) issue();
-          __builtin_amdgcn_sched_barrier(0);
+          if (last) moved();
         }
       }
       done(item, acc, sums);
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // nothing is on its way into LDS that another workgroup may get
   }
 };
 
