@@ -48,9 +48,20 @@ __device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int wide
 // fp32 -> 16 bits, to nearest even; NaN stays NaN
 __device__ __forceinline__ unsigned short to_f16(float x) { return __builtin_bit_cast(unsigned short, (_Float16)x); }
 __device__ __forceinline__ unsigned short to_bf16(float x) { return (unsigned short)(cvt_pk_bf16(x, x) & 0xffffu); }
+// four of them, two at a time
 template <bool F16V>
-__device__ __forceinline__ unsigned short to_16(float x) {
-  if constexpr (F16V) return to_f16(x); else return to_bf16(x);
+__device__ __forceinline__ u16x4_t to_16x4(float a, float b, float c, float d) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+  if constexpr (F16V) {
+    typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+    const u32x2_t u = {__builtin_bit_cast(unsigned, __builtin_convertvector(((f32x2_t){a, b}), f16x2_t)),
+                       __builtin_bit_cast(unsigned, __builtin_convertvector(((f32x2_t){c, d}), f16x2_t))};
+    return __builtin_bit_cast(u16x4_t, u);
+  } else {
+    const u32x2_t u = {cvt_pk_bf16(a, b), cvt_pk_bf16(c, d)};
+    return __builtin_bit_cast(u16x4_t, u);
+  }
 }
 __device__ __forceinline__ float finite_abs(float x) {
   const float a = fabsf(x);
@@ -580,22 +591,20 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
           __builtin_amdgcn_sched_barrier(0);
           const int64_t r = r0 + i * 32 + (lane & 31);
           const bool live = r < count;
-          const float L = live ? lse[r] : 0.f, gr = live ? grow[r] : 0.f;
+          const float L = live ? lse[r] : 1e30f, gr = live ? grow[r] : 0.f;      // (a row past the count: 0 times exp2(-1e30))
           u16x4_t hi[8], lo[8];
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             const float4 b = *reinterpret_cast<const float4*>(bz + c * 8);
             const float bb[4] = {b.x, b.y, b.z, b.w};
+            float v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float v = live ? gr * __builtin_amdgcn_exp2f(fmaf(acc[i][c >> 2][(c & 3) * 4 + e], sc, bb[e]) - L) : 0.f;
-              if constexpr (T::PL == 2) {
-                const _Float16 h = (_Float16)v;
-                hi[c][e] = __builtin_bit_cast(unsigned short, h);
-                lo[c][e] = to_f16(v - (float)h);
-              } else {
-                hi[c][e] = to_16<T::F16>(v);
-              }
+            for (int e = 0; e < 4; ++e) v[e] = gr * __builtin_amdgcn_exp2f(fmaf(acc[i][c >> 2][(c & 3) * 4 + e], sc, bb[e]) - L);
+            hi[c] = to_16x4<T::F16>(v[0], v[1], v[2], v[3]);
+            if constexpr (T::PL == 2) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] -= (float)__builtin_bit_cast(_Float16, (unsigned short)hi[c][e]);
+              lo[c] = to_16x4<true>(v[0], v[1], v[2], v[3]);
             }
           }
           unsigned short* at = dS + (r0 + i * 32) * ldS + c0;
@@ -743,8 +752,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, O
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
   const int count = __builtin_amdgcn_readfirstlane(meta->count), nk = (count + T::BK - 1) / T::BK;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
-  const int sg = *scale;
-  const float un = ldexpf(1.f, -sg), unw = ldexpf(1.f, -meta->sh);       // (two factors: their product may leave fp32's range)
+  const int eb = -*scale, e = eb - meta->sh;       // exponents of the units of db and dW
   unsigned short* scratch = smem + T::LDS + wave * 2048;
   static_assert(T::TN == 2, "64 columns a wave");
   T::template run<true>(
@@ -763,7 +771,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, O
           for (int i = 0; i < T::TM; ++i) {
             const float s = sums[i] + __shfl_xor(sums[i], 32, 64);
             const int64_t j = r0 + i * 32 + (lane & 31);
-            if (lane < 32 && j < vocab) store_as(db, j, bias_dtype, s * un);
+            if (lane < 32 && j < vocab) store_as(db, j, bias_dtype, ldexpf(s, eb));
           }
         }
         if (!dW) return;
@@ -777,7 +785,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, O
               float4 v[4];
 #pragma unroll
               for (int q = 0; q < 4; ++q)
-                v[q] = make_float4(acc[i][n][q * 4] * un * unw, acc[i][n][q * 4 + 1] * un * unw, acc[i][n][q * 4 + 2] * un * unw, acc[i][n][q * 4 + 3] * un * unw);
+                v[q] = make_float4(ldexpf(acc[i][n][q * 4], e), ldexpf(acc[i][n][q * 4 + 1], e), ldexpf(acc[i][n][q * 4 + 2], e), ldexpf(acc[i][n][q * 4 + 3], e));
               rows_of_32(scratch, v, [&](int row, int cc, float4 x) {
                 const int64_t r = r0 + i * 32 + row, c = c0 + n * 32 + cc;
                 if (r >= vocab || c >= K) return;
@@ -794,9 +802,11 @@ __global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, O
             unsigned short* out = reinterpret_cast<unsigned short*>(dW);
             u16x4_t v[8];
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) v[c][e] = to_16<T::F16>(acc[i][c >> 2][(c & 3) * 4 + e] * un * unw);
+            for (int c = 0; c < 8; ++c) {
+              const f32x16_t& x = acc[i][c >> 2];
+              const int q = (c & 3) * 4;
+              v[c] = to_16x4<T::F16>(ldexpf(x[q], e), ldexpf(x[q + 1], e), ldexpf(x[q + 2], e), ldexpf(x[q + 3], e));
+            }
             rows_of_16(scratch, v, [&](int row, int cc, u16x8_t x) {
               const int64_t r = r0 + i * 32 + row, c = c0 + cc;
               if (r >= vocab || c >= K) return;
