@@ -25,7 +25,7 @@ struct FewArgs {
   int rows, vocab, K, slots, wide, dtype, bias_dtype, kd;
   float inv_t, unit, temperature;
   float2* stats;                 // [workgroup][groups RP]
-  float *lse, *zt, *p, *flag;    // saved: [groups RP], [rows][slots], [rows][slots], [groups RP]: 1 for rows that count
+  float *lse, *zt, *p, *flag;    // saved: [groups RP], [rows][slots] (halves), [rows][slots], [groups RP]: 1 for rows that count
   float* loss;
   const float* grad;
   int64_t grad_stride;
@@ -209,7 +209,9 @@ __global__ __launch_bounds__(256) void few_scores_kernel(const FewArgs a) {
       if (g == 0) wst[wave][t * 16 + l15] = make_float2(m, s);
       if (r < a.rows)                           // the scores at the row's targets
         few_targets(a, T, r0, t * 16 + l15, jl, [&](int k, int d) {
-          a.zt[(int64_t)r * a.slots + k] = d < 2 ? (d == 0 ? y[t][0] : y[t][1]) : (d == 2 ? y[t][2] : y[t][3]);
+          const float v = d < 2 ? (d == 0 ? y[t][0] : y[t][1]) : (d == 2 ? y[t][2] : y[t][3]);
+          // half of it: a bias of the lowest finite number, -inf in base 2, is finite so
+          a.zt[(int64_t)r * a.slots + k] = v == -INFINITY && a.bias ? load_as_f32(a.bias, jl + d, a.bias_dtype) * (0.5f * a.unit) : 0.5f * v;
         });
     }
     __syncthreads();
@@ -264,16 +266,16 @@ __global__ __launch_bounds__(256) void few_loss_kernel(const FewArgs a, int64_t 
       const float q = a.p[(int64_t)r * a.slots + k];
       if (id < 0) continue;
       bad |= id >= a.vocab;
-      if (id < a.vocab && !(q == 0.f)) cross += q * (L - a.zt[(int64_t)r * a.slots + k]);
+      if (id < a.vocab && !(q == 0.f)) cross += q * (0.5f * L - a.zt[(int64_t)r * a.slots + k]);
     }
     cross = wave_sum(cross);
-    out = __any(bad) ? NAN : a.temperature * a.temperature * (plogp + cross * LN2);
+    out = __any(bad) ? NAN : a.temperature * a.temperature * (plogp + natural(cross));
     if (__any(bad)) L = NAN;
   } else {
     const int64_t y = load_index(a.index, r * a.ld_index, a.wide);
     live = y != a.ignore;
     if (y < 0 || y >= a.vocab) L = NAN;                 // a label outside the vocabulary spoils its row
-    else out = (L - a.zt[r]) * LN2;
+    else out = natural(0.5f * L - a.zt[r]);
     if (L != L) out = NAN;
   }
   if (lane == 0) {

@@ -14,8 +14,8 @@
 // Rows that do not count (label == ignore_index; no filled slot) are left out on the device: the counted rows are compacted into
 // the packed copy of h, the grids are sized for all rows and workgroups past the count end at once -- no host read-back.
 //
-// Number formats.  bf16 / fp16 operands: one plane, products exact, sums fp32; dS is rounded to the operands' type (2^-9 / 2^-12
-// of an entry, the size of the rounding of the gradients themselves).  fp32 operands: two fp16 planes each (22 bits) after a
+// Number formats.  bf16 / fp16 operands: one plane, products exact, sums fp32; dS is rounded to the operands' type (2^-8 / 2^-11
+// of an entry at most, like the gradients themselves).  fp32 operands: two fp16 planes each (22 bits) after a
 // power-of-two scale from the tensor's largest finite value, so a product is off by ~2^-22: like fp32 sums.  dS is scaled by a power of
 // two from the largest |g T| of the call (fp16 range: entries below 2^-38 of it vanish).
 // Everything runs in the base-2 domain: y = z log2 e, exp2, and ln 2 comes back in the losses.
@@ -97,6 +97,11 @@ __host__ __device__ inline int hidden_splits(int64_t count, int64_t Kp, int64_t 
 __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {        // (maximum, sum of 2^(y - maximum))
   const float M = fmaxf(a.x, b.x), ref = M == -INFINITY ? 0.f : M;        // nothing but masked columns: sum 0
   return make_float2(M, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
+}
+// 2 ln 2 times half a base-2 score or loss; what is finite stays so
+__device__ __forceinline__ float natural(float half) {
+  const float x = half * (2.f * LN2);
+  return fabsf(half) < INFINITY ? fminf(fmaxf(x, -3.4028234664e38f), 3.4028234664e38f) : x;
 }
 __device__ __forceinline__ void store_as(void* p, int64_t i, int dtype, float v) {
   if (dtype == F32) reinterpret_cast<float*>(p)[i] = v;
@@ -356,14 +361,13 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_stats_kernel(Operand A, O
 
 // ---- scores at the targets: one wave a (row, NS slots), fp32 sums over the operands as they came ----
 struct TargetArgs {
-  const void *hidden, *weight, *index;
+  const void *hidden, *weight, *index, *bias;
   int64_t ldh, ldw, ld_index;
-  int K, vocab, slots, wide, kd;      // slots >= 1
+  int K, vocab, slots, wide, kd, bias_dtype;      // slots >= 1
   float unit;
   const Meta* meta;
   const int* rowmap;
-  const float* biasz;
-  float* zt;       // [compacted row][slots], base 2
+  float* zt;       // [compacted row][slots]: HALF the score in base 2, where a bias of the lowest finite number is still finite
 };
 // NS dot products of one row of h with rows of W, their loads in flight together
 template <int DT, int NS>
@@ -426,7 +430,8 @@ __device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block
   for (int s = 0; s < NS; ++s) {
     if (lane != s || s0 + s >= a.slots) continue;
     // an id outside the vocabulary spoils its row; an empty slot has no score
-    a.zt[i * a.slots + s0 + s] = a.kd && id[s] < 0 ? 0.f : id[s] < 0 || id[s] >= a.vocab ? NAN : fmaf(z[s], a.unit, a.biasz[at[s]]);
+    const float half = 0.5f * a.unit, b = a.bias ? load_as_f32(a.bias, at[s], a.bias_dtype) * half : 0.f;
+    a.zt[i * a.slots + s0 + s] = a.kd && id[s] < 0 ? 0.f : id[s] < 0 || id[s] >= a.vocab ? NAN : fmaf(z[s], half, b);
   }
 }
 
@@ -490,7 +495,7 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
       for (int k = lanep; k < slots; k += 16) {
         const float q = p[r * slots + k], z = zt[i * slots + k];
         bad |= z != z;
-        if (!(q == 0.f)) s += q * (L - z);
+        if (!(q == 0.f)) s += q * (0.5f * L - z);
       }
     }
   }
@@ -502,9 +507,9 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
   if (p) {
     s = 0.f;
     for (int w = 0; w < 16; ++w) s += acc[w][rr];
-    out = temperature * temperature * (plogp[r] + s * LN2);
+    out = temperature * temperature * (plogp[r] + natural(s));
   } else {
-    out = (L - zt[i]) * LN2;
+    out = natural(0.5f * L - zt[i]);
     s = zt[i];
   }
   loss[r] = out;
@@ -626,7 +631,7 @@ struct FixArgs {
   unsigned short* dS;
 };
 __device__ __forceinline__ void target_entry(const FixArgs& a, int64_t i, int s, int64_t id, float p) {
-  const float v = a.grow[i] * (__builtin_amdgcn_exp2f(a.zt[i * a.slots + s] - a.lse[i]) - p);
+  const float v = a.grow[i] * (__builtin_amdgcn_exp2f(2.f * a.zt[i * a.slots + s] - a.lse[i]) - p);
   unsigned short* at = a.dS + i * a.ldS + (id - a.j0);
   if (a.dtype == F32) {
     const _Float16 h = (_Float16)v;
@@ -842,10 +847,10 @@ inline size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 constexpr int FEW_ROWS_F32 = 32, FEW_ROWS_16 = 16;
 // and for products of at most this many operations, and target comparisons, whatever the rows.  Forward and backward of 6000 x 512 fp32 at
 // 48, 128, 400 rows (0.3, 0.8, 2.5e9), device us: 71, 118, 265 against 96, 99, 116, and 5 launches against 12 (~4 us of the host each)
-constexpr double FEW_OPS = 6e8, FEW_TARGETS = 1e8;
+constexpr double FEW_OPS = 6e8, FEW_TARGETS = 1e8, FEW_TARGETS_MOST = 4e9;
 bool few_rows(const gridmm_vocab_loss_t* d) {
   const double rv = (double)d->rows * d->vocab;
-  return d->rows <= (d->dtype == F32 ? FEW_ROWS_F32 : FEW_ROWS_16) ||
+  return (d->rows <= (d->dtype == F32 ? FEW_ROWS_F32 : FEW_ROWS_16) && rv * d->slots <= FEW_TARGETS_MOST) ||
          (2. * rv * d->hidden_size <= FEW_OPS && rv * d->slots <= FEW_TARGETS);
 }
 
@@ -867,7 +872,7 @@ struct Plan {
 
 bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   if (!d || d->rows < 0 || d->vocab < 1 || d->hidden_size < 1 || d->slots < 0 || d->dtype < 0 || d->dtype > 2 || d->bias_dtype < 0 ||
-      d->bias_dtype > 2 || !(d->temperature > 0.f) || !(d->temperature < INFINITY) || d->rows > (1 << 20) || d->vocab > (1 << 28) ||
+      d->bias_dtype > 2 || !(d->temperature >= 1e-6f) || !(d->temperature <= 1e6f) || d->rows > (1 << 20) || d->vocab > (1 << 27) ||
       d->hidden_size > (1 << 20) || d->slots > (1 << 16) || (!d->slots && d->temperature != 1.f))
     return false;
   P.PL = d->dtype == F32 ? 2 : 1;
@@ -875,7 +880,8 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.Rp = (int64_t)up(d->rows, 256);
   P.Kp = (int64_t)up(d->hidden_size, 64);
   P.Vp = (int64_t)up(d->vocab, 256);
-  P.pack_w = d->dtype == F32 || d->hidden_size % 64 || d->ld_weight % 8 || ((uintptr_t)d->weight & 15);
+  // (a tile's 256 rows are addressed with 32-bit byte offsets: at most 2^31 from one row to the last where W lies)
+  P.pack_w = d->dtype == F32 || d->hidden_size % 64 || d->ld_weight % 8 || ((uintptr_t)d->weight & 15) || d->ld_weight > (1 << 22);
   // (grids: at most 2^32 threads)
   if ((P.Rp / 128) * (P.Vp / 128) > (1 << 23) || (int64_t)d->rows * ((P.slots + 7) / 8) > (1 << 25)) return false;
   // pieces: packed W and dS at most MOST bytes each, whole tiles, 8 192 columns at least
@@ -1100,7 +1106,7 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   t.hidden = d->hidden; t.weight = d->weight; t.index = d->slots ? d->ids : d->labels;
   t.ldh = d->ld_hidden; t.ldw = d->ld_weight; t.ld_index = d->slots ? d->ld_ids : 1;
   t.K = d->hidden_size; t.vocab = d->vocab; t.slots = P.slots; t.wide = d->index64; t.kd = d->slots > 0;
-  t.unit = unit; t.meta = meta; t.rowmap = rowmap; t.biasz = biasz; t.zt = zt;
+  t.bias = d->bias; t.bias_dtype = d->bias_dtype; t.unit = unit; t.meta = meta; t.rowmap = rowmap; t.zt = zt;
   const int rc = by_dtype(d, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const int hb = (int)(P.Rp / 4);

@@ -20,7 +20,8 @@ from .autograd import DEFERRED
 from .ops import _p, _stream
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-MAX_TOP = 1024
+MAX_TOP, MAX_TOP_ROWS = 1024, 1 << 22
+MAX_ROWS, MAX_VOCAB, MAX_HIDDEN, MAX_SLOTS = 1 << 20, 1 << 27, 1 << 20, 1 << 16
 
 
 class _Desc(ctypes.Structure):
@@ -72,6 +73,9 @@ def _check_head(hidden, weight, bias, *index):
         raise ValueError("hidden (..., K) and weight (V, K), not %s and %s" % (tuple(hidden.shape), tuple(ws)))
     if ws[0] < 1 or ws[1] < 1:
         raise ValueError("an empty weight %s" % (tuple(ws),))
+    if ws[0] > MAX_VOCAB or ws[1] > MAX_HIDDEN or hidden.numel() > MAX_ROWS * ws[1]:
+        raise ValueError("at most %d rows, %d of weight, %d hidden; not %s and %s" % (MAX_ROWS, MAX_VOCAB, MAX_HIDDEN,
+                                                                                      tuple(hidden.shape), tuple(ws)))
     if bias is not None:
         if bias.dim() != 1 or bias.shape[0] != ws[0]:
             raise ValueError("bias (V,), not %s" % (tuple(bias.shape),))
@@ -90,21 +94,23 @@ class _VocabLoss(torch.autograd.Function):
         b = None if bias is None else bias.contiguous()
         d = _Desc()
         d.weight, d.bias = w.data_ptr(), None if b is None else b.data_ptr()
-        d.ld_weight, d.rows, d.vocab, d.hidden_size = ldw, hidden.shape[0], w.shape[0], w.shape[1]
+        K = w.shape[1]
+        d.ld_weight, d.rows, d.vocab, d.hidden_size = ldw, hidden.shape[0], w.shape[0], K
         d.dtype, d.bias_dtype = _DTYPES[w.dtype], 0 if b is None else _DTYPES[b.dtype]
         d.index64, d.temperature, d.ignore_index = int(index.dtype == torch.int64), temperature, ignore_index
         if teacher is None:
             d.labels, d.slots = index.data_ptr(), 0
         else:
-            d.ids, d.ld_ids, d.slots = index.data_ptr(), index.stride(0), index.shape[1]
-            d.teacher, d.ld_teacher = teacher.data_ptr(), teacher.stride(0)
-        d.hidden, d.ld_hidden = hidden.data_ptr(), hidden.stride(0)
+            S = index.shape[1]
+            d.ids, d.ld_ids, d.slots = index.data_ptr(), max(index.stride(0), S), S
+            d.teacher, d.ld_teacher = teacher.data_ptr(), max(teacher.stride(0), S)
+        d.hidden, d.ld_hidden = hidden.data_ptr(), max(hidden.stride(0), K)      # (one row: whatever its stride says)
         need = any(ctx.needs_input_grad[:3])
         dev = hidden.device
         n_saved, n_ws = lib.gridmm_vocab_loss_saved_bytes(ctypes.byref(d)), lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 0)
         if n_saved == 0 or n_ws == 0:
-            raise ValueError("sizes the vocabulary losses do not take: rows %d, vocabulary %d, hidden %d, slots %d"
-                             % (d.rows, d.vocab, d.hidden_size, d.slots))
+            raise ValueError("too many rows for this vocabulary or these slots (rows / 128 x vocabulary / 128 <= 2^23, rows x slots / 8 <= "
+                             "2^25): rows %d, vocabulary %d, slots %d" % (d.rows, d.vocab, d.slots))
         loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
         saved = torch.empty(n_saved, dtype=torch.uint8, device=dev)
         ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
@@ -142,7 +148,10 @@ def vocab_cross_entropy(hidden, weight, labels, bias=None, ignore_index=-1):
     ignore_index (those rows cost nothing and get no gradient).  hidden (..., K) and weight (V, K) in one of fp32 / bf16 / fp16,
     bias (V,) in that type or fp32, labels (...) int64 or int32.  Gradients of hidden, weight and bias in their types.
 
-    A label outside [0, V) that is not ignore_index makes its row's loss NaN, and with it the gradients that it reaches."""
+    A label outside [0, V) that is not ignore_index makes its row's loss NaN, and with it the gradients that it reaches.  A bias of -inf
+    or of the type's lowest number takes its column out of the softmax.  The backward holds one piece of the scores' gradient at a time
+    (512 MB), scaled by one power of two: rows whose upstream gradient is more than 2^20 times smaller than the largest lose bits.  At
+    most 2^20 rows, 2^27 columns, and 2^37 scores."""
     _check_head(hidden, weight, bias, labels)
     if labels.shape != hidden.shape[:-1]:
         raise ValueError("labels %s for hidden %s" % (tuple(labels.shape), tuple(hidden.shape)))
@@ -169,7 +178,8 @@ def vocab_distillation(hidden, weight, teacher_ids, teacher_logits, bias=None, t
     _need(teacher_ids.dtype in (torch.int64, torch.int32), "teacher_ids are int64 or int32, not %s" % teacher_ids.dtype)
     _need(teacher_logits.dtype in _DTYPES, "teacher_logits are fp32, bf16 or fp16, not %s" % teacher_logits.dtype)
     T = float(temperature)
-    _need(0.0 < T < float("inf"), "a temperature above 0, not %r" % (temperature,))
+    _need(1e-6 <= T <= 1e6, "a temperature of 1e-6 to 1e6, not %r" % (temperature,))
+    _need(teacher_ids.shape[-1] <= MAX_SLOTS, "at most %d slots, not %d" % (MAX_SLOTS, teacher_ids.shape[-1]))
     with _on(hidden.device):
         h, _ = _rows(hidden)
         ids, _ = _rows(teacher_ids)
@@ -188,6 +198,8 @@ def top_logits(logits, k):
     k = int(k)
     _need(logits.dim() >= 1 and 1 <= k <= min(logits.shape[-1], MAX_TOP), "1 <= k <= min(V, %d): k = %d of %s"
           % (MAX_TOP, k, tuple(logits.shape)))
+    _need(logits.shape[-1] < 2 ** 31 and logits.numel() <= MAX_TOP_ROWS * logits.shape[-1], "at most %d rows of less than 2^31 logits, not %s"
+          % (MAX_TOP_ROWS, tuple(logits.shape)))
     lib = _lib.load()
     with _on(logits.device):
         x, ld = _rows(logits.detach())

@@ -823,8 +823,10 @@ int gridmm_dropout_add(const float* x, const float* r, float* y, void* y_hi, voi
  *   hidden [rows][hidden_size], weight [vocab][hidden_size] in dtype (0 fp32, 1 bf16, 2 fp16), row strides ld_*; bias [vocab] in
  *   bias_dtype or NULL; labels [rows], ids [rows][slots] int64 (index64 != 0) or int32; teacher fp32 [rows][slots].
  * fp32 operands run as two fp16 planes under a power-of-two scale of the tensor (22 bits; few rows: as fp32), 16-bit ones as
- * they are; sums, maxima and losses are fp32.  rows <= 2^20, vocab <= 2^28, hidden_size <= 2^20, slots <= 2^16.  Deterministic.  Rows that do not count are left out on the device (no read-back): a capture
- * may replay the call with other labels.
+ * they are; sums, maxima and losses are fp32.  dS entries more than 2^38 below the largest |grad T| of the call vanish (bf16: none).
+ * rows <= 2^20, vocab <= 2^27, hidden_size <= 2^20, slots <= 2^16, rows / 128 x vocab / 128 <= 2^23, rows x slots / 8 <= 2^25,
+ * 1e-6 <= T <= 1e6.  Deterministic.  Rows that do not count are left out on the device (no read-back): a capture may replay the call
+ * with other labels.  A column whose bias is -inf or the type's lowest number is out of the sum.
  *   saved      >= gridmm_vocab_loss_saved_bytes, 256-byte aligned: filled by _fwd, read (not changed) by _bwd
  *   workspace  >= gridmm_vocab_loss_workspace(d, 0 forward / 1 backward) bytes, 256-byte aligned
  *   backward   grad: d loss_r at grad[r * grad_stride] (0: one value for all rows); d_hidden [rows][hidden_size],

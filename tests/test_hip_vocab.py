@@ -84,7 +84,7 @@ def _hold(got, want, what):
 
 
 def _leaves(h, w, b):
-    return [t.detach().clone().requires_grad_() if t is not None else None for t in (h, w, b)]
+    return [t.detach().requires_grad_() if t is not None else None for t in (h, w, b)]      # (a clone would lose the strides)
 
 
 def _run_ce(h, w, b, labels, g, ignore=-1):
@@ -195,6 +195,44 @@ def test_cross_entropy_of_strided_operands(dtype, index, R, V, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("R,V,K", [(20, 300, 64), (2000, 300, 520), (2000, 320, 512)])
+def test_rows_of_weight_far_apart(dtype, R, V, K):
+    """2^23 elements and more from one row of W to the next: 32 bits of bytes do not reach over a tile's rows."""
+    g = torch.Generator().manual_seed(8)
+    ld = 2 ** 23 + 64
+    far = torch.empty(V * ld, dtype=DT[dtype], device="cuda").as_strided((V, K), (ld, 1))
+    far.copy_((torch.randn(V, K, generator=g) / 8).to(DT[dtype]))
+    h = torch.randn(R, K, generator=g).to(DT[dtype]).cuda()
+    _check_ce(h, far, None, torch.randint(0, V, (R,), generator=g).cuda(), torch.rand(R, generator=g).cuda())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [200, 40000])
+def test_single_rows_and_broadcast_rows(V):
+    """A single row may carry any stride, and the same row may stand for many."""
+    from gridmm_amd import vocab
+    h, w, b, g = _inputs("fp32", 1, V, 128)
+    y = torch.tensor([3], device="cuda")
+    a = vocab.vocab_cross_entropy(h, w, y, bias=b)
+    assert torch.equal(a, vocab.vocab_cross_entropy(h[0].as_strided((1, 128), (0, 1)), w, y, bias=b))
+    ids, t = torch.tensor([[1, 5, 9]], device="cuda"), torch.tensor([[0.5, 1.0, -1.0]], device="cuda")
+    c = vocab.vocab_distillation(h, w, ids, t, bias=b)
+    assert torch.equal(c, vocab.vocab_distillation(h, w, ids[0].as_strided((1, 3), (0, 1)), t[0].as_strided((1, 3), (0, 1)), bias=b))
+    x = h @ w.t()
+    for one, two in zip(vocab.top_logits(x, 4), vocab.top_logits(x[0].as_strided((1, V), (0, 1)), 4)):
+        assert torch.equal(one, two)
+    hl = h.clone().requires_grad_()
+    many = vocab.vocab_cross_entropy(hl.expand(70, 128), w, y.expand(70), bias=b)
+    assert bool((many == many[0]).all())
+    many.sum().backward()
+    _check_ce(h.expand(70, 128).contiguous(), w, b, y.expand(70).contiguous(), torch.ones(70, device="cuda"))
+    hf = h.expand(70, 128).contiguous().requires_grad_()
+    vocab.vocab_cross_entropy(hf, w, y.expand(70).contiguous(), bias=b).sum().backward()
+    assert torch.equal(hl.grad, hf.grad.sum(0, keepdim=True))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("V,K", [(600, 64), (40000, 256)])
 def test_bias_of_minus_infinity_masks_a_column(dtype, V, K):
@@ -210,8 +248,25 @@ def test_bias_of_minus_infinity_masks_a_column(dtype, V, K):
     want = _oracle(h, w[:300], b[:300], labels[:, None], torch.ones(33, 1, device="cuda", dtype=torch.float64), 1.0, gr)
     for k, t in (("loss", loss.detach()), ("d_hidden", hl.grad), ("d_weight", wl.grad[:300]), ("d_bias", bl.grad[:300])):
         v, e = want[k]
-        _hold(t, (v, e * 8), k)                    # w[400] sets the scale of the fp32 planes: 60 against a spread of 1/4 is 8 bits less range, not precision
+        _hold(t, (v, e), k)                        # (w[400] sets the scale of the fp32 planes, which changes their range and not their 22 bits)
     assert bool((wl.grad[300:] == 0).all()) and bool((bl.grad[300:] == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("V,K", [(600, 64), (40000, 256)])
+def test_bias_of_the_lowest_finite_value(dtype, V, K):
+    """A column masked with the type's lowest number: nothing for the rows that do not aim at it, a huge but finite loss for those that
+    do (the number over log 2 is no longer a fp32 number)."""
+    h, w, b, g = _inputs(dtype, 33, V, K)
+    b[10:300] = torch.finfo(b.dtype).min
+    labels = torch.randint(300, V, (33,), generator=g).cuda()
+    labels[::4], labels[1] = 17, 3
+    got = _check_ce(h, w, b, labels, torch.rand(33, generator=g).cuda())
+    assert bool(torch.isfinite(got["loss"]).all()) and float(got["loss"][0]) > 6e4
+    ids = torch.stack([torch.randperm(V, generator=g)[:7] for _ in range(33)])
+    ids[0, 0] = 17
+    _check_kd(h, w, b, ids.cuda(), torch.randn(33, 7, generator=g).cuda(), torch.rand(33, generator=g).cuda(), 1.0)
 
 
 @pytest.mark.gpu
@@ -271,7 +326,7 @@ def _check_kd(h, w, b, ids, t, g, T):
 
 KD = [("fp32", 300, 9001, 130, 17, 2.0), ("bf16", 200, 20001, 128, 300, 1.0), ("fp16", 1030, 2500, 200, 5, 0.5), ("fp32", 60, 30522, 256, 64, 1.0),
       ("fp32", 1, 1, 64, 1, 1.0), ("fp32", 5, 300, 64, 8, 2.0), ("bf16", 130, 1000, 128, 32, 1.0), ("fp16", 77, 513, 72, 100, 0.5),
-      ("fp32", 300, 2000, 100, 17, 4.0), ("bf16", 3, 40000, 64, 256, 1.5), ("fp32", 64, 256, 64, 256, 1.0)]
+      ("fp32", 300, 2000, 100, 17, 4.0), ("bf16", 3, 40000, 64, 256, 1.5), ("fp32", 64, 256, 64, 256, 1.0), ("fp32", 16, 30522, 64, 8200, 1.0)]
 
 
 @pytest.mark.gpu
@@ -468,6 +523,51 @@ def test_captured_step_replays_with_other_labels_and_other_counts(V):
         want = _run_ce(h, w, b, labels, gr)
         for x, k in zip(out, ("loss", "d_hidden", "d_weight", "d_bias")):
             assert torch.equal(x, want[k]), (drop, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [1500, 30000])
+def test_two_calls_at_once_and_two_captured_ones(V):
+    """Calls on two streams side by side, then each captured (one memory pool) and both replayed in turn: every result is the one that a
+    call alone gives."""
+    from gridmm_amd import vocab
+    sets = []
+    for seed in (1, 2):
+        h, w, b, g = _inputs("bf16", 300, V, 192, True, seed)
+        labels, gr = torch.randint(0, V, (300,), generator=g).cuda(), torch.rand(300, generator=g).cuda()
+        sets.append((_leaves(h, w, b), labels, gr, _run_ce(h, w, b, labels, gr)))
+
+    def step(i):
+        (hl, wl, bl), labels, gr, _ = sets[i]
+        loss = vocab.vocab_cross_entropy(hl, wl, labels, bias=bl)
+        return (loss,) + torch.autograd.grad(loss, (hl, wl, bl), gr)
+
+    def same(i, out):
+        for x, k in zip(out, ("loss", "d_hidden", "d_weight", "d_bias")):
+            assert torch.equal(x, sets[i][3][k]), (i, k)
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs[i].append(step(i))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for out in outs[i]:
+            same(i, out)
+    graphs, pool = [], None
+    for i in (0, 1):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], pool=pool):
+            outs[i] = step(i)
+        pool = graphs[0].pool()
+    for order in ((0, 1), (0, 1, 0), (0, 1, 0, 1)):
+        for i in order:
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            same(i, outs[i])
+            same(1 - i, step(1 - i))                   # eager work between the replays
 
 
 # ---- top logits ----
@@ -697,7 +797,8 @@ def test_the_c_entry_refuses_bad_sizes_and_pointers():
     assert lib.gridmm_vocab_loss_saved_bytes(ctypes.byref(_descriptor())) > 0
     for over in (dict(rows=-1), dict(vocab=0), dict(hidden_size=0), dict(slots=-1), dict(dtype=3), dict(bias_dtype=-1),
                  dict(temperature=0.0), dict(temperature=float("nan")), dict(temperature=float("inf")), dict(temperature=2.0),
-                 dict(rows=2 ** 30), dict(vocab=2 ** 30), dict(hidden_size=2 ** 21), dict(slots=2 ** 17)):
+                 dict(rows=2 ** 30), dict(vocab=2 ** 27 + 1), dict(hidden_size=2 ** 21), dict(slots=2 ** 17), dict(slots=1, temperature=1e-7),
+                 dict(slots=1, temperature=1e7), dict(rows=2 ** 20, vocab=2 ** 20)):
         d = _descriptor(**over)
         assert lib.gridmm_vocab_loss_saved_bytes(ctypes.byref(d)) == 0, over
         assert lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 0) == 0 and lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 1) == 0
@@ -735,6 +836,12 @@ def test_the_wrappers_refuse():
                  lambda: vocab.vocab_distillation(h, w, ids, t, temperature=0.0), lambda: vocab.vocab_distillation(h, w, ids, t, temperature=float("nan")),
                  lambda: vocab.vocab_distillation(h, w, ids.float(), t), lambda: vocab.vocab_distillation(h, w, ids, ids),
                  lambda: vocab.vocab_distillation(h, w, ids[:, :0], t[:, :0]),
+                 lambda: vocab.vocab_distillation(h, w, ids, t, temperature=1e-7), lambda: vocab.vocab_distillation(h, w, ids, t, temperature=1e7),
+                 lambda: vocab.vocab_distillation(h, w, ids[:, :1].expand(4, 2 ** 16 + 1), t[:, :1].expand(4, 2 ** 16 + 1)),
+                 lambda: vocab.vocab_cross_entropy(h[:1].expand(2 ** 20 + 1, 8), w, y[:1].expand(2 ** 20 + 1)),
+                 lambda: vocab.vocab_cross_entropy(h[:1].expand(2 ** 20, 8), w[:1].expand(2 ** 20, 8), y[:1].expand(2 ** 20)),
+                 lambda: vocab.vocab_cross_entropy(h, w[:1].expand(2 ** 27 + 1, 8), y),
+                 lambda: vocab.top_logits(h[:1].expand(2 ** 22 + 1, 8), 1), lambda: vocab.top_logits(h[0, :1].expand(1, 2 ** 31), 1),
                  lambda: vocab.top_logits(h, 0), lambda: vocab.top_logits(h, 9), lambda: vocab.top_logits(h.long(), 1),
                  lambda: vocab.top_logits(torch.zeros(2, 3000).cuda(), 1025)):
         with pytest.raises(ValueError):
