@@ -842,16 +842,31 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------------
 inline size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
-// Up to this many rows the kernels of vocab_few.h.  Forward and backward, us, them against the others: fp32 131072 x 2048, 32 rows 1500 : 2300;
-// bf16 5 rows 530 : 731, 32 rows 860 : 736; 30522 x 768 at one row, forward, fp32 41 : 90.
-constexpr int FEW_ROWS_F32 = 32, FEW_ROWS_16 = 16;
-// and for products of at most this many operations, and target comparisons, whatever the rows.  Forward and backward of 6000 x 512 fp32 at
-// 48, 128, 400 rows (0.3, 0.8, 2.5e9), device us: 71, 118, 265 against 96, 99, 116, and 5 launches against 12 (~4 us of the host each)
-constexpr double FEW_OPS = 6e8, FEW_TARGETS = 1e8, FEW_TARGETS_MOST = 4e9;
+// Which kernels.  Forward and backward, us of wall time (few rows : tiles), 5 launches against 12 (what the host pays for either is ~140 :
+// 158 there):
+//   rows up to 32 fp32, 16 otherwise: fp32 30522 x 2048, 4 rows 303 : 436, 16 rows 318 : 437; bf16 150 : 161, 172 : 160; 131072 x 2048 fp32 at
+//   32 rows 1500 : 2300
+//   or small products.  Each workgroup of the weight gradient goes through m = groups x ceil(hidden / 256) steps one after another (fp32 500 x
+//   2048 at m = 8, 16, 32: 139, 165, 230 : 160; 16 bits, m = 16, 32: 143, 169 : 161), and throughput counts from ~1e9 operations on (fp32 100
+//   hidden, 7.8e8, 1.6e9: 144, 187 : 162; bf16, per score hidden + 400 for its exponential: 512 hidden, 0.9e9, 1.9e9: 143, 176 : 160)
+//   rows that are no whole vectors are loaded value by value: only where the loop over hidden is short (bf16 1379 hidden, 4 rows, forward 73 :
+//   33; 100 hidden x 30522 at 64, 128 rows 143, 203 : 160; fp32 1379 hidden, 16, 32 rows: 142, 200 : 162)
+// and in any case few enough comparisons of the distillation's targets (one pass over all rows' ids a workgroup).
+bool few_vectors(const gridmm_vocab_loss_t* d) {      // rows of h and W are whole 16-byte vectors on their boundaries
+  const int A = d->dtype == F32 ? 4 : 8;
+  return d->hidden_size % A == 0 && d->ld_hidden % A == 0 && d->ld_weight % A == 0 &&
+         (((uintptr_t)d->hidden | (uintptr_t)d->weight) & 15) == 0;
+}
 bool few_rows(const gridmm_vocab_loss_t* d) {
-  const double rv = (double)d->rows * d->vocab;
-  return (d->rows <= (d->dtype == F32 ? FEW_ROWS_F32 : FEW_ROWS_16) && rv * d->slots <= FEW_TARGETS_MOST) ||
-         (2. * rv * d->hidden_size <= FEW_OPS && rv * d->slots <= FEW_TARGETS);
+  const double rv = (double)d->rows * d->vocab, K = d->hidden_size, targets = rv * d->slots;
+  const bool fp32 = d->dtype == F32, vec = few_vectors(d);
+  const int groups = d->rows <= 16 ? 1 : (d->rows + 31) / 32;
+  const double m = (double)groups * ((d->hidden_size + 255) / 256);
+  if (targets > 4e9) return false;
+  if (vec ? d->rows <= (fp32 ? 32 : 16) : d->rows <= 16 && (fp32 || K <= 384)) return true;
+  if (targets > 1e8) return false;
+  if (vec) return fp32 ? m <= 12 && rv * K <= 5e8 : m <= 16 && rv * (K + 400) <= 1.2e9;
+  return K <= 384 && m <= (fp32 ? 4 : 16) && rv * K <= 2e8;
 }
 
 struct Plan {
@@ -914,10 +929,9 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
     P.o_meta = take(GR * 4);                         // 1 for rows that count
     P.o_zt = take(S * 4);
     P.o_p = take(d->slots ? S * 4 : 0);
+    P.f_stats = take(V64 / 64 * GR * 8);             // (small enough to stay: no forward workspace)
     P.saved = o;
-    o = 0;
-    P.f_stats = take(V64 / 64 * GR * 8);
-    P.fwd = o;
+    P.fwd = 0;
     o = 0;
     P.b_ds = take(V64 * GR * 4);
     P.b_part = take((size_t)P.ranges * GR * up(d->hidden_size, 4) * 4);
@@ -1017,9 +1031,7 @@ bool bad_pointers(const gridmm_vocab_loss_t* d, const void* saved, bool forward)
 // calls f(type, tiles of 16 rows, whole vectors)
 template <class F>
 int by_few(const gridmm_vocab_loss_t* d, const Plan& P, F f) {
-  const int A = d->dtype == F32 ? 4 : 8;
-  const bool vec = d->hidden_size % A == 0 && d->ld_hidden % A == 0 && d->ld_weight % A == 0 &&
-                   (((uintptr_t)d->hidden | (uintptr_t)d->weight) & 15) == 0;
+  const bool vec = few_vectors(d);
   auto rows = [&](auto dt) {
     auto one = [&](auto rt) { return vec ? f(dt, rt, std::true_type{}) : f(dt, rt, std::false_type{}); };
     return P.RP == 16 ? one(std::integral_constant<int, 1>{}) : one(std::integral_constant<int, 2>{});
@@ -1056,15 +1068,15 @@ extern "C" size_t gridmm_vocab_loss_workspace(const gridmm_vocab_loss_t* d, int 
 extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, void* saved, size_t saved_bytes, void* workspace,
                                      size_t workspace_bytes, gridmm_stream_t stream) {
   Plan P;
-  if (!make_plan(d, P) || bad_pointers(d, saved, true) || saved_bytes < P.saved || !workspace || workspace_bytes < P.fwd ||
-      ((uintptr_t)workspace & 255) || (d->rows && !loss))
+  if (!make_plan(d, P) || bad_pointers(d, saved, true) || saved_bytes < P.saved || (P.fwd && !workspace) ||
+      workspace_bytes < P.fwd || ((uintptr_t)workspace & 255) || (d->rows && !loss))
     return GRIDMM_EINVAL;
   if (d->rows == 0) return GRIDMM_OK;
   hipStream_t st = as_stream(stream);
   char *sv = (char*)saved, *ws = (char*)workspace;
   if (P.few) {
     FewArgs a = few_args(d, P, saved);
-    a.stats = (float2*)(ws + P.f_stats);
+    a.stats = (float2*)(sv + P.f_stats);
     a.loss = loss;
     const int tiles = (d->vocab + 63) / 64;
     const int rc = by_few(d, P, [&](auto dt, auto rt, auto vec) {

@@ -83,64 +83,65 @@ def _check_head(hidden, weight, bias, *index):
             raise ValueError("bias is %s: fp32 or the weight's type" % bias.dtype)
 
 
+def _vocab_backward(ctx, g):
+    if g is None:
+        return (None,) * 7
+    hidden, w, b, _, saved = ctx.saved_tensors
+    if g.dtype != torch.float32:
+        g = g.float()
+    need_h, need_w, need_b = ctx.needs_input_grad[:3]
+    n_ws, prm = ctx.n_ws, ctx.prm
+    dh = hidden.new_empty(hidden.shape) if need_h else None
+    dw = w.new_empty(w.shape) if need_w else None
+    db = b.new_empty(b.shape) if need_b else None
+    with _on(w.device):
+        ws = saved.new_empty(n_ws)
+        # (addresses as plain numbers: half the time of an object each)
+        _lib.check(_lib.load().gridmm_vocab_loss_bwd(
+            ctypes.byref(ctx.desc), saved.data_ptr(), saved.numel(), g.data_ptr(), g.stride(0), dh.data_ptr() if need_h else None,
+            dw.data_ptr() if need_w else None, db.data_ptr() if need_b else None, ws.data_ptr(), n_ws, _stream()), "gridmm_vocab_loss_bwd")
+    return dh, DEFERRED.hand(prm[0], dw), DEFERRED.hand(prm[1], db), None, None, None, None
+
+
+_vocab_backward_once = once_differentiable(_vocab_backward)
+
+
 class _VocabLoss(torch.autograd.Function):
     """hidden (R, K), weight (V, K), bias (V,) or None, index (R,) labels or (R, S) ids, teacher None or (R, S) -> losses (R,)."""
 
     @staticmethod
     def forward(ctx, hidden, weight, bias, index, teacher, ignore_index, temperature):
         lib = _lib.load()
-        ctx.set_materialize_grads(False)
         w, ldw = _rows(weight)
         b = None if bias is None else bias.contiguous()
-        d = _Desc()
-        d.weight, d.bias = w.data_ptr(), None if b is None else b.data_ptr()
-        K = w.shape[1]
-        d.ld_weight, d.rows, d.vocab, d.hidden_size = ldw, hidden.shape[0], w.shape[0], K
-        d.dtype, d.bias_dtype = _DTYPES[w.dtype], 0 if b is None else _DTYPES[b.dtype]
-        d.index64, d.temperature, d.ignore_index = int(index.dtype == torch.int64), temperature, ignore_index
-        if teacher is None:
-            d.labels, d.slots = index.data_ptr(), 0
-        else:
-            S = index.shape[1]
-            d.ids, d.ld_ids, d.slots = index.data_ptr(), max(index.stride(0), S), S
-            d.teacher, d.ld_teacher = teacher.data_ptr(), max(teacher.stride(0), S)
-        d.hidden, d.ld_hidden = hidden.data_ptr(), max(hidden.stride(0), K)      # (one row: whatever its stride says)
-        need = any(ctx.needs_input_grad[:3])
-        dev = hidden.device
-        n_saved, n_ws = lib.gridmm_vocab_loss_saved_bytes(ctypes.byref(d)), lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 0)
-        if n_saved == 0 or n_ws == 0:
+        (R, K), V, dt = hidden.shape, w.shape[0], w.dtype
+        S = 0 if teacher is None else index.shape[1]
+        at = index.data_ptr()
+        # (a single row: whatever its stride says)
+        d = _Desc(hidden.data_ptr(), w.data_ptr(), None if b is None else b.data_ptr(), None if S else at, at if S else None,
+                  teacher.data_ptr() if S else None, max(hidden.stride(0), K), ldw, max(index.stride(0), S) if S else 0,
+                  max(teacher.stride(0), S) if S else 0, ignore_index, R, V, K, S, _DTYPES[dt], 0 if b is None else _DTYPES[b.dtype],
+                  index.dtype == torch.int64, temperature)
+        ref = ctypes.byref(d)
+        n_saved, n_ws = lib.gridmm_vocab_loss_saved_bytes(ref), lib.gridmm_vocab_loss_workspace(ref, 0)
+        if n_saved == 0:
             raise ValueError("too many rows for this vocabulary or these slots (rows / 128 x vocabulary / 128 <= 2^23, rows x slots / 8 <= "
-                             "2^25): rows %d, vocabulary %d, slots %d" % (d.rows, d.vocab, d.slots))
-        loss = torch.empty(d.rows, dtype=torch.float32, device=dev)
-        saved = torch.empty(n_saved, dtype=torch.uint8, device=dev)
-        ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
-        _lib.check(lib.gridmm_vocab_loss_fwd(ctypes.byref(d), _p(loss), _p(saved), n_saved, _p(ws), n_ws, _stream()),
+                             "2^25): rows %d, vocabulary %d, slots %d" % (R, V, S))
+        loss = hidden.new_empty(R, dtype=torch.float32)
+        saved = hidden.new_empty(n_saved, dtype=torch.uint8)
+        ws = saved.new_empty(n_ws) if n_ws else None
+        _lib.check(lib.gridmm_vocab_loss_fwd(ref, loss.data_ptr(), saved.data_ptr(), n_saved, ws.data_ptr() if n_ws else None, n_ws, _stream()),
                    "gridmm_vocab_loss_fwd")
-        if need:
+        if any(ctx.needs_input_grad[:3]):
+            ctx.set_materialize_grads(False)
             ctx.save_for_backward(hidden, w, b, index, saved)
-            ctx.desc, ctx.prm, ctx.n_ws = d, (weight, bias), lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 1)
+            ctx.desc, ctx.prm, ctx.n_ws = d, (weight, bias), lib.gridmm_vocab_loss_workspace(ref, 1)
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g):
-        if g is None:
-            return (None,) * 7
-        lib = _lib.load()
-        hidden, w, b, index, saved = ctx.saved_tensors
-        if g.dtype != torch.float32:
-            g = g.float()
-        need_h, need_w, need_b = ctx.needs_input_grad[:3]
-        dev = w.device
-        dh = torch.empty(hidden.shape, dtype=w.dtype, device=dev) if need_h else None
-        dw = torch.empty(w.shape, dtype=w.dtype, device=dev) if need_w else None
-        db = torch.empty_like(b) if need_b else None
-        with _on(dev):
-            n_ws = ctx.n_ws
-            ws = torch.empty(n_ws, dtype=torch.uint8, device=dev)
-            _lib.check(lib.gridmm_vocab_loss_bwd(ctypes.byref(ctx.desc), _p(saved), saved.numel(), _p(g), g.stride(0), _p(dh), _p(dw),
-                                                 _p(db), _p(ws), n_ws, _stream()), "gridmm_vocab_loss_bwd")
-        return dh, DEFERRED.hand(ctx.prm[0], dw), DEFERRED.hand(ctx.prm[1], db), None, None, None, None
+        # (a backward that records itself: marked as once differentiable)
+        return (_vocab_backward_once if torch.is_grad_enabled() else _vocab_backward)(ctx, g)
 
 
 def vocab_cross_entropy(hidden, weight, labels, bias=None, ignore_index=-1):

@@ -828,7 +828,8 @@ int gridmm_dropout_add(const float* x, const float* r, float* y, void* y_hi, voi
  * 1e-6 <= T <= 1e6.  Deterministic.  Rows that do not count are left out on the device (no read-back): a capture may replay the call
  * with other labels.  A column whose bias is -inf or the type's lowest number is out of the sum.
  *   saved      >= gridmm_vocab_loss_saved_bytes, 256-byte aligned: filled by _fwd, read (not changed) by _bwd
- *   workspace  >= gridmm_vocab_loss_workspace(d, 0 forward / 1 backward) bytes, 256-byte aligned
+ *   workspace  >= gridmm_vocab_loss_workspace(d, 0 forward / 1 backward) bytes, 256-byte aligned (NULL if that is 0)
+ *              (all four calls take one and the same *d, pointers and strides included: alignment chooses the kernels)
  *   backward   grad: d loss_r at grad[r * grad_stride] (0: one value for all rows); d_hidden [rows][hidden_size],
  *              d_weight [vocab][hidden_size] dense in dtype, d_bias [vocab] in bias_dtype, each overwritten, each may be NULL (one
  *              at least is not); teacher is not read. */

@@ -803,8 +803,8 @@ def test_the_c_entry_refuses_bad_sizes_and_pointers():
         assert lib.gridmm_vocab_loss_saved_bytes(ctypes.byref(d)) == 0, over
         assert lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 0) == 0 and lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 1) == 0
         assert lib.gridmm_vocab_loss_fwd(ctypes.byref(d), 256, 256, 1 << 40, 256, 1 << 40, None) == EINVAL
-    n, ws = lib.gridmm_vocab_loss_saved_bytes(ctypes.byref(_descriptor())), lib.gridmm_vocab_loss_workspace(ctypes.byref(_descriptor()), 0)
-    ok = dict(hidden=256, weight=256, labels=256)
+    ok = dict(hidden=256, weight=256, labels=256, rows=1000, vocab=40000)
+    n, ws = lib.gridmm_vocab_loss_saved_bytes(ctypes.byref(_descriptor(**ok))), lib.gridmm_vocab_loss_workspace(ctypes.byref(_descriptor(**ok)), 0)
     for over, args in ((dict(hidden=0), (256, 256, n, 256, ws)), (dict(weight=0), (256, 256, n, 256, ws)), (dict(labels=0), (256, 256, n, 256, ws)),
                        (dict(ld_hidden=63), (256, 256, n, 256, ws)), (dict(ld_weight=63), (256, 256, n, 256, ws)),
                        ({}, (0, 256, n, 256, ws)), ({}, (256, 0, n, 256, ws)), ({}, (256, 256, n - 1, 256, ws)),
@@ -812,7 +812,7 @@ def test_the_c_entry_refuses_bad_sizes_and_pointers():
                        (dict(slots=4, ids=256, ld_ids=4, ld_teacher=4), (256, 256, 1 << 40, 256, 1 << 40)),
                        (dict(slots=4, ids=256, teacher=256, ld_ids=3, ld_teacher=4), (256, 256, 1 << 40, 256, 1 << 40))):
         assert lib.gridmm_vocab_loss_fwd(ctypes.byref(_descriptor(**{**ok, **over})), *args, None) == EINVAL, (over, args)
-    wb = lib.gridmm_vocab_loss_workspace(ctypes.byref(_descriptor()), 1)
+    wb = lib.gridmm_vocab_loss_workspace(ctypes.byref(_descriptor(**ok)), 1)
     for over, args in (({}, (256, n, 0, 1, 256, 256, 0, 256, wb)), ({}, (256, n, 256, 1, 0, 0, 0, 256, wb)), ({}, (256, n, 256, -1, 256, 0, 0, 256, wb)),
                        ({}, (256, n, 256, 1, 256, 0, 256, 256, wb)), ({}, (256, n, 256, 1, 256, 0, 0, 256, wb - 1))):
         assert lib.gridmm_vocab_loss_bwd(ctypes.byref(_descriptor(**{**ok, **over})), *args, None) == EINVAL, (over, args)
