@@ -8,8 +8,8 @@
 //                   dh = dS W,   dW = dS^T h,   db_j = sum_r dS_rj
 // Forward: the score tile's epilogue leaves each row's (maximum, sum of exponentials) of its columns; a second, small kernel joins
 // them.  Backward: the scores are computed again piece by piece, the epilogue turns them into 16-bit dS (one piece at a time, the
-// workspace bounds its width), and two more products read it.  The entries of dS at a target are written by a kernel of their own
-// from the target's fp32 score: exp(..) - p is rounded once there, whatever cancels.
+// workspace bounds its width), and two more products read it.  The entries of dS at a target come from the target's own fp32
+// score: exp(..) - p is rounded once there, whatever cancels.
 //
 // Rows that do not count (label == ignore_index; no filled slot) are left out on the device: the counted rows are compacted into
 // the packed copy of h, the grids are sized for all rows and workgroups past the count end at once -- no host read-back.
@@ -367,6 +367,7 @@ struct TargetArgs {
   float unit;
   const Meta* meta;
   const int* rowmap;
+  int* label;      // [compacted row], -1 outside the vocabulary; NULL: distillation
   float* zt;       // [compacted row][slots]: HALF the score in base 2, where a bias of the lowest finite number is still finite
 };
 // NS dot products of one row of h with rows of W, their loads in flight together
@@ -430,6 +431,7 @@ __device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block
   for (int s = 0; s < NS; ++s) {
     if (lane != s || s0 + s >= a.slots) continue;
     // an id outside the vocabulary spoils its row; an empty slot has no score
+    if (a.label) a.label[i] = id[s] >= 0 && id[s] < a.vocab ? (int)id[s] : -1;
     const float half = 0.5f * a.unit, b = a.bias ? load_as_f32(a.bias, at[s], a.bias_dtype) * half : 0.f;
     a.zt[i * a.slots + s0 + s] = a.kd && id[s] < 0 ? 0.f : id[s] < 0 || id[s] >= a.vocab ? NAN : fmaf(z[s], half, b);
   }
@@ -517,32 +519,41 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
 }
 
 // ---- backward ----
-// scale exponent of dS from the largest finite |g T| and the scaled factor of every compacted row (zero past the count)
-__global__ __launch_bounds__(PREP_T) void grad_scale_kernel(const float* __restrict__ g, int64_t gs, float temperature,
-                                                            const int* __restrict__ rowmap, const Meta* __restrict__ meta,
-                                                            int* __restrict__ scale, float* __restrict__ grow, int Rp) {
-  __shared__ float part[16];
-  const int tid = threadIdx.x, count = meta->count;
+struct GradArgs {
+  const float* g;              // upstream gradients of the rows as they came
+  int64_t gs;
+  float temperature;
+  const int* rowmap;
+  const int* label;            // of the compacted rows; NULL: distillation, whose targets a kernel of their own writes
+  const float *zt, *lse;
+  int* scale;                  // exponent of the power of two that dS is scaled by
+};
+// That exponent, from the largest finite |g T|: every workgroup finds it for itself (a launch of its own: 10 us).  bf16 has fp32's range
+// and needs none.
+template <class T>
+__device__ __forceinline__ int grad_exponent(const GradArgs& a, int count, float* part) {
+  if constexpr (!T::F16) return 0;
   float m = 0.f;
-  for (int i = tid; i < count; i += PREP_T) m = fmaxf(m, finite_abs(g[(int64_t)rowmap[i] * gs] * temperature));
+#pragma unroll 4
+  for (int i = threadIdx.x; i < count; i += T::THREADS) m = fmaxf(m, finite_abs(a.g[(int64_t)a.rowmap[i] * a.gs] * a.temperature));
   m = wave_max(m);
-  if ((tid & 63) == 0) part[tid >> 6] = m;
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
   __syncthreads();
-  for (int w = 0; w < 16; ++w) m = fmaxf(m, part[w]);
-  const int sg = scale_exp(m, 13);
-  if (tid == 0) *scale = sg;
-  for (int i = tid; i < Rp; i += PREP_T) grow[i] = i < count ? ldexpf(g[(int64_t)rowmap[i] * gs] * temperature, sg) : 0.f;
+#pragma unroll
+  for (int w = 0; w < T::NW; ++w) m = fmaxf(m, part[w]);
+  return __builtin_amdgcn_readfirstlane(scale_exp(m, 13));
 }
 
 // A wave's 32 x 64 values of an epilogue, of 16 or 32 bits, through its own LDS: lane l puts the runs of 4 columns it holds of row
 // l & 31, and takes 16 bytes at a time of rows that lie whole in 8 (16 bits) or 16 (32 bits, 32 columns a pass) lanes: 128 contiguous
 // bytes a row instead of 16 or 32.
-template <class Put>
-__device__ __forceinline__ void rows_of_16(unsigned short* scratch, const u16x4_t (&v)[8], Put put) {
+template <class Patch, class Put>
+__device__ __forceinline__ void rows_of_16(unsigned short* scratch, const u16x4_t (&v)[8], Patch patch, Put put) {
   const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   // run n q (8 columns 8 (4 n + q) ..) half h: 8 bytes at column 32 n + 8 q + 4 h, 16-byte chunks swizzled by the row
 #pragma unroll
   for (int i = 0; i < 8; ++i) *reinterpret_cast<u16x4_t*>(scratch + r * 64 + ((i ^ (r & 7)) * 8) + h * 4) = v[i];
+  patch([&](int c) -> unsigned short& { return scratch[r * 64 + (((c >> 3) ^ (r & 7)) * 8) + (c & 7)]; });      // column c of row r
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
@@ -566,11 +577,11 @@ __device__ __forceinline__ void rows_of_32(unsigned short* scratch, const float4
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// dS of the columns [j0, j0 + C): dS[r][j] = grow_r exp2(y_rj - lse_r), two planes for fp32 operands
+// dS of the columns [j0, j0 + C): dS[r][j] = g_r T exp2(y_rj - lse_r), two planes for fp32 operands; at the row's label, from its fp32
+// score, g_r (exp2(..) - 1)
 template <class T>
 __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Operand B, int nk, int tn, const Meta* __restrict__ meta,
-                                                                const float* __restrict__ biasz, float unit,
-                                                                const float* __restrict__ lse, const float* __restrict__ grow,
+                                                                const float* __restrict__ biasz, float unit, const GradArgs G, int64_t j0,
                                                                 unsigned short* __restrict__ dS, int64_t ldS, int64_t plane) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
   const int count = __builtin_amdgcn_readfirstlane(meta->count), tm = (count + T::BM - 1) / T::BM;
@@ -579,6 +590,8 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
   const float sc = ldexpf(unit, -(meta->sh + meta->sw));
   unsigned short* scratch = smem + T::LDS + wave * 2048;
   static_assert(T::TN == 2, "64 columns a wave");
+  const int sg = grad_exponent<T>(G, count, reinterpret_cast<float*>(smem + T::LDS));
+  if (blockIdx.x == 0 && threadIdx.x == 0) *G.scale = sg;
   T::run(
       A, B, smem,
       [&](int n, Item& it) {
@@ -591,12 +604,22 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
       [&](const Item& it, typename T::Acc& acc, const float*) {
         const int64_t r0 = it.bm + wr * T::WM, c0 = it.bn + wc * T::WN;
         const float* bz = biasz + c0 + (lane >> 5) * 4;
+        // what the rows need, its loads in flight together
+        float Ls[T::TM], gs[T::TM];
+        int ys[T::TM];
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) {
+          const int r = (int)r0 + i * 32 + (lane & 31), rl = min(r, count - 1);
+          const float l = G.lse[rl], g = G.g[G.rowmap[rl] * G.gs] * G.temperature;
+          ys[i] = G.label && r < count && lane < 32 ? G.label[rl] - (int)(j0 + c0) : -1;
+          Ls[i] = r < count ? l : 1e30f;
+          gs[i] = r < count ? ldexpf(g, sg) : 0.f;      // (a row past the count: 0 times exp2(-1e30))
+        }
 #pragma unroll
         for (int i = 0; i < T::TM; ++i) {
           __builtin_amdgcn_sched_barrier(0);
-          const int64_t r = r0 + i * 32 + (lane & 31);
-          const bool live = r < count;
-          const float L = live ? lse[r] : 1e30f, gr = live ? grow[r] : 0.f;      // (a row past the count: 0 times exp2(-1e30))
+          const float L = Ls[i], gr = gs[i];
+          const int y = ys[i];
           u16x4_t hi[8], lo[8];
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
@@ -613,25 +636,31 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
             }
           }
           unsigned short* at = dS + (r0 + i * 32) * ldS + c0;
-          rows_of_16(scratch, hi, [&](int row, int cc, u16x8_t v) { *reinterpret_cast<u16x8_t*>(at + row * ldS + cc) = v; });
+          const bool hit = y >= 0 && y < 64;
+          float target = 0.f;
+          if (hit) target = gr * (__builtin_amdgcn_exp2f(2.f * G.zt[r0 + i * 32 + lane] - L) - 1.f);
+          const unsigned short th = T::F16 ? to_f16(target) : to_bf16(target);
+          rows_of_16(scratch, hi, [&](auto column) { if (hit) column(y) = th; },
+                     [&](int row, int cc, u16x8_t v) { *reinterpret_cast<u16x8_t*>(at + row * ldS + cc) = v; });
           if constexpr (T::PL == 2)
-            rows_of_16(scratch, lo, [&](int row, int cc, u16x8_t v) { *reinterpret_cast<u16x8_t*>(at + plane + row * ldS + cc) = v; });
+            rows_of_16(scratch, lo, [&](auto column) { if (hit) column(y) = to_f16(target - (float)__builtin_bit_cast(_Float16, th)); },
+                       [&](int row, int cc, u16x8_t v) { *reinterpret_cast<u16x8_t*>(at + plane + row * ldS + cc) = v; });
         }
       });
 }
 
-// the entries of dS at the targets in [j0, j0 + C): grow_r (exp2(zt - lse) - sum of p over the slots of the same id), rounded once
+// the entries of dS at a teacher's targets in [j0, j0 + C): g_r T (exp2(z - lse) - sum of p over the slots of the same id), rounded once
 struct FixArgs {
   const void* index;
   int64_t ld_index, j0, ldS, plane;
   int wide, slots, C, vocab, dtype;
   const Meta* meta;
-  const int* rowmap;
-  const float *p, *zt, *lse, *grow;
+  GradArgs G;
+  const float* p;
   unsigned short* dS;
 };
 __device__ __forceinline__ void target_entry(const FixArgs& a, int64_t i, int s, int64_t id, float p) {
-  const float v = a.grow[i] * (__builtin_amdgcn_exp2f(2.f * a.zt[i * a.slots + s] - a.lse[i]) - p);
+  const float v = ldexpf(a.G.g[a.G.rowmap[i] * a.G.gs] * a.G.temperature, *a.G.scale) * (__builtin_amdgcn_exp2f(2.f * a.G.zt[i * a.slots + s] - a.G.lse[i]) - p);
   unsigned short* at = a.dS + i * a.ldS + (id - a.j0);
   if (a.dtype == F32) {
     const _Float16 h = (_Float16)v;
@@ -641,19 +670,13 @@ __device__ __forceinline__ void target_entry(const FixArgs& a, int64_t i, int s,
     at[0] = a.dtype == F16 ? to_f16(v) : to_bf16(v);
   }
 }
-__global__ __launch_bounds__(256) void label_grad_kernel(const FixArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.meta->count) return;
-  const int64_t id = load_index(a.index, a.rowmap[i], a.wide);
-  if (id >= a.j0 && id < a.j0 + a.C && id < a.vocab && id >= 0) target_entry(a, i, 0, id, 1.f);
-}
 // one row a workgroup, 256 of its slots in LDS at a time; several slots may name one id: each of them writes the same value
 __global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
   __shared__ int sid[256];
   __shared__ float sp[256];
   const int64_t i = blockIdx.x;
   if (i >= a.meta->count) return;
-  const int64_t r = a.rowmap[i];
+  const int64_t r = a.G.rowmap[i];
   for (int s0 = 0; s0 < a.slots; s0 += 256) {
     const int s = s0 + threadIdx.x;
     const int64_t id = s < a.slots ? load_index(a.index, r * a.ld_index + s, a.wide) : -1;
@@ -812,7 +835,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, O
               const int q = (c & 3) * 4;
               v[c] = to_16x4<T::F16>(ldexpf(x[q], e), ldexpf(x[q + 1], e), ldexpf(x[q + 2], e), ldexpf(x[q + 3], e));
             }
-            rows_of_16(scratch, v, [&](int row, int cc, u16x8_t x) {
+            rows_of_16(scratch, v, [](auto) {}, [&](int row, int cc, u16x8_t x) {
               const int64_t r = r0 + i * 32 + row, c = c0 + cc;
               if (r >= vocab || c >= K) return;
               if (K % 8 == 0) {
@@ -878,11 +901,11 @@ struct Plan {
   bool keep_w;                 // ... and its copy, one piece, stays for the backward (28 us of 396 at 30522 x 768 fp32)
   int64_t C_fwd, C_bwd;        // columns a piece
   // saved
-  size_t o_meta, o_rowmap, o_rowinv, o_lse, o_zt, o_p, o_biasz, o_h, o_w, saved;
+  size_t o_meta, o_rowmap, o_rowinv, o_lse, o_zt, o_label, o_p, o_biasz, o_h, o_w, saved;
   // forward workspace
   size_t f_counts, f_plogp, f_amax, f_stats, f_w, fwd;
   // backward workspace
-  size_t b_scale, b_grow, b_ds, b_w, b_part, bwd;
+  size_t b_scale, b_ds, b_w, b_part, bwd;
 };
 
 bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
@@ -946,6 +969,7 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.o_rowinv = take(R * 4);
   P.o_lse = take(Rp * 4);
   P.o_zt = take(R * S * 4);
+  P.o_label = take(d->slots ? 0 : R * 4);
   P.o_p = take(d->slots ? R * S * 4 : 0);
   P.o_biasz = take(P.Vp * 4);
   P.o_h = take(Rp * P.Kp * 2 * P.PL);
@@ -960,7 +984,6 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.fwd = o;
   o = 0;
   P.b_scale = take(4);
-  P.b_grow = take(Rp * 4);
   P.b_ds = take(Rp * (size_t)P.C_bwd * 2 * P.PL);
   P.b_w = take(P.pack_w && !P.keep_w ? (size_t)P.C_bwd * P.Kp * 2 * P.PL : 0);
   // with more than one range the ranges' tiles number at most 512 of 128 x 128 or 256 of 256 x 256, else the rows' product once
@@ -1119,6 +1142,7 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   t.ldh = d->ld_hidden; t.ldw = d->ld_weight; t.ld_index = d->slots ? d->ld_ids : 1;
   t.K = d->hidden_size; t.vocab = d->vocab; t.slots = P.slots; t.wide = d->index64; t.kd = d->slots > 0;
   t.bias = d->bias; t.bias_dtype = d->bias_dtype; t.unit = unit; t.meta = meta; t.rowmap = rowmap; t.zt = zt;
+  t.label = d->slots ? nullptr : (int*)(sv + P.o_label);
   const int rc = by_dtype(d, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const int hb = (int)(P.Rp / 4);
@@ -1199,12 +1223,11 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
   const float *lse = (const float*)(sv + P.o_lse), *zt = (const float*)(sv + P.o_zt);
   const float *p = d->slots ? (const float*)(sv + P.o_p) : nullptr, *biasz = (const float*)(sv + P.o_biasz);
   const unsigned short* Hp = (const unsigned short*)(sv + P.o_h);
-  float *grow = (float*)(ws + P.b_grow), *part = (float*)(ws + P.b_part);
+  float* part = (float*)(ws + P.b_part);
   unsigned short *dS = (unsigned short*)(ws + P.b_ds), *wbuf = (unsigned short*)(ws + P.b_w);
   const float unit = LOG2E / d->temperature;
 
-  GRIDMM_LAUNCH(grad_scale_kernel, dim3(1), dim3(PREP_T), 0, st, grad, grad_stride, d->temperature, rowmap, meta, scale, grow, (int)P.Rp);
-  GRIDMM_CHECK_LAUNCH();
+  const GradArgs G{grad, grad_stride, d->temperature, rowmap, d->slots ? nullptr : (const int*)(sv + P.o_label), zt, lse, scale};
   const Operand H{Hp, P.PL * P.Kp, P.Kp, P.Rp, P.Kp};
   for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_bwd) {
     const int64_t C = std::min(P.C_bwd, P.Vp - j0);
@@ -1220,18 +1243,19 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
         using T = TileOf<F, L, decltype(big)::value, false, false>;
         const int64_t tn = C / T::BN, tm = (rows + T::BM - 1) / T::BM;
         GRIDMM_LAUNCH((score_grad_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), (int)tn, meta,
-                      biasz + j0, unit, lse, grow, dS, ldS, C);
+                      biasz + j0, unit, G, j0, dS, ldS, C);
         GRIDMM_CHECK_LAUNCH();
         return GRIDMM_OK;
       });
       if (rc != GRIDMM_OK) return rc;
-      FixArgs f;
-      f.index = d->slots ? d->ids : d->labels; f.ld_index = d->slots ? d->ld_ids : 1; f.j0 = j0; f.ldS = ldS; f.plane = C;
-      f.wide = d->index64; f.slots = P.slots; f.C = (int)C; f.vocab = d->vocab; f.dtype = d->dtype; f.meta = meta; f.rowmap = rowmap;
-      f.p = p; f.zt = zt; f.lse = lse; f.grow = grow; f.dS = dS;
-      if (d->slots) GRIDMM_LAUNCH(target_grad_kernel, dim3(d->rows), dim3(256), 0, st, f);
-      else GRIDMM_LAUNCH(label_grad_kernel, dim3((d->rows + 255) / 256), dim3(256), 0, st, f);
-      GRIDMM_CHECK_LAUNCH();
+      if (d->slots) {
+        FixArgs f;
+        f.index = d->ids; f.ld_index = d->ld_ids; f.j0 = j0; f.ldS = ldS; f.plane = C;
+        f.wide = d->index64; f.slots = P.slots; f.C = (int)C; f.vocab = d->vocab; f.dtype = d->dtype; f.meta = meta; f.G = G;
+        f.p = p; f.dS = dS;
+        GRIDMM_LAUNCH(target_grad_kernel, dim3(d->rows), dim3(256), 0, st, f);
+        GRIDMM_CHECK_LAUNCH();
+      }
       if (d_hidden) {
         rc = by_tile(d->rows, P.C_bwd, [&](auto big, int rows) {
           using T = TileOf<F, L, decltype(big)::value, false, true>;
