@@ -110,10 +110,14 @@ struct Tile {
   // that this one's buffer is free; the transfers of the stage after next -- of the next tile, near a tile's end -- start right there.
   // While done() works on a tile the next one's first fragments are in registers and its second stage is on the way.
   //
+  // twice != 0 (elements): an A of two planes over a B of one, C = (A + A') B with A' that far behind A: an item's nk stages are its range
+  // of the contraction once with A and once with A'.
+  //
   // SUMA: sums also takes the sums of A over the contraction for the waves that want_sums(item) names, lane l those of the steps that
   // it holds of row 32 i + (l & 31); lanes l and l ^ 32 together hold all.
   template <bool SUMA = false, class Work, class Want, class Done>
-  static __device__ __forceinline__ void run(const Operand& A, const Operand& B, unsigned short* smem, Work work, Want want_sums, Done done) {
+  static __device__ __forceinline__ void run(const Operand& A, const Operand& B, unsigned short* smem, Work work, Want want_sums, Done done,
+                                             int64_t twice = 0) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave / WAVES_N, wc = wave % WAVES_N;
@@ -164,14 +168,17 @@ struct Tile {
     auto point = [&] {
       to = __builtin_amdgcn_readfirstlane(lds0 + (issued & 1) * (STAGE * 2));
       if (!have) return;
-      from = base + akt * step;
+      const bool again = twice && akt >= ahead.nk >> 1;
+      const int kt = again ? akt - (ahead.nk >> 1) : akt;
+      from = base + kt * step;
       if (COLA || COLB) {
-        const int64_t first = ahead.k0 + (int64_t)akt * BK, last = O.rows - 1 - first;
-        if (col && last < BK - 1) {              // (the last stages of an item: the next item aims anew)
+        const int64_t first = ahead.k0 + (int64_t)kt * BK, last = O.rows - 1 - first;
+        if (col && (last < BK - 1 || (again && kt == 0))) {       // (the last stages of a range; what follows aims anew)
           if (last < 0) from = O.p + (O.rows - 1) * O.ld;
-          aim(last < 0 ? 0 : (int)last);
+          aim(last < 0 ? 0 : last < BK - 1 ? (int)last : BK - 1);
         }
       }
+      if (again && isA) from += twice;
       from = uniform(from);
     };
     auto piece = [&](int i) { dma16(from, off[i], to + i * 1024); };

@@ -15,7 +15,7 @@
 // the packed copy of h, the grids are sized for all rows and workgroups past the count end at once -- no host read-back.
 //
 // Number formats.  bf16 / fp16 operands: one plane, products exact, sums fp32; dS is rounded to the operands' type (2^-8 / 2^-11
-// of an entry at most, like the gradients themselves).  fp32 operands: two fp16 planes each (22 bits) after a
+// of an entry at most, like the gradients themselves), with few counted rows to two planes of it.  fp32 operands: two fp16 planes each (22 bits) after a
 // power-of-two scale from the tensor's largest finite value, so a product is off by ~2^-22: like fp32 sums.  dS is scaled by a power of
 // two from the largest |g T| of the call (fp16 range: entries below 2^-38 of it vanish).
 // Everything runs in the base-2 domain: y = z log2 e, exp2, and ln 2 comes back in the losses.
@@ -85,7 +85,7 @@ struct Meta {
 // of 4 waves a CU).  The host does not know the count: where both may be right it launches both, each sized for its own range, and the
 // workgroups of the one whose turn it is not end at once.
 constexpr int BIG_TILES = 384;       // 1.5 rounds of 256 CUs
-__host__ __device__ inline bool big_tiles(int64_t count, int64_t C) { return count > 128 && (count + 255) / 256 * (C / 256) >= BIG_TILES; }
+__host__ __device__ inline bool big_tiles(int64_t count, int64_t C) { return count > 256 && (count + 255) / 256 * (C / 256) >= BIG_TILES; }
 // contraction ranges of dh: enough workgroups for two rounds of the chip, at least 8 stages of 64 columns a range
 __host__ __device__ inline int hidden_splits(int64_t count, int64_t Kp, int64_t C, bool big) {
   const int64_t T = big ? 256 : 128, tiles = ((count + T - 1) / T) * ((Kp + T - 1) / T);
@@ -577,12 +577,12 @@ __device__ __forceinline__ void rows_of_32(unsigned short* scratch, const float4
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// dS of the columns [j0, j0 + C): dS[r][j] = g_r T exp2(y_rj - lse_r), two planes for fp32 operands; at the row's label, from its fp32
+// dS of the columns [j0, j0 + C): dS[r][j] = g_r T exp2(y_rj - lse_r), two planes for fp32 operands and few rows (TWO); at the row's label, from its fp32
 // score, g_r (exp2(..) - 1)
-template <class T>
+template <class T, bool TWO>
 __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Operand B, int nk, int tn, const Meta* __restrict__ meta,
                                                                 const float* __restrict__ biasz, float unit, const GradArgs G, int64_t j0,
-                                                                unsigned short* __restrict__ dS, int64_t ldS, int64_t plane) {
+                                                                unsigned short* __restrict__ dS, int64_t plane) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
   const int count = __builtin_amdgcn_readfirstlane(meta->count), tm = (count + T::BM - 1) / T::BM;
   if (big_tiles(count, (int64_t)tn * T::BN) != (T::BM == 256)) return;
@@ -590,6 +590,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
   const float sc = ldexpf(unit, -(meta->sh + meta->sw));
   unsigned short* scratch = smem + T::LDS + wave * 2048;
   static_assert(T::TN == 2, "64 columns a wave");
+  const int64_t ldS = T::PL == 2 || TWO ? 2 * plane : plane;
   const int sg = grad_exponent<T>(G, count, reinterpret_cast<float*>(smem + T::LDS));
   if (blockIdx.x == 0 && threadIdx.x == 0) *G.scale = sg;
   T::run(
@@ -620,31 +621,34 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
           __builtin_amdgcn_sched_barrier(0);
           const float L = Ls[i], gr = gs[i];
           const int y = ys[i];
-          u16x4_t hi[8], lo[8];
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const float4 b = *reinterpret_cast<const float4*>(bz + c * 8);
-            const float bb[4] = {b.x, b.y, b.z, b.w};
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = gr * __builtin_amdgcn_exp2f(fmaf(acc[i][c >> 2][(c & 3) * 4 + e], sc, bb[e]) - L);
-            hi[c] = to_16x4<T::F16>(v[0], v[1], v[2], v[3]);
-            if constexpr (T::PL == 2) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) v[e] -= (float)__builtin_bit_cast(_Float16, (unsigned short)hi[c][e]);
-              lo[c] = to_16x4<true>(v[0], v[1], v[2], v[3]);
-            }
-          }
-          unsigned short* at = dS + (r0 + i * 32) * ldS + c0;
           const bool hit = y >= 0 && y < 64;
           float target = 0.f;
           if (hit) target = gr * (__builtin_amdgcn_exp2f(2.f * G.zt[r0 + i * 32 + lane] - L) - 1.f);
-          const unsigned short th = T::F16 ? to_f16(target) : to_bf16(target);
-          rows_of_16(scratch, hi, [&](auto column) { if (hit) column(y) = th; },
-                     [&](int row, int cc, u16x8_t v) { *reinterpret_cast<u16x8_t*>(at + row * ldS + cc) = v; });
-          if constexpr (T::PL == 2)
-            rows_of_16(scratch, lo, [&](auto column) { if (hit) column(y) = to_f16(target - (float)__builtin_bit_cast(_Float16, th)); },
-                       [&](int row, int cc, u16x8_t v) { *reinterpret_cast<u16x8_t*>(at + plane + row * ldS + cc) = v; });
+          auto rounded = [](float x) {
+            const unsigned short u = T::F16 ? to_f16(x) : to_bf16(x);
+            return T::F16 ? (float)__builtin_bit_cast(_Float16, u) : bf16_bits_to_f32(u);
+          };
+          auto values = [&](int c, float (&v)[4]) {
+            const float4 b = *reinterpret_cast<const float4*>(bz + c * 8);
+            const float bb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = gr * __builtin_amdgcn_exp2f(fmaf(acc[i][c >> 2][(c & 3) * 4 + e], sc, bb[e]) - L);
+          };
+          auto put = [&](const u16x4_t (&x)[8], float at_target, unsigned short* at) {
+            rows_of_16(scratch, x, [&](auto column) { if (hit) column(y) = T::F16 ? to_f16(at_target) : to_bf16(at_target); },
+                       [&](int row, int cc, u16x8_t v) { *reinterpret_cast<u16x8_t*>(at + row * ldS + cc) = v; });
+          };
+          unsigned short* at = dS + (r0 + i * 32) * ldS + c0;
+          u16x4_t hi[8], lo[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float v[4];
+            values(c, v);
+            hi[c] = to_16x4<T::F16>(v[0], v[1], v[2], v[3]);
+            if constexpr (T::PL == 2 || TWO) lo[c] = to_16x4<T::F16>(v[0] - rounded(v[0]), v[1] - rounded(v[1]), v[2] - rounded(v[2]), v[3] - rounded(v[3]));
+          }
+          put(hi, target, at);
+          if constexpr (T::PL == 2 || TWO) put(lo, target - rounded(target), at + plane);
         }
       });
 }
@@ -662,13 +666,8 @@ struct FixArgs {
 __device__ __forceinline__ void target_entry(const FixArgs& a, int64_t i, int s, int64_t id, float p) {
   const float v = ldexpf(a.G.g[a.G.rowmap[i] * a.G.gs] * a.G.temperature, *a.G.scale) * (__builtin_amdgcn_exp2f(2.f * a.G.zt[i * a.slots + s] - a.G.lse[i]) - p);
   unsigned short* at = a.dS + i * a.ldS + (id - a.j0);
-  if (a.dtype == F32) {
-    const _Float16 h = (_Float16)v;
-    at[0] = __builtin_bit_cast(unsigned short, h);
-    at[a.plane] = to_f16(v - (float)h);
-  } else {
-    at[0] = a.dtype == F16 ? to_f16(v) : to_bf16(v);
-  }
+  at[0] = a.dtype == BF16 ? to_bf16(v) : to_f16(v);
+  if (a.ldS > a.plane) at[a.plane] = a.dtype == BF16 ? to_bf16(v - bf16_bits_to_f32(at[0])) : to_f16(v - (float)__builtin_bit_cast(_Float16, at[0]));
 }
 // one row a workgroup, 256 of its slots in LDS at a time; several slots may name one id: each of them writes the same value
 __global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
@@ -700,7 +699,7 @@ __global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
 
 // dh of this piece: partial products over the contraction ranges blockIdx.y, added to those of the pieces before.  `C`: the columns of
 // a whole piece, which fix the tile and the number of ranges for all pieces.
-template <class T>
+template <class T, bool TWO>
 __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, Operand B, int steps, int tn, int64_t C,
                                                                  const Meta* __restrict__ meta, float* __restrict__ part, int64_t Kp,
                                                                  int first) {
@@ -716,7 +715,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, O
       [&](int n, Item& it) {
         unsigned ty, tx, split;
         if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, splits, ty, tx, split)) return false;
-        it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, (int64_t)split * per * T::BK, min(per, steps - (int)split * per), (int)split};
+        it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, (int64_t)split * per * T::BK, min(per, steps - (int)split * per) * (TWO ? 2 : 1), (int)split};
         return true;
       },
       [](const Item&) { return false; },
@@ -738,7 +737,8 @@ __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, O
               *at = x;
             });
           }
-      });
+      },
+      TWO ? A.cols : 0);
 }
 
 // dh = the ranges' partial products in order, unscaled, to the rows they came from; zero for rows that do not count.  A workgroup
@@ -773,12 +773,13 @@ __global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict
 
 // dW of this piece: rows [j0, j0 + C) complete (the contraction is all counted rows), written once in the weight's type; the first
 // tile column also sums dS over the rows: db
-template <class T>
+template <class T, bool TWO>
 __global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, Operand B, int tm, int tn, const Meta* __restrict__ meta,
                                                                  const int* __restrict__ scale, int dtype, int64_t j0, int vocab, int K,
                                                                  void* __restrict__ dW, int bias_dtype, void* __restrict__ db) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
-  const int count = __builtin_amdgcn_readfirstlane(meta->count), nk = (count + T::BK - 1) / T::BK;
+  const int count = __builtin_amdgcn_readfirstlane(meta->count);
+  const int nk = (count + T::BK - 1) / T::BK * (TWO ? 2 : 1);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
   const int eb = -*scale, e = eb - meta->sh;       // exponents of the units of db and dW
   unsigned short* scratch = smem + T::LDS + wave * 2048;
@@ -847,7 +848,8 @@ __global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, O
             });
           }
         }
-      });
+      },
+      TWO ? A.cols : 0);
 }
 
 __global__ void zero_u16_kernel(unsigned short* __restrict__ p, int64_t n) {
@@ -892,9 +894,15 @@ bool few_rows(const gridmm_vocab_loss_t* d) {
   return K <= 384 && m <= (fp32 ? 4 : 16) && rv * K <= 2e8;
 }
 
+// 16-bit operands: dS in two planes, entry = hi + lo, for up to so many rows.  A gradient that a handful of entries makes up shows the
+// rounding of each, a sum over many rows their mean: one plane leaves 1.4 times the error of the gradients' own rounding at thousands of
+// rows, up to twice that at a few.  So few rows are bound by the read of W and the write of dW, not by the products (128 x 128 tiles;
+// in the kernels of the large tile the second plane's registers cost 1.5 % at 8030 x 131072 x 2048).
+constexpr int TWO_PLANES = 256;
+
 struct Plan {
   int PL, slots;               // planes; target slots a row (cross entropy: 1)
-  bool few;
+  bool few, two;
   int RP, groups, ranges, range;      // few rows: rows a group (16 or 32), groups; ranges of the vocabulary in dh and their rows
   int64_t Rp, Kp, Vp;
   bool pack_w;                 // W has to be split or padded; else it is read where it lies
@@ -984,7 +992,8 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.fwd = o;
   o = 0;
   P.b_scale = take(4);
-  P.b_ds = take(Rp * (size_t)P.C_bwd * 2 * P.PL);
+  P.two = P.PL == 1 && d->rows <= TWO_PLANES;
+  P.b_ds = take(Rp * (size_t)P.C_bwd * 2 * (P.two ? 2 : P.PL));
   P.b_w = take(P.pack_w && !P.keep_w ? (size_t)P.C_bwd * P.Kp * 2 * P.PL : 0);
   // with more than one range the ranges' tiles number at most 512 of 128 x 128 or 256 of 256 x 256, else the rows' product once
   P.b_part = take(std::max<size_t>(Rp * (size_t)P.Kp, std::min<size_t>(64 * Rp * (size_t)P.Kp, 256 * 256 * 256)) * 4);
@@ -1019,7 +1028,7 @@ int by_type(const gridmm_vocab_loss_t* d, F f) {
 template <class F>
 int by_tile(int rows, int64_t C, F f) {
   // the largest count that takes the small tile
-  const int64_t small = std::max<int64_t>(128, (BIG_TILES + C / 256 - 1) / (C / 256) * 256 - 256);
+  const int64_t small = std::max<int64_t>(256, (BIG_TILES + C / 256 - 1) / (C / 256) * 256 - 256);
   int rc = f(std::bool_constant<false>{}, (int)std::min<int64_t>(rows, small));
   if (rc == GRIDMM_OK && rows > small) rc = f(std::bool_constant<true>{}, rows);
   return rc;
@@ -1234,18 +1243,26 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
     Operand W;
     int rc = weight_piece(d, P, j0, C, meta, (unsigned short*)(sv + P.o_w), false, wbuf, st, W);
     if (rc != GRIDMM_OK) return rc;
-    const int64_t ldS = P.PL * C;
+    const int64_t ldS = (P.two ? 2 : P.PL) * C;
     const Operand S{dS, ldS, C, P.Rp, C};
     rc = by_type(d, [&](auto f16, auto pl) {
       constexpr bool F = decltype(f16)::value;
       constexpr int L = decltype(pl)::value;
+      // calls f(two planes?): only the small tile has them
+      auto one_or_two = [&](auto big, auto f) {
+        if constexpr (L == 1 && !decltype(big)::value)
+          if (P.two) return f(std::true_type{});
+        return f(std::false_type{});
+      };
       int rc = by_tile(d->rows, C, [&](auto big, int rows) {
         using T = TileOf<F, L, decltype(big)::value, false, false>;
         const int64_t tn = C / T::BN, tm = (rows + T::BM - 1) / T::BM;
-        GRIDMM_LAUNCH((score_grad_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), (int)tn, meta,
-                      biasz + j0, unit, G, j0, dS, ldS, C);
-        GRIDMM_CHECK_LAUNCH();
-        return GRIDMM_OK;
+        return one_or_two(big, [&](auto two) {
+          GRIDMM_LAUNCH((score_grad_kernel<T, decltype(two)::value>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, H, W,
+                        (int)(P.Kp / T::BK), (int)tn, meta, biasz + j0, unit, G, j0, dS, C);
+          GRIDMM_CHECK_LAUNCH();
+          return GRIDMM_OK;
+        });
       });
       if (rc != GRIDMM_OK) return rc;
       if (d->slots) {
@@ -1260,10 +1277,12 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
         rc = by_tile(d->rows, P.C_bwd, [&](auto big, int rows) {
           using T = TileOf<F, L, decltype(big)::value, false, true>;
           const int64_t tn = (P.Kp + T::BN - 1) / T::BN, tm = (rows + T::BM - 1) / T::BM;
-          GRIDMM_LAUNCH((hidden_grad_kernel<T>), dim3(blocks<T>(tm * tn * hidden_splits(1, P.Kp, P.C_bwd, T::BM == 256))), dim3(T::THREADS),
-                        0, st, S, W, (int)(C / T::BK), (int)tn, P.C_bwd, meta, part, P.Kp, j0 == 0);
-          GRIDMM_CHECK_LAUNCH();
-          return GRIDMM_OK;
+          return one_or_two(big, [&](auto two) {
+            GRIDMM_LAUNCH((hidden_grad_kernel<T, decltype(two)::value>), dim3(blocks<T>(tm * tn * hidden_splits(1, P.Kp, P.C_bwd, T::BM == 256))),
+                          dim3(T::THREADS), 0, st, S, W, (int)(C / T::BK), (int)tn, P.C_bwd, meta, part, P.Kp, j0 == 0);
+            GRIDMM_CHECK_LAUNCH();
+            return GRIDMM_OK;
+          });
         });
         if (rc != GRIDMM_OK) return rc;
       }
@@ -1271,12 +1290,14 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
         auto weight = [&](auto big) {
           using T = TileOf<F, L, decltype(big)::value, true, true>;
           const int64_t tn = d_weight ? (P.Kp + T::BN - 1) / T::BN : 1, tm = C / T::BM;      // (db alone: the first tile column)
-          GRIDMM_LAUNCH((weight_grad_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, S, H, (int)tm, (int)tn, meta, scale, d->dtype, j0,
-                        d->vocab, d->hidden_size, d_weight, d->bias_dtype, d_bias);
-          GRIDMM_CHECK_LAUNCH();
-          return GRIDMM_OK;
+          return one_or_two(big, [&](auto two) {
+            GRIDMM_LAUNCH((weight_grad_kernel<T, decltype(two)::value>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, S, H, (int)tm, (int)tn,
+                          meta, scale, d->dtype, j0, d->vocab, d->hidden_size, d_weight, d->bias_dtype, d_bias);
+            GRIDMM_CHECK_LAUNCH();
+            return GRIDMM_OK;
+          });
         };
-        rc = C / 256 * ((P.Kp + 255) / 256) >= BIG_TILES ? weight(std::true_type{}) : weight(std::false_type{});
+        rc = !P.two && C / 256 * ((P.Kp + 255) / 256) >= BIG_TILES ? weight(std::true_type{}) : weight(std::false_type{});
         if (rc != GRIDMM_OK) return rc;
       }
       return GRIDMM_OK;

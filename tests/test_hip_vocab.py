@@ -7,8 +7,8 @@ Tolerances are bounds, derived from the arithmetic (u = 2^-24 is half a step of 
              e_z = (c + K u) |h| . |W| + 4 u |z|,   c = 3 2^-22 (fp32), 0 (16 bits)
   loss       L is off by at most max e_z + the sum of exponentials (V u + 2 steps of exp2 / log2) -> + (V + 8) u (|L| + 1)
   dS entry   exp(z - L) is off by its own size times (e_z + e_L); a target adds its p times 4 u; then one rounding: half a step of
-             the 16-bit type, 2^-22 for two fp16 planes; fp16 has no step below 2^-24, and dS is scaled to 2^13 at most: 2^-36 of
-             the largest |g T|
+             the 16-bit type, its square in two planes (up to 256 rows), 2^-22 for fp32's two fp16 planes; fp16 has no step below
+             2^-24, and dS is scaled to 2^13 at most: 2^-36 of the largest |g T|
   gradients  the entries' errors times the other factor, plus (c + n u) of the sum of sizes, plus half a step of the output's type
 """
 import os
@@ -56,7 +56,7 @@ def _oracle(h, w, b, ids, p, T, g):
     target = torch.zeros_like(q).scatter_add_(1, slot, torch.where(ids >= 0, p, torch.zeros_like(p)))
     gt = (g.double() * T * live)[:, None]
     dS = gt * (q - target)
-    rnd = HALF[dt] if dt != torch.float32 else 2.0 ** -22
+    rnd = 2.0 ** -22 if dt == torch.float32 else HALF[dt] ** 2 if h.shape[0] <= 256 else HALF[dt]
     e_S = gt.abs() * (q * (e_z + e_L[:, None]) * 1.01 + 8 * U * (target + q)) + 4 * U * dS.abs()
     e_S = e_S + rnd * (dS.abs() + e_S) + (2.0 ** -36 * gt.abs().max() if dt != torch.bfloat16 else 0.0)
     out = {"loss": (loss, e_loss)}
