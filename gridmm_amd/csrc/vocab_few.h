@@ -39,20 +39,29 @@ struct FewArgs {
 template <int DT>
 __device__ __forceinline__ float few_1(const void* p, int64_t i) { return load_as_f32(p, i, DT); }
 
-// values k .. k + 3 of a row, widened (zero from K on)
-template <int DT, bool VEC>
+// Vectors on the boundaries of their elements: this chip's global loads take them, at up to twice the cache accesses.  Value by value
+// they took 2 - 3 times as long (16 bits, 1379 hidden).
+typedef float few_f4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned short few_u4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef short few_s8_any __attribute__((ext_vector_type(8), aligned(2)));
+
+// values k .. k + 3 of a row, widened.  FULL: all of them are the row's; else zero from K on
+template <int DT, bool VEC, bool FULL>
 __device__ __forceinline__ few_f4 few_load4(const void* p, int64_t off, int k, int K) {
   few_f4 v = {0.f, 0.f, 0.f, 0.f};
-  if constexpr (VEC) {                       // K % 4 == 0
-    const int at = k < K ? k : 0;
+  if constexpr (VEC || FULL) {               // (VEC: K % 4 == 0)
+    const int at = FULL || k < K ? k : 0;
     if constexpr (DT == F32) {
-      v = *reinterpret_cast<const few_f4*>((const float*)p + off + at);
+      if constexpr (VEC) v = *reinterpret_cast<const few_f4*>((const float*)p + off + at);
+      else v = *reinterpret_cast<const few_f4_any*>((const float*)p + off + at);
     } else {
-      const u16x4_t u = *reinterpret_cast<const u16x4_t*>((const unsigned short*)p + off + at);
+      u16x4_t u;
+      if constexpr (VEC) u = *reinterpret_cast<const u16x4_t*>((const unsigned short*)p + off + at);
+      else u = *reinterpret_cast<const few_u4_any*>((const unsigned short*)p + off + at);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = DT == BF16 ? bf16_bits_to_f32(u[e]) : (float)__builtin_bit_cast(_Float16, (unsigned short)u[e]);
     }
-    if (k >= K) v = (few_f4){0.f, 0.f, 0.f, 0.f};
+    if (!FULL && k >= K) v = (few_f4){0.f, 0.f, 0.f, 0.f};
   } else {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
@@ -60,14 +69,16 @@ __device__ __forceinline__ few_f4 few_load4(const void* p, int64_t off, int k, i
   }
   return v;
 }
-// values k .. k + 7 of a 16-bit row as they are (zero from K on)
-template <bool VEC>
+// values k .. k + 7 of a 16-bit row as they are, likewise
+template <bool VEC, bool FULL>
 __device__ __forceinline__ vocab::s16x8_t few_load8(const void* p, int64_t off, int k, int K) {
   vocab::s16x8_t v = {0, 0, 0, 0, 0, 0, 0, 0};
   const short* x = (const short*)p + off;
   if constexpr (VEC) {                                 // K % 8 == 0
-    v = *reinterpret_cast<const vocab::s16x8_t*>(x + (k < K ? k : 0));
-    if (k >= K) v = (vocab::s16x8_t){0, 0, 0, 0, 0, 0, 0, 0};
+    v = *reinterpret_cast<const vocab::s16x8_t*>(x + (FULL || k < K ? k : 0));
+    if (!FULL && k >= K) v = (vocab::s16x8_t){0, 0, 0, 0, 0, 0, 0, 0};
+  } else if constexpr (FULL) {
+    v = *reinterpret_cast<const few_s8_any*>(x + k);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -89,31 +100,38 @@ __device__ __forceinline__ void few_tile(const FewArgs& a, int r0, int64_t j0, f
     ho[t] = (int64_t)(r < a.rows ? r : a.rows - 1) * a.ldh;
     acc[t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   }
+  using std::bool_constant;
+  using std::integral_constant;
   // 16 bits: U steps' loads in flight together (fp32 measured slower so: 372 against 240 us at 131072 x 2048)
   if constexpr (DT == F32) {
-#pragma unroll 4
-    for (int k0 = 0; k0 < a.K; k0 += 16) {
-      const few_f4 w = few_load4<DT, VEC>(a.weight, j * a.ldw, k0 + 4 * g, a.K);
+    auto step = [&](int k0, auto full) {
+      constexpr bool FULL = decltype(full)::value;
+      const few_f4 w = few_load4<DT, VEC, FULL>(a.weight, j * a.ldw, k0 + 4 * g, a.K);
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
-        const few_f4 h = few_load4<DT, VEC>(a.hidden, ho[t], k0 + 4 * g, a.K);
+        const few_f4 h = few_load4<DT, VEC, FULL>(a.hidden, ho[t], k0 + 4 * g, a.K);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[e], h[e], acc[t], 0, 0, 0);
       }
-    }
+    };
+    const int whole = a.K / 16 * 16;
+#pragma unroll 4
+    for (int k0 = 0; k0 < whole; k0 += 16) step(k0, bool_constant<true>{});
+    if (whole < a.K) step(whole, bool_constant<false>{});
   } else {
-    constexpr int U = RT == 1 ? 8 : RT == 2 ? 6 : 4;
-    for (int k0 = 0; k0 < a.K; k0 += 32 * U) {
-      vocab::s16x8_t w[U], h[U][RT];
+    auto steps = [&](int k0, auto full, auto n) {
+      constexpr bool FULL = decltype(full)::value;
+      constexpr int N = decltype(n)::value;
+      vocab::s16x8_t w[N], h[N][RT];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
+      for (int u = 0; u < N; ++u) {
         const int k = k0 + 32 * u + 8 * g;
-        w[u] = few_load8<VEC>(a.weight, j * a.ldw, k, a.K);
+        w[u] = few_load8<VEC, FULL>(a.weight, j * a.ldw, k, a.K);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) h[u][t] = few_load8<VEC>(a.hidden, ho[t], k, a.K);
+        for (int t = 0; t < RT; ++t) h[u][t] = few_load8<VEC, FULL>(a.hidden, ho[t], k, a.K);
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < N; ++u)
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
           if constexpr (DT == BF16)
@@ -121,6 +139,15 @@ __device__ __forceinline__ void few_tile(const FewArgs& a, int r0, int64_t j0, f
           else
             acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, w[u]), __builtin_bit_cast(f16x8_t, h[u][t]), acc[t], 0, 0, 0);
         }
+    };
+    constexpr int U = RT == 1 ? 8 : 6;
+    if constexpr (VEC) {
+      for (int k0 = 0; k0 < a.K; k0 += 32 * U) steps(k0, bool_constant<false>{}, integral_constant<int, U>{});
+    } else {
+      int k0 = 0;
+      for (; k0 + 32 * U <= a.K; k0 += 32 * U) steps(k0, bool_constant<true>{}, integral_constant<int, U>{});
+      for (; k0 + 32 <= a.K; k0 += 32) steps(k0, bool_constant<true>{}, integral_constant<int, 1>{});
+      if (k0 < a.K) steps(k0, bool_constant<false>{}, integral_constant<int, 1>{});
     }
   }
 #pragma unroll
@@ -303,26 +330,31 @@ __global__ __launch_bounds__(256) void few_products_kernel(const FewArgs a, int 
     for (int e = 0; e < 4; ++e)
 #pragma unroll
       for (int t = 0; t < RT; ++t) acc[e][t] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-    constexpr int U = 8;
-    for (int64_t jb = j0; jb < j1; jb += 4 * U) {
-      few_f4 w[U];
-      float s[U][RT];
+    auto product = [&](auto full) {
+      constexpr bool FULL = decltype(full)::value;
+      constexpr int U = 8;
+      for (int64_t jb = j0; jb < j1; jb += 4 * U) {
+        few_f4 w[U];
+        float s[U][RT];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int64_t j = jb + 4 * u + g, jj = j < j1 ? j : j1 - 1;
-        w[u] = few_load4<DT, VEC>(a.weight, jj * a.ldw, k0 + 4 * perm, a.K);
+        for (int u = 0; u < U; ++u) {
+          const int64_t j = jb + 4 * u + g, jj = j < j1 ? j : j1 - 1;
+          w[u] = few_load4<DT, VEC, FULL>(a.weight, jj * a.ldw, k0 + 4 * perm, a.K);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) s[u][t] = dS[jj * RP + t * 16 + l15];
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          const float v = jb + 4 * u + g < j1 ? s[u][t] : 0.f;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[u][e], v, acc[e][t], 0, 0, 0);
+          for (int t = 0; t < RT; ++t) s[u][t] = dS[jj * RP + t * 16 + l15];
         }
-    }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int t = 0; t < RT; ++t) {
+            const float v = jb + 4 * u + g < j1 ? s[u][t] : 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[u][e], v, acc[e][t], 0, 0, 0);
+          }
+      }
+    };
+    if (k0 + 64 <= a.K) product(std::true_type{});      // (the same for the wave)
+    else product(std::false_type{});
     const int64_t Kq = (a.K + 3) / 4 * 4;
 #pragma unroll
     for (int t = 0; t < RT; ++t)
@@ -351,34 +383,38 @@ __global__ __launch_bounds__(256) void few_products_kernel(const FewArgs a, int 
     f32x4_t acc[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-    for (int group = 0; group < a.groups; ++group) {
-      const int r0 = group * RP;
-      const float* dS = a.dS + group * a.group_dS + j * RP;
+    auto product = [&](auto full) {
+      constexpr bool FULL = decltype(full)::value;
+      for (int group = 0; group < a.groups; ++group) {
+        const int r0 = group * RP;
+        const float* dS = a.dS + group * a.group_dS + j * RP;
 #pragma unroll
-      for (int q = 0; q < 4 * RT; ++q) {
-        const int r = r0 + 4 * q + g;
-        const bool in = r < a.rows && a.flag[r] != 0.f;
-        few_f4 h = few_load4<DT, VEC>(a.hidden, in ? r * a.ldh : 0, k0 + 4 * perm, a.K);
-        if (!in) h = (few_f4){0.f, 0.f, 0.f, 0.f};
-        const float s = dS[4 * q + g];
+        for (int q = 0; q < 4 * RT; ++q) {
+          const int r = r0 + 4 * q + g;
+          const bool in = r < a.rows && a.flag[r] != 0.f;
+          few_f4 h = few_load4<DT, VEC, FULL>(a.hidden, in ? r * a.ldh : 0, k0 + 4 * perm, a.K);
+          if (!in) h = (few_f4){0.f, 0.f, 0.f, 0.f};
+          const float s = dS[4 * q + g];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(h[e], s, acc[e], 0, 0, 0);
+          for (int e = 0; e < 4; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(h[e], s, acc[e], 0, 0, 0);
+        }
       }
-    }
+    };
+    if (k0 + 64 <= a.K) product(std::true_type{});
+    else product(std::false_type{});
     if (j >= a.vocab) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int k = k0 + 16 * i + 4 * g;
       const float f[4] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
-      if (a.K % 4 == 0) {
-        if (k >= a.K) continue;
+      if (k + 4 <= a.K) {                       // (rows of any length: on their elements' boundaries)
         if constexpr (DT == F32) {
-          *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.dW) + j * a.K + k) = make_float4(f[0], f[1], f[2], f[3]);
+          *reinterpret_cast<few_f4_any*>(reinterpret_cast<float*>(a.dW) + j * a.K + k) = (few_f4_any){f[0], f[1], f[2], f[3]};
         } else {
-          u16x4_t u;
+          few_u4_any u;
 #pragma unroll
           for (int e = 0; e < 4; ++e) u[e] = DT == BF16 ? to_bf16(f[e]) : to_f16(f[e]);
-          *reinterpret_cast<u16x4_t*>(reinterpret_cast<unsigned short*>(a.dW) + j * a.K + k) = u;
+          *reinterpret_cast<few_u4_any*>(reinterpret_cast<unsigned short*>(a.dW) + j * a.K + k) = u;
         }
       } else {
 #pragma unroll

@@ -867,15 +867,14 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------------
 inline size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
-// Which kernels.  Forward and backward, us of wall time (few rows : tiles), 5 launches against 12 (what the host pays for either is ~140 :
-// 158 there):
-//   rows up to 32 fp32, 16 otherwise: fp32 30522 x 2048, 4 rows 303 : 436, 16 rows 318 : 437; bf16 150 : 161, 172 : 160; 131072 x 2048 fp32 at
-//   32 rows 1500 : 2300
-//   or small products.  Each workgroup of the weight gradient goes through m = groups x ceil(hidden / 256) steps one after another (fp32 500 x
-//   2048 at m = 8, 16, 32: 139, 165, 230 : 160; 16 bits, m = 16, 32: 143, 169 : 161), and throughput counts from ~1e9 operations on (fp32 100
-//   hidden, 7.8e8, 1.6e9: 144, 187 : 162; bf16, per score hidden + 400 for its exponential: 512 hidden, 0.9e9, 1.9e9: 143, 176 : 160)
-//   rows that are no whole vectors are loaded value by value: only where the loop over hidden is short (bf16 1379 hidden, 4 rows, forward 73 :
-//   33; 100 hidden x 30522 at 64, 128 rows 143, 203 : 160; fp32 1379 hidden, 16, 32 rows: 142, 200 : 162)
+// Which kernels.  Wall time, us, few rows : tiles; what the host pays for 5 launches or 12, the autograd engine and the rest is ~127 : 142 there,
+// 21 : 30 for the forward alone.
+//   rows up to 32 fp32, 16 otherwise: fp32 forward and backward 30522 x 2048, 4 and 16 rows 303 : 436, 318 : 437, 131072 x 2048 at 32 rows
+//   1500 : 2300; bf16 131072 x 2048 at 5 and 32 rows 530 : 731, 951 : 756
+//   small products: a workgroup of the weight gradient goes through groups x ceil(hidden / 256) steps one after another (500 x 2048 at 8, 16,
+//   32 of them: fp32 139, 165, 230 : 160; bf16 -, 143, 169 : 161), and throughput counts from 3e8 scores x hidden on (fp32 452 hidden x 30522 at 16, 64
+//   rows 127, 185 : 160; bf16 8000 x 512 at 128, 256 rows 143, 176 : 160); the forward alone from 1e9 on (fp32 8000 x 2048 at 64 rows 59 : 92,
+//   2216 at 256 92 : 70; bf16 8000 x 452 at 256 rows 27 : 31, 8000 x 64 at 2048 92 : 28)
 // and in any case few enough comparisons of the distillation's targets (one pass over all rows' ids a workgroup).
 bool few_vectors(const gridmm_vocab_loss_t* d) {      // rows of h and W are whole 16-byte vectors on their boundaries
   const int A = d->dtype == F32 ? 4 : 8;
@@ -884,14 +883,13 @@ bool few_vectors(const gridmm_vocab_loss_t* d) {      // rows of h and W are who
 }
 bool few_rows(const gridmm_vocab_loss_t* d) {
   const double rv = (double)d->rows * d->vocab, K = d->hidden_size, targets = rv * d->slots;
-  const bool fp32 = d->dtype == F32, vec = few_vectors(d);
-  const int groups = d->rows <= 16 ? 1 : (d->rows + 31) / 32;
-  const double m = (double)groups * ((d->hidden_size + 255) / 256);
+  const bool fp32 = d->dtype == F32;
   if (targets > 4e9) return false;
-  if (vec ? d->rows <= (fp32 ? 32 : 16) : d->rows <= 16 && (fp32 || K <= 384)) return true;
+  if (d->rows <= (fp32 ? 32 : 16)) return true;
   if (targets > 1e8) return false;
-  if (vec) return fp32 ? m <= 12 && rv * K <= 5e8 : m <= 16 && rv * (K + 400) <= 1.2e9;
-  return K <= 384 && m <= (fp32 ? 4 : 16) && rv * K <= 2e8;
+  if (d->forward_only) return rv * (K + 100) <= 1.1e9;
+  const int steps = (d->rows + 31) / 32 * ((d->hidden_size + 255) / 256);
+  return steps <= 16 && (fp32 ? rv * K <= 2.8e8 : rv * (K + 100) <= 7e8);
 }
 
 // 16-bit operands: dS in two planes, entry = hi + lo, for up to so many rows.  A gradient that a handful of entries makes up shows the
@@ -1193,7 +1191,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
   Plan P;
   if (!make_plan(d, P) || bad_pointers(d, saved, false) || saved_bytes < P.saved || !workspace || workspace_bytes < P.bwd ||
       ((uintptr_t)workspace & 255) || (d->rows && !grad) || (!d_hidden && !d_weight && !d_bias) || grad_stride < 0 ||
-      (d_bias && !d->bias))
+      (d_bias && !d->bias) || d->forward_only)
     return GRIDMM_EINVAL;
   hipStream_t st = as_stream(stream);
   if (d->rows == 0) {                       // nothing counts: the shared gradients are zero

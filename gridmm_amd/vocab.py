@@ -28,7 +28,7 @@ class _Desc(ctypes.Structure):
     """gridmm_vocab_loss_t of include/gridmm.h."""
     _fields_ = ([(n, ctypes.c_void_p) for n in ("hidden", "weight", "bias", "labels", "ids", "teacher")]
                 + [(n, ctypes.c_int64) for n in ("ld_hidden", "ld_weight", "ld_ids", "ld_teacher", "ignore_index")]
-                + [(n, ctypes.c_int) for n in ("rows", "vocab", "hidden_size", "slots", "dtype", "bias_dtype", "index64")]
+                + [(n, ctypes.c_int) for n in ("rows", "vocab", "hidden_size", "slots", "dtype", "bias_dtype", "index64", "forward_only")]
                 + [("temperature", ctypes.c_float)])
 
 
@@ -116,12 +116,12 @@ class _VocabLoss(torch.autograd.Function):
         b = None if bias is None else bias.contiguous()
         (R, K), V, dt = hidden.shape, w.shape[0], w.dtype
         S = 0 if teacher is None else index.shape[1]
-        at = index.data_ptr()
+        at, need = index.data_ptr(), any(ctx.needs_input_grad[:3])
         # (a single row: whatever its stride says)
         d = _Desc(hidden.data_ptr(), w.data_ptr(), None if b is None else b.data_ptr(), None if S else at, at if S else None,
                   teacher.data_ptr() if S else None, max(hidden.stride(0), K), ldw, max(index.stride(0), S) if S else 0,
                   max(teacher.stride(0), S) if S else 0, ignore_index, R, V, K, S, _DTYPES[dt], 0 if b is None else _DTYPES[b.dtype],
-                  index.dtype == torch.int64, temperature)
+                  index.dtype == torch.int64, not need, temperature)
         ref = ctypes.byref(d)
         n_saved, n_ws = lib.gridmm_vocab_loss_saved_bytes(ref), lib.gridmm_vocab_loss_workspace(ref, 0)
         if n_saved == 0:
@@ -132,7 +132,7 @@ class _VocabLoss(torch.autograd.Function):
         ws = saved.new_empty(n_ws) if n_ws else None
         _lib.check(lib.gridmm_vocab_loss_fwd(ref, loss.data_ptr(), saved.data_ptr(), n_saved, ws.data_ptr() if n_ws else None, n_ws, _stream()),
                    "gridmm_vocab_loss_fwd")
-        if any(ctx.needs_input_grad[:3]):
+        if need:
             ctx.set_materialize_grads(False)
             ctx.save_for_backward(hidden, w, b, index, saved)
             ctx.desc, ctx.prm, ctx.n_ws = d, (weight, bias), lib.gridmm_vocab_loss_workspace(ref, 1)

@@ -813,7 +813,7 @@ def test_the_c_entry_refuses_bad_sizes_and_pointers():
                        (dict(slots=4, ids=256, teacher=256, ld_ids=3, ld_teacher=4), (256, 256, 1 << 40, 256, 1 << 40))):
         assert lib.gridmm_vocab_loss_fwd(ctypes.byref(_descriptor(**{**ok, **over})), *args, None) == EINVAL, (over, args)
     wb = lib.gridmm_vocab_loss_workspace(ctypes.byref(_descriptor(**ok)), 1)
-    for over, args in (({}, (256, n, 0, 1, 256, 256, 0, 256, wb)), ({}, (256, n, 256, 1, 0, 0, 0, 256, wb)), ({}, (256, n, 256, -1, 256, 0, 0, 256, wb)),
+    for over, args in ((dict(forward_only=1), (256, 1 << 40, 256, 1, 256, 0, 0, 256, 1 << 40)), ({}, (256, n, 0, 1, 256, 256, 0, 256, wb)), ({}, (256, n, 256, 1, 0, 0, 0, 256, wb)), ({}, (256, n, 256, -1, 256, 0, 0, 256, wb)),
                        ({}, (256, n, 256, 1, 256, 0, 256, 256, wb)), ({}, (256, n, 256, 1, 256, 0, 0, 256, wb - 1))):
         assert lib.gridmm_vocab_loss_bwd(ctypes.byref(_descriptor(**{**ok, **over})), *args, None) == EINVAL, (over, args)
     for a in ((256, 9, 0, 1, 10, 2), (256, 10, 3, 1, 10, 2), (256, 10, 0, -1, 10, 2), (256, 10, 0, 1, 10, 0), (256, 10, 0, 1, 10, 11),
