@@ -286,16 +286,18 @@ __device__ __forceinline__ void pack_row(const void* src, int64_t off, int dtype
   }
 }
 
-// rows [j0, j0 + C) of W -> Wp (zero past the vocabulary)
-__global__ __launch_bounds__(256) void pack_w_kernel(const void* __restrict__ W, int64_t ldw, int dtype, int K, int Kp, int64_t j0,
-                                                     int C, int vocab, const Meta* __restrict__ meta,
-                                                     unsigned short* __restrict__ Wp) {
-  const int lane = threadIdx.x & 63;
-  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+// rows [j0, j0 + C) of W -> Wp (zero past the vocabulary), one row a wave
+__device__ __forceinline__ void pack_w(const void* W, int64_t ldw, int dtype, int K, int Kp, int64_t j0, int i, int C, int vocab, int sw,
+                                       unsigned short* Wp) {
   if (i >= C) return;
   const bool zero = j0 + i >= vocab;
   unsigned short* hi = Wp + (int64_t)i * Kp * (dtype == F32 ? 2 : 1);
-  pack_row(W, zero ? 0 : (j0 + i) * ldw, dtype, K, Kp, lane, meta->sw, zero, hi, hi + Kp);
+  pack_row(W, zero ? 0 : (j0 + i) * ldw, dtype, K, Kp, threadIdx.x & 63, sw, zero, hi, hi + Kp);
+}
+__global__ __launch_bounds__(256) void pack_w_kernel(const void* __restrict__ W, int64_t ldw, int dtype, int K, int Kp, int64_t j0,
+                                                     int C, int vocab, const Meta* __restrict__ meta,
+                                                     unsigned short* __restrict__ Wp) {
+  pack_w(W, ldw, dtype, K, Kp, j0, blockIdx.x * 4 + (threadIdx.x >> 6), C, vocab, meta->sw, Wp);
 }
 
 // ---- forward: per-row (maximum, sum of exponentials) of each tile's columns ----
@@ -438,24 +440,31 @@ __device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block
 }
 
 // One launch behind prep_kernel: the first `blocks` workgroups pack the counted rows of h into Hp (rows past the count up to a multiple
-// of 256: zero), the others compute the scores at the targets.
+// of 256: zero), the next `targets` compute the scores at the targets, the rest pack the first C rows of W.
 template <int DT, int NS>
-__global__ __launch_bounds__(256) void rows_kernel(const TargetArgs t, int blocks, int Kp,
+__global__ __launch_bounds__(256) void rows_kernel(const TargetArgs t, int blocks, int targets, int Kp,
                                                      const float* __restrict__ amax_h,
                                                      const float* __restrict__ amax_w, Meta* __restrict__ meta,
-                                                     unsigned short* __restrict__ Hp) {
-  if ((int)blockIdx.x >= blocks) return target_scores<DT, NS>(t, blockIdx.x - blocks);
-  const int lane = threadIdx.x & 63;
+                                                     unsigned short* __restrict__ Hp, int C, unsigned short* __restrict__ Wp) {
+  const int b = blockIdx.x - blocks, lane = threadIdx.x & 63;
+  if (b >= 0 && b < targets) return target_scores<DT, NS>(t, b);
+  auto scale_w = [&] {
+    float m = 0.f;
+    for (int k = lane; k < AMAX_W; k += 64) m = fmaxf(m, amax_w[k]);
+    return scale_exp(wave_max(m), 14);
+  };
+  if (b >= 0) {
+    const int sw = DT == F32 ? scale_w() : 0;
+    return pack_w(t.weight, t.ldw, DT, t.K, Kp, 0, (b - targets) * 4 + (threadIdx.x >> 6), C, t.vocab, sw, Wp);
+  }
   const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int count = meta->count;
   int sh = 0;
   if constexpr (DT == F32) {
     sh = scale_exp(wave_max(amax_h[lane]), 14);
     if (i == 0) {
-      float m = 0.f;
-      for (int k = lane; k < AMAX_W; k += 64) m = fmaxf(m, amax_w[k]);
-      m = wave_max(m);
-      if (lane == 0) { meta->sh = sh; meta->sw = scale_exp(m, 14); }
+      const int sw = scale_w();
+      if (lane == 0) { meta->sh = sh; meta->sw = sw; }
     }
   }
   if (i >= (count + 255) / 256 * 256) return;
@@ -1040,7 +1049,7 @@ int weight_piece(const gridmm_vocab_loss_t* d, const Plan& P, int64_t j0, int64_
     return GRIDMM_OK;
   }
   if (P.keep_w) buf = kept + j0 * P.PL * P.Kp;
-  if (forward || !P.keep_w) {
+  if (forward ? j0 > 0 : !P.keep_w) {             // (the forward's first piece: rows_kernel)
     GRIDMM_LAUNCH(pack_w_kernel, dim3((unsigned)((C + 3) / 4)), dim3(256), 0, st, d->weight, d->ld_weight, d->dtype, d->hidden_size,
                   (int)P.Kp, j0, (int)C, d->vocab, meta, buf);
     GRIDMM_CHECK_LAUNCH();
@@ -1152,10 +1161,12 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   t.label = d->slots ? nullptr : (int*)(sv + P.o_label);
   const int rc = by_dtype(d, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    const int hb = (int)(P.Rp / 4);
-    const dim3 grid((unsigned)(hb + ((int64_t)d->rows * (d->slots ? (P.slots + 7) / 8 : 1) + 3) / 4));
-    if (d->slots) GRIDMM_LAUNCH((rows_kernel<DT, 8>), grid, dim3(256), 0, st, t, hb, (int)P.Kp, amax, amax + AMAX_H, meta, Hp);
-    else GRIDMM_LAUNCH((rows_kernel<DT, 1>), grid, dim3(256), 0, st, t, hb, (int)P.Kp, amax, amax + AMAX_H, meta, Hp);
+    const int hb = (int)(P.Rp / 4), tb = (int)(((int64_t)d->rows * (d->slots ? (P.slots + 7) / 8 : 1) + 3) / 4);
+    const int C = P.pack_w ? (int)P.C_fwd : 0;
+    unsigned short* Wp = (unsigned short*)(P.keep_w ? sv + P.o_w : ws + P.f_w);
+    const dim3 grid((unsigned)(hb + tb + (C + 3) / 4));
+    if (d->slots) GRIDMM_LAUNCH((rows_kernel<DT, 8>), grid, dim3(256), 0, st, t, hb, tb, (int)P.Kp, amax, amax + AMAX_H, meta, Hp, C, Wp);
+    else GRIDMM_LAUNCH((rows_kernel<DT, 1>), grid, dim3(256), 0, st, t, hb, tb, (int)P.Kp, amax, amax + AMAX_H, meta, Hp, C, Wp);
     GRIDMM_CHECK_LAUNCH();
     return GRIDMM_OK;
   });
