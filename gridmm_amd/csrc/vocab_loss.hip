@@ -86,12 +86,25 @@ struct Meta {
 // workgroups of the one whose turn it is not end at once.
 constexpr int BIG_TILES = 384;       // 1.5 rounds of 256 CUs
 __host__ __device__ inline bool big_tiles(int64_t count, int64_t C) { return count > 256 && (count + 255) / 256 * (C / 256) >= BIG_TILES; }
-// contraction ranges of dh: enough workgroups for two rounds of the chip, at least 8 stages of 64 columns a range
-__host__ __device__ inline int hidden_splits(int64_t count, int64_t Kp, int64_t C, bool big) {
-  const int64_t T = big ? 256 : 128, tiles = ((count + T - 1) / T) * ((Kp + T - 1) / T);
-  int64_t s = (big ? 256 : 512) / (tiles > 0 ? tiles : 1);
-  if (s > C / 512) s = C / 512;
-  return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+// Contraction ranges of dh, so that its few tiles fill whole rounds of the chip: the cheapest of the numbers that fit into the first
+// rounds, in stages of 64 columns a workgroup (1.2 us): rounds x (its share + what a tile costs beside its stages) + the ranges' sums
+// written and read once more at ~4.7 TB/s.  136 tiles at 4099 x 2048 over 32768 columns: 1 range 752 us, 5 ranges 545 us.
+constexpr int64_t PART_MOST = 64 << 20;      // values of the ranges' partial products, if there are more than one
+constexpr int MOST_SPLITS = 64;
+__device__ __forceinline__ int hidden_splits(int64_t count, int64_t Kp, int64_t C, bool big) {
+  const int T = big ? 256 : 128, slots = big ? 256 : 512;
+  const int tiles = (int)((count + T - 1) / T) * (int)((Kp + T - 1) / T);
+  const float stages = (float)(C / 64), join = (float)(count * Kp) * (8.f / 4.7e6f / 1.2f);
+  int most = (int)min((int64_t)MOST_SPLITS, C / 512);                   // at least 8 stages a range
+  if (count > 0) most = (int)min((int64_t)most, PART_MOST / (count * Kp));
+  int best = 1;
+  float least = INFINITY;
+  for (int k = 0, r0 = (tiles + slots - 1) / slots; k < 8; ++k) {
+    const int s = max(1, min(most, (r0 + k) * slots / max(tiles, 1)));
+    const float cost = (float)((tiles * s + slots - 1) / slots) * (stages / (float)s + 6.f) + (float)s * join;
+    if (cost < least) { least = cost; best = s; }
+  }
+  return best;
 }
 
 __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {        // (maximum, sum of 2^(y - maximum))
@@ -721,12 +734,13 @@ __global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
 template <class T, bool TWO>
 __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, Operand B, int steps, int tn, int64_t C,
                                                                  const Meta* __restrict__ meta, float* __restrict__ part, int64_t Kp,
-                                                                 int first) {
+                                                                 int first, int* __restrict__ ranges) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
   const int count = __builtin_amdgcn_readfirstlane(meta->count), tm = (count + T::BM - 1) / T::BM;
   const bool big = big_tiles(count, C);
   if (big != (T::BM == 256)) return;
   const int splits = hidden_splits(count, Kp, C, big), per = (steps + splits - 1) / splits;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ranges = splits;
   const int wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
   unsigned short* scratch = smem + T::LDS + wave * 2048;
   T::run(
@@ -762,9 +776,10 @@ __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, O
 
 // dh = the ranges' partial products in order, unscaled, to the rows they came from; zero for rows that do not count.  A workgroup
 // takes 64 runs of 4 columns of one row, 4 threads a run, each every fourth range.
-__global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict__ part, int64_t C, int64_t Kp, int K, int rows,
+__global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict__ part, int64_t Kp, int K, int rows,
                                                          const int* __restrict__ rowinv, const Meta* __restrict__ meta,
-                                                         const int* __restrict__ scale, int dtype, void* __restrict__ out) {
+                                                         const int* __restrict__ scale, const int* __restrict__ ranges, int dtype,
+                                                         void* __restrict__ out) {
   __shared__ float4 sums[3][64];
   const int t = threadIdx.x & 63, sp = threadIdx.x >> 6;
   const int64_t r = blockIdx.x;
@@ -772,7 +787,7 @@ __global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict
   const int count = __builtin_amdgcn_readfirstlane(meta->count), pos = rowinv[r], e = -(*scale + meta->sw);
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (pos >= 0 && k < Kp) {
-    const int splits = hidden_splits(count, Kp, C, big_tiles(count, C));
+    const int splits = *ranges;
     const float* at = part + (int64_t)pos * Kp + k;
 #pragma unroll 4
     for (int s = sp; s < splits; s += 4) {
@@ -1008,12 +1023,11 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.f_w = take(P.pack_w && !P.keep_w ? (size_t)P.C_fwd * P.Kp * 2 * P.PL : 0);
   P.fwd = o;
   o = 0;
-  P.b_scale = take(4);
+  P.b_scale = take(8);                 // ... and the ranges of dh
   P.two = P.PL == 1 && d->rows <= TWO_PLANES;
   P.b_ds = take(Rp * (size_t)P.C_bwd * 2 * (P.two ? 2 : P.PL));
   P.b_w = take(P.pack_w && !P.keep_w ? (size_t)P.C_bwd * P.Kp * 2 * P.PL : 0);
-  // with more than one range the ranges' tiles number at most 512 of 128 x 128 or 256 of 256 x 256, else the rows' product once
-  P.b_part = take(std::max<size_t>(Rp * (size_t)P.Kp, std::min<size_t>(64 * Rp * (size_t)P.Kp, 256 * 256 * 256)) * 4);
+  P.b_part = take(std::max<size_t>(Rp * (size_t)P.Kp, std::min<size_t>(MOST_SPLITS * Rp * (size_t)P.Kp, PART_MOST)) * 4);
   P.bwd = o;
   return true;
 }
@@ -1297,8 +1311,8 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
           using T = TileOf<F, L, decltype(big)::value, false, true>;
           const int64_t tn = (P.Kp + T::BN - 1) / T::BN, tm = (rows + T::BM - 1) / T::BM;
           return one_or_two(big, [&](auto two) {
-            GRIDMM_LAUNCH((hidden_grad_kernel<T, decltype(two)::value>), dim3(blocks<T>(tm * tn * hidden_splits(1, P.Kp, P.C_bwd, T::BM == 256))),
-                          dim3(T::THREADS), 0, st, S, W, (int)(C / T::BK), (int)tn, P.C_bwd, meta, part, P.Kp, j0 == 0);
+            GRIDMM_LAUNCH((hidden_grad_kernel<T, decltype(two)::value>), dim3(blocks<T>(tm * tn * MOST_SPLITS)),
+                          dim3(T::THREADS), 0, st, S, W, (int)(C / T::BK), (int)tn, P.C_bwd, meta, part, P.Kp, j0 == 0, scale + 1);
             GRIDMM_CHECK_LAUNCH();
             return GRIDMM_OK;
           });
@@ -1324,8 +1338,8 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
     if (rc != GRIDMM_OK) return rc;
   }
   if (d_hidden) {
-    GRIDMM_LAUNCH(hidden_out_kernel, dim3(d->rows, (unsigned)((P.Kp + 255) / 256)), dim3(256), 0, st, part, P.C_bwd, P.Kp,
-                  d->hidden_size, d->rows, rowinv, meta, scale, d->dtype, d_hidden);
+    GRIDMM_LAUNCH(hidden_out_kernel, dim3(d->rows, (unsigned)((P.Kp + 255) / 256)), dim3(256), 0, st, part, P.Kp, d->hidden_size,
+                  d->rows, rowinv, meta, scale, scale + 1, d->dtype, d_hidden);
     GRIDMM_CHECK_LAUNCH();
   }
   return GRIDMM_OK;
