@@ -5,7 +5,8 @@
 //   few_scores   16 vocabulary rows a wave, a group's RT tiles of 16 rows of h: each W value is loaded once, straight into the fragment layout
 //                of the 16x16 matrix instructions (fp32: 16x16x4 fp32, products and sums in fp32; 16 bits: 16x16x32, products exact).
 //                Forward: each row's (maximum, sum of exponentials) of the workgroup's 64 columns, and the targets' scores.
-//                Backward: the same scores again -> dS [group][vocabulary][RP] in fp32
+//                The scores stay for the backward, fp32 [group][vocabulary][RP]: a few percent of W's size, whose third read they save
+//   few_grad     scores -> dS, laid out alike
 //   few_loss     joins the statistics, the teacher's softmax, the losses
 //   few_products dh = dS W over ranges of the vocabulary and dW = dS^T h, db, on the fp32 matrix instruction (16-bit operands are
 //                widened: exact), as two kinds of workgroups of one launch
@@ -26,6 +27,7 @@ struct FewArgs {
   float inv_t, unit, temperature;
   float2* stats;                 // [workgroup][groups RP]
   float *lse, *zt, *p, *flag;    // saved: [groups RP], [rows][slots] (halves), [rows][slots], [groups RP]: 1 for rows that count
+  float* y;                      // saved: the scores, base 2, laid out like dS; NULL: no backward will follow
   float* loss;
   const float* grad;
   int64_t grad_stride;
@@ -209,7 +211,7 @@ __device__ __forceinline__ void few_targets(const FewArgs& a, const FewTargets& 
 }
 
 // VEC: the rows of h and W are whole 16-byte vectors on their boundaries (decided once a call: a choice at each load would wait for it)
-template <int DT, int RT, bool VEC, bool GRAD>
+template <int DT, int RT, bool VEC>
 __global__ __launch_bounds__(256) void few_scores_kernel(const FewArgs a) {
   __shared__ float2 wst[4][RT * 16];
   __shared__ FewTargets T;
@@ -220,50 +222,63 @@ __global__ __launch_bounds__(256) void few_scores_kernel(const FewArgs a) {
   const int r0 = blockIdx.y * RP;
   few_collect<RP>(a, r0, T);
   few_tile<DT, RT, VEC>(a, r0, j0, y);
-  if constexpr (!GRAD) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int r = r0 + t * 16 + l15;
-      float m = fmaxf(fmaxf(y[t][0], y[t][1]), fmaxf(y[t][2], y[t][3]));
-      m = fmaxf(m, __shfl_xor(m, 16, 64));
-      m = fmaxf(m, __shfl_xor(m, 32, 64));
-      const float ref = m == -INFINITY ? 0.f : m;
-      float s = 0.f;
+  for (int t = 0; t < RT; ++t) {
+    const int r = r0 + t * 16 + l15;
+    if (a.y) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f(y[t][i] - ref);
-      s += __shfl_xor(s, 16, 64);
-      s += __shfl_xor(s, 32, 64);
-      if (g == 0) wst[wave][t * 16 + l15] = make_float2(m, s);
-      if (r < a.rows)                           // the scores at the row's targets
-        few_targets(a, T, r0, t * 16 + l15, jl, [&](int k, int d) {
-          const float v = d < 2 ? (d == 0 ? y[t][0] : y[t][1]) : (d == 2 ? y[t][2] : y[t][3]);
-          // half of it: a bias of the lowest finite number, -inf in base 2, is finite so
-          a.zt[(int64_t)r * a.slots + k] = v == -INFINITY && a.bias ? load_as_f32(a.bias, jl + d, a.bias_dtype) * (0.5f * a.unit) : 0.5f * v;
-        });
+      for (int i = 0; i < 4; ++i) a.y[blockIdx.y * a.group_dS + (jl + i) * RP + t * 16 + l15] = y[t][i];
     }
-    __syncthreads();
-    for (int r = threadIdx.x; r < RP; r += 256) {
-      float2 s = wst[0][r];
+    float m = fmaxf(fmaxf(y[t][0], y[t][1]), fmaxf(y[t][2], y[t][3]));
+    m = fmaxf(m, __shfl_xor(m, 16, 64));
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    const float ref = m == -INFINITY ? 0.f : m;
+    float s = 0.f;
 #pragma unroll
-      for (int w = 1; w < 4; ++w) s = join_stats(s, wst[w][r]);
-      a.stats[((int64_t)blockIdx.x * a.groups + blockIdx.y) * RP + r] = s;
-    }
-  } else {
+    for (int i = 0; i < 4; ++i) s += __builtin_amdgcn_exp2f(y[t][i] - ref);
+    s += __shfl_xor(s, 16, 64);
+    s += __shfl_xor(s, 32, 64);
+    if (g == 0) wst[wave][t * 16 + l15] = make_float2(m, s);
+    if (r < a.rows)                           // the scores at the row's targets
+      few_targets(a, T, r0, t * 16 + l15, jl, [&](int k, int d) {
+        const float v = d < 2 ? (d == 0 ? y[t][0] : y[t][1]) : (d == 2 ? y[t][2] : y[t][3]);
+        // half of it: a bias of the lowest finite number, -inf in base 2, is finite so
+        a.zt[(int64_t)r * a.slots + k] = v == -INFINITY && a.bias ? load_as_f32(a.bias, jl + d, a.bias_dtype) * (0.5f * a.unit) : 0.5f * v;
+      });
+  }
+  __syncthreads();
+  for (int r = threadIdx.x; r < RP; r += 256) {
+    float2 s = wst[0][r];
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const int r = r0 + t * 16 + l15;
-      const bool live = r < a.rows && a.flag[r] != 0.f;
-      const float gt = live ? a.grad[r * a.grad_stride] * a.temperature : 0.f, L = live ? a.lse[r] : 0.f;
-      float p[4] = {0.f, 0.f, 0.f, 0.f};
-      if (live)
-        few_targets(a, T, r0, t * 16 + l15, jl, [&](int k, int d) {
-          const float q = a.kd ? a.p[(int64_t)r * a.slots + k] : 1.f;
+    for (int w = 1; w < 4; ++w) s = join_stats(s, wst[w][r]);
+    a.stats[((int64_t)blockIdx.x * a.groups + blockIdx.y) * RP + r] = s;
+  }
+}
+
+template <int RT>
+__global__ __launch_bounds__(256) void few_grad_kernel(const FewArgs a) {
+  __shared__ FewTargets T;
+  constexpr int RP = RT * 16;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l15 = lane & 15, g = lane >> 4;
+  const int64_t jl = (int64_t)blockIdx.x * 64 + wave * 16 + 4 * g;
+  const int r0 = blockIdx.y * RP;
+  few_collect<RP>(a, r0, T);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[i] += d == i ? q : 0.f;
-        });
+  for (int t = 0; t < RT; ++t) {
+    const int r = r0 + t * 16 + l15;
+    const bool live = r < a.rows && a.flag[r] != 0.f;
+    const float gt = live ? a.grad[r * a.grad_stride] * a.temperature : 0.f, L = live ? a.lse[r] : 0.f;
+    float p[4] = {0.f, 0.f, 0.f, 0.f};
+    if (live)
+      few_targets(a, T, r0, t * 16 + l15, jl, [&](int k, int d) {
+        const float q = a.kd ? a.p[(int64_t)r * a.slots + k] : 1.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        a.dS[blockIdx.y * a.group_dS + (jl + i) * RP + t * 16 + l15] = live ? gt * (__builtin_amdgcn_exp2f(y[t][i] - L) - p[i]) : 0.f;
+        for (int i = 0; i < 4; ++i) p[i] += d == i ? q : 0.f;
+      });
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = blockIdx.y * a.group_dS + (jl + i) * RP + t * 16 + l15;
+      a.dS[at] = live ? gt * (__builtin_amdgcn_exp2f(a.y[at] - L) - p[i]) : 0.f;
     }
   }
 }

@@ -992,6 +992,7 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
     P.o_meta = take(GR * 4);                         // 1 for rows that count
     P.o_zt = take(S * 4);
     P.o_p = take(d->slots ? S * 4 : 0);
+    P.o_h = take(d->forward_only ? 0 : V64 * GR * 4);      // the scores
     P.f_stats = take(V64 / 64 * GR * 8);             // (small enough to stay: no forward workspace)
     P.saved = o;
     P.fwd = 0;
@@ -1111,6 +1112,7 @@ FewArgs few_args(const gridmm_vocab_loss_t* d, const Plan& P, const void* saved)
   a.inv_t = 1.f / d->temperature; a.unit = a.inv_t * LOG2E; a.temperature = d->temperature;
   a.lse = (float*)(sv + P.o_lse); a.flag = (float*)(sv + P.o_meta); a.zt = (float*)(sv + P.o_zt);
   a.p = d->slots ? (float*)(sv + P.o_p) : nullptr;
+  a.y = d->forward_only ? nullptr : (float*)(sv + P.o_h);
   a.ranges = P.ranges; a.range = P.range; a.groups = P.groups;
   a.group_dS = (int64_t)up(d->vocab, 64) * P.RP;
   return a;
@@ -1143,7 +1145,7 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
     a.loss = loss;
     const int tiles = (d->vocab + 63) / 64;
     const int rc = by_few(d, P, [&](auto dt, auto rt, auto vec) {
-      GRIDMM_LAUNCH((few_scores_kernel<decltype(dt)::value, decltype(rt)::value, decltype(vec)::value, false>), dim3(tiles, P.groups), dim3(256), 0, st, a);
+      GRIDMM_LAUNCH((few_scores_kernel<decltype(dt)::value, decltype(rt)::value, decltype(vec)::value>), dim3(tiles, P.groups), dim3(256), 0, st, a);
       GRIDMM_CHECK_LAUNCH();
       return GRIDMM_OK;
     });
@@ -1246,7 +1248,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
     const int tiles = (d->vocab + 63) / 64, kb = (d->hidden_size + 255) / 256;
     const int hb = d_hidden ? kb * P.ranges * P.groups : 0, wb = d_weight || d_bias ? (d->vocab + 15) / 16 : 0;
     const int rc = by_few(d, P, [&](auto dt, auto rt, auto vec) {
-      GRIDMM_LAUNCH((few_scores_kernel<decltype(dt)::value, decltype(rt)::value, decltype(vec)::value, true>), dim3(tiles, P.groups), dim3(256), 0, st, a);
+      GRIDMM_LAUNCH((few_grad_kernel<decltype(rt)::value>), dim3(tiles, P.groups), dim3(256), 0, st, a);
       GRIDMM_CHECK_LAUNCH();
       GRIDMM_LAUNCH((few_products_kernel<decltype(dt)::value, decltype(rt)::value, decltype(vec)::value>), dim3(hb + wb), dim3(256), 0, st, a, hb, kb);
       GRIDMM_CHECK_LAUNCH();
