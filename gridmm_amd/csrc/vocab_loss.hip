@@ -313,11 +313,24 @@ __global__ __launch_bounds__(256) void pack_w_kernel(const void* __restrict__ W,
   pack_w(W, ldw, dtype, K, Kp, j0, blockIdx.x * 4 + (threadIdx.x >> 6), C, vocab, meta->sw, Wp);
 }
 
-// ---- forward: per-row (maximum, sum of exponentials) of each tile's columns ----
-template <class T>
+// ---- a teacher's targets by blocks of 64 columns: the score tiles hand over the scores at them ----
+// Dot products of their own read rows x slots rows of W once more (4099 x 128 x 4 KB: 305 us; 2413 x 254 x 15.6 KB: 1.4 ms).
+struct TargetLists {
+  const unsigned short* begin;      // [compacted row][blocks + 1]
+  const unsigned* entry;            // [compacted row][slots]: slot << 6 | column in its block
+  int64_t blocks;
+  int slots;
+  float* zt;
+  const void* bias;
+  int bias_dtype;
+  float half_unit;
+};
+constexpr int LIST_BLOCKS = 4096, LIST_SLOTS = 4096;
+// ---- forward: per-row (maximum, sum of exponentials) of each tile's columns; LISTS: and the scores at the targets among them ----
+template <class T, bool LISTS>
 __global__ __launch_bounds__(T::THREADS, 2) void score_stats_kernel(Operand A, Operand B, int nk, int tn, const Meta* __restrict__ meta,
                                                                  const float* __restrict__ biasz, float unit,
-                                                                 float2* __restrict__ stats, int64_t Rp) {
+                                                                 float2* __restrict__ stats, int64_t Rp, const TargetLists L, int64_t j0) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
   __shared__ float2 wst[T::WAVES_N][T::BM];
   const int count = __builtin_amdgcn_readfirstlane(meta->count), tm = (count + T::BM - 1) / T::BM;
@@ -352,6 +365,39 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_stats_kernel(Operand A, O
               m[i] = fmaxf(m[i], fmaxf(fmaxf(c[q * 4], c[q * 4 + 1]), fmaxf(c[q * 4 + 2], c[q * 4 + 3])));
             }
           }
+        if constexpr (LISTS) {
+          // entries of the rows and 64 columns of this wave; either half of the wave holds 4 of every 8 columns
+          const int64_t block = (j0 + it.bn + wc * T::WN) >> 6;
+          static_assert(T::WN == 64, "64 columns a wave");
+          unsigned e0[T::TM], e1[T::TM], next[T::TM];
+#pragma unroll
+          for (int i = 0; i < T::TM; ++i) {
+            const int64_t r = it.bm + wr * T::WM + i * 32 + (lane & 31);
+            const unsigned short* at = L.begin + (r < count ? r : 0) * (L.blocks + 1) + block;
+            e0[i] = at[0];
+            e1[i] = r < count ? at[1] : 0;
+          }
+#pragma unroll
+          for (int i = 0; i < T::TM; ++i) {
+            const int64_t r = it.bm + wr * T::WM + i * 32 + (lane & 31);
+            next[i] = e0[i] < e1[i] ? L.entry[r * L.slots + e0[i]] : 0;
+          }
+#pragma unroll
+          for (int i = 0; i < T::TM; ++i) {
+            const int64_t r = it.bm + wr * T::WM + i * 32 + (lane & 31);
+            while (e0[i] < e1[i]) {
+              const unsigned v = next[i], c = v & 63;
+              if (++e0[i] < e1[i]) next[i] = L.entry[r * L.slots + e0[i]];
+              if (((c >> 2) & 1) != (unsigned)(lane >> 5)) continue;
+              const int at = (c >> 5) * 16 + ((c & 31) >> 3) * 4 + (c & 3);
+              float y = acc[i][0][0];
+#pragma unroll
+              for (int k = 1; k < 32; ++k) y = at == k ? acc[i][k >> 4][k & 15] : y;
+              // half of it: a bias of the lowest finite number, -inf in base 2, is finite so
+              L.zt[r * L.slots + (v >> 6)] = y == -INFINITY && L.bias ? load_as_f32(L.bias, block * 64 + c, L.bias_dtype) * L.half_unit : 0.5f * y;
+            }
+          }
+        }
 #pragma unroll
         for (int i = 0; i < T::TM; ++i) {
           m[i] = fmaxf(m[i], __shfl_xor(m[i], 32, 64));
@@ -449,6 +495,52 @@ __device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block
     if (a.label) a.label[i] = id[s] >= 0 && id[s] < a.vocab ? (int)id[s] : -1;
     const float half = 0.5f * a.unit, b = a.bias ? load_as_f32(a.bias, at[s], a.bias_dtype) * half : 0.f;
     a.zt[i * a.slots + s0 + s] = a.kd && id[s] < 0 ? 0.f : id[s] < 0 || id[s] >= a.vocab ? NAN : fmaf(z[s], half, b);
+  }
+}
+
+// TargetLists: one compacted row a workgroup (the order within a block is whatever it is: each entry is its slot's own)
+__global__ __launch_bounds__(256) void target_lists_kernel(const TargetArgs t, int blocks, unsigned short* __restrict__ begin,
+                                                           unsigned* __restrict__ entry) {
+  __shared__ unsigned at[LIST_BLOCKS];
+  __shared__ unsigned part[4];
+  const int64_t i = blockIdx.x;
+  if (i >= t.meta->count) return;
+  const int64_t r = t.rowmap[i];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int b = tid; b < blocks; b += 256) at[b] = 0;
+  __syncthreads();
+  for (int s = tid; s < t.slots; s += 256) {
+    const int64_t id = load_index(t.index, r * t.ld_index + s, t.wide);
+    if (id >= 0 && id < t.vocab) atomicAdd(&at[id >> 6], 1u);
+    else t.zt[i * t.slots + s] = id < 0 ? 0.f : NAN;      // an empty slot has no score, an id outside the vocabulary spoils its row
+  }
+  __syncthreads();
+  // thread t owns the blocks [per t, per (t + 1))
+  const int per = (blocks + 255) / 256, b0 = min(blocks, tid * per), b1 = min(blocks, b0 + per);
+  unsigned n = 0;
+  for (int b = b0; b < b1; ++b) n += at[b];
+  unsigned incl = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned up = __shfl_up(incl, o, 64);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 63) part[wave] = incl;
+  __syncthreads();
+  unsigned pos = incl - n;
+  for (int w = 0; w < wave; ++w) pos += part[w];
+  unsigned short* mine = begin + i * (blocks + 1);
+  for (int b = b0; b < b1; ++b) {
+    const unsigned c = at[b];
+    at[b] = pos;
+    mine[b] = (unsigned short)pos;
+    pos += c;
+  }
+  if (tid == 255) mine[blocks] = (unsigned short)pos;
+  __syncthreads();
+  for (int s = tid; s < t.slots; s += 256) {
+    const int64_t id = load_index(t.index, r * t.ld_index + s, t.wide);
+    if (id >= 0 && id < t.vocab) entry[i * t.slots + atomicAdd(&at[id >> 6], 1u)] = (unsigned)s << 6 | (unsigned)(id & 63);
   }
 }
 
@@ -926,6 +1018,15 @@ bool few_rows(const gridmm_vocab_loss_t* d) {
   return steps <= 16 && (fp32 ? rv * K <= 2.8e8 : rv * (K + 100) <= 7e8);
 }
 
+// Scores at a teacher's targets out of the score tiles where that is the cheaper: dot products read rows x slots rows of W at ~7 TB/s,
+// the lists cost ~12 us and each tile's end ~4 us (0.28 us a million scores).  dot products : lists, us of the whole call: 4099 x 65537 x 2048
+// bf16, 128 slots 4520 : 4336, 2413 x 3309 x 3904 fp32, 254 slots 1899 : 748, 2000 x 8000 x 1024 bf16, 64 slots 231 : 202, 2219 x 54900 x 1600
+// fp16, 33 slots 405 : 414
+bool target_lists(const gridmm_vocab_loss_t* d) {
+  const double bytes = (double)d->rows * d->slots * d->hidden_size * (d->dtype == F32 ? 4 : 2);
+  return d->slots && d->slots <= LIST_SLOTS && d->vocab <= LIST_BLOCKS * 64 - 256 && bytes / 7e6 > 12 + 2.8e-7 * d->rows * d->vocab;
+}
+
 // 16-bit operands: dS in two planes, entry = hi + lo, for up to so many rows.  A gradient that a handful of entries makes up shows the
 // rounding of each, a sum over many rows their mean: one plane leaves 1.4 times the error of the gradients' own rounding at thousands of
 // rows, up to twice that at a few.  So few rows are bound by the read of W and the write of dW, not by the products (128 x 128 tiles;
@@ -934,7 +1035,7 @@ constexpr int TWO_PLANES = 256;
 
 struct Plan {
   int PL, slots;               // planes; target slots a row (cross entropy: 1)
-  bool few, two;
+  bool few, two, lists;
   int RP, groups, ranges, range;      // few rows: rows a group (16 or 32), groups; ranges of the vocabulary in dh and their rows
   int64_t Rp, Kp, Vp;
   bool pack_w;                 // W has to be split or padded; else it is read where it lies
@@ -943,7 +1044,7 @@ struct Plan {
   // saved
   size_t o_meta, o_rowmap, o_rowinv, o_lse, o_zt, o_label, o_p, o_biasz, o_h, o_w, saved;
   // forward workspace
-  size_t f_counts, f_plogp, f_amax, f_stats, f_w, fwd;
+  size_t f_counts, f_plogp, f_amax, f_stats, f_w, f_begin, f_entry, fwd;
   // backward workspace
   size_t b_scale, b_ds, b_w, b_part, bwd;
 };
@@ -1022,6 +1123,9 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.f_amax = take((AMAX_H + AMAX_W) * 4);
   P.f_stats = take(Rp * (size_t)(P.Vp / 128) * 8);
   P.f_w = take(P.pack_w && !P.keep_w ? (size_t)P.C_fwd * P.Kp * 2 * P.PL : 0);
+  P.lists = target_lists(d);
+  P.f_begin = take(P.lists ? R * (P.Vp / 64 + 1) * 2 : 0);
+  P.f_entry = take(P.lists ? R * S * 4 : 0);
   P.fwd = o;
   o = 0;
   P.b_scale = take(8);                 // ... and the ranges of dh
@@ -1187,7 +1291,7 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   t.label = d->slots ? nullptr : (int*)(sv + P.o_label);
   const int rc = by_dtype(d, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    const int hb = (int)(P.Rp / 4), tb = (int)(((int64_t)d->rows * (d->slots ? (P.slots + 7) / 8 : 1) + 3) / 4);
+    const int hb = (int)(P.Rp / 4), tb = P.lists ? 0 : (int)(((int64_t)d->rows * (d->slots ? (P.slots + 7) / 8 : 1) + 3) / 4);
     const int C = P.pack_w ? (int)P.C_fwd : 0;
     unsigned short* Wp = (unsigned short*)(P.keep_w ? sv + P.o_w : ws + P.f_w);
     const dim3 grid((unsigned)(hb + tb + (C + 3) / 4));
@@ -1198,6 +1302,14 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   });
   if (rc != GRIDMM_OK) return rc;
 
+  TargetLists lists{};
+  if (P.lists) {
+    unsigned short* begin = (unsigned short*)(ws + P.f_begin);
+    unsigned* entry = (unsigned*)(ws + P.f_entry);
+    lists = TargetLists{begin, entry, P.Vp / 64, P.slots, zt, d->bias, d->bias_dtype, 0.5f * unit};
+    GRIDMM_LAUNCH(target_lists_kernel, dim3(d->rows), dim3(256), 0, st, t, (int)lists.blocks, begin, entry);
+    GRIDMM_CHECK_LAUNCH();
+  }
   const Operand H{Hp, P.PL * P.Kp, P.Kp, P.Rp, P.Kp};
   for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_fwd) {
     const int64_t C = std::min(P.C_fwd, P.Vp - j0);
@@ -1208,10 +1320,13 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
       return by_tile(d->rows, C, [&](auto big, int rows) {
         using T = TileOf<decltype(f16)::value, decltype(pl)::value, decltype(big)::value, false, false>;
         const int64_t tn = C / T::BN, tm = (rows + T::BM - 1) / T::BM;
-        GRIDMM_LAUNCH((score_stats_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), (int)tn, meta,
-                      biasz + j0, unit, stats + j0 / 128 * P.Rp, P.Rp);
-        GRIDMM_CHECK_LAUNCH();
-        return GRIDMM_OK;
+        auto run = [&](auto with) {
+          GRIDMM_LAUNCH((score_stats_kernel<T, decltype(with)::value>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, H, W,
+                        (int)(P.Kp / T::BK), (int)tn, meta, biasz + j0, unit, stats + j0 / 128 * P.Rp, P.Rp, lists, j0);
+          GRIDMM_CHECK_LAUNCH();
+          return GRIDMM_OK;
+        };
+        return P.lists ? run(std::true_type{}) : run(std::false_type{});
       });
     });
     if (rc != GRIDMM_OK) return rc;

@@ -326,7 +326,10 @@ def _check_kd(h, w, b, ids, t, g, T):
 
 KD = [("fp32", 300, 9001, 130, 17, 2.0), ("bf16", 200, 20001, 128, 300, 1.0), ("fp16", 1030, 2500, 200, 5, 0.5), ("fp32", 60, 30522, 256, 64, 1.0),
       ("fp32", 1, 1, 64, 1, 1.0), ("fp32", 5, 300, 64, 8, 2.0), ("bf16", 130, 1000, 128, 32, 1.0), ("fp16", 77, 513, 72, 100, 0.5),
-      ("fp32", 300, 2000, 100, 17, 4.0), ("bf16", 3, 40000, 64, 256, 1.5), ("fp32", 64, 256, 64, 256, 1.0), ("fp32", 16, 30522, 64, 8200, 1.0)]
+      ("fp32", 300, 2000, 100, 17, 4.0), ("bf16", 3, 40000, 64, 256, 1.5), ("fp32", 64, 256, 64, 256, 1.0), ("fp32", 16, 30522, 64, 8200, 1.0),
+      # many slots of long rows: the scores at the targets out of the score tiles (128 x 128, 256 x 256, two pieces of W)
+      ("bf16", 700, 3001, 1024, 100, 1.5), ("fp16", 2100, 11000, 520, 70, 0.5), ("fp32", 300, 5000, 1030, 120, 2.0), ("fp32", 300, 62000, 2200, 60, 2.0),
+      ("fp32", 2100, 11003, 512, 40, 1.0)]
 
 
 @pytest.mark.gpu
@@ -351,10 +354,22 @@ def test_distillation_where_ids_repeat_and_are_int32_columns_of_a_wider_table(V,
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("R,V,K", [(10, 300, 64), (40, 40000, 256)])
-def test_distillation_of_an_id_past_the_vocabulary(R, V, K):
+def test_distillation_from_many_slots_where_ids_repeat_and_columns_are_masked():
+    """The scores at the targets out of the score tiles: repeated ids, all of a row's ids in one block, int32, the lowest bias."""
+    h, w, b, g = _inputs("fp32", 600, 2000, 1024, True, 2)
+    b[40:60] = torch.finfo(torch.float32).min
+    ids = torch.randint(0, 2000, (600, 64), generator=g)
+    ids[1] = torch.randint(70, 75, (64,), generator=g)
+    ids[2] = 1999
+    ids[3, ::2], ids[3, 1::2] = -1, 50
+    _check_kd(h, w, b, ids.int().cuda(), torch.randn(600, 64, generator=g).cuda(), torch.rand(600, generator=g).cuda(), 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,V,K,S", [(10, 300, 64, 4), (40, 40000, 256, 4), (600, 2000, 1024, 80)])
+def test_distillation_of_an_id_past_the_vocabulary(R, V, K, S):
     from gridmm_amd import vocab
-    h, w, b, ids, t, g = _kd_inputs("bf16", R, V, K, 4, seed=1)
+    h, w, b, ids, t, g = _kd_inputs("bf16", R, V, K, S, seed=1)
     good = vocab.vocab_distillation(h, w, ids.cuda(), t.cuda(), bias=b)
     ids[4, 2] = V
     got = vocab.vocab_distillation(h, w, ids.cuda(), t.cuda(), bias=b)
