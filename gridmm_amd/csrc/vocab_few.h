@@ -11,6 +11,7 @@
 //   few_products dh = dS W over ranges of the vocabulary and dW = dS^T h, db, on the fp32 matrix instruction (16-bit operands are
 //                widened: exact), as two kinds of workgroups of one launch
 //   few_hidden   joins the ranges of dh
+// One token of 30522 x 768 fp32: 24 us (3.9 TB/s); 4 rows of 131072 x 2048 fp32 forward 257 us (4.2 TB/s); 32 rows 423, where the reads of h count.
 // dS is never rounded to 16 bits here.  A row that does not count has dS = 0 and its h is read as 0.
 #pragma once
 #include "vocab_gemm.h"

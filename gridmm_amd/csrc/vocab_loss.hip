@@ -18,6 +18,8 @@
 // of an entry at most, like the gradients themselves), with few counted rows to two planes of it.  fp32 operands: two fp16 planes each (22 bits) after a
 // power-of-two scale from the tensor's largest finite value, so a product is off by ~2^-22: like fp32 sums.  dS is scaled by a power of
 // two from the largest |g T| of the call (fp16 range: entries below 2^-38 of it vanish).
+// Bound by the four products (vocab_gemm.h): 8030 x 131072 x 2048 bf16 forward and backward 13.8 - 14.0 ms, of it 3.4 scores, 3.7 dS, 3.4 dh, 3.4 dW;
+// fp32 384 x 30522 x 768 325 us, of it 260 products (1.4 rounds of 128 x 128 tiles) and 53 for W's scale and packing.
 // Everything runs in the base-2 domain: y = z log2 e, exp2, and ln 2 comes back in the losses.
 #include <algorithm>
 
