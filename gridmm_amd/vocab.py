@@ -85,7 +85,7 @@ def _check_head(hidden, weight, bias, *index):
 
 def _vocab_backward(ctx, g):
     if g is None:
-        return (None,) * 7
+        return (None,) * 8
     hidden, w, b, _, saved = ctx.saved_tensors
     if g.dtype != torch.float32:
         g = g.float()
@@ -100,7 +100,7 @@ def _vocab_backward(ctx, g):
         _lib.check(_lib.load().gridmm_vocab_loss_bwd(
             ctypes.byref(ctx.desc), saved.data_ptr(), saved.numel(), g.data_ptr(), g.stride(0), dh.data_ptr() if need_h else None,
             dw.data_ptr() if need_w else None, db.data_ptr() if need_b else None, ws.data_ptr(), n_ws, _stream()), "gridmm_vocab_loss_bwd")
-    return dh, DEFERRED.hand(prm[0], dw), DEFERRED.hand(prm[1], db), None, None, None, None
+    return dh, DEFERRED.hand(prm[0], dw), DEFERRED.hand(prm[1], db), None, None, None, None, None
 
 
 _vocab_backward_once = once_differentiable(_vocab_backward)
@@ -110,13 +110,13 @@ class _VocabLoss(torch.autograd.Function):
     """hidden (R, K), weight (V, K), bias (V,) or None, index (R,) labels or (R, S) ids, teacher None or (R, S) -> losses (R,)."""
 
     @staticmethod
-    def forward(ctx, hidden, weight, bias, index, teacher, ignore_index, temperature):
+    def forward(ctx, hidden, weight, bias, index, teacher, ignore_index, temperature, recording):
         lib = _lib.load()
         w, ldw = _rows(weight)
         b = None if bias is None else bias.contiguous()
         (R, K), V, dt = hidden.shape, w.shape[0], w.dtype
         S = 0 if teacher is None else index.shape[1]
-        at, need = index.data_ptr(), any(ctx.needs_input_grad[:3])
+        at, need = index.data_ptr(), recording and any(ctx.needs_input_grad[:3])
         # (a single row: whatever its stride says)
         d = _Desc(hidden.data_ptr(), w.data_ptr(), None if b is None else b.data_ptr(), None if S else at, at if S else None,
                   teacher.data_ptr() if S else None, max(hidden.stride(0), K), ldw, max(index.stride(0), S) if S else 0,
@@ -160,9 +160,9 @@ def vocab_cross_entropy(hidden, weight, labels, bias=None, ignore_index=-1):
         raise ValueError("labels are int64 or int32, not %s" % labels.dtype)
     with _on(hidden.device):
         if labels.dim() == 1:
-            return _VocabLoss.apply(_rows(hidden)[0], weight, bias, labels.contiguous(), None, int(ignore_index), 1.0)
+            return _VocabLoss.apply(_rows(hidden)[0], weight, bias, labels.contiguous(), None, int(ignore_index), 1.0, torch.is_grad_enabled())
         y = labels.reshape(-1).contiguous()
-        return _VocabLoss.apply(_rows(hidden)[0], weight, bias, y, None, int(ignore_index), 1.0).view(labels.shape)
+        return _VocabLoss.apply(_rows(hidden)[0], weight, bias, y, None, int(ignore_index), 1.0, torch.is_grad_enabled()).view(labels.shape)
 
 
 def vocab_distillation(hidden, weight, teacher_ids, teacher_logits, bias=None, temperature=1.0):
@@ -185,7 +185,7 @@ def vocab_distillation(hidden, weight, teacher_ids, teacher_logits, bias=None, t
         h, _ = _rows(hidden)
         ids, _ = _rows(teacher_ids)
         t, _ = _rows(teacher_logits.detach().float())
-        loss = _VocabLoss.apply(h, weight, bias, ids, t, -1, T)
+        loss = _VocabLoss.apply(h, weight, bias, ids, t, -1, T, torch.is_grad_enabled())
         return loss if hidden.dim() == 2 else loss.view(hidden.shape[:-1])
 
 

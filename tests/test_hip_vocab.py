@@ -435,6 +435,25 @@ def test_only_the_gradients_that_are_asked_for(R, V, K):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("R,V,K", [(20, 500, 64), (600, 2000, 100), (600, 30000, 100)])
+def test_without_recording_a_parameter_is_a_plain_tensor(R, V, K):
+    """Under no_grad leaves that want gradients give what plain tensors give, bit for bit, and nothing is kept for a backward."""
+    from gridmm_amd import vocab
+    h, w, b, g = _inputs("fp32", R, V, K)
+    labels = torch.randint(0, V, (R,), generator=g).cuda()
+    want = vocab.vocab_cross_entropy(h, w, labels, bias=b)
+    hl, wl, bl = _leaves(h, w, b)
+    with torch.no_grad():
+        got = vocab.vocab_cross_entropy(hl, wl, labels, bias=bl)
+    assert torch.equal(got, want) and not got.requires_grad
+    recorded = vocab.vocab_cross_entropy(hl, wl, labels, bias=bl)
+    # the two sets of kernels: fp32 products and sums, or two fp16 planes of each operand (_oracle's e_z, twice)
+    size = (h.double().abs() @ w.double().abs().t() + b.double().abs()).max(1)[0]
+    bound = 2 * (2 * (3 * 2.0 ** -22 + K * U) * size + (V + 32) * U * (want.double().abs() + size + 1))
+    assert bool(((recorded.detach().double() - want.double()).abs() <= bound).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("V", [3000, 30000])
 def test_runs_repeat_bit_for_bit_and_leave_their_inputs(V):
     h, w, b, g = _inputs("bf16", 300, V, 128)
