@@ -328,6 +328,7 @@ __global__ __launch_bounds__(256) void few_loss_kernel(const FewArgs a, int64_t 
   }
 }
 
+constexpr int FEW_J = 2;           // tiles of 16 vocabulary rows a wave of dW
 template <int DT, int RT, bool VEC>
 __global__ __launch_bounds__(256) void few_products_kernel(const FewArgs a, int h_blocks, int k_blocks) {
   constexpr int RP = RT * 16;
@@ -383,9 +384,13 @@ __global__ __launch_bounds__(256) void few_products_kernel(const FewArgs a, int 
       }
     return;
   }
-  // dW: 16 vocabulary rows a workgroup, every fourth run of 64 columns a wave; lane l ends with row j0 + l15, columns k0 + 16 i + 4 g + e
-  const int64_t j = ((int64_t)blockIdx.x - h_blocks) * 16 + l15;      // (dS has rows up to a multiple of 64)
-  if (a.db && wave == 0) {
+  // dW: 16 J vocabulary rows a workgroup, every fourth run of 64 columns a wave; lane l ends with rows jb + 16 u + l15, columns
+  // k0 + 16 i + 4 g + e.  The first group's dS (few rows: all there is) stays in registers for all runs.  dh and dW of 5 x
+  // 131072 x 2048 bf16: 305 us (dh 129 at 4.2 TB/s); loaded at each run, J = 1: 350; J = 4: 320, and 57 : 36 at 128 x 2216 x 512.
+  constexpr int J = FEW_J;
+  const int64_t jb = ((int64_t)blockIdx.x - h_blocks) * (16 * J) + l15;      // (dS has rows up to a multiple of 64)
+  if (a.db && wave < J) {
+    const int64_t j = jb + 16 * wave;
     float sum = 0.f;
     for (int group = 0; group < a.groups; ++group)
 #pragma unroll
@@ -395,47 +400,69 @@ __global__ __launch_bounds__(256) void few_products_kernel(const FewArgs a, int 
     if (g == 0 && j < a.vocab) store_as(a.db, j, a.bias_dtype, sum);
   }
   if (!a.dW) return;
-  for (int k0 = wave * 64; k0 < a.K; k0 += 256) {
-    f32x4_t acc[4];
+  float s0[J][4 * RT];
+  int64_t at0[4 * RT];                // -1: a row that does not count
+  auto load_group = [&](int group, float (&s)[J][4 * RT], int64_t (&at)[4 * RT]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < 4 * RT; ++q) {
+      const int r = group * RP + 4 * q + g;
+      at[q] = r < a.rows && a.flag[r] != 0.f ? r * a.ldh : -1;
+#pragma unroll
+      for (int u = 0; u < J; ++u) s[u][q] = a.dS[group * a.group_dS + (jb + 16 * u) * RP + 4 * q + g];
+    }
+  };
+  load_group(0, s0, at0);
+  for (int k0 = wave * 64; k0 < a.K; k0 += 256) {
+    f32x4_t acc[J][4];
+#pragma unroll
+    for (int u = 0; u < J; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[u][e] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     auto product = [&](auto full) {
       constexpr bool FULL = decltype(full)::value;
-      for (int group = 0; group < a.groups; ++group) {
-        const int r0 = group * RP;
-        const float* dS = a.dS + group * a.group_dS + j * RP;
+      auto add = [&](const float (&s)[J][4 * RT], const int64_t (&at)[4 * RT]) {
+        few_f4 h[4 * RT];
+#pragma unroll
+        for (int q = 0; q < 4 * RT; ++q) h[q] = few_load4<DT, VEC, FULL>(a.hidden, at[q] < 0 ? 0 : at[q], k0 + 4 * perm, a.K);
 #pragma unroll
         for (int q = 0; q < 4 * RT; ++q) {
-          const int r = r0 + 4 * q + g;
-          const bool in = r < a.rows && a.flag[r] != 0.f;
-          few_f4 h = few_load4<DT, VEC, FULL>(a.hidden, in ? r * a.ldh : 0, k0 + 4 * perm, a.K);
-          if (!in) h = (few_f4){0.f, 0.f, 0.f, 0.f};
-          const float s = dS[4 * q + g];
+          if (at[q] < 0) h[q] = (few_f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(h[e], s, acc[e], 0, 0, 0);
+          for (int u = 0; u < J; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[u][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(h[q][e], s[u][q], acc[u][e], 0, 0, 0);
         }
+      };
+      add(s0, at0);
+      for (int group = 1; group < a.groups; ++group) {
+        float s[J][4 * RT];
+        int64_t at[4 * RT];
+        load_group(group, s, at);
+        add(s, at);
       }
     };
     if (k0 + 64 <= a.K) product(std::true_type{});
     else product(std::false_type{});
-    if (j >= a.vocab) continue;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int k = k0 + 16 * i + 4 * g;
-      const float f[4] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
-      if (k + 4 <= a.K) {                       // (rows of any length: on their elements' boundaries)
-        if constexpr (DT == F32) {
-          *reinterpret_cast<few_f4_any*>(reinterpret_cast<float*>(a.dW) + j * a.K + k) = (few_f4_any){f[0], f[1], f[2], f[3]};
+    for (int u = 0; u < J; ++u) {
+      const int64_t j = jb + 16 * u;
+      if (j >= a.vocab) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = k0 + 16 * i + 4 * g;
+        const float f[4] = {acc[u][0][i], acc[u][1][i], acc[u][2][i], acc[u][3][i]};
+        if (k + 4 <= a.K) {                     // (rows of any length: on their elements' boundaries)
+          if constexpr (DT == F32) {
+            *reinterpret_cast<few_f4_any*>(reinterpret_cast<float*>(a.dW) + j * a.K + k) = (few_f4_any){f[0], f[1], f[2], f[3]};
+          } else {
+            const u16x4_t x = to_16x4<DT == F16>(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<few_u4_any*>(reinterpret_cast<unsigned short*>(a.dW) + j * a.K + k) = (few_u4_any){x[0], x[1], x[2], x[3]};
+          }
         } else {
-          few_u4_any u;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) u[e] = DT == BF16 ? to_bf16(f[e]) : to_f16(f[e]);
-          *reinterpret_cast<few_u4_any*>(reinterpret_cast<unsigned short*>(a.dW) + j * a.K + k) = u;
+          for (int e = 0; e < 4; ++e)
+            if (k + e < a.K) store_as(a.dW, j * a.K + k + e, DT, f[e]);
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (k + e < a.K) store_as(a.dW, j * a.K + k + e, DT, f[e]);
       }
     }
   }

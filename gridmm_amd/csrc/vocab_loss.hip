@@ -1363,7 +1363,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
     a.dS = (float*)(ws + P.b_ds); a.part = (float*)(ws + P.b_part);
     a.dh = d_hidden; a.dW = d_weight; a.db = d_bias;
     const int tiles = (d->vocab + 63) / 64, kb = (d->hidden_size + 255) / 256;
-    const int hb = d_hidden ? kb * P.ranges * P.groups : 0, wb = d_weight || d_bias ? (d->vocab + 15) / 16 : 0;
+    const int hb = d_hidden ? kb * P.ranges * P.groups : 0, wb = d_weight || d_bias ? (d->vocab + 16 * FEW_J - 1) / (16 * FEW_J) : 0;
     const int rc = by_few(d, P, [&](auto dt, auto rt, auto vec) {
       GRIDMM_LAUNCH((few_grad_kernel<decltype(rt)::value>), dim3(tiles, P.groups), dim3(256), 0, st, a);
       GRIDMM_CHECK_LAUNCH();
