@@ -85,8 +85,10 @@ struct Meta {
 
 // Tiles of the products over the counted rows.  256 x 256 where they fill the chip (one workgroup of 8 waves a CU), else 128 x 128 (two
 // of 4 waves a CU).  The host does not know the count: where both may be right it launches both, each sized for its own range, and the
-// workgroups of the one whose turn it is not end at once.
-constexpr int BIG_TILES = 384;       // 1.5 rounds of 256 CUs
+// workgroups of the one whose turn it is not end at once.  256 x 256 from 1.5 rounds of 256 CUs on; the forward at 1024 hidden, us, 256 x 256 : 128 x
+// 128, at 314, 384, 512 tiles: bf16 66 : 58, 64 : 64, 72 : 79; fp32 230 : 232, 191 : 205, 206 : 239.  (One full round, 256 tiles, is better off too,
+// 45 : 48 and 127 : 143, but what follows it is not, and the rule has to rise with the count to spare most calls the second launch.)
+constexpr int BIG_TILES = 384;
 __host__ __device__ inline bool big_tiles(int64_t count, int64_t C) { return count > 256 && (count + 255) / 256 * (C / 256) >= BIG_TILES; }
 // Contraction ranges of dh, so that its few tiles fill whole rounds of the chip: the cheapest of the numbers that fit into the first
 // rounds, in stages of 64 columns a workgroup (1.2 us): rounds x (its share + what a tile costs beside its stages) + the ranges' sums
