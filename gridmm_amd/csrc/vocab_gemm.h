@@ -257,6 +257,9 @@ struct Tile {
       // One stage: its products, with the reads of the fragments ahead and the transfers of the stage after next between them, one
       // after each matrix instruction, so that none of them waits for a burst of the others.
       for (int kt = 0; kt < item.nk; ++kt, ++stage) {
+        float part[TM];                      // a stage's sums first: fewer roundings of the long ones
+#pragma unroll
+        for (int i = 0; i < TM; ++i) part[i] = 0.f;
         constexpr int NP = PL == 2 ? 3 : 1, NM = TM * TN, AT = PL == 2 ? NM - 1 : 0;      // the barrier follows product AT of the last sub-step
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -286,8 +289,9 @@ struct Tile {
           if (SUMA && sum) {
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
-              sums[i] = sum8<F16>(a[set][i], sums[i]);
-              if constexpr (PL == 2) sums[i] = sum8<F16>(al[i], sums[i]);
+              part[i] = sum8<F16>(a[set][i], part[i]);
+              if constexpr (PL == 2) part[i] = sum8<F16>(al[i], part[i]);
+              if (last) sums[i] += part[i];
             }
           }
           if (last) moved();
