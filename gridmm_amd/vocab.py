@@ -170,7 +170,8 @@ def vocab_distillation(hidden, weight, teacher_ids, teacher_logits, bias=None, t
     q = softmax((hidden weight^T + bias) / T) over the whole vocabulary, T^2 sum_s p_s (log p_s - log q[id_s]) as fp32 losses of
     hidden's leading shape.  teacher_ids (..., S) int64 or int32: an id < 0 is an empty slot, an id >= V makes its row NaN, ids may
     repeat; teacher_logits (..., S) (top_logits gives both).  A row without a filled slot above -inf: loss 0, no gradient.
-    Gradients of hidden, weight and bias; the teacher gets none."""
+    Gradients of hidden, weight and bias; the teacher gets none.  1e-6 <= T <= 1e6, at most 2^16 slots; sizes else as
+    vocab_cross_entropy."""
     _check_head(hidden, weight, bias, teacher_ids, teacher_logits)
     _need(teacher_ids.dim() >= 1 and teacher_ids.shape == teacher_logits.shape
           and tuple(teacher_ids.shape[:-1]) == tuple(hidden.shape[:-1]) and teacher_ids.shape[-1] >= 1,
