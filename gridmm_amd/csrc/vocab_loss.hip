@@ -14,8 +14,9 @@
 // Rows that do not count (label == ignore_index; no filled slot) are left out on the device: the counted rows are compacted into
 // the packed copy of h, the grids are sized for all rows and workgroups past the count end at once -- no host read-back.
 //
-// Number formats.  bf16 / fp16 operands: one plane, products exact, sums fp32; dS is rounded to the operands' type (2^-8 / 2^-11
-// of an entry at most, like the gradients themselves), with few counted rows to two planes of it.  fp32 operands: two fp16 planes each (22 bits) after a
+// Number formats.  bf16 / fp16 operands: one plane, products exact, sums fp32; dS in two planes of the operands' type, an entry off by
+// 2^-16 (bf16) or 2^-22 (fp16) of itself, so that a gradient is rounded once, to its own type.  (One plane leaves 1.4 times that error, up to
+// twice where a handful of entries makes up a sum; 8030 x 131072 x 2048 13.9 ms against 21.2.)  fp32 operands: two fp16 planes each (22 bits) after a
 // power-of-two scale from the tensor's largest finite value, so a product is off by ~2^-22: like fp32 sums.  dS is scaled by a power of
 // two from the largest |g T| of the call (fp16 range: entries below 2^-38 of it vanish).
 // Bound by the four products (vocab_gemm.h): 8030 x 131072 x 2048 bf16 forward and backward 13.8 - 14.0 ms, of it 3.4 scores, 3.7 dS, 3.4 dh, 3.4 dW;
@@ -705,9 +706,8 @@ __device__ __forceinline__ void rows_of_32(unsigned short* scratch, const float4
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// dS of the columns [j0, j0 + C): dS[r][j] = g_r T exp2(y_rj - lse_r), two planes for fp32 operands and few rows (TWO); at the row's label, from its fp32
-// score, g_r (exp2(..) - 1)
-template <class T, bool TWO>
+// dS of the columns [j0, j0 + C): dS[r][j] = g_r T exp2(y_rj - lse_r) in two planes; at the row's label, from its fp32 score, g_r (exp2(..) - 1)
+template <class T>
 __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Operand B, int nk, int tn, const Meta* __restrict__ meta,
                                                                 const float* __restrict__ biasz, float unit, const GradArgs G, int64_t j0,
                                                                 unsigned short* __restrict__ dS, int64_t plane) {
@@ -718,7 +718,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
   const float sc = ldexpf(unit, -(meta->sh + meta->sw));
   unsigned short* scratch = smem + T::LDS + wave * 2048;
   static_assert(T::TN == 2, "64 columns a wave");
-  const int64_t ldS = T::PL == 2 || TWO ? 2 * plane : plane;
+  const int64_t ldS = 2 * plane;
   const int sg = grad_exponent<T>(G, count, reinterpret_cast<float*>(smem + T::LDS));
   if (blockIdx.x == 0 && threadIdx.x == 0) *G.scale = sg;
   T::run(
@@ -773,10 +773,10 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
             float v[4];
             values(c, v);
             hi[c] = to_16x4<T::F16>(v[0], v[1], v[2], v[3]);
-            if constexpr (T::PL == 2 || TWO) lo[c] = to_16x4<T::F16>(v[0] - rounded(v[0]), v[1] - rounded(v[1]), v[2] - rounded(v[2]), v[3] - rounded(v[3]));
+            lo[c] = to_16x4<T::F16>(v[0] - rounded(v[0]), v[1] - rounded(v[1]), v[2] - rounded(v[2]), v[3] - rounded(v[3]));
           }
           put(hi, target, at);
-          if constexpr (T::PL == 2 || TWO) put(lo, target - rounded(target), at + plane);
+          put(lo, target - rounded(target), at + plane);
         }
       });
 }
@@ -795,7 +795,7 @@ __device__ __forceinline__ void target_entry(const FixArgs& a, int64_t i, int s,
   const float v = ldexpf(a.G.g[a.G.rowmap[i] * a.G.gs] * a.G.temperature, *a.G.scale) * (__builtin_amdgcn_exp2f(2.f * a.G.zt[i * a.slots + s] - a.G.lse[i]) - p);
   unsigned short* at = a.dS + i * a.ldS + (id - a.j0);
   at[0] = a.dtype == BF16 ? to_bf16(v) : to_f16(v);
-  if (a.ldS > a.plane) at[a.plane] = a.dtype == BF16 ? to_bf16(v - bf16_bits_to_f32(at[0])) : to_f16(v - (float)__builtin_bit_cast(_Float16, at[0]));
+  at[a.plane] = a.dtype == BF16 ? to_bf16(v - bf16_bits_to_f32(at[0])) : to_f16(v - (float)__builtin_bit_cast(_Float16, at[0]));
 }
 // one row a workgroup, 256 of its slots in LDS at a time; several slots may name one id: each of them writes the same value
 __global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
@@ -827,7 +827,7 @@ __global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
 
 // dh of this piece: partial products over the contraction ranges blockIdx.y, added to those of the pieces before.  `C`: the columns of
 // a whole piece, which fix the tile and the number of ranges for all pieces.
-template <class T, bool TWO>
+template <class T>
 __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, Operand B, int steps, int tn, int64_t C,
                                                                  const Meta* __restrict__ meta, float* __restrict__ part, int64_t Kp,
                                                                  int first, int* __restrict__ ranges) {
@@ -835,6 +835,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, O
   const int count = __builtin_amdgcn_readfirstlane(meta->count), tm = (count + T::BM - 1) / T::BM;
   const bool big = big_tiles(count, C);
   if (big != (T::BM == 256)) return;
+  constexpr bool TWO = T::PL == 1;       // dS's two planes one after the other
   const int splits = hidden_splits(count, Kp, C, big), per = (steps + splits - 1) / splits;
   if (blockIdx.x == 0 && threadIdx.x == 0) *ranges = splits;
   const int wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
@@ -903,12 +904,13 @@ __global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict
 
 // dW of this piece: rows [j0, j0 + C) complete (the contraction is all counted rows), written once in the weight's type; the first
 // tile column also sums dS over the rows: db
-template <class T, bool TWO>
+template <class T>
 __global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, Operand B, int tm, int tn, const Meta* __restrict__ meta,
                                                                  const int* __restrict__ scale, int dtype, int64_t j0, int vocab, int K,
                                                                  void* __restrict__ dW, int bias_dtype, void* __restrict__ db) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
   const int count = __builtin_amdgcn_readfirstlane(meta->count);
+  constexpr bool TWO = T::PL == 1;
   const int nk = (count + T::BK - 1) / T::BK * (TWO ? 2 : 1);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
   const int eb = -*scale, e = eb - meta->sh;       // exponents of the units of db and dW
@@ -1031,15 +1033,9 @@ bool target_lists(const gridmm_vocab_loss_t* d) {
   return d->slots && d->slots <= LIST_SLOTS && d->vocab <= LIST_BLOCKS * 64 - 256 && bytes / 7e6 > 12 + 2.8e-7 * d->rows * d->vocab;
 }
 
-// 16-bit operands: dS in two planes, entry = hi + lo, for up to so many rows.  A gradient that a handful of entries makes up shows the
-// rounding of each, a sum over many rows their mean: one plane leaves 1.4 times the error of the gradients' own rounding at thousands of
-// rows, up to twice that at a few.  So few rows are bound by the read of W and the write of dW, not by the products (128 x 128 tiles;
-// in the kernels of the large tile the second plane's registers cost 1.5 % at 8030 x 131072 x 2048).
-constexpr int TWO_PLANES = 256;
-
 struct Plan {
   int PL, slots;               // planes; target slots a row (cross entropy: 1)
-  bool few, two, lists;
+  bool few, lists;
   int RP, groups, ranges, range;      // few rows: rows a group (16 or 32), groups; ranges of the vocabulary in dh and their rows
   int64_t Rp, Kp, Vp;
   bool pack_w;                 // W has to be split or padded; else it is read where it lies
@@ -1077,7 +1073,7 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
     return (int64_t)up((P.Vp + n - 1) / n, 256);
   };
   P.C_fwd = P.pack_w ? piece(P.Kp * 2 * P.PL) : P.Vp;
-  P.C_bwd = piece(std::max<int64_t>(P.Rp, 1) * 2 * P.PL);
+  P.C_bwd = piece(std::max<int64_t>(P.Rp, 1) * 4);
   P.keep_w = P.pack_w && P.C_fwd == P.Vp;
   if (P.pack_w) P.C_bwd = std::min(P.C_bwd, P.C_fwd);
   P.few = few_rows(d);
@@ -1133,8 +1129,7 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.fwd = o;
   o = 0;
   P.b_scale = take(8);                 // ... and the ranges of dh
-  P.two = P.PL == 1 && d->rows <= TWO_PLANES;
-  P.b_ds = take(Rp * (size_t)P.C_bwd * 2 * (P.two ? 2 : P.PL));
+  P.b_ds = take(Rp * (size_t)P.C_bwd * 4);
   P.b_w = take(P.pack_w && !P.keep_w ? (size_t)P.C_bwd * P.Kp * 2 * P.PL : 0);
   P.b_part = take(std::max<size_t>(Rp * (size_t)P.Kp, std::min<size_t>(MOST_SPLITS * Rp * (size_t)P.Kp, PART_MOST)) * 4);
   P.bwd = o;
@@ -1397,26 +1392,18 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
     Operand W;
     int rc = weight_piece(d, P, j0, C, meta, (unsigned short*)(sv + P.o_w), false, wbuf, st, W);
     if (rc != GRIDMM_OK) return rc;
-    const int64_t ldS = (P.two ? 2 : P.PL) * C;
+    const int64_t ldS = 2 * C;
     const Operand S{dS, ldS, C, P.Rp, C};
     rc = by_type(d, [&](auto f16, auto pl) {
       constexpr bool F = decltype(f16)::value;
       constexpr int L = decltype(pl)::value;
-      // calls f(two planes?): only the small tile has them
-      auto one_or_two = [&](auto big, auto f) {
-        if constexpr (L == 1 && !decltype(big)::value)
-          if (P.two) return f(std::true_type{});
-        return f(std::false_type{});
-      };
       int rc = by_tile(d->rows, C, [&](auto big, int rows) {
         using T = TileOf<F, L, decltype(big)::value, false, false>;
         const int64_t tn = C / T::BN, tm = (rows + T::BM - 1) / T::BM;
-        return one_or_two(big, [&](auto two) {
-          GRIDMM_LAUNCH((score_grad_kernel<T, decltype(two)::value>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, H, W,
-                        (int)(P.Kp / T::BK), (int)tn, meta, biasz + j0, unit, G, j0, dS, C);
-          GRIDMM_CHECK_LAUNCH();
-          return GRIDMM_OK;
-        });
+        GRIDMM_LAUNCH((score_grad_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), (int)tn, meta, biasz + j0,
+                      unit, G, j0, dS, C);
+        GRIDMM_CHECK_LAUNCH();
+        return GRIDMM_OK;
       });
       if (rc != GRIDMM_OK) return rc;
       if (d->slots) {
@@ -1431,12 +1418,10 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
         rc = by_tile(d->rows, P.C_bwd, [&](auto big, int rows) {
           using T = TileOf<F, L, decltype(big)::value, false, true>;
           const int64_t tn = (P.Kp + T::BN - 1) / T::BN, tm = (rows + T::BM - 1) / T::BM;
-          return one_or_two(big, [&](auto two) {
-            GRIDMM_LAUNCH((hidden_grad_kernel<T, decltype(two)::value>), dim3(blocks<T>(tm * tn * MOST_SPLITS)),
-                          dim3(T::THREADS), 0, st, S, W, (int)(C / T::BK), (int)tn, P.C_bwd, meta, part, P.Kp, j0 == 0, scale + 1);
-            GRIDMM_CHECK_LAUNCH();
-            return GRIDMM_OK;
-          });
+          GRIDMM_LAUNCH((hidden_grad_kernel<T>), dim3(blocks<T>(tm * tn * MOST_SPLITS)), dim3(T::THREADS), 0, st, S, W, (int)(C / T::BK), (int)tn,
+                        P.C_bwd, meta, part, P.Kp, j0 == 0, scale + 1);
+          GRIDMM_CHECK_LAUNCH();
+          return GRIDMM_OK;
         });
         if (rc != GRIDMM_OK) return rc;
       }
@@ -1444,14 +1429,12 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
         auto weight = [&](auto big) {
           using T = TileOf<F, L, decltype(big)::value, true, true>;
           const int64_t tn = d_weight ? (P.Kp + T::BN - 1) / T::BN : 1, tm = C / T::BM;      // (db alone: the first tile column)
-          return one_or_two(big, [&](auto two) {
-            GRIDMM_LAUNCH((weight_grad_kernel<T, decltype(two)::value>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, S, H, (int)tm, (int)tn,
-                          meta, scale, d->dtype, j0, d->vocab, d->hidden_size, d_weight, d->bias_dtype, d_bias);
-            GRIDMM_CHECK_LAUNCH();
-            return GRIDMM_OK;
-          });
+          GRIDMM_LAUNCH((weight_grad_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, S, H, (int)tm, (int)tn, meta, scale, d->dtype, j0,
+                        d->vocab, d->hidden_size, d_weight, d->bias_dtype, d_bias);
+          GRIDMM_CHECK_LAUNCH();
+          return GRIDMM_OK;
         };
-        rc = !P.two && C / 256 * ((P.Kp + 255) / 256) >= BIG_TILES ? weight(std::true_type{}) : weight(std::false_type{});
+        rc = C / 256 * ((P.Kp + 255) / 256) >= BIG_TILES ? weight(std::true_type{}) : weight(std::false_type{});
         if (rc != GRIDMM_OK) return rc;
       }
       return GRIDMM_OK;

@@ -1,0 +1,72 @@
+"""The vocabulary losses and top logits where rounding and range decide: many rows of 16 bits, rows the model is sure of, rows of very
+different size, upstream gradients far apart, columns that one tile holds, teachers' and masks' extreme values.
+
+Tolerances (u = 2^-24, half a step of fp32; they count roundings as independent, where a bound that adds all of them would hide what is
+looked for; the worst-case bounds are those of test_hip_vocab.py):
+  score     an fp32 sum of K products whose partial sums stay below m = max |z| + 1 makes K roundings of at most u m each, in no common
+            direction: 8 standard deviations are 8 sqrt(K) u m / sqrt(3); two fp16 planes add 3 2^-22 of each term: less than that again.
+            e_z = 8 sqrt(K) u m
+  loss      a difference of two such scores, and a sum of positive terms that agree to e_z: 3 e_z
+  q = exp(z - L) is off by 2 e_z of itself; gradients' entries by 3 e_z of the sum of the sizes of their terms, plus half a step of
+            their type
+"""
+import math
+
+import pytest
+import torch
+
+from test_hip_vocab import DT, HALF, U, _inputs, _leaves, _run_ce, _teacher
+
+
+def _e_z(K, z):
+    return 8 * K ** 0.5 * U * (float(z[torch.isfinite(z)].abs().max()) + 1)
+
+
+def _exact(h, w, b, ids, p, T, g):
+    """Losses and gradients in 64 bits, by the formulas; ids / p (R, S), g (R,).  Also the sums of the sizes of the gradients' terms."""
+    H, W = h.double(), w.double()
+    z = H @ W.t()
+    if b is not None:
+        z = z + b.double()
+    z = z / T
+    L = torch.logsumexp(z, 1)
+    zt = z.gather(1, ids)
+    logp = torch.where(p > 0, p.log(), torch.zeros_like(p))
+    loss = T * T * (p * (logp - torch.where(p > 0, zt, torch.zeros_like(zt)) + L[:, None])).sum(1)
+    q = (z - L[:, None]).exp()
+    target = torch.zeros_like(q).scatter_add_(1, ids, p)
+    gt = (g.double() * T)[:, None]
+    dS, size = gt * (q - target), gt.abs() * (q + target)
+    out = {"loss": loss, "d_hidden": dS @ W, "d_weight": dS.t() @ H, "d_bias": dS.sum(0)}
+    sizes = {"d_hidden": size @ W.abs(), "d_weight": size.t() @ H.abs(), "d_bias": size.sum(0)}
+    return z, out, sizes
+
+
+# ---- the gradient of the scores is not what 16-bit gradients show ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("R,V,K", [(300, 5003, 512), (1030, 5003, 264), (3000, 9001, 256)])
+@pytest.mark.parametrize("loss", ["cross_entropy", "distillation"])
+def test_gradients_of_many_16_bit_rows_are_rounded_once(dtype, R, V, K, loss):
+    """The error of a 16-bit gradient is that of its own rounding.  dS in two 16-bit planes is off by at most half a step squared of an
+    entry (2^-16, 2^-22); against the half step of the result that is 2^-8 at most, and the squares of independent errors add: (1 + 2^-16)
+    under the root; sums of K or R fp32 terms are far below.  1.02 leaves room for few entries (d_bias: V of them).  One plane of dS gives 1.4."""
+    from gridmm_amd import vocab
+    h, w, b, g = _inputs(dtype, R, V, K, True, seed=R)
+    gr = (torch.rand(R, generator=g) + 0.5).cuda()
+    hl, wl, bl = _leaves(h, w, b)
+    if loss == "cross_entropy":
+        ids = torch.randint(0, V, (R, 1), generator=g).cuda()
+        p, T = torch.ones(R, 1, dtype=torch.float64, device="cuda"), 1.0
+        vocab.vocab_cross_entropy(hl, wl, ids[:, 0], bias=bl).backward(gr)
+    else:
+        T = 2.0
+        ids = torch.stack([torch.randperm(V, generator=g)[:16] for _ in range(R)]).cuda()
+        t = (torch.randn(R, 16, generator=g) * 3).cuda()
+        p = _teacher(ids, t, T)
+        vocab.vocab_distillation(hl, wl, ids, t, bias=bl, temperature=T).backward(gr)
+    _, want, _ = _exact(h, w, b, ids, p, T, gr)
+    for k, x in (("d_hidden", hl.grad), ("d_weight", wl.grad), ("d_bias", bl.grad)):
+        own = want[k].to(DT[dtype]).double() - want[k]
+        ratio = float((x.double() - want[k]).norm() / own.norm())
+        assert ratio <= 1.02, (k, ratio)
