@@ -70,3 +70,48 @@ def test_gradients_of_many_16_bit_rows_are_rounded_once(dtype, R, V, K, loss):
         own = want[k].to(DT[dtype]).double() - want[k]
         ratio = float((x.double() - want[k]).norm() / own.norm())
         assert ratio <= 1.02, (k, ratio)
+
+
+# ---- no tile is left out ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,R,V,K", [("bf16", 300, 70000, 64), ("fp32", 300, 70000, 64), ("fp16", 300, 33000, 72), ("fp32", 20, 9001, 64),
+                                         ("bf16", 9100, 33001, 72), ("fp32", 2100, 40003, 128), ("fp32", 270, 300001, 520)])
+def test_every_tile_counts(dtype, R, V, K):
+    """Each block of 64 columns in turn holds the column that makes up nearly all of a row's sum, and each in turn the label: a block left
+    out of the sum, the scores or the gradients changes a loss by more than 5.  Then flat rows: the sum of V equal terms is off by less
+    than half of what one block of 64 columns is of it."""
+    from gridmm_amd import vocab
+    g = torch.Generator().manual_seed(V)
+    w = torch.randn(V, K, generator=g)
+    w = (w * (4.0 / w.norm(dim=1, keepdim=True))).to(DT[dtype])
+    blocks = (V + 63) // 64
+    at = torch.arange(max(R, blocks)) % blocks
+    top = (at * 64 + torch.randint(0, 64, at.shape, generator=g)).clamp(max=V - 1)
+    label = ((at * 7919 + 13) % blocks * 64 + torch.randint(0, 64, at.shape, generator=g)).clamp(max=V - 1)
+    w, label, top = w.cuda(), label.cuda(), top.cuda()
+    for r0 in range(0, at.numel(), R):
+        t, y = top[r0:r0 + R], label[r0:r0 + R]
+        h = (w[t].float() * (24.0 / 16.0)).to(DT[dtype])
+        hl = h.requires_grad_()
+        loss = vocab.vocab_cross_entropy(hl, w, y)
+        z = h.detach().double() @ w.double().t()
+        L = torch.logsumexp(z, 1)
+        want = L - z.gather(1, y[:, None])[:, 0]
+        ez = _e_z(K, z)
+        near = (loss.detach().double() - want).abs() <= 3 * ez + 8 * U * 40
+        assert bool(near.all()), (r0, int((~near).sum()))
+        if r0 == 0:
+            assert float((L - torch.logsumexp(z.scatter(1, t[:, None], float("-inf")), 1)).min()) > 5
+        loss.sum().backward()
+        dS = (z - L[:, None]).exp()
+        dS.scatter_add_(1, y[:, None], torch.full_like(y[:, None], -1, dtype=torch.float64))
+        d = hl.grad.double() - dS @ w.double()
+        assert float(d.abs().max()) <= (3 * ez * 2 + HALF[DT[dtype]] * 2) * 4, r0
+        del z, dS, d, hl, loss
+    flat = (torch.randn(min(R, 300), K, generator=g) * 2.0 ** -12).to(DT[dtype]).cuda()
+    y = label[:flat.shape[0]]
+    loss = vocab.vocab_cross_entropy(flat, w, y).double()
+    z = flat.double() @ w.double().t()
+    bound = 3 * _e_z(K, z) + 8 * U * math.log(V)
+    assert bound < 32.0 / V
+    assert float((loss - torch.logsumexp(z, 1) + z.gather(1, y[:, None])[:, 0]).abs().max()) <= bound
