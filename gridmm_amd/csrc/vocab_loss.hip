@@ -1060,7 +1060,7 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.Kp = (int64_t)up(d->hidden_size, 64);
   P.Vp = (int64_t)up(d->vocab, 256);
   // (a tile's 256 rows are addressed with 32-bit byte offsets: at most 2^31 from one row to the last where W lies)
-  P.pack_w = d->dtype == F32 || d->hidden_size % 64 || d->ld_weight % 8 || ((uintptr_t)d->weight & 15) || d->ld_weight > (1 << 22);
+  P.pack_w = d->packed || d->dtype == F32 || d->hidden_size % 64 || d->ld_weight % 8 || ((uintptr_t)d->weight & 15) || d->ld_weight > (1 << 22);
   // (grids: at most 2^32 threads)
   if ((P.Rp / 128) * (P.Vp / 128) > (1 << 23) || (int64_t)d->rows * ((P.slots + 7) / 8) > (1 << 25)) return false;
   // pieces: packed W and dS at most MOST bytes each, whole tiles, 8 192 columns at least

@@ -28,7 +28,7 @@ class _Desc(ctypes.Structure):
     """gridmm_vocab_loss_t of include/gridmm.h."""
     _fields_ = ([(n, ctypes.c_void_p) for n in ("hidden", "weight", "bias", "labels", "ids", "teacher")]
                 + [(n, ctypes.c_int64) for n in ("ld_hidden", "ld_weight", "ld_ids", "ld_teacher", "ignore_index")]
-                + [(n, ctypes.c_int) for n in ("rows", "vocab", "hidden_size", "slots", "dtype", "bias_dtype", "index64", "forward_only")]
+                + [(n, ctypes.c_int) for n in ("rows", "vocab", "hidden_size", "slots", "dtype", "bias_dtype", "index64", "forward_only", "packed")]
                 + [("temperature", ctypes.c_float)])
 
 
@@ -83,10 +83,38 @@ def _check_head(hidden, weight, bias, *index):
             raise ValueError("bias is %s: fp32 or the weight's type" % bias.dtype)
 
 
+def _apart(w, ld):
+    """Rows that the tile products cannot read where they lie (16 bits: 16-byte boundaries, 32-bit offsets within a tile)."""
+    return w.data_ptr() & 15 != 0 or ld % 8 != 0 or ld > 1 << 22
+
+
 def _vocab_backward(ctx, g):
     if g is None:
         return (None,) * 8
-    hidden, w, b, _, saved = ctx.saved_tensors
+    # What saved-tensor hooks give back (checkpointing, offloading) are other tensors than the forward's, which may be gone: the
+    # kernels get the addresses of these.
+    hidden, w, b, index, saved = ctx.saved_tensors
+    d = _Desc.from_buffer_copy(ctx.desc)
+    for t in (hidden, w, index, saved) + (() if b is None else (b,)):
+        if not t.device == g.device:
+            raise RuntimeError("a tensor kept for the backward came back on %s, its gradient is on %s" % (t.device, g.device))
+    if (hidden.shape, w.shape, hidden.dtype, w.dtype, index.shape, index.dtype) != ctx.kept:
+        raise RuntimeError("the tensors kept for the backward came back with other shapes or types")
+    h, ldh = _rows(hidden)
+    w, ldw = _rows(w)
+    if not d.packed and _apart(w, ldw):          # (the forward read W where it lay)
+        w, ldw = w.clone(memory_format=torch.contiguous_format), w.shape[1]
+    if d.slots:
+        index, ldi = _rows(index)
+        d.ids, d.ld_ids = index.data_ptr(), max(ldi, d.slots)
+    else:
+        index = index.contiguous()
+        d.labels = index.data_ptr()
+    # (a single row: whatever its stride says)
+    d.hidden, d.ld_hidden, d.weight, d.ld_weight, d.teacher = h.data_ptr(), max(ldh, d.hidden_size), w.data_ptr(), ldw, None
+    if b is not None:
+        b = b.contiguous()
+        d.bias = b.data_ptr()
     if g.dtype != torch.float32:
         g = g.float()
     need_h, need_w, need_b = ctx.needs_input_grad[:3]
@@ -98,7 +126,7 @@ def _vocab_backward(ctx, g):
         ws = saved.new_empty(n_ws)
         # (addresses as plain numbers: half the time of an object each)
         _lib.check(_lib.load().gridmm_vocab_loss_bwd(
-            ctypes.byref(ctx.desc), saved.data_ptr(), saved.numel(), g.data_ptr(), g.stride(0), dh.data_ptr() if need_h else None,
+            ctypes.byref(d), saved.data_ptr(), saved.numel(), g.data_ptr(), g.stride(0), dh.data_ptr() if need_h else None,
             dw.data_ptr() if need_w else None, db.data_ptr() if need_b else None, ws.data_ptr(), n_ws, _stream()), "gridmm_vocab_loss_bwd")
     return dh, DEFERRED.hand(prm[0], dw), DEFERRED.hand(prm[1], db), None, None, None, None, None
 
@@ -121,7 +149,7 @@ class _VocabLoss(torch.autograd.Function):
         d = _Desc(hidden.data_ptr(), w.data_ptr(), None if b is None else b.data_ptr(), None if S else at, at if S else None,
                   teacher.data_ptr() if S else None, max(hidden.stride(0), K), ldw, max(index.stride(0), S) if S else 0,
                   max(teacher.stride(0), S) if S else 0, ignore_index, R, V, K, S, _DTYPES[dt], 0 if b is None else _DTYPES[b.dtype],
-                  index.dtype == torch.int64, not need, temperature)
+                  index.dtype == torch.int64, not need, _apart(w, ldw), temperature)
         ref = ctypes.byref(d)
         n_saved, n_ws = lib.gridmm_vocab_loss_saved_bytes(ref), lib.gridmm_vocab_loss_workspace(ref, 0)
         if n_saved == 0:
@@ -135,7 +163,9 @@ class _VocabLoss(torch.autograd.Function):
         if need:
             ctx.set_materialize_grads(False)
             ctx.save_for_backward(hidden, w, b, index, saved)
-            ctx.desc, ctx.prm, ctx.n_ws = d, (weight, bias), lib.gridmm_vocab_loss_workspace(ref, 1)
+            ctx.desc, ctx.n_ws = d, lib.gridmm_vocab_loss_workspace(ref, 1)
+            ctx.kept = (hidden.shape, w.shape, dt, dt, index.shape, index.dtype)
+            ctx.prm = [t if isinstance(t, torch.nn.Parameter) else None for t in (weight, bias)]      # (nothing else is kept alive here)
         return loss
 
     @staticmethod

@@ -829,7 +829,9 @@ int gridmm_dropout_add(const float* x, const float* r, float* y, void* y_hi, voi
  * with other labels.  A column whose bias is -inf or the type's lowest number is out of the sum.
  *   saved      >= gridmm_vocab_loss_saved_bytes, 256-byte aligned: filled by _fwd, read (not changed) by _bwd
  *   workspace  >= gridmm_vocab_loss_workspace(d, 0 forward / 1 backward) bytes, 256-byte aligned (NULL if that is 0)
- *              (all four calls take one and the same *d, pointers and strides included: alignment chooses the kernels)
+ *              (all four calls take the same *d.  Pointers and strides of the backward may be others, of copies of the same values, as
+ *              long as the weight's 16 bits stay on 16-byte boundaries, its stride a multiple of 8 and at most 2^22, if they were so)
+ *   packed != 0 weight is not read where it lies, whatever its alignment: no such condition
  *   forward_only != 0: no backward will follow (other kernels may be the faster ones then)
  *   backward   grad: d loss_r at grad[r * grad_stride] (0: one value for all rows); d_hidden [rows][hidden_size],
  *              d_weight [vocab][hidden_size] dense in dtype, d_bias [vocab] in bias_dtype, each overwritten, each may be NULL (one
@@ -838,7 +840,7 @@ typedef struct {
   const void *hidden, *weight, *bias, *labels, *ids;
   const float* teacher;
   int64_t ld_hidden, ld_weight, ld_ids, ld_teacher, ignore_index;
-  int rows, vocab, hidden_size, slots, dtype, bias_dtype, index64, forward_only;
+  int rows, vocab, hidden_size, slots, dtype, bias_dtype, index64, forward_only, packed;
   float temperature;
 } gridmm_vocab_loss_t;
 size_t gridmm_vocab_loss_saved_bytes(const gridmm_vocab_loss_t* d);
