@@ -27,7 +27,8 @@ struct FewArgs {
   int rows, vocab, K, slots, wide, dtype, bias_dtype, kd;
   float inv_t, unit, temperature;
   float2* stats;                 // [workgroup][groups RP]
-  float *lse, *zt, *p, *flag;    // saved: [groups RP], [rows][slots] (halves), [rows][slots], [groups RP]: 1 for rows that count
+  float2* stat;                  // saved: [groups RP] maximum and sum
+  float *zt, *p, *flag;          // saved: [rows][slots] (halves), [rows][slots], [groups RP]: 1 for rows that count
   float* y;                      // saved: the scores, base 2, laid out like dS; NULL: no backward will follow
   float* loss;
   const float* grad;
@@ -268,7 +269,9 @@ __global__ __launch_bounds__(256) void few_grad_kernel(const FewArgs a) {
   for (int t = 0; t < RT; ++t) {
     const int r = r0 + t * 16 + l15;
     const bool live = r < a.rows && a.flag[r] != 0.f;
-    const float gt = live ? a.grad[r * a.grad_stride] * a.temperature : 0.f, L = live ? a.lse[r] : 0.f;
+    const float gt = live ? a.grad[r * a.grad_stride] * a.temperature : 0.f;
+    const float2 st = live ? a.stat[r] : make_float2(0.f, 1.f);
+    const float inv = 1.f / st.y;
     float p[4] = {0.f, 0.f, 0.f, 0.f};
     if (live)
       few_targets(a, T, r0, t * 16 + l15, jl, [&](int k, int d) {
@@ -279,7 +282,7 @@ __global__ __launch_bounds__(256) void few_grad_kernel(const FewArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int64_t at = blockIdx.y * a.group_dS + (jl + i) * RP + t * 16 + l15;
-      a.dS[at] = live ? gt * (__builtin_amdgcn_exp2f(a.y[at] - L) - p[i]) : 0.f;
+      a.dS[at] = live ? gt * fmaf(__builtin_amdgcn_exp2f(a.y[at] - st.x), inv, -p[i]) : 0.f;
     }
   }
 }
@@ -297,33 +300,33 @@ __global__ __launch_bounds__(256) void few_loss_kernel(const FewArgs a, int64_t 
   if (wave) return;
   s = part[0];
   for (int w = 1; w < 4; ++w) s = join_stats(s, part[w]);
-  float L = s.x + __builtin_amdgcn_logf(s.y), out = 0.f;
-  bool live;
+  const float ls = 0.5f * __builtin_amdgcn_logf(s.y);      // (halves, base 2)
+  float out = 0.f;
+  bool live, bad = false;
   if (a.kd) {
     float plogp;
     live = teacher_row(a.index, a.wide, a.ld_index, a.teacher, a.ld_teacher, r, a.slots, a.inv_t, a.p, plogp);
-    float cross = 0.f;
-    bool bad = false;
+    float cross = 0.f, mass = 0.f;
     for (int k = lane; k < a.slots; k += 64) {
       const int64_t id = load_index(a.index, r * a.ld_index + k, a.wide);
       const float q = a.p[(int64_t)r * a.slots + k];
       if (id < 0) continue;
       bad |= id >= a.vocab;
-      if (id < a.vocab && !(q == 0.f)) cross += q * (0.5f * L - a.zt[(int64_t)r * a.slots + k]);
+      if (id < a.vocab && !(q == 0.f)) { cross += q * (0.5f * s.x - a.zt[(int64_t)r * a.slots + k]); mass += q; }
     }
     cross = wave_sum(cross);
-    out = __any(bad) ? NAN : a.temperature * a.temperature * (plogp + natural(cross));
-    if (__any(bad)) L = NAN;
+    mass = wave_sum(mass);
+    bad = __any(bad);
+    out = a.temperature * a.temperature * (plogp + natural(fmaf(mass, ls, cross)));
   } else {
     const int64_t y = load_index(a.index, r * a.ld_index, a.wide);
     live = y != a.ignore;
-    if (y < 0 || y >= a.vocab) L = NAN;                 // a label outside the vocabulary spoils its row
-    else out = natural(0.5f * L - a.zt[r]);
-    if (L != L) out = NAN;
+    bad = y < 0 || y >= a.vocab;                        // a label outside the vocabulary spoils its row
+    if (!bad) out = natural((0.5f * s.x - a.zt[r]) + ls);
   }
   if (lane == 0) {
-    a.loss[r] = live ? out : 0.f;
-    a.lse[r] = L;
+    a.loss[r] = !live ? 0.f : bad ? NAN : out;
+    a.stat[r] = make_float2(s.x, bad ? NAN : s.y);
     a.flag[r] = live ? 1.f : 0.f;
   }
 }

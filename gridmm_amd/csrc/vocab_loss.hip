@@ -8,8 +8,9 @@
 //                   dh = dS W,   dW = dS^T h,   db_j = sum_r dS_rj
 // Forward: the score tile's epilogue leaves each row's (maximum, sum of exponentials) of its columns; a second, small kernel joins
 // them.  Backward: the scores are computed again piece by piece, the epilogue turns them into 16-bit dS (one piece at a time, the
-// workspace bounds its width), and two more products read it.  The entries of dS at a target come from the target's own fp32
-// score: exp(..) - p is rounded once there, whatever cancels.
+// workspace bounds its width), and two more products read it.  The entries of dS at a target come from the target's score as the
+// forward's sums hold it: softmax - p is rounded once there.  A row keeps its maximum and its sum of exponentials apart, as the
+// logarithm of both together has roundings of the maximum's size.
 //
 // Rows that do not count (label == ignore_index; no filled slot) are left out on the device: the counted rows are compacted into
 // the packed copy of h, the grids are sized for all rows and workgroups past the count end at once -- no host read-back.
@@ -178,7 +179,7 @@ struct PrepArgs {
   const unsigned char* counts;       // distillation; NULL: labels
   int64_t ldh, ldw, ignore;
   int rows, vocab, K, wide, dtype, bias_dtype, vp;
-  float inv_t;
+  float unit;
   Meta* meta;
   int *rowmap, *rowinv;
   float *loss, *biasz, *amax_h, *amax_w;
@@ -237,7 +238,7 @@ __global__ __launch_bounds__(PREP_T) void prep_kernel(const PrepArgs a, int nb) 
   if (blk < nb) {
     const int64_t j = (int64_t)blk * PREP_T + tid;
     if (j < a.vp)
-      a.biasz[j] = j >= a.vocab ? -INFINITY : a.bias ? load_as_f32(a.bias, j, a.bias_dtype) * (a.inv_t * LOG2E) : 0.f;
+      a.biasz[j] = j >= a.vocab ? -INFINITY : a.bias ? load_as_f32(a.bias, j, a.bias_dtype) * a.unit : 0.f;
     return;
   }
   blk -= nb;
@@ -425,7 +426,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_stats_kernel(Operand A, O
       });
 }
 
-// ---- scores at the targets: one wave a (row, NS slots), fp32 sums over the operands as they came ----
+// ---- scores at the targets: one wave 32 targets ----
 struct TargetArgs {
   const void *hidden, *weight, *index, *bias;
   int64_t ldh, ldw, ld_index;
@@ -436,71 +437,84 @@ struct TargetArgs {
   int* label;      // [compacted row], -1 outside the vocabulary; NULL: distillation
   float* zt;       // [compacted row][slots]: HALF the score in base 2, where a bias of the lowest finite number is still finite
 };
-// NS dot products of one row of h with rows of W, their loads in flight together
-template <int DT, int NS>
-__device__ __forceinline__ void dots(const TargetArgs& a, int64_t r, const int64_t (&id)[NS], int lane, bool vec, float (&out)[NS]) {
+// Values k .. k + 7 of a row as the tile products take them: one plane, or two under a scale (as pack8 makes them); zero from K on.
+template <int DT, bool VEC>
+__device__ __forceinline__ void planes8(const void* src, int64_t off, int k, int K, int e, vocab::s16x8_t& hi, vocab::s16x8_t& lo) {
+  if constexpr (DT == F32) {
+    const float* x = (const float*)src + off + k;
+    float v[8];
+    if constexpr (VEC) {                               // (K % 8 == 0)
+      const float4 p = k < K ? *reinterpret_cast<const float4*>(x) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const float4 q = k < K ? *reinterpret_cast<const float4*>(x + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
+    } else {
 #pragma unroll
-  for (int s = 0; s < NS; ++s) out[s] = 0.f;
-  if (!vec) {
-    for (int k = lane; k < a.K; k += 64) {
-      const float x = load_as_f32(a.hidden, r * a.ldh + k, DT);
-#pragma unroll
-      for (int s = 0; s < NS; ++s) out[s] = fmaf(x, load_as_f32(a.weight, id[s] * a.ldw + k, DT), out[s]);
+      for (int i = 0; i < 8; ++i) v[i] = k + i < K ? x[i] : 0.f;
     }
-  } else if constexpr (DT == F32) {
-    const float *x = (const float*)a.hidden + r * a.ldh, *W = (const float*)a.weight;
-    for (int k = lane * 4; k < a.K; k += 256) {
-      const float4 p = *reinterpret_cast<const float4*>(x + k);
-      float4 q[NS];
 #pragma unroll
-      for (int s = 0; s < NS; ++s) q[s] = *reinterpret_cast<const float4*>(W + id[s] * a.ldw + k);
-#pragma unroll
-      for (int s = 0; s < NS; ++s) out[s] = fmaf(p.x, q[s].x, fmaf(p.y, q[s].y, fmaf(p.z, q[s].z, fmaf(p.w, q[s].w, out[s]))));
+    for (int i = 0; i < 8; ++i) {
+      const float y = ldexpf(v[i], e);
+      const _Float16 f = (_Float16)y;
+      hi[i] = __builtin_bit_cast(short, f);
+      lo[i] = (short)to_f16(y - (float)f);
     }
   } else {
-    const unsigned short *x = (const unsigned short*)a.hidden + r * a.ldh, *W = (const unsigned short*)a.weight;
-    auto f = [](unsigned short u) { return DT == BF16 ? bf16_bits_to_f32(u) : (float)__builtin_bit_cast(_Float16, u); };
-    for (int k = lane * 8; k < a.K; k += 512) {
-      const u16x8_t p = *reinterpret_cast<const u16x8_t*>(x + k);
-      u16x8_t q[NS];
+    const short* x = (const short*)src + off + k;
+    if constexpr (VEC) {
+      hi = k < K ? *reinterpret_cast<const vocab::s16x8_t*>(x) : (vocab::s16x8_t){0, 0, 0, 0, 0, 0, 0, 0};
+    } else {
 #pragma unroll
-      for (int s = 0; s < NS; ++s) q[s] = *reinterpret_cast<const u16x8_t*>(W + id[s] * a.ldw + k);
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) out[s] = fmaf(f(p[e]), f(q[s][e]), out[s]);
+      for (int i = 0; i < 8; ++i) hi[i] = k + i < K ? x[i] : (short)0;
     }
   }
-#pragma unroll
-  for (int s = 0; s < NS; ++s) out[s] = wave_sum(out[s]);
 }
-template <int DT, int NS>
-__device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block) {
-  const int lane = threadIdx.x & 63;
-  const int groups = (a.slots + NS - 1) / NS;
-  const int64_t w = block * 4 + (threadIdx.x >> 6);
-  const int64_t i = w / groups;
-  if (i >= a.meta->count) return;
-  const int s0 = (int)(w % groups) * NS;
-  const int64_t r = a.rowmap[i];
-  constexpr int A = DT == F32 ? 4 : 8;
-  const bool vec = a.K % A == 0 && a.ldh % A == 0 && a.ldw % A == 0 && (((uintptr_t)a.hidden | (uintptr_t)a.weight) & 15) == 0;
-  int64_t id[NS], at[NS];
+// The score at a target has to be the very number that the log-sum-exp holds for it: where a row is sure of its target their difference
+// is the loss, and a second product with roundings of its own left up to 2e-5 there, of either sign.  So it is computed as the tiles
+// do, by the same matrix instructions in the same order, and equals the tile's bit for bit: the diagonal of a 32 x 32 product of 32
+// targets' rows of W and their rows of h.  (32 times the operations of a dot product, and the same reads, which bound it.)
+template <int DT>
+__device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block, int sh, int sw) {
+  const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
+  const int64_t pair = (block * 4 + (threadIdx.x >> 6)) * 32 + n, pairs = (int64_t)a.meta->count * a.slots;
+  if (pair - n >= pairs) return;
+  const int64_t i = (pair < pairs ? pair : pairs - 1) / a.slots;
+  const int s = (int)((pair < pairs ? pair : pairs - 1) - i * a.slots);
+  const int64_t r = a.rowmap[i], id = load_index(a.index, r * a.ld_index + s, a.wide), at = id >= 0 && id < a.vocab ? id : 0;
+  const bool vec = a.K % 8 == 0 && a.ldh % 8 == 0 && a.ldw % 8 == 0 && (((uintptr_t)a.hidden | (uintptr_t)a.weight) & 15) == 0;
+  f32x16_t acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  auto product = [&](auto v) {
+    constexpr int U = 4;              // steps whose loads are in flight together
+    for (int k0 = 0; k0 < a.K; k0 += 16 * U) {
+      vocab::s16x8_t h[U], hl[U], w[U], wl[U];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    id[s] = s0 + s < a.slots ? load_index(a.index, r * a.ld_index + s0 + s, a.wide) : -1;
-    at[s] = id[s] >= 0 && id[s] < a.vocab ? id[s] : 0;      // (row 0 in place of a row that is not there)
-  }
-  float z[NS];
-  dots<DT, NS>(a, r, at, lane, vec, z);
+      for (int u = 0; u < U; ++u) {
+        planes8<DT, decltype(v)::value>(a.hidden, r * a.ldh, k0 + 16 * u + 8 * half, a.K, sh, h[u], hl[u]);
+        planes8<DT, decltype(v)::value>(a.weight, at * a.ldw, k0 + 16 * u + 8 * half, a.K, sw, w[u], wl[u]);
+      }
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    if (lane != s || s0 + s >= a.slots) continue;
-    // an id outside the vocabulary spoils its row; an empty slot has no score
-    if (a.label) a.label[i] = id[s] >= 0 && id[s] < a.vocab ? (int)id[s] : -1;
-    const float half = 0.5f * a.unit, b = a.bias ? load_as_f32(a.bias, at[s], a.bias_dtype) * half : 0.f;
-    a.zt[i * a.slots + s0 + s] = a.kd && id[s] < 0 ? 0.f : id[s] < 0 || id[s] >= a.vocab ? NAN : fmaf(z[s], half, b);
-  }
+      for (int u = 0; u < U; ++u) {
+        acc = vocab::mma<DT != BF16>(w[u], h[u], acc);
+        if constexpr (DT == F32) {
+          acc = vocab::mma<true>(wl[u], h[u], acc);
+          acc = vocab::mma<true>(w[u], hl[u], acc);
+        }
+      }
+    }
+  };
+  if (vec) product(std::true_type{});
+  else product(std::false_type{});
+  // lane l holds column l & 31 at rows 8 (q >> 2) + 4 (l >> 5) + (q & 3)
+  const int q = (n >> 3) * 4 + (n & 3);
+  float z = acc[0];
+#pragma unroll
+  for (int k = 1; k < 16; ++k) z = q == k ? acc[k] : z;
+  if (pair >= pairs || half != ((n >> 2) & 1)) return;
+  // an id outside the vocabulary spoils its row; an empty slot has no score
+  if (a.label) a.label[i] = id >= 0 && id < a.vocab ? (int)id : -1;
+  const float b = a.bias ? load_as_f32(a.bias, at, a.bias_dtype) * a.unit : 0.f, y = fmaf(z, ldexpf(a.unit, -(sh + sw)), b);
+  // half of it: a bias of the lowest finite number, -inf in base 2, is finite so
+  const float out = y == -INFINITY && a.bias ? load_as_f32(a.bias, at, a.bias_dtype) * (0.5f * a.unit) : 0.5f * y;
+  a.zt[pair] = a.kd && id < 0 ? 0.f : id < 0 || id >= a.vocab ? NAN : out;
 }
 
 // TargetLists: one compacted row a workgroup (the order within a block is whatever it is: each entry is its slot's own)
@@ -551,18 +565,21 @@ __global__ __launch_bounds__(256) void target_lists_kernel(const TargetArgs t, i
 
 // One launch behind prep_kernel: the first `blocks` workgroups pack the counted rows of h into Hp (rows past the count up to a multiple
 // of 256: zero), the next `targets` compute the scores at the targets, the rest pack the first C rows of W.
-template <int DT, int NS>
+template <int DT>
 __global__ __launch_bounds__(256) void rows_kernel(const TargetArgs t, int blocks, int targets, int Kp,
                                                      const float* __restrict__ amax_h,
                                                      const float* __restrict__ amax_w, Meta* __restrict__ meta,
                                                      unsigned short* __restrict__ Hp, int C, unsigned short* __restrict__ Wp) {
   const int b = blockIdx.x - blocks, lane = threadIdx.x & 63;
-  if (b >= 0 && b < targets) return target_scores<DT, NS>(t, b);
   auto scale_w = [&] {
     float m = 0.f;
     for (int k = lane; k < AMAX_W; k += 64) m = fmaxf(m, amax_w[k]);
     return scale_exp(wave_max(m), 14);
   };
+  if (b >= 0 && b < targets) {
+    if constexpr (DT == F32) return target_scores<DT>(t, b, scale_exp(wave_max(amax_h[lane]), 14), scale_w());
+    else return target_scores<DT>(t, b, 0, 0);
+  }
   if (b >= 0) {
     const int sw = DT == F32 ? scale_w() : 0;
     return pack_w(t.weight, t.ldw, DT, t.K, Kp, 0, (b - targets) * 4 + (threadIdx.x >> 6), C, t.vocab, sw, Wp);
@@ -587,9 +604,9 @@ __global__ __launch_bounds__(256) void rows_kernel(const TargetArgs t, int block
 __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ stats, int64_t Vp, int64_t C, int64_t Rp, const Meta* __restrict__ meta,
                                                    const int* __restrict__ rowmap, const float* __restrict__ zt, int slots,
                                                    const float* __restrict__ p, const float* __restrict__ plogp, float temperature,
-                                                   float* __restrict__ lse, float* __restrict__ loss) {
+                                                   float2* __restrict__ stat, float* __restrict__ loss) {
   __shared__ float2 part[16][17];
-  __shared__ float acc[16][17];
+  __shared__ float2 acc[16][17];
   const int rr = threadIdx.x & 15, lanep = threadIdx.x >> 4;
   const int count = meta->count;
   const int64_t T = big_tiles(count, C) ? 256 : 128;
@@ -616,9 +633,10 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
   __syncthreads();
   a = part[0][rr];
   for (int w = 1; w < 16; ++w) a = join_stats(a, part[w][rr]);
-  const float L = a.x + __builtin_amdgcn_logf(a.y);        // base 2
-  float s = 0.f;
-  bool bad = L != L;
+  // The log-sum-exp stays in its two parts, maximum and logarithm of the sum: as one number it has the maximum's roundings, 2e-6 at 46
+  const float ls = 0.5f * __builtin_amdgcn_logf(a.y);        // (halves, base 2)
+  float s = 0.f, mass = 0.f;
+  bool bad = !(a.x == a.x && ls == ls);
   if (i < count) {
     if (p) {
       const int64_t r = rowmap[i];
@@ -626,25 +644,25 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
       for (int k = lanep; k < slots; k += 16) {
         const float q = p[r * slots + k], z = zt[i * slots + k];
         bad |= z != z;
-        if (!(q == 0.f)) s += q * (0.5f * L - z);
+        if (!(q == 0.f)) { s += q * (0.5f * a.x - z); mass += q; }
       }
     }
   }
-  acc[lanep][rr] = bad ? NAN : s;
+  acc[lanep][rr] = make_float2(bad ? NAN : s, mass);
   __syncthreads();
   if (lanep != 0 || i >= count) return;
   const int64_t r = rowmap[i];
   float out;
   if (p) {
-    s = 0.f;
-    for (int w = 0; w < 16; ++w) s += acc[w][rr];
-    out = temperature * temperature * (plogp[r] + natural(s));
+    s = mass = 0.f;
+    for (int w = 0; w < 16; ++w) { s += acc[w][rr].x; mass += acc[w][rr].y; }
+    out = temperature * temperature * (plogp[r] + natural(fmaf(mass, ls, s)));
   } else {
-    out = natural(0.5f * L - zt[i]);
+    out = natural((0.5f * a.x - zt[i]) + ls);
     s = zt[i];
   }
   loss[r] = out;
-  lse[i] = s != s ? NAN : L;                                // a bad target: its row's gradient is NaN too
+  stat[i] = make_float2(a.x, s != s ? NAN : a.y);           // a bad target: its row's gradient is NaN too
 }
 
 // ---- backward ----
@@ -654,7 +672,8 @@ struct GradArgs {
   float temperature;
   const int* rowmap;
   const int* label;            // of the compacted rows; NULL: distillation, whose targets a kernel of their own writes
-  const float *zt, *lse;
+  const float* zt;
+  const float2* stat;          // (maximum, sum of 2^(y - maximum)): a softmax entry is 2^(y - maximum) / sum
   int* scale;                  // exponent of the power of two that dS is scaled by
 };
 // That exponent, from the largest finite |g T|: every workgroup finds it for itself (a launch of its own: 10 us).  bf16 has fp32's range
@@ -706,7 +725,7 @@ __device__ __forceinline__ void rows_of_32(unsigned short* scratch, const float4
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
-// dS of the columns [j0, j0 + C): dS[r][j] = g_r T exp2(y_rj - lse_r) in two planes; at the row's label, from its fp32 score, g_r (exp2(..) - 1)
+// dS of the columns [j0, j0 + C): dS[r][j] = g_r T q_rj in two planes; at the row's label, from its fp32 score, g_r (q - 1)
 template <class T>
 __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Operand B, int nk, int tn, const Meta* __restrict__ meta,
                                                                 const float* __restrict__ biasz, float unit, const GradArgs G, int64_t j0,
@@ -734,24 +753,26 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
         const int64_t r0 = it.bm + wr * T::WM, c0 = it.bn + wc * T::WN;
         const float* bz = biasz + c0 + (lane >> 5) * 4;
         // what the rows need, its loads in flight together
-        float Ls[T::TM], gs[T::TM];
+        float Ms[T::TM], inv[T::TM], gs[T::TM];
         int ys[T::TM];
 #pragma unroll
         for (int i = 0; i < T::TM; ++i) {
           const int r = (int)r0 + i * 32 + (lane & 31), rl = min(r, count - 1);
-          const float l = G.lse[rl], g = G.g[G.rowmap[rl] * G.gs] * G.temperature;
+          const float2 st = G.stat[rl];
+          const float g = G.g[G.rowmap[rl] * G.gs] * G.temperature;
           ys[i] = G.label && r < count && lane < 32 ? G.label[rl] - (int)(j0 + c0) : -1;
-          Ls[i] = r < count ? l : 1e30f;
-          gs[i] = r < count ? ldexpf(g, sg) : 0.f;      // (a row past the count: 0 times exp2(-1e30))
+          Ms[i] = r < count ? st.x : INFINITY;          // (a row past the count: 0 times exp2(-inf))
+          inv[i] = r < count ? 1.f / st.y : 1.f;
+          gs[i] = r < count ? ldexpf(g, sg) : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < T::TM; ++i) {
           __builtin_amdgcn_sched_barrier(0);
-          const float L = Ls[i], gr = gs[i];
+          const float M = Ms[i], gr = gs[i], gq = gr * inv[i];
           const int y = ys[i];
           const bool hit = y >= 0 && y < 64;
           float target = 0.f;
-          if (hit) target = gr * (__builtin_amdgcn_exp2f(2.f * G.zt[r0 + i * 32 + lane] - L) - 1.f);
+          if (hit) target = gr * fmaf(__builtin_amdgcn_exp2f(2.f * G.zt[r0 + i * 32 + lane] - M), inv[i], -1.f);
           auto rounded = [](float x) {
             const unsigned short u = T::F16 ? to_f16(x) : to_bf16(x);
             return T::F16 ? (float)__builtin_bit_cast(_Float16, u) : bf16_bits_to_f32(u);
@@ -760,7 +781,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
             const float4 b = *reinterpret_cast<const float4*>(bz + c * 8);
             const float bb[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = gr * __builtin_amdgcn_exp2f(fmaf(acc[i][c >> 2][(c & 3) * 4 + e], sc, bb[e]) - L);
+            for (int e = 0; e < 4; ++e) v[e] = gq * __builtin_amdgcn_exp2f(fmaf(acc[i][c >> 2][(c & 3) * 4 + e], sc, bb[e]) - M);
           };
           auto put = [&](const u16x4_t (&x)[8], float at_target, unsigned short* at) {
             rows_of_16(scratch, x, [&](auto column) { if (hit) column(y) = T::F16 ? to_f16(at_target) : to_bf16(at_target); },
@@ -781,7 +802,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
       });
 }
 
-// the entries of dS at a teacher's targets in [j0, j0 + C): g_r T (exp2(z - lse) - sum of p over the slots of the same id), rounded once
+// the entries of dS at a teacher's targets in [j0, j0 + C): g_r T (q - sum of p over the slots of the same id)
 struct FixArgs {
   const void* index;
   int64_t ld_index, j0, ldS, plane;
@@ -792,7 +813,8 @@ struct FixArgs {
   unsigned short* dS;
 };
 __device__ __forceinline__ void target_entry(const FixArgs& a, int64_t i, int s, int64_t id, float p) {
-  const float v = ldexpf(a.G.g[a.G.rowmap[i] * a.G.gs] * a.G.temperature, *a.G.scale) * (__builtin_amdgcn_exp2f(2.f * a.G.zt[i * a.slots + s] - a.G.lse[i]) - p);
+  const float2 st = a.G.stat[i];
+  const float v = ldexpf(a.G.g[a.G.rowmap[i] * a.G.gs] * a.G.temperature, *a.G.scale) * fmaf(__builtin_amdgcn_exp2f(2.f * a.G.zt[i * a.slots + s] - st.x), 1.f / st.y, -p);
   unsigned short* at = a.dS + i * a.ldS + (id - a.j0);
   at[0] = a.dtype == BF16 ? to_bf16(v) : to_f16(v);
   at[a.plane] = a.dtype == BF16 ? to_bf16(v - bf16_bits_to_f32(at[0])) : to_f16(v - (float)__builtin_bit_cast(_Float16, at[0]));
@@ -1042,7 +1064,7 @@ struct Plan {
   bool keep_w;                 // ... and its copy, one piece, stays for the backward (28 us of 396 at 30522 x 768 fp32)
   int64_t C_fwd, C_bwd;        // columns a piece
   // saved
-  size_t o_meta, o_rowmap, o_rowinv, o_lse, o_zt, o_label, o_p, o_biasz, o_h, o_w, saved;
+  size_t o_meta, o_rowmap, o_rowinv, o_stat, o_zt, o_label, o_p, o_biasz, o_h, o_w, saved;
   // forward workspace
   size_t f_counts, f_plogp, f_amax, f_stats, f_w, f_begin, f_entry, fwd;
   // backward workspace
@@ -1089,7 +1111,7 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
     size_t o = 0;
     auto take = [&](size_t bytes) { const size_t at = o; o += up(bytes, 256); return at; };
     const size_t V64 = up(d->vocab, 64), S = (size_t)d->rows * P.slots, GR = (size_t)P.groups * P.RP;
-    P.o_lse = take(GR * 4);
+    P.o_stat = take(GR * 8);
     P.o_meta = take(GR * 4);                         // 1 for rows that count
     P.o_zt = take(S * 4);
     P.o_p = take(d->slots ? S * 4 : 0);
@@ -1109,7 +1131,7 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.o_meta = take(sizeof(Meta));
   P.o_rowmap = take(R * 4);
   P.o_rowinv = take(R * 4);
-  P.o_lse = take(Rp * 4);
+  P.o_stat = take(Rp * 8);
   P.o_zt = take(R * S * 4);
   P.o_label = take(d->slots ? 0 : R * 4);
   P.o_p = take(d->slots ? R * S * 4 : 0);
@@ -1213,7 +1235,7 @@ FewArgs few_args(const gridmm_vocab_loss_t* d, const Plan& P, const void* saved)
   a.rows = d->rows; a.vocab = d->vocab; a.K = d->hidden_size; a.slots = P.slots; a.wide = d->index64; a.dtype = d->dtype;
   a.bias_dtype = d->bias_dtype; a.kd = d->slots > 0;
   a.inv_t = 1.f / d->temperature; a.unit = a.inv_t * LOG2E; a.temperature = d->temperature;
-  a.lse = (float*)(sv + P.o_lse); a.flag = (float*)(sv + P.o_meta); a.zt = (float*)(sv + P.o_zt);
+  a.stat = (float2*)(sv + P.o_stat); a.flag = (float*)(sv + P.o_meta); a.zt = (float*)(sv + P.o_zt);
   a.p = d->slots ? (float*)(sv + P.o_p) : nullptr;
   a.y = d->forward_only ? nullptr : (float*)(sv + P.o_h);
   a.ranges = P.ranges; a.range = P.range; a.groups = P.groups;
@@ -1259,7 +1281,8 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   }
   Meta* meta = (Meta*)(sv + P.o_meta);
   int *rowmap = (int*)(sv + P.o_rowmap), *rowinv = (int*)(sv + P.o_rowinv);
-  float *lse = (float*)(sv + P.o_lse), *zt = (float*)(sv + P.o_zt), *p = d->slots ? (float*)(sv + P.o_p) : nullptr;
+  float2* stat = (float2*)(sv + P.o_stat);
+  float *zt = (float*)(sv + P.o_zt), *p = d->slots ? (float*)(sv + P.o_p) : nullptr;
   float* biasz = (float*)(sv + P.o_biasz);
   unsigned short* Hp = (unsigned short*)(sv + P.o_h);
   unsigned char* counts = (unsigned char*)(ws + P.f_counts);
@@ -1277,7 +1300,7 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   a.counts = d->slots ? counts : nullptr;
   a.ldh = d->ld_hidden; a.ldw = d->ld_weight; a.ignore = d->ignore_index;
   a.rows = d->rows; a.vocab = d->vocab; a.K = d->hidden_size; a.wide = d->index64; a.dtype = d->dtype; a.bias_dtype = d->bias_dtype;
-  a.vp = (int)P.Vp; a.inv_t = inv_t; a.meta = meta; a.rowmap = rowmap; a.rowinv = rowinv; a.loss = loss; a.biasz = biasz;
+  a.vp = (int)P.Vp; a.unit = unit; a.meta = meta; a.rowmap = rowmap; a.rowinv = rowinv; a.loss = loss; a.biasz = biasz;
   a.amax_h = amax; a.amax_w = amax + AMAX_H;
   const int nb = (int)((P.Vp + PREP_T - 1) / PREP_T);
   GRIDMM_LAUNCH(prep_kernel, dim3(1 + nb + (d->dtype == F32 ? AMAX_H + AMAX_W : 0)), dim3(PREP_T), 0, st, a, nb);
@@ -1290,12 +1313,11 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   t.label = d->slots ? nullptr : (int*)(sv + P.o_label);
   const int rc = by_dtype(d, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    const int hb = (int)(P.Rp / 4), tb = P.lists ? 0 : (int)(((int64_t)d->rows * (d->slots ? (P.slots + 7) / 8 : 1) + 3) / 4);
+    const int hb = (int)(P.Rp / 4), tb = P.lists ? 0 : (int)(((int64_t)d->rows * P.slots + 127) / 128);
     const int C = P.pack_w ? (int)P.C_fwd : 0;
     unsigned short* Wp = (unsigned short*)(P.keep_w ? sv + P.o_w : ws + P.f_w);
     const dim3 grid((unsigned)(hb + tb + (C + 3) / 4));
-    if (d->slots) GRIDMM_LAUNCH((rows_kernel<DT, 8>), grid, dim3(256), 0, st, t, hb, tb, (int)P.Kp, amax, amax + AMAX_H, meta, Hp, C, Wp);
-    else GRIDMM_LAUNCH((rows_kernel<DT, 1>), grid, dim3(256), 0, st, t, hb, tb, (int)P.Kp, amax, amax + AMAX_H, meta, Hp, C, Wp);
+    GRIDMM_LAUNCH((rows_kernel<DT>), grid, dim3(256), 0, st, t, hb, tb, (int)P.Kp, amax, amax + AMAX_H, meta, Hp, C, Wp);
     GRIDMM_CHECK_LAUNCH();
     return GRIDMM_OK;
   });
@@ -1331,7 +1353,7 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
     if (rc != GRIDMM_OK) return rc;
   }
   GRIDMM_LAUNCH(loss_kernel, dim3((d->rows + 15) / 16), dim3(256), 0, st, stats, P.Vp, P.C_fwd, P.Rp, meta, rowmap, zt, P.slots, p,
-                plogp, d->temperature, lse, loss);
+                plogp, d->temperature, stat, loss);
   GRIDMM_CHECK_LAUNCH();
   return GRIDMM_OK;
 }
@@ -1378,14 +1400,15 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
   const Meta* meta = (const Meta*)(sv + P.o_meta);
   int* scale = (int*)(ws + P.b_scale);
   const int *rowmap = (const int*)(sv + P.o_rowmap), *rowinv = (const int*)(sv + P.o_rowinv);
-  const float *lse = (const float*)(sv + P.o_lse), *zt = (const float*)(sv + P.o_zt);
+  const float2* stat = (const float2*)(sv + P.o_stat);
+  const float* zt = (const float*)(sv + P.o_zt);
   const float *p = d->slots ? (const float*)(sv + P.o_p) : nullptr, *biasz = (const float*)(sv + P.o_biasz);
   const unsigned short* Hp = (const unsigned short*)(sv + P.o_h);
   float* part = (float*)(ws + P.b_part);
   unsigned short *dS = (unsigned short*)(ws + P.b_ds), *wbuf = (unsigned short*)(ws + P.b_w);
   const float unit = LOG2E / d->temperature;
 
-  const GradArgs G{grad, grad_stride, d->temperature, rowmap, d->slots ? nullptr : (const int*)(sv + P.o_label), zt, lse, scale};
+  const GradArgs G{grad, grad_stride, d->temperature, rowmap, d->slots ? nullptr : (const int*)(sv + P.o_label), zt, stat, scale};
   const Operand H{Hp, P.PL * P.Kp, P.Kp, P.Rp, P.Kp};
   for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_bwd) {
     const int64_t C = std::min(P.C_bwd, P.Vp - j0);

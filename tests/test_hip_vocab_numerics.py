@@ -72,6 +72,60 @@ def test_gradients_of_many_16_bit_rows_are_rounded_once(dtype, R, V, K, loss):
         assert ratio <= 1.02, (k, ratio)
 
 
+# ---- rows that the model is sure of ----
+def _sure(dtype, R, V, K, margin, seed):
+    """Hidden states that lie along the row of W of their label: the label's score is `margin` above everything else's typical one."""
+    g = torch.Generator().manual_seed(seed)
+    w = torch.randn(V, K, generator=g) / K ** 0.5
+    y = torch.randperm(V, generator=g)[:R]
+    h = w[y] * (margin / (w[y] * w[y]).sum(1, keepdim=True)) + 0.1 * torch.randn(R, K, generator=g)
+    return h.to(DT[dtype]).cuda(), w.to(DT[dtype]).cuda(), y.cuda(), g
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("R,V,K", [(20, 700, 256), (300, 4000, 768), (400, 30011, 260), (2600, 11000, 256)])
+@pytest.mark.parametrize("margin", [14.0, 34.0])
+@pytest.mark.parametrize("loss", ["cross_entropy", "one slot", "three slots"])
+def test_rows_that_the_model_is_sure_of(dtype, R, V, K, margin, loss):
+    """loss = (M - z_y) + log sum 2^(y - M): where the label's score is the maximum M the first term is 0 if both come from one product,
+    and the second one is a sum that starts at 1: at most 64 additions next to 1 (a lane's columns, the lanes, the tiles), each off by
+    u, exponentials off by 3 e_z of themselves, a logarithm off by 4 u: never below 0.  The label's entry of dS is
+    g (1 / sum - 1) likewise."""
+    from gridmm_amd import vocab
+    h, w, y, g = _sure(dtype, R, V, K, margin, seed=V)
+    # distinct powers of two: d_bias of a label is its row's entry of dS plus what other rows leave there
+    gr = torch.ones(R, device="cuda")
+    b = torch.zeros(V, dtype=torch.float32, device="cuda")
+    hl, wl, bl = _leaves(h, w, b)
+    if loss == "cross_entropy":
+        ids, p = y[:, None], torch.ones(R, 1, dtype=torch.float64, device="cuda")
+        got = vocab.vocab_cross_entropy(hl, wl, y, bias=bl)
+    else:
+        S = 1 if loss == "one slot" else 3
+        ids = torch.stack([y] + [(y + 1 + s) % V for s in range(S - 1)], 1)
+        t = torch.full((R, S), -200.0, device="cuda")      # (the others' share: e^-300, nothing in fp32)
+        t[:, 0] = 100.0
+        p = torch.zeros(R, S, dtype=torch.float64, device="cuda")
+        p[:, 0] = 1.0
+        got = vocab.vocab_distillation(hl, wl, ids, t, bias=bl)
+    got.backward(gr)
+    z, want, _ = _exact(h, w, b, ids, p, 1.0, gr)
+    ez = _e_z(K, z)
+    bound = want["loss"] * 3 * ez + 68 * U
+    sure = z.gather(1, y[:, None])[:, 0] == z.max(1)[0]
+    assert int(sure.sum()) > 0.9 * R
+    got = got.detach().double()
+    assert bool((got[sure] >= 0).all()), float(got[sure].min())
+    err = ((got - want["loss"]).abs() - bound)[sure]
+    assert float(err.max()) <= 0, (float(err.max()), float(bound.max()))
+    # d_bias[y_r] = (q - 1) + the q of the other rows there: the entry, rounded to two 16-bit planes, and a sum of R terms
+    e = (1 - want["loss"].neg().exp()) * (3 * ez + 2.0 ** -16) + 68 * U
+    q = (z - torch.logsumexp(z, 1, keepdim=True)).exp().sum(0)[y] - want["loss"].neg().exp()
+    d = (bl.grad.double()[y] - want["d_bias"][y]).abs() - e - q.abs() * (3 * ez + 2.0 ** -16 + R * U) - R * 2.0 ** -38
+    assert float(d[sure].max()) <= 0, float(d[sure].max())
+
+
 # ---- no tile is left out ----
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,R,V,K", [("bf16", 300, 70000, 64), ("fp32", 300, 70000, 64), ("fp16", 300, 33000, 72), ("fp32", 20, 9001, 64),
