@@ -426,7 +426,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_stats_kernel(Operand A, O
       });
 }
 
-// ---- scores at the targets: one wave 32 targets ----
+// ---- scores at the targets: one workgroup 32 targets ----
 struct TargetArgs {
   const void *hidden, *weight, *index, *bias;
   int64_t ldh, ldw, ld_index;
@@ -437,72 +437,99 @@ struct TargetArgs {
   int* label;      // [compacted row], -1 outside the vocabulary; NULL: distillation
   float* zt;       // [compacted row][slots]: HALF the score in base 2, where a bias of the lowest finite number is still finite
 };
-// Values k .. k + 7 of a row as the tile products take them: one plane, or two under a scale (as pack8 makes them); zero from K on.
+// Values k .. k + 7 of a row as they lie, zero from K on
 template <int DT, bool VEC>
-__device__ __forceinline__ void planes8(const void* src, int64_t off, int k, int K, int e, vocab::s16x8_t& hi, vocab::s16x8_t& lo) {
-  if constexpr (DT == F32) {
-    const float* x = (const float*)src + off + k;
-    float v[8];
-    if constexpr (VEC) {                               // (K % 8 == 0)
-      const float4 p = k < K ? *reinterpret_cast<const float4*>(x) : make_float4(0.f, 0.f, 0.f, 0.f);
-      const float4 q = k < K ? *reinterpret_cast<const float4*>(x + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-      v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = k + i < K ? x[i] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = ldexpf(v[i], e);
-      const _Float16 f = (_Float16)y;
-      hi[i] = __builtin_bit_cast(short, f);
-      lo[i] = (short)to_f16(y - (float)f);
-    }
+__device__ __forceinline__ void load8(const void* src, int64_t off, int k, int K, float (&v)[8]) {
+  const float* x = (const float*)src + off + k;
+  if constexpr (VEC) {                                 // (K % 8 == 0)
+    const float4 p = k < K ? *reinterpret_cast<const float4*>(x) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 q = k < K ? *reinterpret_cast<const float4*>(x + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    v[0] = p.x; v[1] = p.y; v[2] = p.z; v[3] = p.w; v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
   } else {
-    const short* x = (const short*)src + off + k;
-    if constexpr (VEC) {
-      hi = k < K ? *reinterpret_cast<const vocab::s16x8_t*>(x) : (vocab::s16x8_t){0, 0, 0, 0, 0, 0, 0, 0};
-    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) hi[i] = k + i < K ? x[i] : (short)0;
-    }
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? x[i] : 0.f;
   }
 }
+template <int DT, bool VEC>
+__device__ __forceinline__ void load8(const void* src, int64_t off, int k, int K, vocab::s16x8_t& v) {
+  const short* x = (const short*)src + off + k;
+  if constexpr (VEC) {
+    v = k < K ? *reinterpret_cast<const vocab::s16x8_t*>(x) : (vocab::s16x8_t){0, 0, 0, 0, 0, 0, 0, 0};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? x[i] : (short)0;
+  }
+}
+// ... and as the tile products take them: one plane, or two under a scale (as pack8 makes them), `apart` vectors from each other
+__device__ __forceinline__ void put8(vocab::s16x8_t* at, int apart, const float (&v)[8], int e) {
+  vocab::s16x8_t hi, lo;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = ldexpf(v[i], e);
+    const _Float16 f = (_Float16)y;
+    hi[i] = __builtin_bit_cast(short, f);
+    lo[i] = (short)to_f16(y - (float)f);
+  }
+  at[0] = hi;
+  at[apart] = lo;
+}
+__device__ __forceinline__ void put8(vocab::s16x8_t* at, int, const vocab::s16x8_t& v, int) { at[0] = v; }
 // The score at a target has to be the very number that the log-sum-exp holds for it: where a row is sure of its target their difference
 // is the loss, and a second product with roundings of its own left up to 2e-5 there, of either sign.  So it is computed as the tiles
 // do, by the same matrix instructions in the same order, and equals the tile's bit for bit: the diagonal of a 32 x 32 product of 32
-// targets' rows of W and their rows of h.  (32 times the operations of a dot product, and the same reads, which bound it.)
+// targets' rows of W and their rows of h.  (32 times the operations of a dot product, and the same reads, which bound it.)  The four waves
+// fetch and split the operands, the first one multiplies: one wave for all of it took 62 us at 384 x 768 fp32, longer than the packing beside it.
+constexpr int TARGET_LDS = 1024;      // vectors of 8 values: 16 KB
 template <int DT>
-__device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block, int sh, int sw) {
-  const int lane = threadIdx.x & 63, n = lane & 31, half = lane >> 5;
-  const int64_t pair = (block * 4 + (threadIdx.x >> 6)) * 32 + n, pairs = (int64_t)a.meta->count * a.slots;
-  if (pair - n >= pairs) return;
+__device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block, int sh, int sw, vocab::s16x8_t* lds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, half = lane >> 5;
+  const int64_t pair = block * 32 + n, pairs = (int64_t)a.meta->count * a.slots;
+  if (block * 32 >= pairs) return;
   const int64_t i = (pair < pairs ? pair : pairs - 1) / a.slots;
   const int s = (int)((pair < pairs ? pair : pairs - 1) - i * a.slots);
   const int64_t r = a.rowmap[i], id = load_index(a.index, r * a.ld_index + s, a.wide), at = id >= 0 && id < a.vocab ? id : 0;
   const bool vec = a.K % 8 == 0 && a.ldh % 8 == 0 && a.ldw % 8 == 0 && (((uintptr_t)a.hidden | (uintptr_t)a.weight) & 15) == 0;
   f32x16_t acc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  constexpr int FR = DT == F32 ? 4 : 2, U = DT == F32 ? 1 : 2;      // fragments a step (16 columns), steps a wave fetches at a time
+  static_assert(4 * U * FR * 64 == TARGET_LDS, "the steps of a round in LDS");
+  using Raw = typename std::conditional<DT == F32, float[8], vocab::s16x8_t>::type;
   auto product = [&](auto v) {
-    constexpr int U = 4;              // steps whose loads are in flight together
-    for (int k0 = 0; k0 < a.K; k0 += 16 * U) {
-      vocab::s16x8_t h[U], hl[U], w[U], wl[U];
+    Raw h[U], w[U];
+    auto fetch = [&](int k0) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        planes8<DT, decltype(v)::value>(a.hidden, r * a.ldh, k0 + 16 * u + 8 * half, a.K, sh, h[u], hl[u]);
-        planes8<DT, decltype(v)::value>(a.weight, at * a.ldw, k0 + 16 * u + 8 * half, a.K, sw, w[u], wl[u]);
+        const int k = k0 + 16 * (wave * U + u) + 8 * half;
+        load8<DT, decltype(v)::value>(a.hidden, r * a.ldh, k, a.K, h[u]);
+        load8<DT, decltype(v)::value>(a.weight, at * a.ldw, k, a.K, w[u]);
       }
+    };
+    fetch(0);
+    for (int k0 = 0; k0 < a.K; k0 += 64 * U) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        acc = vocab::mma<DT != BF16>(w[u], h[u], acc);
-        if constexpr (DT == F32) {
-          acc = vocab::mma<true>(wl[u], h[u], acc);
-          acc = vocab::mma<true>(w[u], hl[u], acc);
+        vocab::s16x8_t* to = lds + (wave * U + u) * FR * 64 + lane;
+        put8(to, 64, h[u], sh);
+        put8(to + FR / 2 * 64, 64, w[u], sw);
+      }
+      fetch(k0 + 64 * U);                    // (past the end: zeros, nothing is read)
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int u = 0; u < 4 * U; ++u) {
+          const vocab::s16x8_t* from = lds + u * FR * 64 + lane;
+          acc = vocab::mma<DT != BF16>(from[FR / 2 * 64], from[0], acc);
+          if constexpr (DT == F32) {
+            acc = vocab::mma<true>(from[3 * 64], from[0], acc);
+            acc = vocab::mma<true>(from[2 * 64], from[64], acc);
+          }
         }
       }
+      __syncthreads();
     }
   };
   if (vec) product(std::true_type{});
   else product(std::false_type{});
+  if (wave) return;
   // lane l holds column l & 31 at rows 8 (q >> 2) + 4 (l >> 5) + (q & 3)
   const int q = (n >> 3) * 4 + (n & 3);
   float z = acc[0];
@@ -570,6 +597,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const TargetArgs t, int block
                                                      const float* __restrict__ amax_h,
                                                      const float* __restrict__ amax_w, Meta* __restrict__ meta,
                                                      unsigned short* __restrict__ Hp, int C, unsigned short* __restrict__ Wp) {
+  __shared__ vocab::s16x8_t lds[TARGET_LDS];
   const int b = blockIdx.x - blocks, lane = threadIdx.x & 63;
   auto scale_w = [&] {
     float m = 0.f;
@@ -577,8 +605,8 @@ __global__ __launch_bounds__(256) void rows_kernel(const TargetArgs t, int block
     return scale_exp(wave_max(m), 14);
   };
   if (b >= 0 && b < targets) {
-    if constexpr (DT == F32) return target_scores<DT>(t, b, scale_exp(wave_max(amax_h[lane]), 14), scale_w());
-    else return target_scores<DT>(t, b, 0, 0);
+    if constexpr (DT == F32) return target_scores<DT>(t, b, scale_exp(wave_max(amax_h[lane]), 14), scale_w(), lds);
+    else return target_scores<DT>(t, b, 0, 0, lds);
   }
   if (b >= 0) {
     const int sw = DT == F32 ? scale_w() : 0;
@@ -1313,7 +1341,7 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   t.label = d->slots ? nullptr : (int*)(sv + P.o_label);
   const int rc = by_dtype(d, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    const int hb = (int)(P.Rp / 4), tb = P.lists ? 0 : (int)(((int64_t)d->rows * P.slots + 127) / 128);
+    const int hb = (int)(P.Rp / 4), tb = P.lists ? 0 : (int)(((int64_t)d->rows * P.slots + 31) / 32);
     const int C = P.pack_w ? (int)P.C_fwd : 0;
     unsigned short* Wp = (unsigned short*)(P.keep_w ? sv + P.o_w : ws + P.f_w);
     const dim3 grid((unsigned)(hb + tb + (C + 3) / 4));
