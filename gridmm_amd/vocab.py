@@ -88,17 +88,22 @@ def _apart(w, ld):
     return w.data_ptr() & 15 != 0 or ld % 8 != 0 or ld > 1 << 22
 
 
-def _vocab_backward(ctx, g):
-    if g is None:
-        return (None,) * 8
-    # What saved-tensor hooks give back (checkpointing, offloading) are other tensors than the forward's, which may be gone: the
-    # kernels get the addresses of these.
-    hidden, w, b, index, saved = ctx.saved_tensors
-    d = _Desc.from_buffer_copy(ctx.desc)
+def _place(hidden, w, b, index):
+    return (hidden.data_ptr(), w.data_ptr(), 0 if b is None else b.data_ptr(), index.data_ptr(), hidden.stride(0), w.stride(0), index.stride(0),
+            hidden.numel(), w.numel(), index.numel())
+
+
+def _moved(ctx, g, hidden, w, b, index, saved):
+    """What saved-tensor hooks give back (checkpointing, offloading) are other tensors than the forward's, which may be gone: a descriptor
+    with the addresses of these, and what it points to."""
     for t in (hidden, w, index, saved) + (() if b is None else (b,)):
-        if not t.device == g.device:
+        if t.device != g.device:
             raise RuntimeError("a tensor kept for the backward came back on %s, its gradient is on %s" % (t.device, g.device))
-    if (hidden.shape, w.shape, hidden.dtype, w.dtype, index.shape, index.dtype) != ctx.kept:
+    d = _Desc.from_buffer_copy(ctx.desc)
+    dt = hidden.dtype
+    if ((tuple(hidden.shape), tuple(w.shape), index.numel()) != ((d.rows, d.hidden_size), (d.vocab, d.hidden_size), d.rows * max(d.slots, 1))
+            or dt not in _DTYPES or _DTYPES[dt] != d.dtype or w.dtype != dt or index.dtype != (torch.int64 if d.index64 else torch.int32)
+            or (b is not None and (b.numel() != d.vocab or _DTYPES.get(b.dtype) != d.bias_dtype))):
         raise RuntimeError("the tensors kept for the backward came back with other shapes or types")
     h, ldh = _rows(hidden)
     w, ldw = _rows(w)
@@ -111,10 +116,20 @@ def _vocab_backward(ctx, g):
         index = index.contiguous()
         d.labels = index.data_ptr()
     # (a single row: whatever its stride says)
-    d.hidden, d.ld_hidden, d.weight, d.ld_weight, d.teacher = h.data_ptr(), max(ldh, d.hidden_size), w.data_ptr(), ldw, None
+    d.hidden, d.ld_hidden, d.weight, d.ld_weight = h.data_ptr(), max(ldh, d.hidden_size), w.data_ptr(), ldw
     if b is not None:
         b = b.contiguous()
         d.bias = b.data_ptr()
+    return d, (h, w, b, index)
+
+
+def _vocab_backward(ctx, g):
+    if g is None:
+        return (None,) * 8
+    hidden, w, b, index, saved = ctx.saved_tensors
+    d, keep = ctx.desc, None
+    if _place(hidden, w, b, index) != ctx.place:
+        d, keep = _moved(ctx, g, hidden, w, b, index, saved)
     if g.dtype != torch.float32:
         g = g.float()
     need_h, need_w, need_b = ctx.needs_input_grad[:3]
@@ -163,9 +178,9 @@ class _VocabLoss(torch.autograd.Function):
         if need:
             ctx.set_materialize_grads(False)
             ctx.save_for_backward(hidden, w, b, index, saved)
-            ctx.desc, ctx.n_ws = d, lib.gridmm_vocab_loss_workspace(ref, 1)
-            ctx.kept = (hidden.shape, w.shape, dt, dt, index.shape, index.dtype)
-            ctx.prm = [t if isinstance(t, torch.nn.Parameter) else None for t in (weight, bias)]      # (nothing else is kept alive here)
+            ctx.desc, ctx.place, ctx.n_ws = d, _place(hidden, w, b, index), lib.gridmm_vocab_loss_workspace(ref, 1)
+            P = torch.nn.Parameter                   # (nothing else is kept alive here)
+            ctx.prm = [weight if isinstance(weight, P) else None, bias if isinstance(bias, P) else None]
         return loss
 
     @staticmethod
