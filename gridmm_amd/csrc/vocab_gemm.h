@@ -75,6 +75,8 @@ __device__ __forceinline__ const unsigned short* uniform(const unsigned short* p
                                  (unsigned)__builtin_amdgcn_readfirstlane((int)u));
 }
 
+__device__ __forceinline__ f32x16_t mma2(float a, float b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+
 struct Operand {
   const unsigned short* p;
   int64_t ld;       // elements between rows of the stored matrix
@@ -116,14 +118,19 @@ struct Tile {
   // that this one's buffer is free; the transfers of the stage after next -- of the next tile, near a tile's end -- start right there.
   // While done() works on a tile the next one's first fragments are in registers and its second stage is on the way.
   //
-  // twice != 0 (elements): an A of two planes over a B of one, C = (A + A') B with A' that far behind A: an item's nk stages are its range
-  // of the contraction once with A and once with A'.
+  // twice != 0 (elements): an A of two planes over a B of one, C = (A + A') B with A' that far behind A: an item's range of the
+  // contraction once with A and once with A'.
   //
   // SUMA: sums also takes the sums of A over the contraction for the waves that want_sums(item) names, lane l those of the steps that
   // it holds of row 32 i + (l & 31); lanes l and l ^ 32 together hold all.
   template <bool SUMA = false, class Work, class Want, class Done>
-  static __device__ __forceinline__ void run(const Operand& A, const Operand& B, unsigned short* smem, Work work, Want want_sums, Done done,
+  static __device__ __forceinline__ void run(const Operand& A, const Operand& B, unsigned short* smem, Work work_once, Want want_sums, Done done,
                                              int64_t twice = 0) {
+    auto work = [&](int n, Item& it) {
+      const bool is = work_once(n, it);
+      if (twice) it.nk *= 2;
+      return is;
+    };
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave / WAVES_N, wc = wave % WAVES_N;
@@ -300,6 +307,59 @@ struct Tile {
       done(item, acc, sums);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // nothing is on its way into LDS that another workgroup may get
+  }
+
+  // The same loop over items in fp32, values straight from where they lie, for operands that 16-bit planes do not hold: two contraction
+  // steps a matrix instruction, lane l the step k + (l >> 5).  rows(item) gives two functions of (i, k), the values of output row
+  // wr WM + 32 i + (l & 31) and of output column wc WN + 32 i + (l & 31) of the tile at contraction step k, 0 where there is none.
+  template <bool SUMA = false, class Work, class Want, class Rows, class Done>
+  static __device__ __forceinline__ void run_exact(Work work, Want want_sums, Rows rows, Done done) {
+    const int half = (threadIdx.x & 63) >> 5;
+    Item item;
+    for (int n = 0; work(n, item); ++n) {
+      Acc acc;
+      float sums[TM];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) {
+        sums[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < TN; ++c)
+#pragma unroll
+          for (int q = 0; q < 16; ++q) acc[i][c][q] = 0.f;
+      }
+      const bool sum = SUMA && want_sums(item);
+      rows(item, [&](auto fa, auto fb) {
+        for (int kt = 0; kt < item.nk; ++kt) {
+          float part[TM];                      // a stage's sums first, as above
+#pragma unroll
+          for (int i = 0; i < TM; ++i) part[i] = 0.f;
+#pragma unroll 1
+          for (int k0 = 0; k0 < BK; k0 += 8) {
+            float a[4][TM], b[4][TN];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int64_t k = item.k0 + (int64_t)kt * BK + k0 + 2 * u + half;
+#pragma unroll
+              for (int i = 0; i < TM; ++i) a[u][i] = fa(i, k);
+#pragma unroll
+              for (int c = 0; c < TN; ++c) b[u][c] = fb(c, k);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+              for (int i = 0; i < TM; ++i) {
+#pragma unroll
+                for (int c = 0; c < TN; ++c) acc[i][c] = mma2(b[u][c], a[u][i], acc[i][c]);
+                if (sum) part[i] += a[u][i];
+              }
+          }
+#pragma unroll
+          for (int i = 0; i < TM; ++i) sums[i] += part[i];
+        }
+      });
+      done(item, acc, sums);
+      __syncthreads();                         // (what done() leaves in LDS is read before the next one writes)
+    }
   }
 };
 

@@ -17,8 +17,9 @@
 //
 // Number formats.  bf16 / fp16 operands: one plane, products exact, sums fp32; dS in two planes of the operands' type, an entry off by
 // 2^-16 (bf16) or 2^-22 (fp16) of itself, so that a gradient is rounded once, to its own type.  (One plane leaves 1.4 times that error, up to
-// twice where a handful of entries makes up a sum; 8030 x 131072 x 2048 13.9 ms against 21.2.)  fp32 operands: two fp16 planes each (22 bits) after a
-// power-of-two scale from the tensor's largest finite value, so a product is off by ~2^-22: like fp32 sums.  dS is scaled by a power of
+// twice where a handful of entries makes up a sum; 8030 x 131072 x 2048 13.9 ms against 21.2.)  fp32 operands: two fp16 planes each after a
+// power-of-two scale from the tensor's largest finite value: 22 bits of a value, or 25 of its row's largest, as long as the rows' largest
+// values lie within 2^14 of each other, which the device finds out; rows further apart run on fp32 matrix instructions.  dS is scaled by a power of
 // two from the largest |g T| of the call (fp16 range: entries below 2^-38 of it vanish).
 // Bound by the four products (vocab_gemm.h): 8030 x 131072 x 2048 bf16 forward and backward 13.8 - 14.0 ms, of it 3.4 scores, 3.7 dS, 3.4 dh, 3.4 dW;
 // fp32 384 x 30522 x 768 325 us, of it 260 products (1.4 rounds of 128 x 128 tiles) and 53 for W's scale and packing.
@@ -83,6 +84,19 @@ __device__ __forceinline__ int scale_exp(float amax, int top) {
 struct Meta {
   int count;         // rows that count
   int sh, sw;        // power-of-two exponents of the packed h and W
+  int wide;          // fp32 rows too far apart for one scale: nothing is packed, the products are fp32
+};
+// One scale leaves 22 bits of a value, but none below 2^-40 of the tensor's largest: with the rows' largest values within 2^14 of each
+// other (rows of zeros aside) every value keeps 22 bits, or 25 of its row's largest.  Rows further apart -- an outlier row, be it of a
+// column that its bias masks -- take the products on fp32 matrix instructions, from the operands as they
+// lie: 384 x 30522 x 768 2.0 ms against 0.33, 2048 x 32000 x 1024 11.3 against 1.5.
+constexpr int SPREAD = 14;
+// the operands as they lie, for those products
+struct Raw {
+  const void *hidden, *weight;
+  int64_t ldh, ldw, j0;          // j0: the piece's first column
+  int K, vocab;
+  const int* rowmap;
 };
 
 // Tiles of the products over the counted rows.  256 x 256 where they fill the chip (one workgroup of 8 waves a CU), else 128 x 128 (two
@@ -182,7 +196,8 @@ struct PrepArgs {
   float unit;
   Meta* meta;
   int *rowmap, *rowinv;
-  float *loss, *biasz, *amax_h, *amax_w;
+  float *loss, *biasz;
+  int *amax_h, *amax_w;
 };
 
 __device__ __forceinline__ float amax_row(const float* x, int K, int lane) {
@@ -202,7 +217,7 @@ __device__ __forceinline__ float amax_row(const float* x, int K, int lane) {
 // operands the rest find the largest finite |h| of the counted rows and |W|, one partial value a workgroup.
 __global__ __launch_bounds__(PREP_T) void prep_kernel(const PrepArgs a, int nb) {
   __shared__ int part[16];
-  __shared__ float fpart[16];
+  __shared__ int part2[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   auto counted = [&](int r) {
     return a.counts ? a.counts[r] != 0 : load_index(a.labels, r, a.wide) != a.ignore;
@@ -231,7 +246,7 @@ __global__ __launch_bounds__(PREP_T) void prep_kernel(const PrepArgs a, int nb) 
       if (c) a.rowmap[pos++] = (int)r;
       else a.loss[r] = 0.f;
     }
-    if (tid == 0) { a.meta->count = total; a.meta->sh = a.meta->sw = 0; }
+    if (tid == 0) { a.meta->count = total; a.meta->sh = a.meta->sw = a.meta->wide = 0; }
     return;
   }
   blk -= 1;
@@ -248,16 +263,38 @@ __global__ __launch_bounds__(PREP_T) void prep_kernel(const PrepArgs a, int nb) 
   const float* x = reinterpret_cast<const float*>(is_h ? a.hidden : a.weight);
   const int64_t ld = is_h ? a.ldh : a.ldw;
   const int rows = is_h ? a.rows : a.vocab;
-  float m = 0.f;
+  int top = 1 << 14, least = -(1 << 14);          // exponents of the scales that fit the largest row and the smallest one
   for (int64_t r = blk * 16 + wave; r < rows; r += blocks * 16)
-    if (!is_h || counted((int)r)) m = fmaxf(m, amax_row(x + r * ld, a.K, lane));
-  m = wave_max(m);
-  if (lane == 0) fpart[wave] = m;
+    if (!is_h || counted((int)r)) {
+      const float v = wave_max(amax_row(x + r * ld, a.K, lane));
+      if (v > 0.f) { const int e = scale_exp(v, 14); top = min(top, e); least = max(least, e); }
+    }
+  if (lane == 0) { part[wave] = top; part2[wave] = least; }
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < 16; ++w) m = fmaxf(m, fpart[w]);
-    (is_h ? a.amax_h : a.amax_w)[blk] = m;
+    for (int w = 1; w < 16; ++w) { top = min(top, part[w]); least = max(least, part2[w]); }
+    (is_h ? a.amax_h : a.amax_w)[blk] = top + (least << 16);
   }
+}
+// what comes of them, by a whole wave: the exponent of the scale that brings the tensor's largest value under 2^15, and whether the rows
+// lie too far apart for it
+__device__ __forceinline__ int tensor_scale(const int* amax, int n, bool& wide) {
+  int top = 1 << 14, least = -(1 << 14);
+  for (int k = threadIdx.x & 63; k < n; k += 64) {
+    const int v = amax[k], t = (short)(v & 0xffff);
+    top = min(top, t);
+    least = max(least, (v - t) >> 16);
+  }
+  top = -(int)wave_max((float)-top);
+  least = (int)wave_max((float)least);
+  wide |= least - top > SPREAD;
+  return top == 1 << 14 ? 0 : top;                // (nothing but zeros)
+}
+struct Scales { int sh, sw, wide; };
+__device__ __forceinline__ Scales scales(const int* amax_h, const int* amax_w) {
+  bool wide = false;
+  const int sh = tensor_scale(amax_h, AMAX_H, wide), sw = tensor_scale(amax_w, AMAX_W, wide);
+  return wide ? Scales{0, 0, 1} : Scales{sh, sw, 0};
 }
 
 // ---- packing: rows -> 16-bit rows of Kp columns (zero past K), fp32 as two fp16 planes under a power-of-two scale ----
@@ -316,7 +353,28 @@ __device__ __forceinline__ void pack_w(const void* W, int64_t ldw, int dtype, in
 __global__ __launch_bounds__(256) void pack_w_kernel(const void* __restrict__ W, int64_t ldw, int dtype, int K, int Kp, int64_t j0,
                                                      int C, int vocab, const Meta* __restrict__ meta,
                                                      unsigned short* __restrict__ Wp) {
+  if (meta->wide) return;
   pack_w(W, ldw, dtype, K, Kp, j0, blockIdx.x * 4 + (threadIdx.x >> 6), C, vocab, meta->sw, Wp);
+}
+
+// The scores' operands in fp32, for Tile::run_exact: counted rows of h, rows of W of the piece
+template <class T>
+__device__ __forceinline__ auto exact_scores(const Raw& raw, int count) {
+  return [&raw, count](const Item& it, auto f) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N, K = raw.K;
+    const float *h[T::TM], *w[T::TN];
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i) {
+      const int64_t r = it.bm + wr * T::WM + i * 32 + (lane & 31);
+      h[i] = (const float*)raw.hidden + (int64_t)raw.rowmap[r < count ? r : count - 1] * raw.ldh;
+    }
+#pragma unroll
+    for (int c = 0; c < T::TN; ++c) {
+      const int64_t j = raw.j0 + it.bn + wc * T::WN + c * 32 + (lane & 31);
+      w[c] = (const float*)raw.weight + (j < raw.vocab ? j : raw.vocab - 1) * raw.ldw;
+    }
+    f([&](int i, int64_t k) { return k < K ? h[i][k] : 0.f; }, [&](int c, int64_t k) { return k < K ? w[c][k] : 0.f; });
+  };
 }
 
 // ---- a teacher's targets by blocks of 64 columns: the score tiles hand over the scores at them ----
@@ -336,23 +394,20 @@ constexpr int LIST_BLOCKS = 4096, LIST_SLOTS = 4096;
 template <class T, bool LISTS>
 __global__ __launch_bounds__(T::THREADS, 2) void score_stats_kernel(Operand A, Operand B, int nk, int tn, const Meta* __restrict__ meta,
                                                                  const float* __restrict__ biasz, float unit,
-                                                                 float2* __restrict__ stats, int64_t Rp, const TargetLists L, int64_t j0) {
+                                                                 float2* __restrict__ stats, int64_t Rp, const TargetLists L, const Raw raw) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS];
   __shared__ float2 wst[T::WAVES_N][T::BM];
   const int count = __builtin_amdgcn_readfirstlane(meta->count), tm = (count + T::BM - 1) / T::BM;
   if (big_tiles(count, (int64_t)tn * T::BN) != (T::BM == 256)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
   const float sc = ldexpf(unit, -(meta->sh + meta->sw));
-  T::run(
-      A, B, smem,
-      [&](int n, Item& it) {
-        unsigned ty, tx, layer;
-        if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, 1, ty, tx, layer)) return false;
-        it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, 0, nk, 0};
-        return true;
-      },
-      [](const Item&) { return false; },
-      [&](const Item& it, typename T::Acc& acc, const float*) {
+  auto work = [&](int n, Item& it) {
+    unsigned ty, tx, layer;
+    if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, 1, ty, tx, layer)) return false;
+    it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, 0, nk, 0};
+    return true;
+  };
+  auto done = [&](const Item& it, typename T::Acc& acc, const float*) {
         float m[T::TM];
 #pragma unroll
         for (int i = 0; i < T::TM; ++i) m[i] = -INFINITY;
@@ -373,7 +428,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_stats_kernel(Operand A, O
           }
         if constexpr (LISTS) {
           // entries of the rows and 64 columns of this wave; either half of the wave holds 4 of every 8 columns
-          const int64_t block = (j0 + it.bn + wc * T::WN) >> 6;
+          const int64_t block = (raw.j0 + it.bn + wc * T::WN) >> 6;
           static_assert(T::WN == 64, "64 columns a wave");
           unsigned e0[T::TM], e1[T::TM], next[T::TM];
 #pragma unroll
@@ -423,7 +478,10 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_stats_kernel(Operand A, O
           for (int w = 1; w < T::WAVES_N; ++w) a = join_stats(a, wst[w][r]);
           stats[it.bn / 128 * Rp + it.bm + r] = a;
         }
-      });
+  };
+  if constexpr (T::PL == 2)
+    if (meta->wide) return T::run_exact(work, [](const Item&) { return false; }, exact_scores<T>(raw, count), done);
+  T::run(A, B, smem, work, [](const Item&) { return false; }, done);
 }
 
 // ---- scores at the targets: one workgroup 32 targets ----
@@ -481,7 +539,7 @@ __device__ __forceinline__ void put8(vocab::s16x8_t* at, int, const vocab::s16x8
 // fetch and split the operands, the first one multiplies: one wave for all of it took 62 us at 384 x 768 fp32, longer than the packing beside it.
 constexpr int TARGET_LDS = 1024;      // vectors of 8 values: 16 KB
 template <int DT>
-__device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block, int sh, int sw, vocab::s16x8_t* lds) {
+__device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block, const Scales sc, vocab::s16x8_t* lds) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, half = lane >> 5;
   const int64_t pair = block * 32 + n, pairs = (int64_t)a.meta->count * a.slots;
   if (block * 32 >= pairs) return;
@@ -508,8 +566,8 @@ __device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         vocab::s16x8_t* to = lds + (wave * U + u) * FR * 64 + lane;
-        put8(to, 64, h[u], sh);
-        put8(to + FR / 2 * 64, 64, w[u], sw);
+        put8(to, 64, h[u], sc.sh);
+        put8(to + FR / 2 * 64, 64, w[u], sc.sw);
       }
       fetch(k0 + 64 * U);                    // (past the end: zeros, nothing is read)
       __syncthreads();
@@ -527,8 +585,19 @@ __device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block
       __syncthreads();
     }
   };
-  if (vec) product(std::true_type{});
-  else product(std::false_type{});
+  if (DT == F32 && sc.wide) {
+    if (wave) return;
+    const float *h = (const float*)a.hidden + r * a.ldh, *w = (const float*)a.weight + at * a.ldw;
+#pragma unroll 8
+    for (int k0 = 0; k0 < a.K; k0 += 2) {
+      const bool in = k0 + half < a.K;
+      acc = vocab::mma2(in ? w[k0 + half] : 0.f, in ? h[k0 + half] : 0.f, acc);
+    }
+  } else if (vec) {
+    product(std::true_type{});
+  } else {
+    product(std::false_type{});
+  }
   if (wave) return;
   // lane l holds column l & 31 at rows 8 (q >> 2) + 4 (l >> 5) + (q & 3)
   const int q = (n >> 3) * 4 + (n & 3);
@@ -538,7 +607,7 @@ __device__ __forceinline__ void target_scores(const TargetArgs& a, int64_t block
   if (pair >= pairs || half != ((n >> 2) & 1)) return;
   // an id outside the vocabulary spoils its row; an empty slot has no score
   if (a.label) a.label[i] = id >= 0 && id < a.vocab ? (int)id : -1;
-  const float b = a.bias ? load_as_f32(a.bias, at, a.bias_dtype) * a.unit : 0.f, y = fmaf(z, ldexpf(a.unit, -(sh + sw)), b);
+  const float b = a.bias ? load_as_f32(a.bias, at, a.bias_dtype) * a.unit : 0.f, y = fmaf(z, ldexpf(a.unit, -(sc.sh + sc.sw)), b);
   // half of it: a bias of the lowest finite number, -inf in base 2, is finite so
   const float out = y == -INFINITY && a.bias ? load_as_f32(a.bias, at, a.bias_dtype) * (0.5f * a.unit) : 0.5f * y;
   a.zt[pair] = a.kd && id < 0 ? 0.f : id < 0 || id >= a.vocab ? NAN : out;
@@ -594,34 +663,23 @@ __global__ __launch_bounds__(256) void target_lists_kernel(const TargetArgs t, i
 // of 256: zero), the next `targets` compute the scores at the targets, the rest pack the first C rows of W.
 template <int DT>
 __global__ __launch_bounds__(256) void rows_kernel(const TargetArgs t, int blocks, int targets, int Kp,
-                                                     const float* __restrict__ amax_h,
-                                                     const float* __restrict__ amax_w, Meta* __restrict__ meta,
+                                                     const int* __restrict__ amax_h,
+                                                     const int* __restrict__ amax_w, Meta* __restrict__ meta,
                                                      unsigned short* __restrict__ Hp, int C, unsigned short* __restrict__ Wp) {
   __shared__ vocab::s16x8_t lds[TARGET_LDS];
   const int b = blockIdx.x - blocks, lane = threadIdx.x & 63;
-  auto scale_w = [&] {
-    float m = 0.f;
-    for (int k = lane; k < AMAX_W; k += 64) m = fmaxf(m, amax_w[k]);
-    return scale_exp(wave_max(m), 14);
-  };
-  if (b >= 0 && b < targets) {
-    if constexpr (DT == F32) return target_scores<DT>(t, b, scale_exp(wave_max(amax_h[lane]), 14), scale_w(), lds);
-    else return target_scores<DT>(t, b, 0, 0, lds);
-  }
+  Scales sc{0, 0, 0};
+  if constexpr (DT == F32) sc = scales(amax_h, amax_w);
+  const int sh = sc.sh;
+  if (b >= 0 && b < targets) return target_scores<DT>(t, b, sc, lds);
   if (b >= 0) {
-    const int sw = DT == F32 ? scale_w() : 0;
-    return pack_w(t.weight, t.ldw, DT, t.K, Kp, 0, (b - targets) * 4 + (threadIdx.x >> 6), C, t.vocab, sw, Wp);
+    if (sc.wide) return;
+    return pack_w(t.weight, t.ldw, DT, t.K, Kp, 0, (b - targets) * 4 + (threadIdx.x >> 6), C, t.vocab, sc.sw, Wp);
   }
   const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int count = meta->count;
-  int sh = 0;
-  if constexpr (DT == F32) {
-    sh = scale_exp(wave_max(amax_h[lane]), 14);
-    if (i == 0) {
-      const int sw = scale_w();
-      if (lane == 0) { meta->sh = sh; meta->sw = sw; }
-    }
-  }
+  if (DT == F32 && i == 0 && lane == 0) { meta->sh = sh; meta->sw = sc.sw; meta->wide = sc.wide; }
+  if (sc.wide) return;
   if (i >= (count + 255) / 256 * 256) return;
   const bool zero = i >= count;
   unsigned short* hi = Hp + (int64_t)i * Kp * (DT == F32 ? 2 : 1);
@@ -707,8 +765,8 @@ struct GradArgs {
 // That exponent, from the largest finite |g T|: every workgroup finds it for itself (a launch of its own: 10 us).  bf16 has fp32's range
 // and needs none.
 template <class T>
-__device__ __forceinline__ int grad_exponent(const GradArgs& a, int count, float* part) {
-  if constexpr (!T::F16) return 0;
+__device__ __forceinline__ int grad_exponent(const GradArgs& a, int count, bool wide, float* part) {
+  if (!T::F16 || wide) return 0;
   float m = 0.f;
 #pragma unroll 4
   for (int i = threadIdx.x; i < count; i += T::THREADS) m = fmaxf(m, finite_abs(a.g[(int64_t)a.rowmap[i] * a.gs] * a.temperature));
@@ -756,7 +814,7 @@ __device__ __forceinline__ void rows_of_32(unsigned short* scratch, const float4
 // dS of the columns [j0, j0 + C): dS[r][j] = g_r T q_rj in two planes; at the row's label, from its fp32 score, g_r (q - 1)
 template <class T>
 __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Operand B, int nk, int tn, const Meta* __restrict__ meta,
-                                                                const float* __restrict__ biasz, float unit, const GradArgs G, int64_t j0,
+                                                                const float* __restrict__ biasz, float unit, const GradArgs G, const Raw raw,
                                                                 unsigned short* __restrict__ dS, int64_t plane) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
   const int count = __builtin_amdgcn_readfirstlane(meta->count), tm = (count + T::BM - 1) / T::BM;
@@ -766,18 +824,18 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
   unsigned short* scratch = smem + T::LDS + wave * 2048;
   static_assert(T::TN == 2, "64 columns a wave");
   const int64_t ldS = 2 * plane;
-  const int sg = grad_exponent<T>(G, count, reinterpret_cast<float*>(smem + T::LDS));
+  const bool wide = T::PL == 2 && meta->wide;
+  const int sg = grad_exponent<T>(G, count, wide, reinterpret_cast<float*>(smem + T::LDS));
   if (blockIdx.x == 0 && threadIdx.x == 0) *G.scale = sg;
-  T::run(
-      A, B, smem,
-      [&](int n, Item& it) {
-        unsigned ty, tx, layer;
-        if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, 1, ty, tx, layer)) return false;
-        it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, 0, nk, 0};
-        return true;
-      },
-      [](const Item&) { return false; },
-      [&](const Item& it, typename T::Acc& acc, const float*) {
+  auto work = [&](int n, Item& it) {
+    unsigned ty, tx, layer;
+    if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, 1, ty, tx, layer)) return false;
+    it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, 0, nk, 0};
+    return true;
+  };
+  // in planes of 16 bits, or in fp32 (which takes the same room)
+  auto done = [&](auto in_fp32) {
+    return [&](const Item& it, typename T::Acc& acc, const float*) {
         const int64_t r0 = it.bm + wr * T::WM, c0 = it.bn + wc * T::WN;
         const float* bz = biasz + c0 + (lane >> 5) * 4;
         // what the rows need, its loads in flight together
@@ -788,7 +846,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
           const int r = (int)r0 + i * 32 + (lane & 31), rl = min(r, count - 1);
           const float2 st = G.stat[rl];
           const float g = G.g[G.rowmap[rl] * G.gs] * G.temperature;
-          ys[i] = G.label && r < count && lane < 32 ? G.label[rl] - (int)(j0 + c0) : -1;
+          ys[i] = G.label && r < count ? G.label[rl] - (int)(raw.j0 + c0) : -1;
           Ms[i] = r < count ? st.x : INFINITY;          // (a row past the count: 0 times exp2(-inf))
           inv[i] = r < count ? 1.f / st.y : 1.f;
           gs[i] = r < count ? ldexpf(g, sg) : 0.f;
@@ -800,7 +858,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
           const int y = ys[i];
           const bool hit = y >= 0 && y < 64;
           float target = 0.f;
-          if (hit) target = gr * fmaf(__builtin_amdgcn_exp2f(2.f * G.zt[r0 + i * 32 + lane] - M), inv[i], -1.f);
+          if (hit) target = gr * fmaf(__builtin_amdgcn_exp2f(2.f * G.zt[r0 + i * 32 + (lane & 31)] - M), inv[i], -1.f);
           auto rounded = [](float x) {
             const unsigned short u = T::F16 ? to_f16(x) : to_bf16(x);
             return T::F16 ? (float)__builtin_bit_cast(_Float16, u) : bf16_bits_to_f32(u);
@@ -812,9 +870,26 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
             for (int e = 0; e < 4; ++e) v[e] = gq * __builtin_amdgcn_exp2f(fmaf(acc[i][c >> 2][(c & 3) * 4 + e], sc, bb[e]) - M);
           };
           auto put = [&](const u16x4_t (&x)[8], float at_target, unsigned short* at) {
-            rows_of_16(scratch, x, [&](auto column) { if (hit) column(y) = T::F16 ? to_f16(at_target) : to_bf16(at_target); },
+            rows_of_16(scratch, x, [&](auto column) { if (hit && lane < 32) column(y) = T::F16 ? to_f16(at_target) : to_bf16(at_target); },
                        [&](int row, int cc, u16x8_t v) { *reinterpret_cast<u16x8_t*>(at + row * ldS + cc) = v; });
           };
+          if constexpr (decltype(in_fp32)::value) {
+            float* at = reinterpret_cast<float*>(dS) + (r0 + i * 32) * plane + c0;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              float4 v[4];
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                float x[4];
+                values(4 * n + c, x);
+                // (half of the wave holds 4 of every 8 columns; the label's among them)
+                const int e = y - 32 * n - 8 * c - 4 * (lane >> 5);
+                v[c] = make_float4(e == 0 ? target : x[0], e == 1 ? target : x[1], e == 2 ? target : x[2], e == 3 ? target : x[3]);
+              }
+              rows_of_32(scratch, v, [&](int row, int cc, float4 f) { *reinterpret_cast<float4*>(at + row * plane + n * 32 + cc) = f; });
+            }
+            continue;
+          }
           unsigned short* at = dS + (r0 + i * 32) * ldS + c0;
           u16x4_t hi[8], lo[8];
 #pragma unroll
@@ -827,7 +902,11 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
           put(hi, target, at);
           put(lo, target - rounded(target), at + plane);
         }
-      });
+    };
+  };
+  if constexpr (T::PL == 2)
+    if (wide) return T::run_exact(work, [](const Item&) { return false; }, exact_scores<T>(raw, count), done(std::true_type{}));
+  T::run(A, B, smem, work, [](const Item&) { return false; }, done(std::false_type{}));
 }
 
 // the entries of dS at a teacher's targets in [j0, j0 + C): g_r T (q - sum of p over the slots of the same id)
@@ -843,6 +922,10 @@ struct FixArgs {
 __device__ __forceinline__ void target_entry(const FixArgs& a, int64_t i, int s, int64_t id, float p) {
   const float2 st = a.G.stat[i];
   const float v = ldexpf(a.G.g[a.G.rowmap[i] * a.G.gs] * a.G.temperature, *a.G.scale) * fmaf(__builtin_amdgcn_exp2f(2.f * a.G.zt[i * a.slots + s] - st.x), 1.f / st.y, -p);
+  if (a.meta->wide) {
+    reinterpret_cast<float*>(a.dS)[i * a.plane + (id - a.j0)] = v;
+    return;
+  }
   unsigned short* at = a.dS + i * a.ldS + (id - a.j0);
   at[0] = a.dtype == BF16 ? to_bf16(v) : to_f16(v);
   at[a.plane] = a.dtype == BF16 ? to_bf16(v - bf16_bits_to_f32(at[0])) : to_f16(v - (float)__builtin_bit_cast(_Float16, at[0]));
@@ -880,7 +963,7 @@ __global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
 template <class T>
 __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, Operand B, int steps, int tn, int64_t C,
                                                                  const Meta* __restrict__ meta, float* __restrict__ part, int64_t Kp,
-                                                                 int first, int* __restrict__ ranges) {
+                                                                 int first, int* __restrict__ ranges, const Raw raw) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
   const int count = __builtin_amdgcn_readfirstlane(meta->count), tm = (count + T::BM - 1) / T::BM;
   const bool big = big_tiles(count, C);
@@ -890,35 +973,55 @@ __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, O
   if (blockIdx.x == 0 && threadIdx.x == 0) *ranges = splits;
   const int wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
   unsigned short* scratch = smem + T::LDS + wave * 2048;
-  T::run(
-      A, B, smem,
-      [&](int n, Item& it) {
-        unsigned ty, tx, split;
-        if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, splits, ty, tx, split)) return false;
-        it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, (int64_t)split * per * T::BK, min(per, steps - (int)split * per) * (TWO ? 2 : 1), (int)split};
-        return true;
-      },
-      [](const Item&) { return false; },
-      [&](const Item& it, typename T::Acc& acc, const float*) {
-        float* out = part + (int64_t)it.extra * count * Kp;
+  auto work = [&](int n, Item& it) {
+    unsigned ty, tx, split;
+    if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, splits, ty, tx, split)) return false;
+    it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, (int64_t)split * per * T::BK, min(per, steps - (int)split * per), (int)split};
+    return true;
+  };
+  auto done = [&](const Item& it, typename T::Acc& acc, const float*) {
+    float* out = part + (int64_t)it.extra * count * Kp;
 #pragma unroll
-        for (int i = 0; i < T::TM; ++i)
+    for (int i = 0; i < T::TM; ++i)
 #pragma unroll
-          for (int n = 0; n < T::TN; ++n) {
-            __builtin_amdgcn_sched_barrier(0);
-            const int64_t r0 = it.bm + wr * T::WM + i * 32, c0 = it.bn + wc * T::WN + n * 32;
-            float4 v[4];
+      for (int n = 0; n < T::TN; ++n) {
+        __builtin_amdgcn_sched_barrier(0);
+        const int64_t r0 = it.bm + wr * T::WM + i * 32, c0 = it.bn + wc * T::WN + n * 32;
+        float4 v[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = make_float4(acc[i][n][q * 4], acc[i][n][q * 4 + 1], acc[i][n][q * 4 + 2], acc[i][n][q * 4 + 3]);
-            rows_of_32(scratch, v, [&](int row, int cc, float4 x) {
-              if (r0 + row >= count || c0 + cc >= Kp) return;
-              float4* at = reinterpret_cast<float4*>(out + (r0 + row) * Kp + c0 + cc);
-              if (!first) { const float4 o = *at; x.x += o.x; x.y += o.y; x.z += o.z; x.w += o.w; }
-              *at = x;
-            });
-          }
-      },
-      TWO ? A.cols : 0);
+        for (int q = 0; q < 4; ++q) v[q] = make_float4(acc[i][n][q * 4], acc[i][n][q * 4 + 1], acc[i][n][q * 4 + 2], acc[i][n][q * 4 + 3]);
+        rows_of_32(scratch, v, [&](int row, int cc, float4 x) {
+          if (r0 + row >= count || c0 + cc >= Kp) return;
+          float4* at = reinterpret_cast<float4*>(out + (r0 + row) * Kp + c0 + cc);
+          if (!first) { const float4 o = *at; x.x += o.x; x.y += o.y; x.z += o.z; x.w += o.w; }
+          *at = x;
+        });
+      }
+  };
+  if constexpr (T::PL == 2)
+    if (meta->wide) {
+      // dS in fp32, W where it lies
+      auto rows = [&](const Item& it, auto f) {
+        const int lane = threadIdx.x & 63;
+        const float *s[T::TM], *w[T::TN];
+        bool in[T::TN];
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) {
+          const int64_t r = it.bm + wr * T::WM + i * 32 + (lane & 31);
+          s[i] = reinterpret_cast<const float*>(A.p) + (r < count ? r : count - 1) * A.cols;
+        }
+#pragma unroll
+        for (int c = 0; c < T::TN; ++c) {
+          const int64_t k = it.bn + wc * T::WN + c * 32 + (lane & 31);
+          in[c] = k < raw.K;
+          w[c] = (const float*)raw.weight + (in[c] ? k : 0);
+        }
+        f([&](int i, int64_t j) { return j < A.cols && raw.j0 + j < raw.vocab ? s[i][j] : 0.f; },
+          [&](int c, int64_t j) { return in[c] && raw.j0 + j < raw.vocab ? w[c][(raw.j0 + j) * raw.ldw] : 0.f; });
+      };
+      return T::run_exact(work, [](const Item&) { return false; }, rows, done);
+    }
+  T::run(A, B, smem, work, [](const Item&) { return false; }, done, TWO ? A.cols : 0);
 }
 
 // dh = the ranges' partial products in order, unscaled, to the rows they came from; zero for rows that do not count.  A workgroup
@@ -957,81 +1060,97 @@ __global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict
 template <class T>
 __global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, Operand B, int tm, int tn, const Meta* __restrict__ meta,
                                                                  const int* __restrict__ scale, int dtype, int64_t j0, int vocab, int K,
-                                                                 void* __restrict__ dW, int bias_dtype, void* __restrict__ db) {
+                                                                 void* __restrict__ dW, int bias_dtype, void* __restrict__ db, const Raw raw) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
   const int count = __builtin_amdgcn_readfirstlane(meta->count);
   constexpr bool TWO = T::PL == 1;
-  const int nk = (count + T::BK - 1) / T::BK * (TWO ? 2 : 1);
+  const int nk = (count + T::BK - 1) / T::BK;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
   const int eb = -*scale, e = eb - meta->sh;       // exponents of the units of db and dW
   unsigned short* scratch = smem + T::LDS + wave * 2048;
   static_assert(T::TN == 2, "64 columns a wave");
-  T::template run<true>(
-      A, B, smem,
-      [&](int n, Item& it) {
-        unsigned ty, tx, layer;
-        if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, 1, ty, tx, layer)) return false;
-        it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, 0, nk, 0};
-        return true;
-      },
-      [&](const Item& it) { return db && it.bn == 0 && wc == 0; },
-      [&](const Item& it, typename T::Acc& acc, const float* sums) {
-        const int64_t r0 = j0 + it.bm + wr * T::WM, c0 = it.bn + wc * T::WN;
-        if (db && it.bn == 0 && wc == 0) {
+  auto work = [&](int n, Item& it) {
+    unsigned ty, tx, layer;
+    if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, 1, ty, tx, layer)) return false;
+    it = Item{(int64_t)ty * T::BM, (int64_t)tx * T::BN, 0, nk, 0};
+    return true;
+  };
+  auto want = [&](const Item& it) { return db && it.bn == 0 && wc == 0; };
+  auto done = [&](const Item& it, typename T::Acc& acc, const float* sums) {
+    const int64_t r0 = j0 + it.bm + wr * T::WM, c0 = it.bn + wc * T::WN;
+    if (db && it.bn == 0 && wc == 0) {
 #pragma unroll
-          for (int i = 0; i < T::TM; ++i) {
-            const float s = sums[i] + __shfl_xor(sums[i], 32, 64);
-            const int64_t j = r0 + i * 32 + (lane & 31);
-            if (lane < 32 && j < vocab) store_as(db, j, bias_dtype, ldexpf(s, eb));
-          }
-        }
-        if (!dW) return;
+      for (int i = 0; i < T::TM; ++i) {
+        const float s = sums[i] + __shfl_xor(sums[i], 32, 64);
+        const int64_t j = r0 + i * 32 + (lane & 31);
+        if (lane < 32 && j < vocab) store_as(db, j, bias_dtype, ldexpf(s, eb));
+      }
+    }
+    if (!dW) return;
 #pragma unroll
-        for (int i = 0; i < T::TM; ++i) {
-          __builtin_amdgcn_sched_barrier(0);
-          if (dtype == F32) {
-            float* out = reinterpret_cast<float*>(dW);
+    for (int i = 0; i < T::TM; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (dtype == F32) {
+        float* out = reinterpret_cast<float*>(dW);
 #pragma unroll
-            for (int n = 0; n < T::TN; ++n) {
-              float4 v[4];
+        for (int n = 0; n < T::TN; ++n) {
+          float4 v[4];
 #pragma unroll
-              for (int q = 0; q < 4; ++q)
-                v[q] = make_float4(ldexpf(acc[i][n][q * 4], e), ldexpf(acc[i][n][q * 4 + 1], e), ldexpf(acc[i][n][q * 4 + 2], e), ldexpf(acc[i][n][q * 4 + 3], e));
-              rows_of_32(scratch, v, [&](int row, int cc, float4 x) {
-                const int64_t r = r0 + i * 32 + row, c = c0 + n * 32 + cc;
-                if (r >= vocab || c >= K) return;
-                if (K % 4 == 0) {
-                  *reinterpret_cast<float4*>(out + r * K + c) = x;
-                } else {
-                  const float f[4] = {x.x, x.y, x.z, x.w};
-                  for (int e = 0; e < 4; ++e)
-                    if (c + e < K) out[r * K + c + e] = f[e];
-                }
-              });
+          for (int q = 0; q < 4; ++q)
+            v[q] = make_float4(ldexpf(acc[i][n][q * 4], e), ldexpf(acc[i][n][q * 4 + 1], e), ldexpf(acc[i][n][q * 4 + 2], e), ldexpf(acc[i][n][q * 4 + 3], e));
+          rows_of_32(scratch, v, [&](int row, int cc, float4 x) {
+            const int64_t r = r0 + i * 32 + row, c = c0 + n * 32 + cc;
+            if (r >= vocab || c >= K) return;
+            if (K % 4 == 0) {
+              *reinterpret_cast<float4*>(out + r * K + c) = x;
+            } else {
+              const float f[4] = {x.x, x.y, x.z, x.w};
+              for (int e = 0; e < 4; ++e)
+                if (c + e < K) out[r * K + c + e] = f[e];
             }
+          });
+        }
+      } else {
+        unsigned short* out = reinterpret_cast<unsigned short*>(dW);
+        u16x4_t v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const f32x16_t& x = acc[i][c >> 2];
+          const int q = (c & 3) * 4;
+          v[c] = to_16x4<T::F16>(ldexpf(x[q], e), ldexpf(x[q + 1], e), ldexpf(x[q + 2], e), ldexpf(x[q + 3], e));
+        }
+        rows_of_16(scratch, v, [](auto) {}, [&](int row, int cc, u16x8_t x) {
+          const int64_t r = r0 + i * 32 + row, c = c0 + cc;
+          if (r >= vocab || c >= K) return;
+          if (K % 8 == 0) {
+            *reinterpret_cast<u16x8_t*>(out + r * K + c) = x;
           } else {
-            unsigned short* out = reinterpret_cast<unsigned short*>(dW);
-            u16x4_t v[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              const f32x16_t& x = acc[i][c >> 2];
-              const int q = (c & 3) * 4;
-              v[c] = to_16x4<T::F16>(ldexpf(x[q], e), ldexpf(x[q + 1], e), ldexpf(x[q + 2], e), ldexpf(x[q + 3], e));
-            }
-            rows_of_16(scratch, v, [](auto) {}, [&](int row, int cc, u16x8_t x) {
-              const int64_t r = r0 + i * 32 + row, c = c0 + cc;
-              if (r >= vocab || c >= K) return;
-              if (K % 8 == 0) {
-                *reinterpret_cast<u16x8_t*>(out + r * K + c) = x;
-              } else {
-                for (int e = 0; e < 8; ++e)
-                  if (c + e < K) out[r * K + c + e] = x[e];
-              }
-            });
+            for (int e = 0; e < 8; ++e)
+              if (c + e < K) out[r * K + c + e] = x[e];
           }
+        });
+      }
+    }
+  };
+  if constexpr (T::PL == 2)
+    if (meta->wide) {
+      auto rows = [&](const Item& it, auto f) {
+        const float *s[T::TM], *h[T::TN];
+        bool in[T::TN];
+#pragma unroll
+        for (int i = 0; i < T::TM; ++i) s[i] = reinterpret_cast<const float*>(A.p) + it.bm + wr * T::WM + i * 32 + (lane & 31);
+#pragma unroll
+        for (int c = 0; c < T::TN; ++c) {
+          const int64_t k = it.bn + wc * T::WN + c * 32 + (lane & 31);
+          in[c] = k < raw.K;
+          h[c] = (const float*)raw.hidden + (in[c] ? k : 0);
         }
-      },
-      TWO ? A.cols : 0);
+        f([&](int i, int64_t r) { return r < count ? s[i][r * A.cols] : 0.f; },
+          [&](int c, int64_t r) { return in[c] && r < count ? h[c][(int64_t)raw.rowmap[r] * raw.ldh] : 0.f; });
+      };
+      return T::template run_exact<true>(work, want, rows, done);
+    }
+  T::template run<true>(A, B, smem, work, want, done, TWO ? A.cols : 0);
 }
 
 __global__ void zero_u16_kernel(unsigned short* __restrict__ p, int64_t n) {
@@ -1314,7 +1433,8 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   float* biasz = (float*)(sv + P.o_biasz);
   unsigned short* Hp = (unsigned short*)(sv + P.o_h);
   unsigned char* counts = (unsigned char*)(ws + P.f_counts);
-  float *plogp = (float*)(ws + P.f_plogp), *amax = (float*)(ws + P.f_amax);
+  float* plogp = (float*)(ws + P.f_plogp);
+  int* amax = (int*)(ws + P.f_amax);
   float2* stats = (float2*)(ws + P.f_stats);
   const float inv_t = 1.f / d->temperature, unit = inv_t * LOG2E;
 
@@ -1362,6 +1482,7 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
   const Operand H{Hp, P.PL * P.Kp, P.Kp, P.Rp, P.Kp};
   for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_fwd) {
     const int64_t C = std::min(P.C_fwd, P.Vp - j0);
+    const Raw raw{d->hidden, d->weight, d->ld_hidden, d->ld_weight, j0, d->hidden_size, d->vocab, rowmap};
     Operand W;
     int rc = weight_piece(d, P, j0, C, meta, (unsigned short*)(sv + P.o_w), true, (unsigned short*)(ws + P.f_w), st, W);
     if (rc != GRIDMM_OK) return rc;
@@ -1371,7 +1492,7 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
         const int64_t tn = C / T::BN, tm = (rows + T::BM - 1) / T::BM;
         auto run = [&](auto with) {
           GRIDMM_LAUNCH((score_stats_kernel<T, decltype(with)::value>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, H, W,
-                        (int)(P.Kp / T::BK), (int)tn, meta, biasz + j0, unit, stats + j0 / 128 * P.Rp, P.Rp, lists, j0);
+                        (int)(P.Kp / T::BK), (int)tn, meta, biasz + j0, unit, stats + j0 / 128 * P.Rp, P.Rp, lists, raw);
           GRIDMM_CHECK_LAUNCH();
           return GRIDMM_OK;
         };
@@ -1440,6 +1561,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
   const Operand H{Hp, P.PL * P.Kp, P.Kp, P.Rp, P.Kp};
   for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_bwd) {
     const int64_t C = std::min(P.C_bwd, P.Vp - j0);
+    const Raw raw{d->hidden, d->weight, d->ld_hidden, d->ld_weight, j0, d->hidden_size, d->vocab, rowmap};
     Operand W;
     int rc = weight_piece(d, P, j0, C, meta, (unsigned short*)(sv + P.o_w), false, wbuf, st, W);
     if (rc != GRIDMM_OK) return rc;
@@ -1452,7 +1574,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
         using T = TileOf<F, L, decltype(big)::value, false, false>;
         const int64_t tn = C / T::BN, tm = (rows + T::BM - 1) / T::BM;
         GRIDMM_LAUNCH((score_grad_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, H, W, (int)(P.Kp / T::BK), (int)tn, meta, biasz + j0,
-                      unit, G, j0, dS, C);
+                      unit, G, raw, dS, C);
         GRIDMM_CHECK_LAUNCH();
         return GRIDMM_OK;
       });
@@ -1470,7 +1592,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
           using T = TileOf<F, L, decltype(big)::value, false, true>;
           const int64_t tn = (P.Kp + T::BN - 1) / T::BN, tm = (rows + T::BM - 1) / T::BM;
           GRIDMM_LAUNCH((hidden_grad_kernel<T>), dim3(blocks<T>(tm * tn * MOST_SPLITS)), dim3(T::THREADS), 0, st, S, W, (int)(C / T::BK), (int)tn,
-                        P.C_bwd, meta, part, P.Kp, j0 == 0, scale + 1);
+                        P.C_bwd, meta, part, P.Kp, j0 == 0, scale + 1, raw);
           GRIDMM_CHECK_LAUNCH();
           return GRIDMM_OK;
         });
@@ -1481,7 +1603,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
           using T = TileOf<F, L, decltype(big)::value, true, true>;
           const int64_t tn = d_weight ? (P.Kp + T::BN - 1) / T::BN : 1, tm = C / T::BM;      // (db alone: the first tile column)
           GRIDMM_LAUNCH((weight_grad_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, S, H, (int)tm, (int)tn, meta, scale, d->dtype, j0,
-                        d->vocab, d->hidden_size, d_weight, d->bias_dtype, d_bias);
+                        d->vocab, d->hidden_size, d_weight, d->bias_dtype, d_bias, raw);
           GRIDMM_CHECK_LAUNCH();
           return GRIDMM_OK;
         };

@@ -126,6 +126,88 @@ def test_rows_that_the_model_is_sure_of(dtype, R, V, K, margin, loss):
     assert float(d[sure].max()) <= 0, float(d[sure].max())
 
 
+# ---- rows of very different size ----
+def _neighbours(got, want, sizes, z, h, rows, columns, dtype):
+    """Losses and gradients of `rows`, and the gradients of `columns` of the vocabulary, to what fp32 products leave."""
+    K, half = h.shape[1], HALF[DT[dtype]]
+    ez = _e_z(K, z[rows])
+    assert float(((got["loss"].double() - want["loss"]).abs()[rows]).max()) <= 3 * ez + 8 * U * float(want["loss"][rows].abs().max())
+    for k, at in (("d_hidden", rows), ("d_weight", columns), ("d_bias", columns)):
+        v, n = want[k][at], sizes[k][at]
+        d = (got[k].double()[at] - v).abs() - 3 * ez * n - half * v.abs()
+        if dtype == "fp16":
+            d = d - 2.0 ** -25
+        assert float(d.max()) <= 0, (k, float(d.max()), float(n.max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("R,V,K", [(20, 500, 64), (300, 4000, 768), (500, 30011, 100), (2600, 11000, 96)])
+@pytest.mark.parametrize("factor", [1e4, 1e8, 1e12, 1e30])
+def test_one_large_hidden_row_leaves_the_others_alone(dtype, R, V, K, factor):
+    h, w, b, g = _inputs(dtype, R, V, K, True, seed=3)
+    h[5] *= factor
+    labels = torch.randint(0, V, (R,), generator=g).cuda()
+    gr = (torch.rand(R, generator=g) + 0.5).cuda()
+    got = _run_ce(h, w, b, labels, gr)
+    z, want, sizes = _exact(h, w, b, labels[:, None], torch.ones(R, 1, dtype=torch.float64, device="cuda"), 1.0, gr)
+    rows = torch.arange(R, device="cuda") != 5
+    columns = torch.ones(V, dtype=torch.bool, device="cuda")
+    columns[labels[5]] = False                     # the large row reaches these two
+    columns[z[5].argmax()] = False
+    _neighbours(got, want, sizes, z, h, rows, columns, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("R,V,K", [(20, 500, 64), (300, 4000, 768), (500, 30011, 100), (2600, 11000, 96)])
+@pytest.mark.parametrize("factor", [1e4, 1e8, 1e12, 1e30])
+@pytest.mark.parametrize("masked", [True, False])
+def test_one_large_row_of_the_weight_leaves_the_others_alone(dtype, R, V, K, factor, masked):
+    """A column masked by its bias; or one whose large scores are negative for half of the rows, which keep theirs."""
+    h, w, b, g = _inputs(dtype, R, V, K, True, seed=4)
+    w[7] *= factor
+    if masked:
+        b[7] = float("-inf")
+    labels = torch.randint(8, V, (R,), generator=g).cuda()
+    gr = (torch.rand(R, generator=g) + 0.5).cuda()
+    z7 = h.double() @ w[7].double()
+    rows = torch.ones(R, dtype=torch.bool, device="cuda") if masked else z7 < -200
+    gr = torch.where(rows, gr, torch.zeros_like(gr))
+    got = _run_ce(h, w, b, labels, gr)
+    keep = torch.arange(V, device="cuda") != 7
+    z, want, sizes = _exact(h, w[keep], b[keep], (labels - 1)[:, None], torch.ones(R, 1, dtype=torch.float64, device="cuda"), 1.0, gr)
+    assert int(rows.sum()) > R // 8
+    got["d_weight"], got["d_bias"], seven = got["d_weight"][keep], got["d_bias"][keep], got["d_weight"][7]
+    _neighbours(got, want, sizes, z, h, rows, torch.ones(V - 1, dtype=torch.bool, device="cuda"), dtype)
+    assert bool((seven == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [3, 90])
+def test_distillation_beside_one_large_row(S):
+    from gridmm_amd import vocab
+    R, V, K, T = 600, 3000, 1000, 2.0
+    h, w, b, g = _inputs("fp32", R, V, K, True, seed=6)
+    h[5] *= 1e10
+    w[7] *= 1e10
+    b[7] = float("-inf")
+    ids = torch.stack([8 + torch.randperm(V - 8, generator=g)[:S] for _ in range(R)]).cuda()
+    t = torch.randn(R, S, generator=g).cuda()
+    gr = (torch.rand(R, generator=g) + 0.5).cuda()
+    hl, wl, bl = _leaves(h, w, b)
+    loss = vocab.vocab_distillation(hl, wl, ids, t, bias=bl, temperature=T)
+    loss.backward(gr)
+    keep = torch.arange(V, device="cuda") != 7
+    z, want, sizes = _exact(h, w[keep], b[keep], ids - 1, _teacher(ids, t, T), T, gr)
+    got = {"loss": loss.detach() / (T * T), "d_hidden": hl.grad, "d_weight": wl.grad[keep], "d_bias": bl.grad[keep]}
+    want["loss"] = want["loss"] / (T * T)
+    columns = torch.ones(V - 1, dtype=torch.bool, device="cuda")
+    columns[ids[5] - 1] = False
+    columns[z[5].argmax()] = False
+    _neighbours(got, want, sizes, z, h, torch.arange(R, device="cuda") != 5, columns, "fp32")
+
+
 # ---- no tile is left out ----
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,R,V,K", [("bf16", 300, 70000, 64), ("fp32", 300, 70000, 64), ("fp16", 300, 33000, 72), ("fp32", 20, 9001, 64),
