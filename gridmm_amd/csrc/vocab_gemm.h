@@ -48,22 +48,27 @@ __device__ __forceinline__ f32x16_t mma(s16x8_t a, s16x8_t b, f32x16_t c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
 
-// sum of 8 16-bit values + c
-template <bool F16>
+// sum of 8 bf16 values + c
 __device__ __forceinline__ float sum8(s16x8_t v, float c) {
-  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
   typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
   typedef short s16x2_t __attribute__((ext_vector_type(2)));
+  const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const s16x2_t x = {v[2 * e], v[2 * e + 1]};
-    if constexpr (F16) {
-      const f16x2_t one = {(_Float16)1.f, (_Float16)1.f};
-      c = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, x), one, c, false);
-    } else {
-      const bf16x2_t one = {(__bf16)1.f, (__bf16)1.f};
-      c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x), one, c, false);
-    }
+    c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x), one, c, false);
+  }
+  return c;
+}
+
+// sum of 8 fp16 values times weights + c
+__device__ __forceinline__ float dot8(s16x8_t v, s16x8_t w, float c) {
+  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+  typedef short s16x2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const s16x2_t x = {v[2 * e], v[2 * e + 1]}, y = {w[2 * e], w[2 * e + 1]};
+    c = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, x), __builtin_bit_cast(f16x2_t, y), c, false);
   }
   return c;
 }
@@ -103,6 +108,7 @@ struct Tile {
   static constexpr int PIECES = (BM + BN) / 8, PPW = PIECES / NW;
   static constexpr int LDS = 2 * STAGE;                  // u16 of the two-stage ring
   static constexpr int SCRATCH = NW * 2048;              // u16: 4 KB a wave for an epilogue's stores
+  static constexpr int WEIGHTS = 2048;                   // of a wave's sums, in its SCRATCH
   static constexpr int PER_CU = BM == 256 ? 1 : 2;       // workgroups that a CU's 160 KB of LDS take
   static_assert(PIECES % NW == 0 && WM % 32 == 0 && WN % 32 == 0 && BM % 64 == 0 && BN % 64 == 0, "tile shape");
   static_assert(BM / 8 % PPW == 0 || PPW % (BM / 8) == 0, "a wave's pieces belong to one operand");
@@ -122,10 +128,13 @@ struct Tile {
   // contraction once with A and once with A'.
   //
   // SUMA: sums also takes the sums of A over the contraction for the waves that want_sums(item) names, lane l those of the steps that
-  // it holds of row 32 i + (l & 31); lanes l and l ^ 32 together hold all.
+  // it holds of row 32 i + (l & 31); lanes l and l ^ 32 together hold all.  fp16: each step times its fp16
+  // weight, WEIGHTS at a time in the wave's own LDS `room`, and readable that far past the contraction.  (Scalar loads wait for all of
+  // the fragments' reads, and those for them: 4096 x 65536 x 2048 fp16 7.1 ms
+  // against 6.1.)
   template <bool SUMA = false, class Work, class Want, class Done>
   static __device__ __forceinline__ void run(const Operand& A, const Operand& B, unsigned short* smem, Work work_once, Want want_sums, Done done,
-                                             int64_t twice = 0) {
+                                             int64_t twice = 0, const unsigned short* weights = nullptr, unsigned short* room = nullptr) {
     auto work = [&](int n, Item& it) {
       const bool is = work_once(n, it);
       if (twice) it.nk *= 2;
@@ -267,11 +276,19 @@ struct Tile {
         float part[TM];                      // a stage's sums first: fewer roundings of the long ones
 #pragma unroll
         for (int i = 0; i < TM; ++i) part[i] = 0.f;
+        const int first_k = (twice && kt >= item.nk >> 1 ? kt - (item.nk >> 1) : kt) * BK;
+        if (SUMA && F16 && sum && first_k % WEIGHTS == 0) {
+#pragma unroll
+          for (int i = 0; i < WEIGHTS / 512; ++i)
+            *reinterpret_cast<s16x8_t*>(room + i * 512 + lane * 8) = *reinterpret_cast<const s16x8_t*>(weights + item.k0 + first_k + i * 512 + lane * 8);
+        }
         constexpr int NP = PL == 2 ? 3 : 1, NM = TM * TN, AT = PL == 2 ? NM - 1 : 0;      // the barrier follows product AT of the last sub-step
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           const int set = ks & 1;
           const bool last = ks == KS - 1;
+          s16x8_t w = {0, 0, 0, 0, 0, 0, 0, 0};
+          if (SUMA && F16 && sum) w = *reinterpret_cast<const s16x8_t*>(room + first_k % WEIGHTS + ks * 16 + half * 8);
 #pragma unroll
           for (int m = 0; m < NP * NM; ++m) {
             const int p = m / NM, i = m % NM / TN, n2 = m % TN;
@@ -296,8 +313,9 @@ struct Tile {
           if (SUMA && sum) {
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
-              part[i] = sum8<F16>(a[set][i], part[i]);
-              if constexpr (PL == 2) part[i] = sum8<F16>(al[i], part[i]);
+              if constexpr (F16) part[i] = dot8(a[set][i], w, part[i]);
+              else part[i] = sum8(a[set][i], part[i]);
+              if constexpr (PL == 2) part[i] = dot8(al[i], w, part[i]);
               if (last) sums[i] += part[i];
             }
           }

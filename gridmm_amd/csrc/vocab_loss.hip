@@ -19,8 +19,8 @@
 // 2^-16 (bf16) or 2^-22 (fp16) of itself, so that a gradient is rounded once, to its own type.  (One plane leaves 1.4 times that error, up to
 // twice where a handful of entries makes up a sum; 8030 x 131072 x 2048 13.9 ms against 21.2.)  fp32 operands: two fp16 planes each after a
 // power-of-two scale from the tensor's largest finite value: 22 bits of a value, or 25 of its row's largest, as long as the rows' largest
-// values lie within 2^14 of each other, which the device finds out; rows further apart run on fp32 matrix instructions.  dS is scaled by a power of
-// two from the largest |g T| of the call (fp16 range: entries below 2^-38 of it vanish).
+// values lie within 2^14 of each other, which the device finds out; rows further apart run on fp32 matrix instructions.  fp16
+// planes of dS take a power-of-two scale for each row, from its |g T|.
 // Bound by the four products (vocab_gemm.h): 8030 x 131072 x 2048 bf16 forward and backward 13.8 - 14.0 ms, of it 3.4 scores, 3.7 dS, 3.4 dh, 3.4 dW;
 // fp32 384 x 30522 x 768 325 us, of it 260 products (1.4 rounds of 128 x 128 tiles) and 53 for W's scale and packing.
 // Everything runs in the base-2 domain: y = z log2 e, exp2, and ln 2 comes back in the losses.
@@ -659,13 +659,26 @@ __global__ __launch_bounds__(256) void target_lists_kernel(const TargetArgs t, i
   }
 }
 
+// exponent of the scale that brings a row of fp32 or fp16 under 2^15; NO_ROW: nothing but zeros
+constexpr int NO_ROW = 1 << 14;
+template <int DT>
+__device__ __forceinline__ int row_exp(const void* h, int64_t off, int K, int lane) {
+  float m = 0.f;
+  if constexpr (DT == F32) m = amax_row((const float*)h + off, K, lane);
+  else
+    for (int k = lane; k < K; k += 64) m = fmaxf(m, finite_abs(load_as_f32(h, off + k, DT)));
+  m = wave_max(m);
+  return m > 0.f ? scale_exp(m, 14) : NO_ROW;
+}
+
 // One launch behind prep_kernel: the first `blocks` workgroups pack the counted rows of h into Hp (rows past the count up to a multiple
 // of 256: zero), the next `targets` compute the scores at the targets, the rest pack the first C rows of W.
 template <int DT>
 __global__ __launch_bounds__(256) void rows_kernel(const TargetArgs t, int blocks, int targets, int Kp,
                                                      const int* __restrict__ amax_h,
                                                      const int* __restrict__ amax_w, Meta* __restrict__ meta,
-                                                     unsigned short* __restrict__ Hp, int C, unsigned short* __restrict__ Wp) {
+                                                     unsigned short* __restrict__ Hp, int* __restrict__ hexp, int C,
+                                                     unsigned short* __restrict__ Wp) {
   __shared__ vocab::s16x8_t lds[TARGET_LDS];
   const int b = blockIdx.x - blocks, lane = threadIdx.x & 63;
   Scales sc{0, 0, 0};
@@ -683,7 +696,13 @@ __global__ __launch_bounds__(256) void rows_kernel(const TargetArgs t, int block
   if (i >= (count + 255) / 256 * 256) return;
   const bool zero = i >= count;
   unsigned short* hi = Hp + (int64_t)i * Kp * (DT == F32 ? 2 : 1);
-  pack_row(t.hidden, zero ? 0 : (int64_t)t.rowmap[i] * t.ldh, DT, t.K, Kp, lane, sh, zero, hi, hi + Kp);
+  const int64_t off = zero ? 0 : (int64_t)t.rowmap[i] * t.ldh;
+  pack_row(t.hidden, off, DT, t.K, Kp, lane, sh, zero, hi, hi + Kp);
+  if constexpr (DT != BF16)
+    if (!zero && hexp) {
+      const int e = row_exp<DT>(t.hidden, off, t.K, lane);
+      if (lane == 0) hexp[i] = e;
+    }
 }
 
 // ---- joins the tiles' statistics and writes the losses: 16 rows a workgroup, 16 threads a row ----
@@ -752,6 +771,17 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
 }
 
 // ---- backward ----
+// dS in fp16 planes takes a scale for each row, from its |g T|: 2^13 at most, so that a row's entries keep 22 bits, or 2^-38 of its
+// own |g T|, whatever the others are.  dh takes the scales out again row by row; dW = dS^T h sums over the rows, so h is laid out once
+// more with the scales' inverses in it, and db's sums carry them as weights (2^15 to 2^-24).  Rows whose |g T| |h| are more than 2^20 apart do not
+// fit into one layout of h, |g T| more than 2^39 apart not into the weights: dS is fp32 then and dh and dW are products on fp32 matrix
+// instructions.  bf16 has fp32's range and needs none of it.
+constexpr int GRAD_SPREAD = 20, WEIGHT_SPREAD = 39;
+struct Back {
+  int wide;          // dS is fp32
+  int c, least;      // dW's unit is 2^-c, db's 2^-least (fp32 dS: 1)
+  int ranges;        // of dh
+};
 struct GradArgs {
   const float* g;              // upstream gradients of the rows as they came
   int64_t gs;
@@ -760,22 +790,66 @@ struct GradArgs {
   const int* label;            // of the compacted rows; NULL: distillation, whose targets a kernel of their own writes
   const float* zt;
   const float2* stat;          // (maximum, sum of 2^(y - maximum)): a softmax entry is 2^(y - maximum) / sum
-  int* scale;                  // exponent of the power of two that dS is scaled by
+  const int* rowexp;           // of the compacted rows: dS is 2^this times as large; NULL: 1
+  const Back* back;            // NULL: bf16
+  __device__ float scaled(int i) const {
+    const float v = g[rowmap[i] * gs] * temperature;
+    return rowexp ? ldexpf(v, rowexp[i]) : v;
+  }
 };
-// That exponent, from the largest finite |g T|: every workgroup finds it for itself (a launch of its own: 10 us).  bf16 has fp32's range
-// and needs none.
-template <class T>
-__device__ __forceinline__ int grad_exponent(const GradArgs& a, int count, bool wide, float* part) {
-  if (!T::F16 || wide) return 0;
-  float m = 0.f;
+// The rows' scales, what they come to, and h with their inverses: H2 and weights.  Every workgroup goes through all rows' exponents for
+// itself, one wave then lays a row out.
+__global__ __launch_bounds__(256) void grad_scales_kernel(const GradArgs a, const Meta* __restrict__ meta, const int* __restrict__ hexp, int planes, int Kp,
+                                                          const unsigned short* __restrict__ Hp, unsigned short* __restrict__ H2,
+                                                          unsigned short* __restrict__ weights, int* __restrict__ rowexp, Back* __restrict__ back) {
+  __shared__ int part[4][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, count = meta->count;
+  auto exponent = [&](int i) {       // NO_ROW: a gradient of 0, or none that is a number
+    const float v = finite_abs(a.g[a.rowmap[i] * a.gs] * a.temperature);
+    return v > 0.f ? scale_exp(v, 13) : NO_ROW;
+  };
+  int e0 = NO_ROW, e1 = -NO_ROW, least = NO_ROW, most = -NO_ROW;
+  if (!meta->wide) {
 #pragma unroll 4
-  for (int i = threadIdx.x; i < count; i += T::THREADS) m = fmaxf(m, finite_abs(a.g[(int64_t)a.rowmap[i] * a.gs] * a.temperature));
-  m = wave_max(m);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+    for (int i = tid; i < count; i += 256) {
+      const int x = exponent(i), h = hexp[i];
+      if (x == NO_ROW) continue;
+      least = min(least, x);
+      most = max(most, x);
+      if (h != NO_ROW) { e0 = min(e0, x + h); e1 = max(e1, x + h); }
+    }
+  }
+  e0 = -(int)wave_max((float)-e0);
+  e1 = (int)wave_max((float)e1);
+  least = -(int)wave_max((float)-least);
+  most = (int)wave_max((float)most);
+  if (lane == 0) { part[wave][0] = e0; part[wave][1] = e1; part[wave][2] = least; part[wave][3] = most; }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < T::NW; ++w) m = fmaxf(m, part[w]);
-  return __builtin_amdgcn_readfirstlane(scale_exp(m, 13));
+  for (int w = 0; w < 4; ++w) {
+    e0 = min(e0, part[w][0]); e1 = max(e1, part[w][1]);
+    least = min(least, part[w][2]); most = max(most, part[w][3]);
+  }
+  const bool wide = meta->wide || e1 - e0 > GRAD_SPREAD || most - least > WEIGHT_SPREAD;
+  const int c = wide || e0 == NO_ROW ? 0 : e0;
+  if (wide || least == NO_ROW) least = 0;
+  if (blockIdx.x == 0 && tid == 0) { back->wide = wide; back->c = c; back->least = wide ? 0 : least + 15; }
+  for (int i = blockIdx.x * 4 + wave; i < (count + 255) / 256 * 256; i += gridDim.x * 4) {
+    const int x = i < count && !wide ? exponent(i) : NO_ROW;
+    if (lane == 0) {
+      rowexp[i] = x == NO_ROW ? 0 : x;
+      weights[i] = x == NO_ROW ? (unsigned short)0 : to_f16(ldexpf(1.f, 15 + least - x));
+    }
+    if (wide) continue;
+    // (zeros past the count and for a row whose gradient is 0 or no number, which its dS has already)
+    const int64_t at = (int64_t)i * Kp * planes;
+    for (int k = lane * 8; k < Kp * planes; k += 512) {
+      u16x8_t v = *reinterpret_cast<const u16x8_t*>(Hp + at + k);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = x == NO_ROW ? (unsigned short)0 : to_f16(ldexpf((float)__builtin_bit_cast(_Float16, (unsigned short)v[e]), c - x - meta->sh));
+      *reinterpret_cast<u16x8_t*>(H2 + at + k) = v;
+    }
+  }
 }
 
 // A wave's 32 x 64 values of an epilogue, of 16 or 32 bits, through its own LDS: lane l puts the runs of 4 columns it holds of row
@@ -824,9 +898,6 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
   unsigned short* scratch = smem + T::LDS + wave * 2048;
   static_assert(T::TN == 2, "64 columns a wave");
   const int64_t ldS = 2 * plane;
-  const bool wide = T::PL == 2 && meta->wide;
-  const int sg = grad_exponent<T>(G, count, wide, reinterpret_cast<float*>(smem + T::LDS));
-  if (blockIdx.x == 0 && threadIdx.x == 0) *G.scale = sg;
   auto work = [&](int n, Item& it) {
     unsigned ty, tx, layer;
     if (!tile_of(blockIdx.x, gridDim.x, n, tm, tn, 1, ty, tx, layer)) return false;
@@ -845,11 +916,11 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
         for (int i = 0; i < T::TM; ++i) {
           const int r = (int)r0 + i * 32 + (lane & 31), rl = min(r, count - 1);
           const float2 st = G.stat[rl];
-          const float g = G.g[G.rowmap[rl] * G.gs] * G.temperature;
+          const float g = G.scaled(rl);
           ys[i] = G.label && r < count ? G.label[rl] - (int)(raw.j0 + c0) : -1;
           Ms[i] = r < count ? st.x : INFINITY;          // (a row past the count: 0 times exp2(-inf))
           inv[i] = r < count ? 1.f / st.y : 1.f;
-          gs[i] = r < count ? ldexpf(g, sg) : 0.f;
+          gs[i] = r < count ? g : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < T::TM; ++i) {
@@ -904,9 +975,12 @@ __global__ __launch_bounds__(T::THREADS, 2) void score_grad_kernel(Operand A, Op
         }
     };
   };
+  auto none = [](const Item&) { return false; };
   if constexpr (T::PL == 2)
-    if (wide) return T::run_exact(work, [](const Item&) { return false; }, exact_scores<T>(raw, count), done(std::true_type{}));
-  T::run(A, B, smem, work, [](const Item&) { return false; }, done(std::false_type{}));
+    if (meta->wide) return T::run_exact(work, none, exact_scores<T>(raw, count), done(std::true_type{}));
+  if constexpr (T::F16)
+    if (G.back->wide) return T::run(A, B, smem, work, none, done(std::true_type{}));
+  T::run(A, B, smem, work, none, done(std::false_type{}));
 }
 
 // the entries of dS at a teacher's targets in [j0, j0 + C): g_r T (q - sum of p over the slots of the same id)
@@ -921,8 +995,8 @@ struct FixArgs {
 };
 __device__ __forceinline__ void target_entry(const FixArgs& a, int64_t i, int s, int64_t id, float p) {
   const float2 st = a.G.stat[i];
-  const float v = ldexpf(a.G.g[a.G.rowmap[i] * a.G.gs] * a.G.temperature, *a.G.scale) * fmaf(__builtin_amdgcn_exp2f(2.f * a.G.zt[i * a.slots + s] - st.x), 1.f / st.y, -p);
-  if (a.meta->wide) {
+  const float v = a.G.scaled((int)i) * fmaf(__builtin_amdgcn_exp2f(2.f * a.G.zt[i * a.slots + s] - st.x), 1.f / st.y, -p);
+  if (a.G.back && a.G.back->wide) {
     reinterpret_cast<float*>(a.dS)[i * a.plane + (id - a.j0)] = v;
     return;
   }
@@ -963,14 +1037,14 @@ __global__ __launch_bounds__(256) void target_grad_kernel(const FixArgs a) {
 template <class T>
 __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, Operand B, int steps, int tn, int64_t C,
                                                                  const Meta* __restrict__ meta, float* __restrict__ part, int64_t Kp,
-                                                                 int first, int* __restrict__ ranges, const Raw raw) {
+                                                                 int first, Back* __restrict__ back, const Raw raw) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
   const int count = __builtin_amdgcn_readfirstlane(meta->count), tm = (count + T::BM - 1) / T::BM;
   const bool big = big_tiles(count, C);
   if (big != (T::BM == 256)) return;
   constexpr bool TWO = T::PL == 1;       // dS's two planes one after the other
   const int splits = hidden_splits(count, Kp, C, big), per = (steps + splits - 1) / splits;
-  if (blockIdx.x == 0 && threadIdx.x == 0) *ranges = splits;
+  if (blockIdx.x == 0 && threadIdx.x == 0) back->ranges = splits;
   const int wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
   unsigned short* scratch = smem + T::LDS + wave * 2048;
   auto work = [&](int n, Item& it) {
@@ -998,12 +1072,13 @@ __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, O
         });
       }
   };
-  if constexpr (T::PL == 2)
-    if (meta->wide) {
+  if constexpr (T::F16)
+    if (back->wide) {
       // dS in fp32, W where it lies
       auto rows = [&](const Item& it, auto f) {
         const int lane = threadIdx.x & 63;
-        const float *s[T::TM], *w[T::TN];
+        const float* s[T::TM];
+        int64_t w[T::TN];
         bool in[T::TN];
 #pragma unroll
         for (int i = 0; i < T::TM; ++i) {
@@ -1014,10 +1089,10 @@ __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, O
         for (int c = 0; c < T::TN; ++c) {
           const int64_t k = it.bn + wc * T::WN + c * 32 + (lane & 31);
           in[c] = k < raw.K;
-          w[c] = (const float*)raw.weight + (in[c] ? k : 0);
+          w[c] = in[c] ? k : 0;
         }
         f([&](int i, int64_t j) { return j < A.cols && raw.j0 + j < raw.vocab ? s[i][j] : 0.f; },
-          [&](int c, int64_t j) { return in[c] && raw.j0 + j < raw.vocab ? w[c][(raw.j0 + j) * raw.ldw] : 0.f; });
+          [&](int c, int64_t j) { return in[c] && raw.j0 + j < raw.vocab ? load_as_f32(raw.weight, w[c] + (raw.j0 + j) * raw.ldw, T::PL == 2 ? F32 : F16) : 0.f; });
       };
       return T::run_exact(work, [](const Item&) { return false; }, rows, done);
     }
@@ -1028,16 +1103,17 @@ __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, O
 // takes 64 runs of 4 columns of one row, 4 threads a run, each every fourth range.
 __global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict__ part, int64_t Kp, int K, int rows,
                                                          const int* __restrict__ rowinv, const Meta* __restrict__ meta,
-                                                         const int* __restrict__ scale, const int* __restrict__ ranges, int dtype,
+                                                         const int* __restrict__ rowexp, const Back* __restrict__ back, int dtype,
                                                          void* __restrict__ out) {
   __shared__ float4 sums[3][64];
   const int t = threadIdx.x & 63, sp = threadIdx.x >> 6;
   const int64_t r = blockIdx.x;
   const int k = blockIdx.y * 256 + t * 4;
-  const int count = __builtin_amdgcn_readfirstlane(meta->count), pos = rowinv[r], e = -(*scale + meta->sw);
+  const int count = __builtin_amdgcn_readfirstlane(meta->count), pos = rowinv[r];
+  const int e = !rowexp || pos < 0 || back->wide ? 0 : -(rowexp[pos] + meta->sw);
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (pos >= 0 && k < Kp) {
-    const int splits = *ranges;
+    const int splits = back->ranges;
     const float* at = part + (int64_t)pos * Kp + k;
 #pragma unroll 4
     for (int s = sp; s < splits; s += 4) {
@@ -1059,14 +1135,14 @@ __global__ __launch_bounds__(256) void hidden_out_kernel(const float* __restrict
 // tile column also sums dS over the rows: db
 template <class T>
 __global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, Operand B, int tm, int tn, const Meta* __restrict__ meta,
-                                                                 const int* __restrict__ scale, int dtype, int64_t j0, int vocab, int K,
+                                                                 const Back* __restrict__ back, const unsigned short* __restrict__ weights, int dtype, int64_t j0, int vocab, int K,
                                                                  void* __restrict__ dW, int bias_dtype, void* __restrict__ db, const Raw raw) {
   __shared__ __attribute__((aligned(16))) unsigned short smem[T::LDS + T::SCRATCH];
   const int count = __builtin_amdgcn_readfirstlane(meta->count);
   constexpr bool TWO = T::PL == 1;
   const int nk = (count + T::BK - 1) / T::BK;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
-  const int eb = -*scale, e = eb - meta->sh;       // exponents of the units of db and dW
+  const int eb = T::F16 ? -back->least : 0, e = T::F16 ? -back->c : 0;       // exponents of the units of db and dW
   unsigned short* scratch = smem + T::LDS + wave * 2048;
   static_assert(T::TN == 2, "64 columns a wave");
   auto work = [&](int n, Item& it) {
@@ -1132,10 +1208,11 @@ __global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, O
       }
     }
   };
-  if constexpr (T::PL == 2)
-    if (meta->wide) {
+  if constexpr (T::F16)
+    if (back->wide) {
       auto rows = [&](const Item& it, auto f) {
-        const float *s[T::TM], *h[T::TN];
+        const float* s[T::TM];
+        int64_t h[T::TN];
         bool in[T::TN];
 #pragma unroll
         for (int i = 0; i < T::TM; ++i) s[i] = reinterpret_cast<const float*>(A.p) + it.bm + wr * T::WM + i * 32 + (lane & 31);
@@ -1143,14 +1220,14 @@ __global__ __launch_bounds__(T::THREADS, 2) void weight_grad_kernel(Operand A, O
         for (int c = 0; c < T::TN; ++c) {
           const int64_t k = it.bn + wc * T::WN + c * 32 + (lane & 31);
           in[c] = k < raw.K;
-          h[c] = (const float*)raw.hidden + (in[c] ? k : 0);
+          h[c] = in[c] ? k : 0;
         }
         f([&](int i, int64_t r) { return r < count ? s[i][r * A.cols] : 0.f; },
-          [&](int c, int64_t r) { return in[c] && r < count ? h[c][(int64_t)raw.rowmap[r] * raw.ldh] : 0.f; });
+          [&](int c, int64_t r) { return in[c] && r < count ? load_as_f32(raw.hidden, h[c] + (int64_t)raw.rowmap[r] * raw.ldh, T::PL == 2 ? F32 : F16) : 0.f; });
       };
       return T::template run_exact<true>(work, want, rows, done);
     }
-  T::template run<true>(A, B, smem, work, want, done, TWO ? A.cols : 0);
+  T::template run<true>(A, B, smem, work, want, done, TWO ? A.cols : 0, weights, scratch);
 }
 
 __global__ void zero_u16_kernel(unsigned short* __restrict__ p, int64_t n) {
@@ -1211,11 +1288,11 @@ struct Plan {
   bool keep_w;                 // ... and its copy, one piece, stays for the backward (28 us of 396 at 30522 x 768 fp32)
   int64_t C_fwd, C_bwd;        // columns a piece
   // saved
-  size_t o_meta, o_rowmap, o_rowinv, o_stat, o_zt, o_label, o_p, o_biasz, o_h, o_w, saved;
+  size_t o_meta, o_rowmap, o_rowinv, o_stat, o_zt, o_label, o_p, o_biasz, o_hexp, o_h, o_w, saved;
   // forward workspace
   size_t f_counts, f_plogp, f_amax, f_stats, f_w, f_begin, f_entry, fwd;
   // backward workspace
-  size_t b_scale, b_ds, b_w, b_part, bwd;
+  size_t b_back, b_rowexp, b_weights, b_h2, b_ds, b_w, b_part, bwd;
 };
 
 bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
@@ -1283,6 +1360,7 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.o_label = take(d->slots ? 0 : R * 4);
   P.o_p = take(d->slots ? R * S * 4 : 0);
   P.o_biasz = take(P.Vp * 4);
+  P.o_hexp = take(d->dtype == BF16 ? 0 : Rp * 4);
   P.o_h = take(Rp * P.Kp * 2 * P.PL);
   P.o_w = take(P.keep_w ? (size_t)P.Vp * P.Kp * 2 * P.PL : 0);
   P.saved = o;
@@ -1297,7 +1375,10 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.f_entry = take(P.lists ? R * S * 4 : 0);
   P.fwd = o;
   o = 0;
-  P.b_scale = take(8);                 // ... and the ranges of dh
+  P.b_back = take(sizeof(Back));
+  P.b_rowexp = take(d->dtype == BF16 ? 0 : Rp * 4);
+  P.b_weights = take(d->dtype == BF16 ? 0 : (Rp + 2048) * 2);
+  P.b_h2 = take(d->dtype == BF16 ? 0 : Rp * P.Kp * 2 * P.PL);
   P.b_ds = take(Rp * (size_t)P.C_bwd * 4);
   P.b_w = take(P.pack_w && !P.keep_w ? (size_t)P.C_bwd * P.Kp * 2 * P.PL : 0);
   P.b_part = take(std::max<size_t>(Rp * (size_t)P.Kp, std::min<size_t>(MOST_SPLITS * Rp * (size_t)P.Kp, PART_MOST)) * 4);
@@ -1465,7 +1546,8 @@ extern "C" int gridmm_vocab_loss_fwd(const gridmm_vocab_loss_t* d, float* loss, 
     const int C = P.pack_w ? (int)P.C_fwd : 0;
     unsigned short* Wp = (unsigned short*)(P.keep_w ? sv + P.o_w : ws + P.f_w);
     const dim3 grid((unsigned)(hb + tb + (C + 3) / 4));
-    GRIDMM_LAUNCH((rows_kernel<DT>), grid, dim3(256), 0, st, t, hb, tb, (int)P.Kp, amax, amax + AMAX_H, meta, Hp, C, Wp);
+    GRIDMM_LAUNCH((rows_kernel<DT>), grid, dim3(256), 0, st, t, hb, tb, (int)P.Kp, amax, amax + AMAX_H, meta, Hp,
+                  d->forward_only ? nullptr : (int*)(sv + P.o_hexp), C, Wp);
     GRIDMM_CHECK_LAUNCH();
     return GRIDMM_OK;
   });
@@ -1547,7 +1629,10 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
     return GRIDMM_OK;
   }
   const Meta* meta = (const Meta*)(sv + P.o_meta);
-  int* scale = (int*)(ws + P.b_scale);
+  Back* back = (Back*)(ws + P.b_back);
+  const bool scaled = d->dtype != BF16;
+  int* rowexp = scaled ? (int*)(ws + P.b_rowexp) : nullptr;
+  unsigned short* weights = scaled ? (unsigned short*)(ws + P.b_weights) : nullptr;
   const int *rowmap = (const int*)(sv + P.o_rowmap), *rowinv = (const int*)(sv + P.o_rowinv);
   const float2* stat = (const float2*)(sv + P.o_stat);
   const float* zt = (const float*)(sv + P.o_zt);
@@ -1557,8 +1642,16 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
   unsigned short *dS = (unsigned short*)(ws + P.b_ds), *wbuf = (unsigned short*)(ws + P.b_w);
   const float unit = LOG2E / d->temperature;
 
-  const GradArgs G{grad, grad_stride, d->temperature, rowmap, d->slots ? nullptr : (const int*)(sv + P.o_label), zt, stat, scale};
+  const GradArgs G{grad, grad_stride, d->temperature, rowmap, d->slots ? nullptr : (const int*)(sv + P.o_label), zt, stat, rowexp, scaled ? back : nullptr};
   const Operand H{Hp, P.PL * P.Kp, P.Kp, P.Rp, P.Kp};
+  Operand H2 = H;                          // of dW
+  if (scaled) {
+    unsigned short* h2 = (unsigned short*)(ws + P.b_h2);
+    GRIDMM_LAUNCH(grad_scales_kernel, dim3((unsigned)std::min<int64_t>(P.Rp / 4, 1024)), dim3(256), 0, st, G, meta, (const int*)(sv + P.o_hexp), P.PL,
+                  (int)P.Kp, Hp, h2, weights, rowexp, back);
+    GRIDMM_CHECK_LAUNCH();
+    H2.p = h2;
+  }
   for (int64_t j0 = 0; j0 < P.Vp; j0 += P.C_bwd) {
     const int64_t C = std::min(P.C_bwd, P.Vp - j0);
     const Raw raw{d->hidden, d->weight, d->ld_hidden, d->ld_weight, j0, d->hidden_size, d->vocab, rowmap};
@@ -1592,7 +1685,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
           using T = TileOf<F, L, decltype(big)::value, false, true>;
           const int64_t tn = (P.Kp + T::BN - 1) / T::BN, tm = (rows + T::BM - 1) / T::BM;
           GRIDMM_LAUNCH((hidden_grad_kernel<T>), dim3(blocks<T>(tm * tn * MOST_SPLITS)), dim3(T::THREADS), 0, st, S, W, (int)(C / T::BK), (int)tn,
-                        P.C_bwd, meta, part, P.Kp, j0 == 0, scale + 1, raw);
+                        P.C_bwd, meta, part, P.Kp, j0 == 0, back, raw);
           GRIDMM_CHECK_LAUNCH();
           return GRIDMM_OK;
         });
@@ -1602,7 +1695,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
         auto weight = [&](auto big) {
           using T = TileOf<F, L, decltype(big)::value, true, true>;
           const int64_t tn = d_weight ? (P.Kp + T::BN - 1) / T::BN : 1, tm = C / T::BM;      // (db alone: the first tile column)
-          GRIDMM_LAUNCH((weight_grad_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, S, H, (int)tm, (int)tn, meta, scale, d->dtype, j0,
+          GRIDMM_LAUNCH((weight_grad_kernel<T>), dim3(blocks<T>(tm * tn)), dim3(T::THREADS), 0, st, S, H2, (int)tm, (int)tn, meta, back, weights, d->dtype, j0,
                         d->vocab, d->hidden_size, d_weight, d->bias_dtype, d_bias, raw);
           GRIDMM_CHECK_LAUNCH();
           return GRIDMM_OK;
@@ -1616,7 +1709,7 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
   }
   if (d_hidden) {
     GRIDMM_LAUNCH(hidden_out_kernel, dim3(d->rows, (unsigned)((P.Kp + 255) / 256)), dim3(256), 0, st, part, P.Kp, d->hidden_size,
-                  d->rows, rowinv, meta, scale, scale + 1, d->dtype, d_hidden);
+                  d->rows, rowinv, meta, rowexp, back, d->dtype, d_hidden);
     GRIDMM_CHECK_LAUNCH();
   }
   return GRIDMM_OK;

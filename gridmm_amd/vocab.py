@@ -196,8 +196,7 @@ def vocab_cross_entropy(hidden, weight, labels, bias=None, ignore_index=-1):
 
     A label outside [0, V) that is not ignore_index makes its row's loss NaN, and with it the gradients that it reaches.  A bias of -inf
     or of the type's lowest number takes its column out of the softmax.  The backward holds one piece of the scores' gradient at a time
-    (512 MB), scaled by one power of two: rows whose upstream gradient is more than 2^20 times smaller than the largest lose bits.  At
-    most 2^20 rows, 2^27 columns, and 2^37 scores."""
+    (512 MB).  At most 2^20 rows, 2^27 columns, and 2^37 scores."""
     _check_head(hidden, weight, bias, labels)
     if labels.shape != hidden.shape[:-1]:
         raise ValueError("labels %s for hidden %s" % (tuple(labels.shape), tuple(hidden.shape)))

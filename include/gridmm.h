@@ -823,7 +823,7 @@ int gridmm_dropout_add(const float* x, const float* r, float* y, void* y_hi, voi
  *   hidden [rows][hidden_size], weight [vocab][hidden_size] in dtype (0 fp32, 1 bf16, 2 fp16), row strides ld_*; bias [vocab] in
  *   bias_dtype or NULL; labels [rows], ids [rows][slots] int64 (index64 != 0) or int32; teacher fp32 [rows][slots].
  * fp32 operands run as two fp16 planes under a power-of-two scale of the tensor (22 bits of a value or 25 of its row's largest; few rows,
- * and rows whose largest values are more than 2^14 apart, counted rows of hidden or rows of weight: as fp32), 16-bit ones as they are; sums, maxima and losses are fp32.  dS entries more than 2^38 below the largest |grad T| of the call vanish (bf16: none).
+ * and rows whose largest values are more than 2^14 apart, counted rows of hidden or rows of weight: as fp32), 16-bit ones as they are; sums, maxima and losses are fp32.  dS entries more than 2^38 below their row's |grad T| vanish (bf16, few rows: none).
  * rows <= 2^20, vocab <= 2^27, hidden_size <= 2^20, slots <= 2^16, rows / 128 x vocab / 128 <= 2^23, rows x slots / 8 <= 2^25,
  * 1e-6 <= T <= 1e6.  Deterministic.  Rows that do not count are left out on the device (no read-back): a capture may replay the call
  * with other labels.  A column whose bias is -inf or the type's lowest number is out of the sum.

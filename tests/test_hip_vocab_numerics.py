@@ -208,6 +208,28 @@ def test_distillation_beside_one_large_row(S):
     _neighbours(got, want, sizes, z, h, torch.arange(R, device="cuda") != 5, columns, "fp32")
 
 
+# ---- upstream gradients far apart ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("R,V,K", [(30, 20000, 64), (300, 30011, 96), (2600, 11000, 96)])
+@pytest.mark.parametrize("ratio", [10, 18, 30])
+def test_rows_of_small_upstream_gradients_keep_their_own(dtype, R, V, K, ratio):
+    """Nearly flat rows against a weight with a mean of its own: the many small entries of dS make up as much of dh as the label's.  Rows
+    whose upstream gradient is 2^-ratio of the others' are held to their own size."""
+    h, w, b, g = _inputs(dtype, R, V, K, True, seed=2, spread=0.3)
+    w = (w.float() + torch.randn(K, generator=g).cuda()).to(DT[dtype])
+    h = (h.float() * 0.05).to(DT[dtype])
+    labels = torch.randint(0, V, (R,), generator=g).cuda()
+    gr = (torch.rand(R, generator=g) + 0.5).cuda()
+    gr[::2] *= 2.0 ** -ratio
+    if dtype == "fp16":
+        gr *= 2.0 ** min(ratio, 14)                # (dh itself has fp16's range)
+    got = _run_ce(h, w, b, labels, gr)
+    z, want, sizes = _exact(h, w, b, labels[:, None], torch.ones(R, 1, dtype=torch.float64, device="cuda"), 1.0, gr)
+    every = torch.ones(R, dtype=torch.bool, device="cuda")
+    _neighbours(got, want, sizes, z, h, every, torch.ones(V, dtype=torch.bool, device="cuda"), dtype)
+
+
 # ---- no tile is left out ----
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,R,V,K", [("bf16", 300, 70000, 64), ("fp32", 300, 70000, 64), ("fp16", 300, 33000, 72), ("fp32", 20, 9001, 64),
