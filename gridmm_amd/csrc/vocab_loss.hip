@@ -1594,11 +1594,12 @@ extern "C" int gridmm_vocab_loss_bwd(const gridmm_vocab_loss_t* d, const void* s
                                      size_t workspace_bytes, gridmm_stream_t stream) {
   Plan P;
   if (!make_plan(d, P) || bad_pointers(d, saved, false) || saved_bytes < P.saved || !workspace || workspace_bytes < P.bwd ||
-      ((uintptr_t)workspace & 255) || (d->rows && !grad) || (!d_hidden && !d_weight && !d_bias) || grad_stride < 0 ||
+      ((uintptr_t)workspace & 255) || (d->rows && (!grad || (!d_hidden && !d_weight && !d_bias))) || grad_stride < 0 ||
       (d_bias && !d->bias) || d->forward_only)
     return GRIDMM_EINVAL;
   hipStream_t st = as_stream(stream);
   if (d->rows == 0) {                       // nothing counts: the shared gradients are zero
+    if (!d_weight && !d_bias) return GRIDMM_OK;
     const int64_t nw = (int64_t)d->vocab * d->hidden_size * (d->dtype == F32 ? 2 : 1), nb = (int64_t)d->vocab * (d->bias_dtype == F32 ? 2 : 1);
     if (d_weight) GRIDMM_LAUNCH(zero_u16_kernel, dim3((unsigned)std::min<int64_t>((nw + 255) / 256, 4096)), dim3(256), 0, st, (unsigned short*)d_weight, nw);
     if (d_bias) GRIDMM_LAUNCH(zero_u16_kernel, dim3((unsigned)std::min<int64_t>((nb + 255) / 256, 4096)), dim3(256), 0, st, (unsigned short*)d_bias, nb);

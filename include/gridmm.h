@@ -835,7 +835,7 @@ int gridmm_dropout_add(const float* x, const float* r, float* y, void* y_hi, voi
  *   forward_only != 0: no backward will follow (other kernels may be the faster ones then)
  *   backward   grad: d loss_r at grad[r * grad_stride] (0: one value for all rows); d_hidden [rows][hidden_size],
  *              d_weight [vocab][hidden_size] dense in dtype, d_bias [vocab] in bias_dtype, each overwritten, each may be NULL (one
- *              at least is not); teacher is not read. */
+ *              at least is not, unless rows == 0); teacher is not read. */
 typedef struct {
   const void *hidden, *weight, *bias, *labels, *ids;
   const float* teacher;

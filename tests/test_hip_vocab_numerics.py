@@ -273,3 +273,28 @@ def test_every_tile_counts(dtype, R, V, K):
     bound = 3 * _e_z(K, z) + 8 * U * math.log(V)
     assert bound < 32.0 / V
     assert float((loss - torch.logsumexp(z, 1) + z.gather(1, y[:, None])[:, 0]).abs().max()) <= bound
+
+
+# ---- no rows ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_no_rows_under_a_frozen_decoder(dtype):
+    """A batch without a masked token whose decoder is not trained: an empty gradient, not an error."""
+    from gridmm_amd import vocab
+    h, w, b, _ = _inputs(dtype, 0, 100, 64)
+    hl = h.requires_grad_()
+    vocab.vocab_cross_entropy(hl, w, torch.zeros(0, dtype=torch.long, device="cuda"), bias=b).sum().backward()
+    assert hl.grad.shape == (0, 64)
+    hl.grad = None
+    vocab.vocab_distillation(hl, w, torch.zeros(0, 3, dtype=torch.long, device="cuda"), torch.zeros(0, 3, device="cuda"), bias=b).sum().backward()
+    assert hl.grad.shape == (0, 64)
+
+
+def test_no_rows_and_no_outputs_at_the_c_entry():
+    """Nothing is launched: an empty hidden gradient has no address."""
+    import ctypes
+    from test_hip_vocab import _descriptor
+    from gridmm_amd import _lib
+    lib = _lib.load()
+    d = _descriptor(rows=0, weight=256)
+    assert lib.gridmm_vocab_loss_bwd(ctypes.byref(d), 256, 1 << 40, None, 1, None, None, None, 256, 1 << 40, None) == 0
