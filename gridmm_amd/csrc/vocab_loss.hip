@@ -1309,17 +1309,19 @@ bool make_plan(const gridmm_vocab_loss_t* d, Plan& P) {
   P.pack_w = d->packed || d->dtype == F32 || d->hidden_size % 64 || d->ld_weight % 8 || ((uintptr_t)d->weight & 15) || d->ld_weight > (1 << 22);
   // (grids: at most 2^32 threads)
   if ((P.Rp / 128) * (P.Vp / 128) > (1 << 23) || (int64_t)d->rows * ((P.slots + 7) / 8) > (1 << 25)) return false;
-  // pieces: packed W and dS at most MOST bytes each, whole tiles, 8 192 columns at least
-  const int64_t most = PIECE_MB << 20, least = 8192;
-  auto piece = [&](int64_t bytes_a_column) {
+  // pieces: packed W and dS of at most `most` bytes each, whole tiles; but of dS 8192 columns (32 KB a row: more than that from 16384 rows
+  // on), as dh's sums are read and written once a piece, and of W a tile's 256.  Forward and backward with 2048 : 8192 columns, ms:
+  // 32768 x 32768 x 1024 bf16 16.3 : 12.8, 131072 rows of it 100 : 51, 131072 x 16384 x 4096 97 : 85, 131072 x 16384 x 1024 fp32 68 : 46
+  const int64_t most = PIECE_MB << 20;
+  auto piece = [&](int64_t bytes_a_column, int64_t least) {
     int64_t c = most / bytes_a_column / 256 * 256;
     if (c < least) c = least;
     if (c >= P.Vp) return P.Vp;
     const int64_t n = (P.Vp + c - 1) / c;                      // equal pieces
     return (int64_t)up((P.Vp + n - 1) / n, 256);
   };
-  P.C_fwd = P.pack_w ? piece(P.Kp * 2 * P.PL) : P.Vp;
-  P.C_bwd = piece(std::max<int64_t>(P.Rp, 1) * 4);
+  P.C_fwd = P.pack_w ? piece(P.Kp * 2 * P.PL, 256) : P.Vp;
+  P.C_bwd = piece(std::max<int64_t>(P.Rp, 1) * 4, 8192);
   P.keep_w = P.pack_w && P.C_fwd == P.Vp;
   if (P.pack_w) P.C_bwd = std::min(P.C_bwd, P.C_fwd);
   P.few = few_rows(d);

@@ -195,8 +195,12 @@ def vocab_cross_entropy(hidden, weight, labels, bias=None, ignore_index=-1):
     bias (V,) in that type or fp32, labels (...) int64 or int32.  Gradients of hidden, weight and bias in their types.
 
     A label outside [0, V) that is not ignore_index makes its row's loss NaN, and with it the gradients that it reaches.  A bias of -inf
-    or of the type's lowest number takes its column out of the softmax.  The backward holds one piece of the scores' gradient at a time
-    (512 MB).  At most 2^20 rows, 2^27 columns, and 2^37 scores."""
+    or of the type's lowest number takes its column out of the softmax.  At most 2^20 rows, 2^27 columns, and 2^37 scores.
+
+    Memory beside the results: what is kept for the backward is a copy of hidden, and one of weight where it is fp32 or cannot be read in
+    place and takes at most 512 MB; the backward holds one piece of the scores' gradient at a time, of 512 MB, or of 32 KB a row where that is more
+    (from 16384 rows on), fp32 sums of d_hidden (256 MB at most, or 4 bytes a value) and, fp32 and fp16, one more copy of hidden; the forward 8
+    bytes for 128 columns of a row.  A few rows, and small heads, keep their scores (4 bytes each)."""
     _check_head(hidden, weight, bias, labels)
     if labels.shape != hidden.shape[:-1]:
         raise ValueError("labels %s for hidden %s" % (tuple(labels.shape), tuple(hidden.shape)))

@@ -832,6 +832,8 @@ int gridmm_dropout_add(const float* x, const float* r, float* y, void* y_hi, voi
  *              (all four calls take the same *d.  Pointers and strides of the backward may be others, of copies of the same values, as
  *              long as the weight's 16 bits stay on 16-byte boundaries, its stride a multiple of 8 and at most 2^22, if they were so)
  *   packed != 0 weight is not read where it lies, whatever its alignment: no such condition
+ *              The backward's is mostly one piece of dS, 512 MB, or 32 KB a row where that is more (from 16384 rows on), and fp32 sums of
+ *              d_hidden (256 MB at most, or 4 bytes a value); the forward's 8 bytes for 128 columns of a row
  *   forward_only != 0: no backward will follow (other kernels may be the faster ones then)
  *   backward   grad: d loss_r at grad[r * grad_stride] (0: one value for all rows); d_hidden [rows][hidden_size],
  *              d_weight [vocab][hidden_size] dense in dtype, d_bias [vocab] in bias_dtype, each overwritten, each may be NULL (one

@@ -298,3 +298,26 @@ def test_no_rows_and_no_outputs_at_the_c_entry():
     lib = _lib.load()
     d = _descriptor(rows=0, weight=256)
     assert lib.gridmm_vocab_loss_bwd(ctypes.byref(d), 256, 1 << 40, None, 1, None, None, None, 256, 1 << 40, None) == 0
+
+
+# ---- memory ----
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("rows", [1000, 16384, 40000, 2 ** 17, 2 ** 20])
+@pytest.mark.parametrize("vocab,hidden", [(30522, 768), (131072, 2048), (131072, 33001), (5000, 64), (2 ** 17, 2 ** 20)])
+def test_workspaces_stay_within_what_is_said_of_them(dtype, rows, vocab, hidden):
+    """The library is asked without a GPU."""
+    import ctypes
+    from test_hip_vocab import _descriptor
+    from gridmm_amd import _lib
+    lib = _lib.load()
+    d = _descriptor(rows=rows, vocab=vocab, hidden_size=hidden, dtype=dtype, bias_dtype=dtype, ld_hidden=hidden, ld_weight=hidden, hidden=256, weight=256)
+    size, MB = 4 if dtype == 0 else 2, 2 ** 20
+    rp, vp, kp = (rows + 255) // 256 * 256, (vocab + 255) // 256 * 256, (hidden + 63) // 64 * 64
+    piece_w = max(512 * MB, 256 * kp * size)
+    saved = lib.gridmm_vocab_loss_saved_bytes(ctypes.byref(d))
+    assert 0 < saved <= rp * kp * size + 512 * MB + 64 * rp + 4 * vp + 4096
+    forward = lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 0)
+    assert 0 < forward <= rp * vp // 16 + piece_w + 64 * rp + 65536
+    backward = lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 1)
+    scores_grad, sums, layout = max(512 * MB, 32768 * rp), max(256 * MB, 4 * rp * kp), 0 if dtype == 1 else rp * kp * size
+    assert 0 < backward <= scores_grad + sums + layout + piece_w + 64 * rp + 65536
