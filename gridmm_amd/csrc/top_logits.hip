@@ -275,7 +275,9 @@ __global__ __launch_bounds__(T, 4) void top_scan_kernel(const void* __restrict__
     for (int e = 1; e < E; ++e) top = fmaxf(top, x[e]);
     const float ref = fmaxf(m, fminf(top, HUGE_F));
     float t = 0.f;
-    if (__all(fabsf(ref) < 1e38f)) {          // (a product of the reference that stays finite: one instruction less)
+    // One instruction less with the reference's product rounded: 2^-24 of the reference on the log-sum-exp, half its own step.  Only for
+    // references up to 2^16: of 1e10, a mask's or a value's, that rounding is an exponent of its own, and the sum infinite
+    if (__all(fabsf(ref) < 65536.f)) {
       const float r2 = ref * LOG2E;
 #pragma unroll
       for (int e = 0; e < E; ++e) t += __builtin_amdgcn_exp2f(fmaf(x[e], LOG2E, -r2));

@@ -321,3 +321,32 @@ def test_workspaces_stay_within_what_is_said_of_them(dtype, rows, vocab, hidden)
     backward = lib.gridmm_vocab_loss_workspace(ctypes.byref(d), 1)
     scores_grad, sums, layout = max(512 * MB, 32768 * rp), max(256 * MB, 4 * rp * kp), 0 if dtype == 1 else rp * kp * size
     assert 0 < backward <= scores_grad + sums + layout + piece_w + 64 * rp + 65536
+
+
+# ---- extreme values: top logits ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("R,V", [(1, 70001), (3, 300), (300, 9001), (2000, 3000)])
+def test_top_logits_of_rows_masked_with_large_finite_numbers(dtype, R, V):
+    """Masks of -1e9 to -1e38 and the lowest number, in whole stretches and here and there, and rows whose own values are that large: the
+    log-sum-exp is that of the rest, sums of V exponentials (sqrt(V) + 16) u off, or as large as the largest value."""
+    from gridmm_amd import vocab
+    g = torch.Generator().manual_seed(V)
+    for mask in (-1e9, -3e10, -1e20, -1e30, -9e37, float(torch.finfo(DT[dtype]).min)):
+        x = torch.randn(R, V, generator=g) * 3
+        x[:, : V // 2] = mask
+        x[torch.rand(R, V, generator=g) < 0.3] = mask
+        x[:, -1] = 1.0
+        x = x.to(DT[dtype]).cuda()
+        values, ids, lse = vocab.top_logits(x, 5)
+        want, order = x.float().sort(dim=1, descending=True, stable=True)
+        assert torch.equal(ids, order[:, :5]) and torch.equal(values.float(), want[:, :5])
+        z = torch.logsumexp(x.double(), 1)
+        assert float((lse.double() - z).abs().max()) <= (V ** 0.5 + 16) * U * 30, mask
+    for size in (1e9, 3e10, 1e20, 1e37, 2e38):
+        x = (torch.randn(R, V, generator=g) * size / 8).to(DT[dtype]).cuda()
+        lse = vocab.top_logits(x, 1)[2].double()
+        z = torch.logsumexp(x.double(), 1)
+        # (2e38: rows that hold an infinity have it as their log-sum-exp, exactly)
+        off = torch.where(lse == z, torch.zeros_like(z), (lse - z).abs() / z.abs())
+        assert float(off.max()) <= 4 * U, size
