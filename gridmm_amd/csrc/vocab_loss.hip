@@ -149,7 +149,7 @@ __device__ __forceinline__ bool teacher_row(const void* ids, int wide, int64_t l
   bool nan = false;
   for (int s = lane; s < slots; s += 64) {
     if (load_index(ids, r * ld_ids + s, wide) < 0) continue;
-    const float v = t[r * ld_t + s] * inv_t;
+    const float v = t[r * ld_t + s];
     nan |= v != v;
     m = fmaxf(m, v);
   }
@@ -161,14 +161,14 @@ __device__ __forceinline__ bool teacher_row(const void* ids, int wide, int64_t l
   }
   float sum = 0.f;
   for (int s = lane; s < slots; s += 64)
-    if (load_index(ids, r * ld_ids + s, wide) >= 0) sum += expf(t[r * ld_t + s] * inv_t - m);
+    if (load_index(ids, r * ld_ids + s, wide) >= 0) sum += expf((t[r * ld_t + s] - m) * inv_t);
   sum = wave_sum(sum);
   const float ls = logf(sum);
   float h = 0.f;
   for (int s = lane; s < slots; s += 64) {
     float q = 0.f;
     if (load_index(ids, r * ld_ids + s, wide) >= 0) {
-      const float lp = t[r * ld_t + s] * inv_t - m - ls;
+      const float lp = (t[r * ld_t + s] - m) * inv_t - ls;      // (t / T may be past fp32 where the difference is not)
       q = expf(lp);
       if (q > 0.f || q != q) h += q * lp;
     }

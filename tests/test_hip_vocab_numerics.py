@@ -350,3 +350,29 @@ def test_top_logits_of_rows_masked_with_large_finite_numbers(dtype, R, V):
         # (2e38: rows that hold an infinity have it as their log-sum-exp, exactly)
         off = torch.where(lse == z, torch.zeros_like(z), (lse - z).abs() / z.abs())
         assert float(off.max()) <= 4 * U, size
+
+
+# ---- extreme values: teachers ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,V,K", [(10, 300, 64), (300, 4000, 768)])
+@pytest.mark.parametrize("T", [0.25, 1.0, 4.0])
+def test_a_teacher_with_extreme_values(R, V, K, T):
+    """Slots masked with the lowest number, rows of nothing else, and logits whose quotient by T is no longer a number of fp32."""
+    from gridmm_amd import vocab
+    h, w, b, g = _inputs("fp32", R, V, K, True, seed=1)
+    ids = torch.stack([torch.randperm(V, generator=g)[:6] for _ in range(R)]).cuda()
+    t = torch.randn(R, 6, generator=g).cuda()
+    low = torch.finfo(torch.float32).min
+    t[0, 2:] = low                                 # two slots count
+    t[1] = low                                     # all alike
+    t[2] = 3e38
+    t[3, 1:] = -3e38
+    t[4, 0] = 3e38                                 # one slot has it all
+    hl = h.clone().requires_grad_()
+    gr = torch.ones(R, device="cuda")
+    loss = vocab.vocab_distillation(hl, w, ids, t, bias=b, temperature=T)
+    loss.backward(gr)
+    z, want, sizes = _exact(h, w, b, ids, _teacher(ids, t, T), T, gr)
+    ez = _e_z(K, z)
+    assert float((loss.detach().double() - want["loss"]).abs().max()) <= T * T * (3 * ez + 16 * U * 8)
+    assert float(((hl.grad.double() - want["d_hidden"]).abs() - 3 * ez * sizes["d_hidden"]).max()) <= 0
