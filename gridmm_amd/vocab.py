@@ -128,7 +128,7 @@ def _vocab_backward(ctx, g):
         return (None,) * 8
     hidden, w, b, index, saved = ctx.saved_tensors
     d, keep = ctx.desc, None
-    if _place(hidden, w, b, index) != ctx.place:
+    if _place(hidden, w, b, index) != ctx.place or not saved.is_cuda:
         d, keep = _moved(ctx, g, hidden, w, b, index, saved)
     if g.dtype != torch.float32:
         g = g.float()

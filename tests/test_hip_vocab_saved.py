@@ -69,9 +69,8 @@ def test_a_checkpointed_backward_reads_what_the_second_forward_kept(library, slo
     keep = []
 
     def head(x):
-        h = x * 2.0
-        keep.append(torch.empty_like(h))           # (so that the second forward's lie elsewhere)
-        return _call(h, w, b, index, t)
+        keep.extend(torch.empty_like(x) for _ in range(256))      # (the memory of the first forward's h is taken: the second's lies elsewhere)
+        return _call(x * 2.0, w, b, index, t)
     checkpoint(head, x, use_reentrant=False).sum().backward()
     assert len(library.forward) == 2 and len(library.backward) == 1
     first, second, back = library.forward[0], library.forward[1], library.backward[0]
