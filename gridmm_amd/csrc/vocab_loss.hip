@@ -1245,15 +1245,19 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------------
 inline size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
-// Which kernels.  Wall time, us, few rows : tiles; what the host pays for 5 launches or 12, the autograd engine and the rest is ~127 : 142 there,
-// 21 : 30 for the forward alone.
-//   rows up to 32 fp32, 16 otherwise: fp32 forward and backward 30522 x 2048, 4 and 16 rows 303 : 436, 318 : 437, 131072 x 2048 at 32 rows
-//   1500 : 2300; bf16 131072 x 2048 at 5 and 32 rows 530 : 731, 951 : 756
-//   small products: a workgroup of the weight gradient goes through groups x ceil(hidden / 256) steps one after another (500 x 2048 at 8, 16,
-//   32 of them: fp32 139, 165, 230 : 160; bf16 -, 143, 169 : 161), and throughput counts from 3e8 scores x hidden on (fp32 452 hidden x 30522 at 16, 64
-//   rows 127, 185 : 160; bf16 8000 x 512 at 128, 256 rows 143, 176 : 160); the forward alone from 1e9 on (fp32 8000 x 2048 at 64 rows 59 : 92,
-//   2216 at 256 92 : 70; bf16 8000 x 452 at 256 rows 27 : 31, 8000 x 64 at 2048 92 : 28)
-// and in any case few enough comparisons of the distillation's targets (one pass over all rows' ids a workgroup).
+// Which kernels.  Wall time of a call alone, us, few rows : tiles; a small call is the host's time, ~140 : 175 forward and backward, ~35 : 40
+// - 50 the forward alone.
+//   up to 32 rows (the forward alone of 16 bits: 16): forward and backward bf16 131072 x 2048 at 5, 16, 32, 48 rows 506 : 783, 507 : 777, 667 : 782,
+//   1172 : 780; 30522 x 768 at 32, 48 rows 158 : 177, 193 : 176; fp32 131072 x 2048 at 16, 32 rows 810 : 2286, 989 : 2294; the forward alone
+//   bf16 131072 x 2048 at 17, 32 rows 177 : 184, 221 : 179
+//   small products: a workgroup of the weight gradient goes through groups x ceil(hidden / 256) steps one after another (bf16 8000 x 512 at 8, 16
+//   of them 163 : 172, 233 : 173; 2216 x 512 at 16, 32 178 : 172, 284 : 174), and throughput counts from 3e8 scores x hidden on (fp32 30522 x
+//   768 at 32, 64, 96 rows 162 : 223, 222 : 229, 305 : 234), where a score costs as much as 100 columns beside its product (16 bits);
+//   the forward alone from 1e9 on (fp32 8000 x 2048 at 64, 128 rows 80 : 129, 114 : 130; bf16 8000 x 452 at 256, 512 rows 48 : 57, 66 : 58;
+//   8000 x 16 at 512, 1024, 2048 rows 37 : 40, 48 : 41, 67 : 45)
+//   a teacher's slots: every workgroup looks through all rows' ids; fp32 256 rows x 2000 x 64 at 64, 256, 1024 slots (3e7, 1e8, 5e8 comparisons)
+//   147 : 191, 167 : 190, 691 : 463, the forward alone 44 : 53, 65 : 62, 318 : 103.  With few rows it is the tiles that suffer more (each row's slots
+//   against each other, one workgroup): 16 rows x 131072 x 768 bf16 at 2048, 8192 slots (4e9, 2e10) 422 : 1507, 1018 : 18184
 bool few_vectors(const gridmm_vocab_loss_t* d) {      // rows of h and W are whole 16-byte vectors on their boundaries
   const int A = d->dtype == F32 ? 4 : 8;
   return d->hidden_size % A == 0 && d->ld_hidden % A == 0 && d->ld_weight % A == 0 &&
@@ -1262,8 +1266,8 @@ bool few_vectors(const gridmm_vocab_loss_t* d) {      // rows of h and W are who
 bool few_rows(const gridmm_vocab_loss_t* d) {
   const double rv = (double)d->rows * d->vocab, K = d->hidden_size, targets = rv * d->slots;
   const bool fp32 = d->dtype == F32;
-  if (targets > 4e9) return false;
-  if (d->rows <= (fp32 ? 32 : 16)) return true;
+  if (targets > 2e10) return false;
+  if (d->rows <= (fp32 || !d->forward_only ? 32 : 16)) return true;
   if (targets > 1e8) return false;
   if (d->forward_only) return rv * (K + 100) <= 1.1e9;
   const int steps = (d->rows + 31) / 32 * ((d->hidden_size + 255) / 256);
