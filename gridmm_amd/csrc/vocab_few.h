@@ -300,7 +300,7 @@ __global__ __launch_bounds__(256) void few_loss_kernel(const FewArgs a, int64_t 
   if (wave) return;
   s = part[0];
   for (int w = 1; w < 4; ++w) s = join_stats(s, part[w]);
-  const float ls = 0.5f * __builtin_amdgcn_logf(s.y);      // (halves, base 2)
+  const float ls = s.x == -INFINITY ? NAN : 0.5f * __builtin_amdgcn_logf(s.y);      // (halves, base 2; no column left: no number)
   float out = 0.f;
   bool live, bad = false;
   if (a.kd) {

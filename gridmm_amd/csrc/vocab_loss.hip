@@ -745,7 +745,7 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
   a = part[0][rr];
   for (int w = 1; w < 16; ++w) a = join_stats(a, part[w][rr]);
   // The log-sum-exp stays in its two parts, maximum and logarithm of the sum: as one number it has the maximum's roundings, 2e-6 at 46
-  const float ls = 0.5f * __builtin_amdgcn_logf(a.y);        // (halves, base 2)
+  const float ls = a.x == -INFINITY ? NAN : 0.5f * __builtin_amdgcn_logf(a.y);        // (halves, base 2; no column left: no number)
   float s = 0.f, mass = 0.f;
   bool bad = !(a.x == a.x && ls == ls);
   if (i < count) {

@@ -195,7 +195,9 @@ def vocab_cross_entropy(hidden, weight, labels, bias=None, ignore_index=-1):
     bias (V,) in that type or fp32, labels (...) int64 or int32.  Gradients of hidden, weight and bias in their types.
 
     A label outside [0, V) that is not ignore_index makes its row's loss NaN, and with it the gradients that it reaches.  A bias of -inf
-    or of the type's lowest number takes its column out of the softmax.  At most 2^20 rows, 2^27 columns, and 2^37 scores.
+    or of the type's lowest number takes its column out of the softmax; with no column left a row is NaN.  At most 2^20 rows, 2^27
+    columns, and 2^37 scores.  fp32 rows (of hidden, or of weight) whose largest values are more than 2^14 apart, and fp32 and fp16 rows whose
+    upstream gradients times largest values are more than 2^20 apart, keep their accuracy on slower matrix instructions: 5 to 7 times the time.
 
     Memory beside the results: what is kept for the backward is a copy of hidden, and one of weight where it is fp32 or cannot be read in
     place and takes at most 512 MB; the backward holds one piece of the scores' gradient at a time, of 512 MB, or of 32 KB a row where that is more

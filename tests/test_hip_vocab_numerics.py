@@ -230,6 +230,44 @@ def test_rows_of_small_upstream_gradients_keep_their_own(dtype, R, V, K, ratio):
     _neighbours(got, want, sizes, z, h, every, torch.ones(V, dtype=torch.bool, device="cuda"), dtype)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+def test_a_captured_step_finds_out_anew_at_each_replay(dtype):
+    """Whether one scale serves all rows is decided on the device: a graph captured with ordinary rows is replayed with an outlier, with
+    upstream gradients far apart, and with ordinary ones again; every replay equals the eager call."""
+    from gridmm_amd import vocab
+    R, V, K = 300, 20011, 192
+    h, w, b, g = _inputs(dtype, R, V, K, True, seed=8)
+    hl, wl, bl = _leaves(h, w, b)
+    labels = torch.randint(0, V, (R,), generator=g).cuda()
+    gr = (torch.rand(R, generator=g) + 0.5).cuda()
+    plain = gr.clone()
+
+    def step():
+        loss = vocab.vocab_cross_entropy(hl, wl, labels, bias=bl)
+        return (loss,) + torch.autograd.grad(loss, (hl, wl, bl), gr)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        step()
+    torch.cuda.current_stream().wait_stream(st)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for large, ratio in ((1.0, 0), (3e4, 0), (1.0, 30), (1.0, 0), (3e4, 30)):
+        with torch.no_grad():
+            hl.copy_(h)
+            hl[7] *= large
+        gr.copy_(plain)
+        gr[::3] *= 2.0 ** -ratio
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _run_ce(hl.detach(), w, b, labels, gr)
+        for x, k in zip(out, ("loss", "d_hidden", "d_weight", "d_bias")):
+            assert torch.equal(torch.nan_to_num(x), torch.nan_to_num(want[k])), (large, ratio, k)
+
+
 # ---- no tile is left out ----
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype,R,V,K", [("bf16", 300, 70000, 64), ("fp32", 300, 70000, 64), ("fp16", 300, 33000, 72), ("fp32", 20, 9001, 64),
@@ -376,3 +414,25 @@ def test_a_teacher_with_extreme_values(R, V, K, T):
     ez = _e_z(K, z)
     assert float((loss.detach().double() - want["loss"]).abs().max()) <= T * T * (3 * ez + 16 * U * 8)
     assert float(((hl.grad.double() - want["d_hidden"]).abs() - 3 * ez * sizes["d_hidden"]).max()) <= 0
+
+
+# ---- extreme values: nothing left ----
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("R,V,K", [(10, 300, 64), (300, 4000, 768)])
+@pytest.mark.parametrize("mask", ["-inf", "lowest"])
+def test_rows_without_a_column_are_no_number(dtype, R, V, K, mask):
+    """All columns out of the softmax: 0 / 0."""
+    from gridmm_amd import vocab
+    h, w, b, g = _inputs(dtype, R, V, K, True, seed=1)
+    b[:] = float("-inf") if mask == "-inf" else torch.finfo(b.dtype).min
+    y = torch.randint(0, V, (R,), generator=g).cuda()
+    y[1] = -1
+    hl = h.requires_grad_()
+    for loss in (vocab.vocab_cross_entropy(hl, w, y, bias=b),
+                 vocab.vocab_distillation(hl, w, torch.stack([y, y], 1), torch.zeros(R, 2, device="cuda"), bias=b)):
+        assert float(loss[1]) == 0.0
+        rest = torch.arange(R, device="cuda") != 1
+        assert bool(torch.isnan(loss[rest]).all())
+        d, = torch.autograd.grad(loss.sum(), hl)
+        assert bool(torch.isnan(d[rest]).all()) and bool((d[1] == 0).all())
