@@ -17,9 +17,10 @@
 //                c ^ (((row >> 1) & 1) << 2): the 4 rows x 64 bytes that half a wave's transpose read takes are 256 different bytes
 // Both hand lane l of a 32x32x16 fragment its row (or column) l & 31 at contraction steps 8 (l >> 5) .. + 7.
 //
-// Bound by the way of the operands from L2 to the CU: the 256 x 256 tile asks for 32 bytes a clock at full matrix rate and gets ~21 (10.0 - 10.6
-// TB/s over the chip at 1.7 GHz, matrix pipes 63 - 72 % busy, no bank conflicts); ~10 % of a tile's time is its end, which nothing overlaps.
-// 8030 x 131072 x 2048 bf16: scores 3.35 - 3.43 ms = 1.26 - 1.29 PFLOP/s, dh and dW 1.26 - 1.31 (a large library product 1.36 - 1.41).  128 x 128 tiles
+// Bound by the way of the operands from L2 to the CU: the 256 x 256 tile asks for 32 bytes a clock at full matrix rate and gets ~21 (9.2 - 10.3
+// TB/s over the chip at 1.7 GHz, matrix pipes 58 - 72 % busy, no bank conflicts); ~10 % of a tile's time is its end, which nothing overlaps.
+// 8030 x 131072 x 2048 bf16: scores 3.36 ms = 1.28 PFLOP/s, dh and dW, each over two planes of dS, 1.27 - 1.28 (a large library product 1.36 - 1.41;
+// boxes and hours differ by 6 %).  128 x 128 tiles
 // (two workgroups a CU, 64 bytes a clock) only where the larger ones leave CUs idle.  Measured and not kept: 4 waves of 128 x 128 (278 : 246 us
 // a piece), a raised wave priority around the products (the same).
 #pragma once

@@ -21,8 +21,8 @@
 // power-of-two scale from the tensor's largest finite value: 22 bits of a value, or 25 of its row's largest, as long as the rows' largest
 // values lie within 2^14 of each other, which the device finds out; rows further apart run on fp32 matrix instructions.  fp16
 // planes of dS take a power-of-two scale for each row, from its |g T|.
-// Bound by the four products (vocab_gemm.h): 8030 x 131072 x 2048 bf16 forward and backward 13.8 - 14.0 ms, of it 3.4 scores, 3.7 dS, 3.4 dh, 3.4 dW;
-// fp32 384 x 30522 x 768 325 us, of it 260 products (1.4 rounds of 128 x 128 tiles) and 53 for W's scale and packing.
+// Bound by the products (vocab_gemm.h): 8030 x 131072 x 2048 bf16 forward and backward 21.1 ms, of it 3.4 scores, 4.1 dS, 6.7 dh, 6.8 dW (two planes
+// of dS each); fp32 384 x 30522 x 768 334 - 350 us, of it 255 products (1.4 rounds of 128 x 128 tiles) and 60 for W's scale and packing.
 // Everything runs in the base-2 domain: y = z log2 e, exp2, and ln 2 comes back in the losses.
 #include <algorithm>
 
@@ -107,14 +107,15 @@ struct Raw {
 constexpr int BIG_TILES = 384;
 __host__ __device__ inline bool big_tiles(int64_t count, int64_t C) { return count > 256 && (count + 255) / 256 * (C / 256) >= BIG_TILES; }
 // Contraction ranges of dh, so that its few tiles fill whole rounds of the chip: the cheapest of the numbers that fit into the first
-// rounds, in stages of 64 columns a workgroup (1.2 us): rounds x (its share + what a tile costs beside its stages) + the ranges' sums
-// written and read once more at ~4.7 TB/s.  136 tiles at 4099 x 2048 over 32768 columns: 1 range 752 us, 5 ranges 545 us.
+// rounds, in stages of 64 columns a workgroup (1.2 us, and as much again for the second plane of 16 bits): rounds x (its share + what a
+// tile costs beside its stages) + the ranges' sums written and read once more at ~4.7 TB/s.  136 tiles at 4099 x 2048 over 32768 columns of one
+// plane: 1 range 752 us, 5 ranges 545 us; over 22016 of two planes 3 ranges 749, 5 ranges 717.
 constexpr int64_t PART_MOST = 64 << 20;      // values of the ranges' partial products, if there are more than one
 constexpr int MOST_SPLITS = 64;
-__device__ __forceinline__ int hidden_splits(int64_t count, int64_t Kp, int64_t C, bool big) {
+__device__ __forceinline__ int hidden_splits(int64_t count, int64_t Kp, int64_t C, bool big, bool two) {
   const int T = big ? 256 : 128, slots = big ? 256 : 512;
   const int tiles = (int)((count + T - 1) / T) * (int)((Kp + T - 1) / T);
-  const float stages = (float)(C / 64), join = (float)(count * Kp) * (8.f / 4.7e6f / 1.2f);
+  const float stages = (float)(C / 64) * (two ? 2.f : 1.f), join = (float)(count * Kp) * (8.f / 4.7e6f / 1.2f);
   int most = (int)min((int64_t)MOST_SPLITS, C / 512);                   // at least 8 stages a range
   if (count > 0) most = (int)min((int64_t)most, PART_MOST / (count * Kp));
   int best = 1;
@@ -1049,7 +1050,7 @@ __global__ __launch_bounds__(T::THREADS, 2) void hidden_grad_kernel(Operand A, O
   const bool big = big_tiles(count, C);
   if (big != (T::BM == 256)) return;
   constexpr bool TWO = T::PL == 1;       // dS's two planes one after the other
-  const int splits = hidden_splits(count, Kp, C, big), per = (steps + splits - 1) / splits;
+  const int splits = hidden_splits(count, Kp, C, big, TWO), per = (steps + splits - 1) / splits;
   if (blockIdx.x == 0 && threadIdx.x == 0) back->ranges = splits;
   const int wave = threadIdx.x >> 6, wr = wave / T::WAVES_N, wc = wave % T::WAVES_N;
   unsigned short* scratch = smem + T::LDS + wave * 2048;
