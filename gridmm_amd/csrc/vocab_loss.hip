@@ -781,7 +781,7 @@ __global__ __launch_bounds__(256) void loss_kernel(const float2* __restrict__ st
 // dS in fp16 planes takes a scale for each row, from its |g T|: 2^13 at most, so that a row's entries keep 22 bits, or 2^-38 of its
 // own |g T|, whatever the others are.  dh takes the scales out again row by row; dW = dS^T h sums over the rows, so h is laid out once
 // more with the scales' inverses in it, and db's sums carry them as weights (2^15 to 2^-24).  Rows whose |g T| |h| are more than 2^20 apart do not
-// fit into one layout of h, |g T| more than 2^39 apart not into the weights: dS is fp32 then and dh and dW are products on fp32 matrix
+// fit into one layout of h (up to there a value is off by 2^-19 of its row's largest at most), |g T| more than 2^39 apart not into the weights: dS is fp32 then and dh and dW are products on fp32 matrix
 // instructions.  bf16 has fp32's range and needs none of it.
 constexpr int GRAD_SPREAD = 20, WEIGHT_SPREAD = 39;
 struct Back {

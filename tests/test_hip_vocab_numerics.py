@@ -208,6 +208,52 @@ def test_distillation_beside_one_large_row(S):
     _neighbours(got, want, sizes, z, h, torch.arange(R, device="cuda") != 5, columns, "fp32")
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("loss", ["cross_entropy", "distillation"])
+@pytest.mark.parametrize("dtype,R,V,K", [("fp32", 9100, 33001, 72), ("fp16", 9100, 33001, 72), ("fp32", 270, 200003, 700)])
+def test_rows_far_apart_over_several_pieces(dtype, R, V, K, loss):
+    """More columns than a piece of dS or a packed piece of W holds, rows of wider matrices off 16-byte boundaries, ignored rows among them: an
+    outlier row of each operand (fp32), upstream gradients far apart."""
+    from gridmm_amd import vocab
+    h, w, b, g = _inputs(dtype, R, V, K, True, seed=7)
+    if dtype == "fp32":
+        h[5] *= 1e9
+        w[7] *= 1e9
+    b[7] = float("-inf")
+
+    def strided(t):
+        return torch.zeros(t.shape[0], t.shape[1] + 5, dtype=t.dtype, device="cuda")[:, 3:3 + t.shape[1]].copy_(t)
+    hl, wl, bl = _leaves(strided(h), strided(w), b)
+    gr = (torch.rand(R, generator=g) + 0.5).cuda()
+    gr[::3] *= 2.0 ** -24
+    if dtype == "fp16":
+        gr *= 2.0 ** 12
+    live = torch.rand(R, generator=g).cuda() > 0.2
+    live[5] = True
+    S, T = (1, 1.0) if loss == "cross_entropy" else (4, 2.0)
+    ids = (8 + torch.stack([torch.randperm(V - 8, generator=g)[:S] for _ in range(R)])).cuda()
+    p = torch.ones(R, S, dtype=torch.float64, device="cuda")
+    if loss == "cross_entropy":
+        got = vocab.vocab_cross_entropy(hl, wl, torch.where(live, ids[:, 0], torch.full_like(ids[:, 0], -1)), bias=bl)
+    else:
+        t = torch.randn(R, S, generator=g).cuda()
+        p = _teacher(ids, t, T)
+        got = vocab.vocab_distillation(hl, wl, torch.where(live[:, None], ids, torch.full_like(ids, -1)), t, bias=bl, temperature=T)
+    got.backward(gr)
+    keep = torch.arange(V, device="cuda") != 7
+    z, want, sizes = _exact(h, w[keep], b[keep], ids - 1, p, T, torch.where(live, gr, torch.zeros_like(gr)))
+    want["loss"] = torch.where(live, want["loss"], torch.zeros_like(want["loss"])) / (T * T)
+    rows = torch.arange(R, device="cuda") != 5 if dtype == "fp32" else torch.ones(R, dtype=torch.bool, device="cuda")
+    columns = torch.ones(V - 1, dtype=torch.bool, device="cuda")
+    if dtype == "fp32":
+        columns[ids[5] - 1] = False
+        columns[z[5].argmax()] = False
+    out = {"loss": got.detach() / (T * T), "d_hidden": hl.grad, "d_weight": wl.grad[keep], "d_bias": bl.grad[keep]}
+    z[~live] = 0.0
+    _neighbours(out, want, sizes, z, h, rows, columns, dtype)
+    assert bool((hl.grad[~live] == 0).all()) and bool((wl.grad[7] == 0).all())
+
+
 # ---- upstream gradients far apart ----
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
@@ -228,6 +274,44 @@ def test_rows_of_small_upstream_gradients_keep_their_own(dtype, R, V, K, ratio):
     z, want, sizes = _exact(h, w, b, labels[:, None], torch.ones(R, 1, dtype=torch.float64, device="cuda"), 1.0, gr)
     every = torch.ones(R, dtype=torch.bool, device="cuda")
     _neighbours(got, want, sizes, z, h, every, torch.ones(V, dtype=torch.bool, device="cuda"), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("R,V,K,apart", [(300, 4000, 768, 32), (300, 4000, 768, 17), (2600, 11000, 256, 32)])
+def test_columns_that_only_rows_of_small_gradients_reach(dtype, R, V, K, apart):
+    """Rows that put everything on one column, their label another: the label's entry of dS is -g, the column's +g.  The rows of the even half
+    have upstream gradients 2^-apart of the others' and hidden states up to 2^12 times as large (another bias holds their scores down), so that the
+    columns that only they reach have sums of their own size."""
+    g = torch.Generator().manual_seed(apart)
+    w = torch.randn(V, K, generator=g) / K ** 0.5
+    order = torch.randperm(V, generator=g)[:2 * R]
+    top, labels = order[:R], order[R:2 * R].cuda()
+    h = w[top] * (40.0 / (w[top] * w[top]).sum(1, keepdim=True))
+    up = 12 if apart == 32 else 0
+    h[::2] *= 2.0 ** up
+    h, w = h.to(DT[dtype]).cuda(), w.to(DT[dtype]).cuda()
+    gr = (torch.rand(R, generator=g) + 0.5).cuda()
+    gr[::2] *= 2.0 ** -apart
+    b = torch.zeros(V, device="cuda")
+    hl, wl, bl = _leaves(h, w, b)
+    from gridmm_amd import vocab
+    vocab.vocab_cross_entropy(hl, wl, labels, bias=bl).backward(gr * 2.0 ** 14 if dtype == "fp16" else gr)
+    gx = gr * 2.0 ** 14 if dtype == "fp16" else gr
+    z, want, sizes = _exact(h, w, b, labels[:, None], torch.ones(R, 1, dtype=torch.float64, device="cuda"), 1.0, gx)
+    half = HALF[DT[dtype]]
+    # a row's other entries of dS: softmax of scores 40 apart at least less what 8 standard deviations make up; far below fp32 where h is larger
+    for k, got in (("d_bias", bl.grad), ("d_weight", wl.grad)):
+        at = labels[::2]
+        v = want[k][at]
+        # the entry itself: (1 - q) g, two 16-bit planes (2^-16).  The layout of h has rows' |g h| up to 2^20 apart, the largest in [2^14, 2^15): a row's
+        # largest value lies at 2^-6 at least, and half of fp16's last step is 2^-25, so a value is off by 2^-19 of its row's largest at most
+        bound = (2.0 ** -15 + (half if k == "d_weight" else 0.0)) * sizes[k][at] + (2.0 ** -25 if dtype == "fp16" else 0.0)
+        if k == "d_weight":
+            bound = bound + 2.0 ** -19 * (gx[::2].double() * h[::2].double().abs().amax(1))[:, None]
+        d = (got.double()[at] - v).abs() - bound
+        assert float(d.max()) <= 0, (k, float(d.max()), float(v.abs().max()))
+        assert float(v.abs().max()) > 0
 
 
 @pytest.mark.gpu
